@@ -75,6 +75,9 @@ _SIGNATURES = {
     "frb_expert_gemm_tc": "pipippppiipiiipif",
     "frb_gather_rows_bf16": "pppii",
     "frb_attention_prefill_tc": "pippipippipppppiiifippipf" "iiii",
+    "frb_qkv_prepare_8bit": "pippif" "ppi" "pppii" "ppppp" "ii" "iiiiiiiii" "i" "pfi" "i",
+    "frb_cache_read_8bit": "ppppi" "ipii" "ppi" "pppi" "pp" "iiii",
+    "frb_attention_decode_8bit": "pppppi" "ipii" "pp" "ppp" "iiiiii" "f" "iii" "ii" "pp" "f" "pff" "p",
     "frb_attention_pair_tc": "pippi" "pippi" "ppppp" "iiiifiif" "pffp",
     "frb_dyt_rows": "ppppp" "ppp" "pp" "iii" "p" "pppp" "pll",
     "frb_stream_copies": "pip" "pp" "ppppp" "ip" "ppp" "ppp" "pip" "iii",
@@ -112,6 +115,7 @@ _ENTRY_GROUPS = {
                "frb_latent_attention_mma", "frb_latent_attention_tc"),
     "attention": ("frb_attention_decode_mma", "frb_attention_prefill_mma", "frb_attention_decode_tma", "frb_attention_prefill_tc",
                   "frb_attention_pair_tc"),
+    "cache8": ("frb_qkv_prepare_8bit", "frb_cache_read_8bit", "frb_attention_decode_8bit"),
     "attention32": ("frb_attention_f32_tiles", "frb_attention_f32_tc", "frb_attention_f32_token"),
     "streams": ("frb_weight_stream", "frb_expert_gemm_mma", "frb_rows_f32", "frb_dense_rows_f32"),
     "experts": ("frb_router_topk", "frb_expert_plan", "frb_expert_combine", "frb_expert_gemm_generic", "frb_route_plan_small",
@@ -207,7 +211,7 @@ def _stream() -> int:
 
 
 _LAUNCHES = 0
-_KERNELS_PER_CALL = {"frb_gated_delta_rule": 2, "frb_gated_recurrence": 2, "frb_sample_floor": 3, "frb_argmax_rows": 2, "frb_expert_plan": 3, "frb_attention_decode_mma": 2, "frb_attention_decode_tma": 2, "frb_attention_f32_token": 2, "frb_gla_chunks": 3, "frb_state_space_chunks": 3, "frb_delta_chunks": 4, "frb_products_f32": 2, "frb_attention_f32_tc": 2}
+_KERNELS_PER_CALL = {"frb_gated_delta_rule": 2, "frb_gated_recurrence": 2, "frb_sample_floor": 3, "frb_argmax_rows": 2, "frb_expert_plan": 3, "frb_attention_decode_mma": 2, "frb_attention_decode_tma": 2, "frb_attention_f32_token": 2, "frb_attention_decode_8bit": 2, "frb_gla_chunks": 3, "frb_state_space_chunks": 3, "frb_delta_chunks": 4, "frb_products_f32": 2, "frb_attention_f32_tc": 2}
 
 
 def launches() -> int:
@@ -1528,6 +1532,8 @@ _WAIT_CODES = {
     3: "expert products: the epilogue waiting for the accumulators",
     6: "expert products: the MMA thread waiting for the epilogue to have read the accumulators",
     4: "one-token attention: waiting for a page's copy",
+    7: "one-token attention over 8-bit pages: waiting for a page's copy",
+    8: "one-token attention over 8-bit pages: a sequence has more keys than the launch was sized for (max_chunks); keys were left out",
     5: "one-token attention: a sequence has more keys than the launch was sized for (max_chunks); keys were left out",
     21: "weight stream: the producer waiting for a free stage",
     22: "weight stream: a compute warp waiting for a loaded stage",
@@ -1710,6 +1716,170 @@ def attention_pair_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
           page_table.shape[1], _ptr(tile_seq), _ptr(tile_q0), tile_seq.numel(), _ptr(seq_slot), _ptr(seq_start), _ptr(seq_q_len),
           _ptr(cu_q_len), _ptr(out), int(heads), int(v_heads), int(head_dim), int(v_dim), float(scale), int(window or 0),
           int(keep_first or 0), float(softcap or 0.0), _ptr(lam), float(eps), float(factor), _ptr(tc_status(q.device)))
+
+
+# ------------------------------------------------------------------------------------------------ a cache in 8 bits
+
+CACHE_8BIT_TYPES = {torch.float8_e4m3fn: 0, torch.int8: 1}      # types of the codes (FRB_E4M3, FRB_INT8)
+
+
+def _want_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor, *others) -> int:
+    """Checks a store of 8-bit pages against itself and that it and the other tensors lie on the current device; the codes' type."""
+    if k_pages.dtype not in CACHE_8BIT_TYPES or v_pages.dtype != k_pages.dtype:
+        raise KernelError(f"8-bit pages hold float8_e4m3fn or int8, keys and values alike: found {k_pages.dtype} and {v_pages.dtype}")
+    _want(k_scales, torch.float32, "the keys' scales")
+    _want(v_scales, torch.float32, "the values' scales")
+    for pages, scales, what in ((k_pages, k_scales, "keys"), (v_pages, v_scales, "values")):
+        if pages.dim() != 4 or pages.shape[2] != PAGE or tuple(scales.shape) != tuple(pages.shape[:3]):
+            raise KernelError(f"8-bit {what} of shape {list(pages.shape)} with scales of {list(scales.shape)}: pages are "
+                              f"[pages, heads, {PAGE}, entries], scales [pages, heads, {PAGE}]")
+    if k_pages.shape[0] != v_pages.shape[0]:
+        raise KernelError(f"{k_pages.shape[0]} pages of keys and {v_pages.shape[0]} of values")
+    device = k_pages.device
+    for t in (k_scales, v_pages, v_scales, *others):
+        if t is not None and t.device != device:
+            raise KernelError(f"tensors on {device} and {t.device} in one call")
+    if device.type == "cuda" and device.index != torch.cuda.current_device():
+        raise KernelError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    return CACHE_8BIT_TYPES[k_pages.dtype]
+
+
+def _want_ints(tensors: dict) -> None:
+    for what, t in tensors.items():
+        _want(t, torch.int32, what)
+
+
+def qkv_prepare_8bit(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
+                     cos_table: Optional[torch.Tensor], sin_table: Optional[torch.Tensor], tok_pos: torch.Tensor, tok_slot: torch.Tensor,
+                     page_table: torch.Tensor, q_out: torch.Tensor, k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor,
+                     v_scales: torch.Tensor, *, num_heads: int, num_kv_heads: int, head_dim: int, rotary_dim: int, interleaved: bool,
+                     per_head: bool = False, tables_final: bool = False, bias: Optional[torch.Tensor] = None, v_dim: Optional[int] = None,
+                     q_temp: Optional[tuple[float, int]] = None, num_v_heads: Optional[int] = None, values_from_keys: bool = False) -> None:
+    """As :func:`qkv_prepare`, keys and values written as 8-bit codes with a scale a row (one token, one head): scale = max |x| / Q,
+    code = x * Q / max |x| rounded half to even, Q = 448 (float8_e4m3fn) or 127 (int8).  ``k_pages`` and ``v_pages`` are [pages, heads,
+    64, entries] (values not transposed), ``k_scales`` and ``v_scales`` float32 [pages, heads, 64].  A row whose largest entry is below
+    2^-96 is stored as zeros; one with an entry that is not finite reads back as NaN.  No two different rows of a call go to one place.  A token whose slot, position or page does
+    not exist (a table entry of -1) leaves the store as it was.  Queries come out in bfloat16.  Head sizes: ``MMA_HEAD_SIZES``."""
+    v_dim = int(v_dim or head_dim)
+    num_v_heads = num_kv_heads if num_v_heads is None else int(num_v_heads)
+    codes = _want_8bit(k_pages, k_scales, v_pages, v_scales, qkv, q_weight, k_weight, cos_table, sin_table, tok_pos, tok_slot, page_table, q_out, bias)
+    if (q_weight is None) != (k_weight is None):
+        raise KernelError("q and k norm weights come together or not at all")
+    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
+        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
+    tokens = qkv.shape[0]
+    row = (num_heads + num_kv_heads) * head_dim + (0 if values_from_keys else num_v_heads * v_dim)
+    if qkv.dim() != 2 or qkv.shape[1] != row:
+        raise KernelError(f"projected rows of shape {list(qkv.shape)}, not [tokens, {row}]")
+    if tuple(k_pages.shape[1:]) != (num_kv_heads, PAGE, head_dim) or tuple(v_pages.shape[1:]) != (num_v_heads, PAGE, v_dim):
+        raise KernelError(f"8-bit pages of {list(k_pages.shape[1:])} and {list(v_pages.shape[1:])} for {num_kv_heads} key heads of {head_dim} "
+                          f"and {num_v_heads} value heads of {v_dim}")
+    _want(q_out, torch.bfloat16, "queries")
+    if q_out.numel() != tokens * num_heads * head_dim:
+        raise KernelError(f"{q_out.numel()} query entries for {tokens} tokens of {num_heads} heads of {head_dim}")
+    _want_ints({"positions": tok_pos, "slots": tok_slot, "the page table": page_table})
+    if tok_pos.numel() != tokens or tok_slot.numel() != tokens or page_table.dim() != 2:
+        raise KernelError(f"{tok_pos.numel()} positions and {tok_slot.numel()} slots for {tokens} tokens")
+    wdtype = torch.float32
+    if q_weight is not None:
+        wdtype = q_weight.dtype
+        widths = (head_dim, head_dim) if per_head else (num_heads * head_dim, num_kv_heads * head_dim)
+        if k_weight.dtype != wdtype or (q_weight.numel(), k_weight.numel()) != widths:
+            raise KernelError(f"q and k norm weights of {q_weight.numel()} and {k_weight.numel()} entries ({wdtype}, {k_weight.dtype}), not {widths}")
+    if bias is not None:
+        _want(bias, torch.float32, "the projections' bias")
+        if bias.numel() != row:
+            raise KernelError(f"a bias of {bias.numel()} entries for rows of {row}")
+    if rotary_dim:
+        if cos_table is None or sin_table is None:
+            raise KernelError("rotary tables are missing")
+        for table in (cos_table, sin_table):
+            _want(table, torch.float32, "rotary tables")
+            if table.dim() != 2 or table.shape[1] != rotary_dim // 2 or table.shape[0] != cos_table.shape[0]:
+                raise KernelError(f"a rotary table of shape {list(table.shape)} for {rotary_dim} rotated entries")
+    _call("frb_qkv_prepare_8bit", _ptr(qkv), _code(qkv.dtype), _ptr(q_weight), _ptr(k_weight), _code(wdtype), float(eps),
+          _ptr(cos_table), _ptr(sin_table), cos_table.shape[0] if cos_table is not None else 0, _ptr(tok_pos), _ptr(tok_slot),
+          _ptr(page_table), page_table.shape[0], page_table.shape[1], _ptr(q_out), _ptr(k_pages), _ptr(k_scales), _ptr(v_pages),
+          _ptr(v_scales), codes, k_pages.shape[0], tokens, num_heads, num_kv_heads, num_v_heads, head_dim, v_dim, rotary_dim,
+          int(interleaved), int(per_head), int(tables_final), _ptr(bias), float(q_temp[0]) if q_temp else 0.0,
+          int(q_temp[1]) if q_temp else 1, int(values_from_keys))
+
+
+def cache_read_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
+                    page_seq: torch.Tensor, page_index: torch.Tensor, seq_slot: torch.Tensor, seq_start: torch.Tensor, seq_q_len: torch.Tensor,
+                    keys: torch.Tensor, values: torch.Tensor) -> None:
+    """Pages of a cache of 8-bit pages as bfloat16 pages in the layout of the prompt kernels: ``keys[n]`` and ``values[n]`` (transposed,
+    [heads, entries, 64]) are page number ``page_index[n]`` of sequence ``page_seq[n]``, code times scale rounded once.  Sequence b is
+    slot ``seq_slot[b]`` and holds ``seq_start[b] + seq_q_len[b]`` tokens; places behind them, and pages that the table does not have, become zero."""
+    codes = _want_8bit(k_pages, k_scales, v_pages, v_scales, page_table, page_seq, page_index, seq_slot, seq_start, seq_q_len, keys, values)
+    _want_ints({"the page table": page_table, "pages' sequences": page_seq, "pages' numbers": page_index, "slots": seq_slot,
+                "positions": seq_start, "new tokens": seq_q_len})
+    _want(keys, torch.bfloat16, "keys read back")
+    _want(values, torch.bfloat16, "values read back")
+    kv_heads, head_dim, v_heads, v_dim = k_pages.shape[1], k_pages.shape[3], v_pages.shape[1], v_pages.shape[3]
+    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
+        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
+    count = page_seq.numel()
+    if page_index.numel() != count or tuple(keys.shape) != (count, kv_heads, PAGE, head_dim) or tuple(values.shape) != (count, v_heads, v_dim, PAGE):
+        raise KernelError(f"{count} sequences and {page_index.numel()} numbers of pages with keys of shape {list(keys.shape)} and values of "
+                          f"{list(values.shape)}")
+    if seq_start.numel() != seq_slot.numel() or seq_q_len.numel() != seq_slot.numel() or page_table.dim() != 2:
+        raise KernelError(f"{seq_slot.numel()} slots with {seq_start.numel()} positions and {seq_q_len.numel()} numbers of new tokens")
+    _call("frb_cache_read_8bit", _ptr(k_pages), _ptr(k_scales), _ptr(v_pages), _ptr(v_scales), codes, k_pages.shape[0], _ptr(page_table),
+          page_table.shape[0], page_table.shape[1], _ptr(page_seq), _ptr(page_index), count, _ptr(seq_slot), _ptr(seq_start), _ptr(seq_q_len),
+          seq_slot.numel(), _ptr(keys), _ptr(values), kv_heads, v_heads, head_dim, v_dim)
+
+
+def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor,
+                          page_table: torch.Tensor, seq_pos: torch.Tensor, seq_slot: torch.Tensor, part_o: torch.Tensor,
+                          part_ml: torch.Tensor, out: torch.Tensor, *, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                          window: Optional[int], max_chunks: int, chunks_per_block: Optional[int] = None,
+                          slopes: Optional[torch.Tensor] = None, chunk: Optional[int] = None, sinks: Optional[torch.Tensor] = None,
+                          softcap: Optional[float] = None, v_dim: Optional[int] = None, keep_first: int = 0, maps: int = 1,
+                          difference: Optional[dict] = None) -> None:
+    """As :func:`attention_decode_tma` over 8-bit pages (see :func:`qkv_prepare_8bit`), for every head size of ``MMA_HEAD_SIZES`` and
+    groups of any size; queries and output are bfloat16.  ``part_o`` and ``part_ml`` (float32) hold a partial result per (sequence, head,
+    run of ``chunks_per_block`` chunks): ``[sequences, heads, max_chunks, v_dim]`` and ``[..., 2]`` always suffice.  A sequence
+    at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
+    v_dim = int(v_dim or head_dim)
+    codes = _want_8bit(k_pages, k_scales, v_pages, v_scales, q, page_table, seq_pos, seq_slot, part_o, part_ml, out, slopes, sinks,
+                       difference["lam"] if difference is not None else None)
+    if maps < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or num_kv_heads % maps:
+        raise KernelError(f"{num_heads} heads over {num_kv_heads} key heads with {maps} maps")
+    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
+        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
+    if tuple(k_pages.shape[1:]) != (num_kv_heads, PAGE, head_dim) or tuple(v_pages.shape[1:]) != (num_kv_heads // maps, PAGE, v_dim):
+        raise KernelError(f"8-bit pages of {list(k_pages.shape[1:])} and {list(v_pages.shape[1:])} for {num_kv_heads} key heads of {head_dim} "
+                          f"and {num_kv_heads // maps} value heads of {v_dim}")
+    _want(q, torch.bfloat16, "queries")
+    _want(out, torch.bfloat16, "the attention output")
+    _want(part_o, torch.float32, "partial outputs")
+    _want(part_ml, torch.float32, "partial maxima and sums")
+    _want_slopes(slopes, num_heads)
+    _want_slopes(sinks, num_heads)
+    _want_ints({"the page table": page_table, "positions": seq_pos, "slots": seq_slot})
+    seqs = q.shape[0]
+    lam, eps, factor = _difference_args(difference, maps)
+    heads_out = num_heads // 2 if difference is not None else num_heads
+    if q.numel() != seqs * num_heads * head_dim or out.numel() != seqs * heads_out * v_dim:
+        raise KernelError(f"queries of shape {list(q.shape)} and an output of {list(out.shape)} for {num_heads} heads of {head_dim} and {v_dim}")
+    if seq_pos.numel() != seqs or seq_slot.numel() != seqs or page_table.dim() != 2:
+        raise KernelError(f"{seq_pos.numel()} positions and {seq_slot.numel()} slots for {seqs} sequences")
+    if window is not None and window < 0 or chunk is not None and chunk < 0 or keep_first < 0:
+        raise KernelError(f"a window of {window}, chunks of {chunk}, {keep_first} first tokens")
+    if max_chunks < 1 or (chunks_per_block is not None and chunks_per_block < 1):
+        raise KernelError(f"{max_chunks} chunks, {chunks_per_block} per block")
+    if chunks_per_block is None:
+        _ptr(q)                                                         # refuses a tensor on the host before the device is asked
+        chunks_per_block = decode_chunks_per_block(seqs, num_kv_heads, max_chunks, sm_count(q.device))
+    rows = seqs * num_heads * -(-max_chunks // chunks_per_block)
+    if part_o.numel() < rows * v_dim or part_ml.numel() < rows * 2:
+        raise KernelError(f"room for {part_o.numel()} partial outputs and {part_ml.numel()} maxima and sums, {rows * v_dim} and {rows * 2} are needed")
+    _call("frb_attention_decode_8bit", _ptr(q), _ptr(k_pages), _ptr(k_scales), _ptr(v_pages), _ptr(v_scales), codes, k_pages.shape[0],
+          _ptr(page_table), page_table.shape[0], page_table.shape[1], _ptr(seq_pos), _ptr(seq_slot), _ptr(part_o), _ptr(part_ml), _ptr(out),
+          seqs, num_heads, num_kv_heads, num_kv_heads // maps, head_dim, v_dim, float(scale), int(window or 0), int(chunk or 0),
+          int(keep_first or 0), max_chunks, int(chunks_per_block), _ptr(slopes), _ptr(sinks), float(softcap or 0.0), lam, eps, factor,
+          _ptr(tc_status(q.device)))
 
 
 def wait_probe(device, limit_cycles: int = 100_000) -> int:
