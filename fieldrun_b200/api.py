@@ -29,8 +29,8 @@ from .sampling import SamplingParams
 from .weights import FolderSource, MemorySource, RandomInit, write_model_folder
 
 
-def build_model(arch: Architecture, config: ModelConfig, dtype) -> DecoderModel:
-    return DecoderModel(arch.plan(config), dtype)
+def build_model(arch: Architecture, config: ModelConfig, dtype, cache_dtype=None) -> DecoderModel:
+    return DecoderModel(arch.plan(config), dtype, cache_dtype)
 
 
 def write_random_model(folder: str, config: ModelConfig | dict, init: RandomInit = RandomInit()) -> None:
@@ -104,12 +104,14 @@ class LanguageModel:
 
 
 def load(model_dir: str, *, dtype="bfloat16", max_tokens: int = 8192, num_slots: Optional[int] = None,
-         device="cuda", max_batch: int = 64) -> LanguageModel:
-    """Load a model folder (config.json + safetensors); the model class is chosen by config.json."""
+         device="cuda", max_batch: int = 64, cache_dtype=None) -> LanguageModel:
+    """Load a model folder (config.json + safetensors); the model class is chosen by config.json.  ``cache_dtype``:
+    "float8_e4m3fn" or "int8" holds keys and values in 8 bits with a scale per token and head (bfloat16 models; half the cache's
+    memory and of what a token reads of it), None in the model's dtype."""
     if not os.path.isdir(model_dir):
         raise FileNotFoundError(f"{model_dir}: no such model folder")
     arch, config = load_config(model_dir)
-    model = build_model(arch, config, dtype)
+    model = build_model(arch, config, dtype, cache_dtype)
     source = FolderSource(model_dir, model.tensor_needs(), parse_dtype(dtype), device)
     try:
         model.load(source)
@@ -119,14 +121,14 @@ def load(model_dir: str, *, dtype="bfloat16", max_tokens: int = 8192, num_slots:
 
 
 def random_model(config: ModelConfig | dict, init: RandomInit = RandomInit(), *, dtype="bfloat16", max_tokens: int = 8192,
-                 num_slots: Optional[int] = None, device="cuda", max_batch: int = 64) -> LanguageModel:
-    """A model of ``config`` with random weights drawn on the device (nothing is written)."""
+                 num_slots: Optional[int] = None, device="cuda", max_batch: int = 64, cache_dtype=None) -> LanguageModel:
+    """A model of ``config`` with random weights drawn on the device (nothing is written); ``cache_dtype`` as for :func:`load`."""
     if isinstance(config, dict):
         arch = architecture_for(config, "config")
         config = arch.config_from_dict(config, "config")
     else:
         arch = architecture_for({"architectures": [config.architecture]}, "config")
-    model = build_model(arch, config, dtype)
+    model = build_model(arch, config, dtype, cache_dtype)
     source = MemorySource(lambda need: init.draw(need, device), init.stored, parse_dtype(dtype), device)
     model.load(source)
     return LanguageModel(model, config, max_tokens=max_tokens, num_slots=num_slots, device=device, max_batch=max_batch)

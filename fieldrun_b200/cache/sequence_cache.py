@@ -10,7 +10,8 @@ of key/value heads, key and value head sizes, all keys, a window of them or chun
 a store, a page pool and a table of its own; a windowed group gives a page back
 as soon as every key on it lies outside the window (pages that hold the first tokens of a line that keeps those stay), a chunked group as soon as the
 sequence has left the chunks that the page holds.  What is cached is K after
-norm and rotary and V as projected (src/minimax.rs:262-268).
+norm and rotary and V as projected (src/minimax.rs:262-268), in the cache's dtype or, where the need says so, as 8-bit
+codes with a scale per token and head (the reference's 8-bit cache has a scale per row, too: src/minimax.rs:291-347).
 
 The state area holds, per cache line that asks for one, a tensor of a fixed
 shape and type per slot, zeroed when the slot is given out.  MiniMax-M2 has no such
@@ -27,6 +28,8 @@ import torch
 from .pools import CacheFull, IndexPool
 
 PAGE_TOKENS = 64
+# types that keys and values can be held in besides the model's: 8-bit codes with a float32 scale per token and head
+CODE_DTYPES = {"float8_e4m3fn": torch.float8_e4m3fn, "int8": torch.int8}
 _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
 
 
@@ -44,13 +47,14 @@ class CacheNeed:
     values_in_keys: bool = False         # a key's value is a part of its key row: the line has no value pages
     value_heads: int = 0                 # value heads, where several key heads share one; 0: one for every key head
     keep_first: int = 0                  # with a window: the sequence's first tokens stay visible beside it
+    codes: str = ""                      # keys and values in 8 bits: a key of CODE_DTYPES; "" holds them in the cache's dtype
 
     @property
     def group_key(self) -> tuple | None:
         if not self.kv_heads:
             return None
         return (self.kv_heads, self.head_dim, self.window, 0 if self.values_in_keys else self.value_dim or self.head_dim, self.chunk,
-                self.value_heads or self.kv_heads, self.keep_first if self.window is not None else 0)
+                self.value_heads or self.kv_heads, self.keep_first if self.window is not None else 0, self.codes)
 
     @property
     def copy_floats(self) -> int:
@@ -94,11 +98,18 @@ class LineView:
     page_table: torch.Tensor | None      # int32 [num_slots, max_pages]; -1 where no page is held
     window: int | None
     state: torch.Tensor | None           # [num_slots, *state_shape] in the need's state_dtype
+    # Only where keys and values are held in 8 bits: ``keys`` and ``values`` are then codes, the values' pages as the keys'
+    # ([num_pages, value heads, PAGE_TOKENS, value_dim]), and every row (a token's of one head) is its codes times its scale here
+    key_scales: torch.Tensor | None = None       # float32 [num_pages, kv_heads, PAGE_TOKENS]
+    value_scales: torch.Tensor | None = None     # float32 [num_pages, value heads, PAGE_TOKENS]
 
 
 class _Group:
     def __init__(self, key, lines, num_pages, num_slots, dtype, device, allocate):
-        self.kv_heads, self.head_dim, self.window, self.value_dim, self.chunk, self.value_heads, keep_first = key
+        self.kv_heads, self.head_dim, self.window, self.value_dim, self.chunk, self.value_heads, keep_first, self.codes = key
+        if self.codes and (self.codes not in CODE_DTYPES or not self.value_dim):
+            raise ValueError(f"keys and values of {self.head_dim} and {self.value_dim} entries in {self.codes!r}; known: {sorted(CODE_DTYPES)}, "
+                             "for lines that hold values beside their keys")
         self.keep_pages = pages_for(keep_first)                      # pages that a sequence keeps to its end
         self.lines = list(lines)
         self.num_pages = num_pages
@@ -110,14 +121,22 @@ class _Group:
         self.dirty: list[tuple[int, int, int]] = []
         self.fresh: list[int] = []           # pages given out since the last sync whose old contents may be read
         shape = (len(self.lines), num_pages, self.kv_heads, PAGE_TOKENS, self.head_dim)
-        if allocate:
+        self.key_scales = self.value_scales = None
+        if allocate and self.codes:
+            # zeros of any of these types are bytes of zero
+            self.keys = torch.zeros(shape, dtype=torch.uint8, device=device).view(CODE_DTYPES[self.codes])
+            self.values = torch.zeros(shape[:2] + (self.value_heads, PAGE_TOKENS, self.value_dim), dtype=torch.uint8,
+                                      device=device).view(CODE_DTYPES[self.codes])
+            self.key_scales = torch.zeros(shape[:4], dtype=torch.float32, device=device)
+            self.value_scales = torch.zeros(shape[:2] + (self.value_heads, PAGE_TOKENS), dtype=torch.float32, device=device)
+        elif allocate:
             self.keys = torch.zeros(shape, dtype=dtype, device=device)
             # within a page the values lie transposed, [head_dim, PAGE_TOKENS]: the product P @ V then reads
             # runs of neighbouring keys
             self.values = torch.zeros(shape[:2] + (self.value_heads, self.value_dim, PAGE_TOKENS), dtype=dtype, device=device)
-            self.table_dev = torch.full((num_slots, num_pages), -1, dtype=torch.int32, device=device)
         else:
-            self.keys = self.values = self.table_dev = None
+            self.keys = self.values = None
+        self.table_dev = torch.full((num_slots, num_pages), -1, dtype=torch.int32, device=device) if allocate else None
 
     def pages_needed(self, slot: int, new_len: int) -> int:
         return max(0, pages_for(new_len) - int(self.end_page[slot]))
@@ -132,8 +151,9 @@ class _Group:
         self.dirty.append((slot, lo, hi))
         # A page that the new tokens do not fill keeps, beyond them, what an earlier sequence left there.  The
         # attention kernels give such keys no weight, but 0 x NaN is NaN: whatever was there must be finite.
-        # So the last page handed out is cleared unless the sequence's tokens fill it to the end.
-        if new_len % PAGE_TOKENS:
+        # So the last page handed out is cleared unless the sequence's tokens fill it to the end.  (The kernels over
+        # 8-bit pages take nothing from the places of keys that a token may not see.)
+        if new_len % PAGE_TOKENS and not self.codes:
             self.fresh.append(int(self.table[slot, hi - 1]))
 
     def release_outside_window(self, slot: int, length: int) -> None:
@@ -300,6 +320,8 @@ class SequenceCache:
             group, index = self._line_group[line]
             keys = group.keys[index] if group.keys is not None else None
             values = group.values[index] if group.values is not None else None
+            if group.codes and keys is not None:
+                return LineView(keys, values, group.table_dev, need.window, state, group.key_scales[index], group.value_scales[index])
             return LineView(keys, values, group.table_dev, need.window, state)
         return LineView(None, None, None, None, state)
 

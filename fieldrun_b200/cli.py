@@ -7,7 +7,7 @@ next-token top-1 over ``--n-eval`` positions (default 500) with a sliding contex
 and ``--dump`` writes the predictions one id per line (src/main.rs:3933-3941,
 4096-4104).  Here ``--model`` names a model folder (``--bundle`` is accepted for
 it), and ``--temperature``, ``--seed``, ``--top-k``, ``--top-p``, ``--eos``, ``--dtype`` and ``--prompts`` are
-what a batch engine with sampling adds; ``--device cpu`` and ``--kv-int8`` are recognised and refused with a reason.  ``random`` writes a model folder with
+what a batch engine with sampling adds, ``--cache-dtype`` the types of a cache in 8 bits; ``--device cpu`` and ``--kv-int8`` are recognised and refused with a reason.  ``random`` writes a model folder with
 random weights, the counterpart of the reference's offline ``convert`` step.
 
     python -m fieldrun_b200 --model DIR --ids ids.json --ctx 64 --generate 32
@@ -88,14 +88,17 @@ def _main(argv: list[str] | None = None) -> int:
     parser.add_argument("--batch", type=int, default=64, help="most sequences in one batch")
     parser.add_argument("--device", default="auto", choices=["auto", "gpu", "cpu"],
                         help="the reference's switch (src/main.rs:4036-4094); this library runs on the GPU only")
-    parser.add_argument("--kv-int8", action="store_true", help="the reference's 8-bit cache; not part of this library")
+    parser.add_argument("--cache-dtype", choices=["float8_e4m3fn", "int8"], help="hold keys and values in 8 bits, with a scale per token "
+                        "and head (bfloat16 models; default: the model's dtype)")
+    parser.add_argument("--kv-int8", action="store_true", help="the reference's 8-bit cache; here: --cache-dtype")
     parser.add_argument("--profile", action="store_true",
                         help="time every kernel with CUDA events (steps run directly, slower) and print the sums as JSON lines")
     args = parser.parse_args(argv)
     if args.device == "cpu":
         raise SystemExit("[fieldrun_b200] --device cpu: this library has no CPU path; it runs on one CUDA device (sm_100a)")
     if args.kv_int8:
-        raise SystemExit("[fieldrun_b200] --kv-int8: quantized caches are not part of this library; the cache holds the model's dtype")
+        raise SystemExit("[fieldrun_b200] --kv-int8: the reference's quantized caches have a scale per row; here they are --cache-dtype int8, a scale "
+                         "per token and head")
 
     import fieldrun_b200 as fr
 
@@ -117,7 +120,8 @@ def _main(argv: list[str] | None = None) -> int:
         need = sum((len(p) + new + 63) // 64 * 64 for p in prompts[:args.batch])
     else:
         need = min(args.batch, args.n_eval) * ((args.ctx + 64) // 64 * 64)
-    lm = fr.load(args.model, dtype=args.dtype, max_tokens=max(args.max_tokens, need, 64), max_batch=args.batch)
+    lm = fr.load(args.model, dtype=args.dtype, max_tokens=max(args.max_tokens, need, 64), max_batch=args.batch,
+                 cache_dtype=args.cache_dtype)
 
     if args.logits_dump:
         # every position's logits of one sequence run whole (src/main.rs:1146-1156 runs each prefix anew)

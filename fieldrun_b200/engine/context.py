@@ -198,6 +198,39 @@ class StepContext:
             kept[key] = total
         return kept[key]
 
+    def pages_in_sight(self, window: Optional[int], chunk: Optional[int], keep_first: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The cache pages that the new tokens may see (those that :meth:`visible_pages` counts), sequence by sequence: the sequence
+        of each (of the step) and its number there, and a table [sequences, pages] of each one's place in that list, -1 elsewhere; int32 on
+        the device.  For steps of prompts only, as :meth:`token_chunks`."""
+        kept = self.__dict__.setdefault("_pages_in_sight", {})
+        key = (window, chunk, keep_first)
+        if key not in kept:
+            pages = [-(-(start + n) // PAGE_TOKENS) for start, n in zip(self.seq_starts, self.seq_q_lens)]
+            table = np.full((self.num_seqs, max(pages)), -1, dtype=np.int32)
+            seqs, numbers, count = [], [], 0
+            for b, (start, n) in enumerate(zip(self.seq_starts, self.seq_q_lens)):
+                if n == 0:
+                    continue
+                low = max(0, start - int(window) + 1) if window else 0
+                if chunk:
+                    low = max(low, start // chunk * chunk)
+                first = low // PAGE_TOKENS
+                own = np.concatenate([np.arange(min(-(-(keep_first if window else 0) // PAGE_TOKENS), first)), np.arange(first, pages[b])])
+                table[b, own] = np.arange(count, count + len(own))
+                seqs.append(np.full(len(own), b))
+                numbers.append(own)
+                count += len(own)
+            flat = torch.from_numpy(np.concatenate([*seqs, *numbers, table.reshape(-1)]).astype(np.int32)).to(self.device)
+            kept[key] = (flat[:count], flat[count:2 * count], flat[2 * count:].view(table.shape))
+        return kept[key]
+
+    @property
+    def seq_rows(self) -> torch.Tensor:
+        """0, 1, ... for the step's sequences, int32 on the device."""
+        if "_seq_rows" not in self.__dict__:
+            self._seq_rows = torch.arange(self.num_seqs, dtype=torch.int32, device=self.device)
+        return self._seq_rows
+
     def query_tiles(self, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Tiles of ``rows`` consecutive new tokens that never span two sequences: (sequence of each tile,
         first row of each tile among its sequence's new tokens), on the device."""

@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from ..cache import CacheNeed, SequenceCache
+from ..cache import CODE_DTYPES, CacheNeed, SequenceCache
 from ..config.plan import ModelPlan
 from ..parts import build_block, build_part
 from ..parts.linear import full_sums, require_true_float32, split_products_reach
@@ -34,8 +34,19 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"dtype {name!r} is neither bfloat16 nor float32") from None
 
 
+def parse_cache_dtype(name) -> str:
+    """What keys and values are held in: "" (the model's dtype; also None) or a key of ``CODE_DTYPES``."""
+    if name is None or name == "":
+        return ""
+    for codes, dtype in CODE_DTYPES.items():
+        if name == dtype or (isinstance(name, str) and name.lower() == codes):
+            return codes
+    raise ValueError(f"a cache of type {name!r}: known are {sorted(CODE_DTYPES)}, or None for the model's dtype")
+
+
 class DecoderModel:
-    def __init__(self, plan: ModelPlan, dtype):
+    def __init__(self, plan: ModelPlan, dtype, cache_dtype=None):
+        """``cache_dtype``: "float8_e4m3fn" or "int8" holds the keys and values of every attention layer in 8 bits."""
         plan.check()
         self.plan = plan
         self.dtype = parse_dtype(dtype)
@@ -55,6 +66,12 @@ class DecoderModel:
                 block.set_mixer_input(build_part("mixer_input", layer.mixer_input, self.dtype))
             if layer.connections is not None:
                 block.set_connections(build_part("stream_connection", layer.connections, self.dtype))
+        self.cache_codes = parse_cache_dtype(cache_dtype)
+        if self.cache_codes:
+            if not any(block.cache_need().kv_heads for block in self.blocks):
+                raise ValueError(f"a cache in {self.cache_codes} was asked for, but no layer keeps keys and values")
+            for block in self.blocks:
+                block.mixer.store_cache_as(self.cache_codes)
         self.additions = [build_part("addition", layer.addition, self.dtype) if layer.addition is not None else None
                           for layer in plan.layers]
         self.connectors = [build_part("connector", spec, self.dtype) for spec in plan.connectors]

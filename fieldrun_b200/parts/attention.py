@@ -35,6 +35,10 @@ A projection's rows are laid out head by head as [map 1, map 2]; the kernels see
 their own (rows are put into the order key head, map, query head of the group at load), two key heads sharing a value head.
 The difference is taken in float32: of the one-token kernels' partial results where those are joined, inside the kernel that
 runs both maps of a prompt's head, of float32 outputs otherwise.
+
+The keys and values may be held in 8 bits (``store_cache_as``): they are written as codes with a scale per token and head, single
+tokens attend over the codes, and for a prompt the pages in sight are read back into bfloat16 pages first, which the same
+kernels then take as those of a bfloat16 cache.  Every query, a prompt's as well, sees what the cache holds.
 """
 from __future__ import annotations
 
@@ -42,7 +46,7 @@ from typing import Optional
 
 import torch
 
-from ..cache import CacheNeed, LineView
+from ..cache import CODE_DTYPES, PAGE_TOKENS, CacheNeed, LineView
 from ..csrc import ops
 from ..weights.loader import MATRIX, VECTOR, TensorNeed, TensorSource
 from .base import BiasedRows, Mixer, build_position, register_part
@@ -140,6 +144,7 @@ class GQAAttention(Mixer):
         self.kv_width = self.k_heads * self.head_dim
         self.v_width = self.num_kv_heads * self.value_dim
         self.out_width = self.num_heads * self.value_dim
+        self.codes = ""                       # type of the cache line's codes, "" for keys and values in the model's dtype
         self.b_qkv: Optional[torch.Tensor] = None
         self.w_qkv: Optional[torch.Tensor] = None
         self.w_o: Optional[torch.Tensor] = None
@@ -220,7 +225,16 @@ class GQAAttention(Mixer):
         return CacheNeed(kv_heads=self.k_heads, head_dim=self.head_dim, keep_first=self.keep_first,
                          value_heads=self.num_kv_heads if self.maps == 2 else 0,
                          window=int(self.window) if self.window is not None else None,
-                         value_dim=self.value_dim if self.value_dim != self.head_dim else 0, chunk=self.chunk)
+                         value_dim=self.value_dim if self.value_dim != self.head_dim else 0, chunk=self.chunk, codes=self.codes)
+
+    def store_cache_as(self, codes: str) -> None:
+        if codes not in CODE_DTYPES:
+            raise ValueError(f"keys and values in {codes!r}: known are {sorted(CODE_DTYPES)}")
+        if not self.tensor_cores:
+            raise ValueError(f"keys and values in 8 bits are for bfloat16 models and the (key, value) head sizes {sorted(ops.MMA_HEAD_SIZES)}: "
+                             f"this layer has {(self.head_dim, self.value_dim)} in {str(self.dtype).replace('torch.', '')}")
+        self.codes = codes
+        self.kernel_groups = ("common", "streams", "attention", "cache8")
 
     def prepare(self, num_positions: int, device) -> None:
         if self.position is not None and self.position.rotary_dim > 0:
@@ -238,16 +252,19 @@ class GQAAttention(Mixer):
         qkv = part_linear(act, self.w_qkv)                                   # float32 [T, q + k + v] (or [T, q + k], [T, q])
         q = ctx.buffer("attention.q", (tokens, self.q_width), self.dtype)
         rotary_dim = self.position.rotary_dim if self.position is not None else 0
-        ops.qkv_prepare(qkv, self.q_norm, self.k_norm, self.qk_norm_eps, self.cos, self.sin, ctx.tok_pos, ctx.tok_slot,
-                        line.page_table, q, line.keys, line.values, num_heads=self.q_heads,
-                        num_kv_heads=0 if self.shares_kv else self.k_heads, num_v_heads=0 if self.shares_kv else self.num_kv_heads,
-                        head_dim=self.head_dim,
-                        rotary_dim=rotary_dim,
-                        interleaved=bool(self.position.interleaved) if self.position is not None else False,
-                        write_cache=writes_cache, per_head=self.qk_norm == "per_head",
-                        tables_final=True,      # the step's tables were there before the projection above began
-                        bias=self.b_qkv, v_dim=self.value_dim, q_temp=self.q_temp,
-                        values_from_keys=self.values_from_keys and not self.shares_kv)
+        prepare = dict(num_heads=self.q_heads, num_kv_heads=0 if self.shares_kv else self.k_heads,
+                       num_v_heads=0 if self.shares_kv else self.num_kv_heads, head_dim=self.head_dim, rotary_dim=rotary_dim,
+                       interleaved=bool(self.position.interleaved) if self.position is not None else False,
+                       per_head=self.qk_norm == "per_head",
+                       tables_final=True,       # the step's tables were there before the projection above began
+                       bias=self.b_qkv, v_dim=self.value_dim, q_temp=self.q_temp,
+                       values_from_keys=self.values_from_keys and not self.shares_kv)
+        tables = (qkv, self.q_norm, self.k_norm, self.qk_norm_eps, self.cos, self.sin, ctx.tok_pos, ctx.tok_slot, line.page_table, q)
+        if self.codes and writes_cache:
+            ops.qkv_prepare_8bit(*tables, line.keys, line.key_scales, line.values, line.value_scales, **prepare)
+        else:
+            pages = (None, None) if self.codes else (line.keys, line.values)
+            ops.qkv_prepare(*tables, *pages, write_cache=writes_cache, **prepare)
         out = ctx.buffer("attention.out", (tokens, self.out_width), self.dtype)
         gate = part_linear(act, self.w_gate) if self.has_head_gate else None     # float32 [T, heads], before the sigmoid
         self.attend(ctx, q, line, out, gate)
@@ -266,6 +283,25 @@ class GQAAttention(Mixer):
                       softcap=self.softcap, keep_first=self.keep_first, maps=self.maps)
         difference = dict(lam=self.lam, eps=self.diff_eps, factor=1.0 - self.diff)
         both = self.softcap is not None and self.slopes is not None     # the tcgen05 kernel has either, not both
+        if self.codes and ctx.is_decode:
+            chunks = (ctx.max_kv_len + ops.ATTENTION_CHUNK - 1) // ops.ATTENTION_CHUNK
+            part_o = ctx.buffer("attention.part_o", (ctx.num_seqs, self.q_heads, chunks, self.value_dim), torch.float32)
+            part_ml = ctx.buffer("attention.part_ml", (ctx.num_seqs, self.q_heads, chunks, 2), torch.float32)
+            ops.attention_decode_8bit(q, line.keys, line.key_scales, line.values, line.value_scales, line.page_table, ctx.seq_start,
+                                      ctx.seq_slot, part_o, part_ml, out, max_chunks=chunks,
+                                      difference=difference if self.maps == 2 else None, **common)
+            if gate is not None:
+                ops.head_gate(out, gate, self.num_heads, self.value_dim)
+            return
+        keys, values, table, seq_slot, tok_slot = line.keys, line.values, line.page_table, ctx.seq_slot, ctx.tok_slot
+        if self.codes:
+            # the pages in sight as bfloat16 pages of the step's own: sequence b of the step is row b of their table
+            page_seq, page_index, table = ctx.pages_in_sight(self.window, self.chunk, self.keep_first)
+            keys = ctx.buffer("attention.keys", (page_seq.numel(), self.k_heads, PAGE_TOKENS, self.head_dim), torch.bfloat16)
+            values = ctx.buffer("attention.values", (page_seq.numel(), self.num_kv_heads, self.value_dim, PAGE_TOKENS), torch.bfloat16)
+            ops.cache_read_8bit(line.keys, line.key_scales, line.values, line.value_scales, line.page_table, page_seq, page_index,
+                                ctx.seq_slot, ctx.seq_start, ctx.seq_q_len, keys, values)
+            seq_slot, tok_slot = ctx.seq_rows, ctx.tok_seq
         maps_out = out if self.maps == 1 else ctx.buffer("attention.maps", (out.shape[0], self.maps * self.out_width), torch.float32)
         if self.tensor_cores and not both:
             if ctx.is_decode and self.num_heads // self.num_kv_heads <= 16:
@@ -274,7 +310,7 @@ class GQAAttention(Mixer):
                 part_ml = ctx.buffer("attention.part_ml", (ctx.num_seqs, self.q_heads, chunks, 2), torch.float32)
                 # head sizes 64 and 128: the pages come into shared memory by TMA; others: loads into registers
                 decode = ops.attention_decode_tma if self.head_dim in ops.TC_ATTENTION_HEAD_DIMS else ops.attention_decode_mma
-                decode(q, line.keys, line.values, line.page_table, ctx.seq_start, ctx.seq_slot, part_o, part_ml, out,
+                decode(q, keys, values, table, ctx.seq_start, seq_slot, part_o, part_ml, out,
                        max_chunks=chunks, difference=difference if self.maps == 2 else None, **common)
                 maps_out = out
             elif self.head_dim in ops.TC_ATTENTION_HEAD_DIMS and ctx.max_q_len >= TC_ATTENTION_MIN_QUERIES:
@@ -282,16 +318,16 @@ class GQAAttention(Mixer):
                 tile_seq, tile_q0 = ctx.query_tiles(ops.TC_ATTENTION_QUERIES)
                 if self.maps == 2 and self.chunk is None and ops.attention_pair_takes(self.head_dim, self.value_dim):
                     # both maps, their difference and its norm in one kernel
-                    ops.attention_pair_tc(q, line.keys, line.values, line.page_table, tile_seq, tile_q0, ctx.seq_slot, ctx.seq_start,
+                    ops.attention_pair_tc(q, keys, values, table, tile_seq, tile_q0, seq_slot, ctx.seq_start,
                                           ctx.seq_q_len, ctx.cu_q_len, out, heads=self.num_heads, v_heads=self.num_kv_heads,
                                           head_dim=self.head_dim, v_dim=self.value_dim, scale=self.softmax_scale, window=self.window,
                                           keep_first=self.keep_first, softcap=self.softcap, **difference)
                     return
-                ops.attention_prefill_tc(q, line.keys, line.values, line.page_table, tile_seq, tile_q0, ctx.seq_slot,
+                ops.attention_prefill_tc(q, keys, values, table, tile_seq, tile_q0, seq_slot,
                                          ctx.seq_start, ctx.seq_q_len, ctx.cu_q_len, maps_out, **common)
             else:
                 tile_seq, tile_q0 = ctx.query_tiles(16)
-                ops.attention_prefill_mma(q, line.keys, line.values, line.page_table, tile_seq, tile_q0, ctx.seq_slot,
+                ops.attention_prefill_mma(q, keys, values, table, tile_seq, tile_q0, seq_slot,
                                           ctx.seq_start, ctx.seq_q_len, ctx.cu_q_len, maps_out, **common)
             if gate is not None:
                 ops.head_gate(out, gate, self.num_heads, self.value_dim)
@@ -301,7 +337,7 @@ class GQAAttention(Mixer):
             chunks = (ctx.max_kv_len + ops.ATTENTION_CHUNK - 1) // ops.ATTENTION_CHUNK
             part_o = ctx.buffer("attention.part_o", (ctx.num_seqs, self.q_heads, chunks, self.value_dim), torch.float32)
             part_ml = ctx.buffer("attention.part_ml", (ctx.num_seqs, self.q_heads, chunks, 2), torch.float32)
-            ops.attention_f32_token(q, line.keys, line.values, line.page_table, ctx.tok_pos, ctx.tok_slot, part_o, part_ml, maps_out,
+            ops.attention_f32_token(q, keys, values, table, ctx.tok_pos, tok_slot, part_o, part_ml, maps_out,
                                     max_chunks=chunks, gate=gate, **common)
         elif (self.float32_tiles and not ctx.is_decode
               and ops.attention_f32_tiles_take(self.head_dim, self.value_dim, ctx.query_tiles(ops.TC_ATTENTION_QUERIES)[0].numel())):
@@ -311,14 +347,14 @@ class GQAAttention(Mixer):
                 pages = ctx.visible_pages(self.window, self.chunk, self.keep_first)
                 floats = ops.attention_f32_tc_scratch(pages, self.k_heads, self.head_dim, self.value_dim, self.maps)
             if 0 < floats <= F32_TC_SCRATCH:
-                ops.attention_f32_tc(q, line.keys, line.values, line.page_table, tile_seq, tile_q0, ctx.seq_slot, ctx.seq_start,
+                ops.attention_f32_tc(q, keys, values, table, tile_seq, tile_q0, seq_slot, ctx.seq_start,
                                      ctx.seq_q_len, ctx.cu_q_len, ctx.buffer("attention.parts", (floats,), torch.float32), pages, maps_out,
                                      gate=gate, **common)
             else:
-                ops.attention_f32_tiles(q, line.keys, line.values, line.page_table, tile_seq, tile_q0, ctx.seq_slot, ctx.seq_start,
+                ops.attention_f32_tiles(q, keys, values, table, tile_seq, tile_q0, seq_slot, ctx.seq_start,
                                         ctx.seq_q_len, ctx.cu_q_len, maps_out, gate=gate, **common)
         else:
-            ops.attention_generic(q, line.keys, line.values, line.page_table, ctx.tok_pos, ctx.tok_slot, maps_out, gate=gate, **common)
+            ops.attention_generic(q, keys, values, table, ctx.tok_pos, tok_slot, maps_out, gate=gate, **common)
         if maps_out is not out:
             ops.map_difference(maps_out, out, heads=self.num_heads, kv_heads=self.num_kv_heads, v_dim=self.value_dim, **difference)
 

@@ -14,6 +14,8 @@ Interfaces
 ``Mixer.forward(ctx, act, line, writes_cache)`` -> float32 update [T, width]
     ``line`` is the :class:`~fieldrun_b200.cache.LineView` of the run's cache line.
 ``Mixer.cache_need()`` -> :class:`~fieldrun_b200.cache.CacheNeed`
+``Mixer.store_cache_as(codes)``
+    keys and values in 8 bits from now on (a key of ``CODE_DTYPES``), or a ValueError from a mixer that has no kernels for it.
 ``FeedForward.forward(ctx, act, act32)`` -> float32 update [T, width]
 ``Position.tables(num_positions, device)`` -> (cos, sin) float32 [positions, dim/2]
 ``Block.forward(ctx, x, pending, line, writes_cache)`` -> (x, pending)
@@ -278,6 +280,13 @@ class Position:
 class Mixer(Part):
     def cache_need(self) -> CacheNeed:
         return CacheNeed()
+
+    def store_cache_as(self, codes: str) -> None:
+        """Hold the keys and values of the part's cache line in 8 bits, ``codes`` a key of ``CODE_DTYPES``; called before the
+        model's cache is made.  A mixer that keeps no keys and values has nothing to do; one that keeps some, and has no kernels
+        for 8-bit pages, refuses."""
+        if self.cache_need().kv_heads:
+            raise ValueError(f"mixer {self.spec.kind!r} holds its keys and values in the model's dtype only, not in {codes}")
 
     def prepare(self, num_positions: int, device) -> None:
         """Called once the cache's size is known (tables over positions are made here)."""

@@ -79,3 +79,31 @@ def difference(out, lam, heads, kv_heads, eps, factor):
     o = out.reshape(kv_heads, 2, heads // kv_heads, -1)
     o = (o[:, 0] - lam * o[:, 1]).reshape(heads, -1)
     return o / np.sqrt((o * o).mean(-1, keepdims=True) + eps) * factor
+
+
+def output_bound(want, size, top, reach, position, *, dim, group, maps=1, softcap=None, slopes=None, lam=None, eps=None, factor=None,
+                 rounding=2.0 ** -11):
+    """What one token's output (bfloat16) may be off by, and the value itself with two maps' difference taken; ``rounding``: of a weight.
+
+    Scores: exact products (float16 of 11 bits and codes of 8, or bfloat16) added in float32, up to 2^-23 of the terms' size a step, and a few
+    roundings of the score itself, of a slope's product and of a cap; twice that is the relative error of a weight over the sum.
+    Weights: their rounding, the hardware's exponential, sums of position + 1 terms in float32; a weight below 2^-22 of the largest has an
+    absolute error instead.  Then the output's own rounding."""
+    score = 2.0 ** -23 * (dim + 16) * reach + (2.0 ** -20 * softcap if softcap else 0.0)
+    if slopes is not None:
+        score = score + 2.0 ** -22 * slopes * position
+    weight = rounding + 2.0 ** -16 + (position + 1) * 2.0 ** -26 + 4 * score[:, None]
+    bound = weight * size + (position + 1) * 2.0 ** -31 * top[:, None]
+    if maps == 2:
+        heads = want.shape[0] // 2
+        kv_heads = heads // group
+        raw = want.reshape(kv_heads, 2, group, -1)
+        raw = (raw[:, 0] - lam * raw[:, 1]).reshape(heads, -1)
+        b = bound.reshape(kv_heads, 2, group, -1)
+        b = (b[:, 0] + abs(lam) * b[:, 1]).reshape(heads, -1)
+        want = difference(want, lam, heads, kv_heads, eps, factor)
+        # the norm's factor is off by at most the largest relative error of the row
+        rms = np.sqrt((raw * raw).mean(-1, keepdims=True) + eps)
+        shift = np.sqrt((b * b).mean(-1, keepdims=True)) / rms
+        bound = factor * b / rms * (1 + 2 * shift) + 2 * shift * np.abs(want) + 2.0 ** -18 * np.abs(want)
+    return want, bound + 2.0 ** -8 * (np.abs(want) + bound) + 1e-37

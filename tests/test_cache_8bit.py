@@ -1,8 +1,15 @@
 """A cache in 8 bits on the host: what its calls refuse, its pages and tables."""
+import importlib
+
+import numpy as np
 import pytest
 import torch
 
+import fieldrun_b200 as fr
+from fieldrun_b200.cache import CacheNeed, SequenceCache
+from fieldrun_b200.config.registry import architecture_for
 from fieldrun_b200.csrc import ops
+from fieldrun_b200.engine.context import StepContext
 
 PAGE = 64
 E4M3, INT8 = torch.float8_e4m3fn, torch.int8
@@ -111,3 +118,90 @@ def test_entry_points_refuse_sizes_by_a_message():
     assert lib.frb_qkv_prepare_8bit(None, 0, None, None, 0, 1e-6, None, None, 0, None, None, None, 1, 1, *[None] * 5, 0, 1, 1, 900, 2, 2, 64, 64, 0, 0, 0, 0,
                                     None, 0.0, 1, 0, None) == -1
     assert b"more than 200 KB" in lib.frb_last_error()
+
+
+# ------------------------------------------------------------------------------------------------ pages and tables
+
+@pytest.mark.parametrize("codes,dtype", [("int8", INT8), ("float8_e4m3fn", E4M3)])
+def test_lines_in_8_bits_have_a_group_of_their_own(codes, dtype):
+    needs = [CacheNeed(2, 64), CacheNeed(2, 64, codes=codes), CacheNeed(4, 32, value_dim=64, value_heads=2, window=70, codes=codes), CacheNeed(2, 64, codes=codes)]
+    cache = SequenceCache(needs, max_tokens=640, num_slots=3, device="cpu")
+    assert [g.lines for g in cache.groups] == [[0], [1, 3], [2]]
+    plain, line, other = cache.line(0), cache.line(3), cache.line(2)
+    assert plain.key_scales is None and plain.keys.dtype == torch.bfloat16 and tuple(plain.values.shape) == (10, 2, 64, 64)
+    assert line.keys.dtype == dtype and tuple(line.values.shape) == (10, 2, 64, 64) and tuple(line.key_scales.shape) == (10, 2, 64)
+    assert tuple(other.keys.shape) == (10, 4, 64, 32) and tuple(other.values.shape) == (10, 2, 64, 64) and tuple(other.value_scales.shape) == (10, 2, 64)
+    assert other.window == 70 and all(t.is_contiguous() for t in (line.keys, line.values, line.key_scales, other.values))
+    s = cache.alloc()
+    cache.begin_step([s], [100])
+    assert cache.groups[0].table_dev[s, 1] >= 0 and torch.equal(cache.groups[1].table_dev, torch.from_numpy(cache.groups[1].table))
+    cache.end_step([s], [100])
+    for _ in range(100):
+        cache.begin_step([s], [1])
+        cache.end_step([s], [1])
+    assert cache.groups[2].pool.num_held == 2
+    cache.check()
+    cache.free(s)
+    cache.check()
+
+
+def test_lines_in_8_bits_are_refused_where_they_make_no_sense():
+    with pytest.raises(ValueError, match="'int4'"):
+        SequenceCache([CacheNeed(2, 64, codes="int4")], max_tokens=64, device="cpu")
+    with pytest.raises(ValueError, match="hold values beside their keys"):
+        SequenceCache([CacheNeed(1, 48, value_dim=40, values_in_keys=True, codes="int8")], max_tokens=64, device="cpu")
+    writer, reader = CacheNeed(2, 64, window=50, codes="int8"), CacheNeed(2, 64, codes="int8")
+    assert writer.shared_with(reader) == reader
+    with pytest.raises(ValueError, match="cannot read"):
+        writer.shared_with(CacheNeed(2, 64))
+
+
+@pytest.mark.parametrize("window,chunk,keep_first", [(None, None, 0), (64, None, 0), (1, None, 0), (100, None, 130), (None, 100, 0), (70, 170, 0), (5000, None, 3)])
+def test_pages_in_sight(window, chunk, keep_first):
+    starts, new = [0, 700, 63, 64, 1000, 129], [1, 5, 1, 200, 0, 64]
+    ctx = StepContext.__new__(StepContext)
+    ctx.seq_starts, ctx.seq_q_lens, ctx.num_seqs, ctx.device = starts, new, len(starts), torch.device("cpu")
+    seqs, numbers, table = ctx.pages_in_sight(window, chunk, keep_first)
+    assert seqs.numel() == ctx.visible_pages(window, chunk, keep_first) and table.is_contiguous() and table.dtype == torch.int32
+    want = set()
+    for b, (start, n) in enumerate(zip(starts, new)):
+        for pos in range(start, start + n):
+            for key in range(pos + 1):
+                lo = max(0, pos - window + 1) if window else 0
+                lo = max(lo, pos // chunk * chunk) if chunk else lo
+                if key >= lo or (window and key < keep_first):
+                    want.add((b, key // PAGE))
+    got = list(zip(seqs.tolist(), numbers.tolist()))
+    assert set(got) == want and len(got) == len(want)
+    for b in range(len(starts)):
+        for page in range(table.shape[1]):
+            assert int(table[b, page]) == (got.index((b, page)) if (b, page) in want else -1)
+    assert ctx.pages_in_sight(window, chunk, keep_first)[2] is table
+
+
+def build(design, name, dtype, cache_dtype):
+    config = importlib.import_module(f"{design}_configs").ALL[name][0]
+    arch = architecture_for(config, "config")
+    return fr.build_model(arch, arch.config_from_dict(config, "config"), dtype, cache_dtype)
+
+
+@pytest.mark.parametrize("design,name", [("tiny", "b"), ("tiny", "d"), ("bamasun", "C"), ("fotanex", "C"), ("bakasun", "C"), ("duzinex", "C"), ("kifunex", "C")])
+def test_models_with_a_cache_in_8_bits(design, name):
+    for given, codes in (("int8", "int8"), (torch.float8_e4m3fn, "float8_e4m3fn"), (None, ""), ("", "")):
+        model = build(design, name, "bfloat16", given)
+        needs = model.cache_needs()
+        assert any(n.kv_heads for n in needs) and all(n.codes == (codes if n.kv_heads else "") for n in needs)
+        assert ("cache8" in model.kernel_groups()) == bool(codes)
+        assert model.replayable
+
+
+def test_models_that_cannot_hold_their_cache_in_8_bits_say_so():
+    with pytest.raises(ValueError, match="for bfloat16 models"):
+        build("tiny", "d", "float32", "int8")
+    with pytest.raises(ValueError, match=r"\(16, 16\)"):
+        build("tiny", "a", "bfloat16", "int8")
+    with pytest.raises(ValueError, match="latent_attention.*model's dtype only"):
+        build("depelix", "C", "bfloat16", "float8_e4m3fn")
+    for name in ("int4", "bfloat16", torch.uint8, 8):
+        with pytest.raises(ValueError, match="a cache of type"):
+            build("tiny", "d", "bfloat16", name)

@@ -316,29 +316,10 @@ class Attended:
             want, size, top, reach = plain.attend(q, self.rows_of(i, self.k, self.ks), self.rows_of(i, self.v, self.vs), position,
                                                   scale=o["scale"], group=self.heads // self.kv_heads, maps=self.maps, window=o["window"],
                                                   chunk=o.get("chunk"), keep_first=o.get("keep_first", 0), softcap=o.get("softcap"), **arrays)
-            # Scores: exact products (float16 of 11 bits, codes of 8) added in float32, up to 2^-23 of the terms' size a step, and a few
-            # roundings of the score itself, of a slope's product and of a cap; twice that is the relative error of a weight over the sum.
-            score = 2.0 ** -23 * (self.dim + 16) * reach + (2.0 ** -20 * o["softcap"] if o.get("softcap") else 0.0)
-            if arrays["slopes"] is not None:
-                score = score + 2.0 ** -22 * arrays["slopes"] * position
-            # Weights: rounded to float16 (2^-11), the hardware's exponential, sums of position + 1 terms in float32; a weight below 2^-22 of the
-            # largest has an absolute error instead.  Then the output's own rounding.
-            weight = 2.0 ** -11 + 2.0 ** -16 + (position + 1) * 2.0 ** -26 + 4 * score[:, None]
-            bound = weight * size + (position + 1) * 2.0 ** -31 * top[:, None]
-            if self.maps == 2:
-                d = o["difference"]
-                group = self.heads // self.kv_heads
-                lam = float(d["lam"].double())
-                b = bound.reshape(self.v_heads, 2, group, -1)
-                raw = want.reshape(self.v_heads, 2, group, -1)
-                raw = (raw[:, 0] - lam * raw[:, 1]).reshape(self.heads // 2, -1)
-                b = (b[:, 0] + lam * b[:, 1]).reshape(self.heads // 2, -1)
-                want = plain.difference(want, lam, self.heads // 2, self.v_heads, d["eps"], d["factor"])
-                # the norm's factor is off by at most the largest relative error of the row
-                rms = np.sqrt((raw * raw).mean(-1, keepdims=True) + d["eps"])
-                shift = np.sqrt((b * b).mean(-1, keepdims=True)) / rms
-                bound = d["factor"] * b / rms * (1 + 2 * shift) + 2 * shift * np.abs(want) + 2.0 ** -18 * np.abs(want)
-            bound = bound + 2.0 ** -8 * (np.abs(want) + bound) + 1e-37
+            d = o.get("difference")
+            more = dict(lam=float(d["lam"].double()), eps=d["eps"], factor=d["factor"]) if d else {}
+            want, bound = plain.output_bound(want, size, top, reach, position, dim=self.dim, group=self.heads // self.kv_heads, maps=self.maps,
+                                             softcap=o.get("softcap"), slopes=arrays["slopes"], **more)
             off = np.abs(got[i] - want)
             assert np.isfinite(got[i]).all() and (off <= bound).all(), (i, position, float((off / bound).max()))
         return self
