@@ -11,26 +11,31 @@
 // both types; the queries are brought to float16 by a power of two per head (exact down to 2^-29 of a head's largest entry); a
 // key's scale multiplies its scores, a value's scale its weight.
 //
-// A block takes a run of pages of one key head of one sequence, its warps the pages in turn.  A warp asks for its own pages by TMA
-// (keys, then values, each announced on an mbarrier of the warp's own), the next page's keys as soon as the present page's scores are
-// done and its values as soon as they are multiplied, so that a warp waits for nothing but its own copies; the page's number
-// comes a page ahead.  The warps' results are combined through shared memory and written as one partial result; a second kernel
-// joins the partial results in order.
-//
 // Weights: p_j = 2^(s_j - m) with m a running maximum that follows a page's only beyond a margin.  The weight that multiplies codes is
 // w_j = p_j vs_j, rounded to float16 after division by a unit U per head, a power of two that follows the largest w seen: w / U is at most
 // 2^15, and full precision (2^-11) reaches down to 2^-22 of the largest.  The sum of the p_j stays in float32.
 //
-// Which key a row of the score tile stands for, and which dimension a row of the output tile, is free; both are chosen so that the
-// lanes of a quarter warp read shared memory from different banks under the copies' swizzle (key_of_row, below).
+// A page of 64 keys is one warp's work: its keys and values come by TMA into tiles of the warp's own, each announced on an mbarrier of
+// the warp's own.  Which key a row of the score tile stands for, and which dimension a row of the output tile, is free; both are
+// chosen so that the lanes of a quarter warp read shared memory from different banks under the copies' swizzle (key_of_row).
 //
-// Every wait on an mbarrier gives up after about a second and sets `status`; the block then waits (with the same limit) for the copies
-// that are in flight and returns.
+// Two kernels cut the work differently (the entry point chooses), a third joins the partial results in order:
+// chunks: a block takes four pages of a key head, a page a warp, and combines the four through shared memory.  Where there are few pages
+//   nothing is faster: every page is read at once.
+// pieces: all pages that the step's tokens see, sequence by sequence and key head by key head, are one line that is cut into pieces of one
+//   length, a warp's each, about as many as warps are resident.  A warp runs through its piece without waiting for any other: the
+//   next page's keys are asked for as soon as the present page's scores are done and its values as soon as they are multiplied, also from
+//   one key head or sequence to the next, where the warp leaves a partial result.  Sequences of unequal lengths need no more time than
+//   their pages, and there is no last wave of a few blocks.
+//
+// Every wait on an mbarrier gives up after about a second and sets `status`; the warps then wait (with the same limit) for the copies
+// that are in flight and return.
 #include "cache_8bit.cuh"
 #include "tma.cuh"
 
 #define D8_WARPS 4
 #define D8_THREADS (32 * D8_WARPS)
+#define D8_RESIDENT(NT) ((NT) == 1 ? 3 : 2)     // blocks that an SM holds
 #define D8_CHUNK_PAGES 4               // a chunk is 256 keys
 #define D8_RAISE 8.0f                  // the running maximum follows a page's maximum only beyond this margin (in units of log2)
 #define D8_STATUS_WAIT 7               // a wait gave up
@@ -46,22 +51,44 @@ struct Decode8Params {
     const int* page_table;     // [slots, max_pages]
     const int* seq_pos;        // [B] position of the sequence's token; negative: the sequence has none, its output is zero
     const int* seq_slot;       // [B]
-    float* part_o;             // [B, nh, parts, VD]
-    float* part_ml;            // [B, nh, parts, 2]
+    float* part_o;             // [B, nh, max_chunks, VD]
+    float* part_ml;            // [B, nh, max_chunks, 2]
     bf16* out;                 // [B, nh * VD], or with two maps per head [B, nh / 2 * VD]
-    const float* slopes;       // as in DecodeAttnParams, like all below
-    const float* sinks;
-    const float* lam;
+    const float* slopes;       // null, or one slope per query head: key j's score is lowered by slope * (position - j)
+    const float* sinks;        // null, or one number per query head whose exponential joins the softmax's denominator
+    const float* lam;          // not null: two maps per head; query heads lie as [value head, map, query head of the group]
     int* status;
     float scale, softcap, diff_eps, diff_factor;
-    int window, chunk, keep_first, max_pages, num_slots, num_pages, num_heads, num_kv_heads, v_heads;
-    int parts, pages_per_block, head_tiles, early;
+    int window, chunk, keep_first, max_pages, num_slots, num_pages, num_heads, num_kv_heads, v_heads, num_seqs;
+    int max_chunks;            // partial results that there is room for per (sequence, head); a sequence has at most four times as many pages
+    int head_tiles;            // tiles of query heads per key head
+    int pieces;                // warps that the line of pages is cut for; 0: chunks
+    int early;                 // copies go out before the kernel before this one has ended (0: FIELDRUN_B200_ATTENTION_EARLY=0)
 };
 
 // The position that the kernels work with: none (-1) for a slot that does not exist.
 __device__ __forceinline__ int held_position(const Decode8Params& p, int b) {
     const int slot = p.seq_slot[b];
     return slot >= 0 && slot < p.num_slots ? min(p.seq_pos[b], p.max_pages * FRB_PAGE - 1) : -1;
+}
+
+// The pages that hold a key which a sequence's token may see: those of the first tokens that stay visible, then the window's.
+struct Sight {
+    int lo_key, hi_key, kept, first_page, count;
+    bool cut;                                           // there are more, which the launch has no room for
+    __device__ __forceinline__ int number(int n) const { return n < kept ? n : first_page + n - kept; }     // the n-th one's place in the sequence
+};
+
+__device__ __forceinline__ Sight sight_of(const Decode8Params& p, int b) {
+    Sight s;
+    s.hi_key = held_position(p, b);
+    s.lo_key = first_visible_key(max(s.hi_key, 0), p.window, p.chunk);
+    s.first_page = s.lo_key / FRB_PAGE;
+    s.kept = kept_runs(p.keep_first, FRB_PAGE, s.first_page);
+    const int pages = s.hi_key < 0 ? 0 : s.kept + s.hi_key / FRB_PAGE + 1 - s.first_page;
+    s.cut = pages > D8_CHUNK_PAGES * p.max_chunks;
+    s.count = s.cut ? D8_CHUNK_PAGES * p.max_chunks : pages;
+    return s;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -156,145 +183,136 @@ __device__ __forceinline__ void load_row_of_scales(void* dst, const float* src, 
                  ::"r"(smem_addr(dst)), "l"(src), "r"(4 * FRB_PAGE), "r"(smem_addr(bar)) : "memory");
 }
 
-// HD, VD: entries of a key and of a value head.  NT: query heads of a key head in tiles of eight (1 or 2); a block takes NT tiles.
-template <int HD, int VD, int NT, int CODES>
-__global__ void __launch_bounds__(D8_THREADS, NT == 1 ? 3 : 2)
-attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Params p) {
-    // as attention_decode_tma: the copies of every page but the sequence's last go out before the kernel before this one has ended
-    let_next_kernel_start();
-    constexpr int K_TILE = FRB_PAGE * HD, V_TILE = FRB_PAGE * VD, SCALES = 4 * FRB_PAGE;
-    constexpr int KU = HD % 64 == 0 ? 16 : 8, K_STEPS = HD / (4 * KU), K_WORDS = KU / 4;     // a lane's bytes of a key at a time
-    constexpr int VB = VD / 8, MT = VD / 16;                                                // a lane's bytes of a value; output tiles
-    constexpr int O_STRIDE = VD + 4;
-    static_assert(NT * 8 * O_STRIDE * 4 <= K_TILE + V_TILE, "a warp's partial result fits into its pages");
-    extern __shared__ uint8_t dynamic[];
-    __shared__ uint64_t full_k[D8_WARPS], full_v[D8_WARPS];
-    __shared__ float sm_m[D8_WARPS][8 * NT], sm_l[D8_WARPS][8 * NT];
-    __shared__ int failed;
-    uint8_t* tiles = reinterpret_cast<uint8_t*>(((uintptr_t)dynamic + 1023) & ~(uintptr_t)1023);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    uint8_t* k_tile = tiles + (size_t)warp * (K_TILE + V_TILE);
-    uint8_t* v_tile = k_tile + K_TILE;
-    float* k_scale = reinterpret_cast<float*>(tiles + (size_t)D8_WARPS * (K_TILE + V_TILE) + (size_t)warp * 2 * SCALES);
-    float* v_scale = k_scale + FRB_PAGE;
+// What a warp has in shared memory: a page's keys and values with their scales, and the mbarriers that announce them.
+template <int HD, int VD>
+struct WarpTiles {
+    static constexpr int K_TILE = FRB_PAGE * HD, V_TILE = FRB_PAGE * VD, SCALES = 4 * FRB_PAGE;
+    static constexpr int BYTES = D8_WARPS * (K_TILE + V_TILE + 2 * SCALES);
+    uint8_t* keys;
+    uint8_t* values;
+    float* key_scales;
+    float* value_scales;
+    uint64_t* keys_full;
+    uint64_t* values_full;
+    uint32_t keys_parity, values_parity;
+    bool keys_out, values_out;          // a copy is in flight
 
-    const int part = blockIdx.x, kvh = blockIdx.y / p.head_tiles, tile = blockIdx.y - kvh * p.head_tiles, b = blockIdx.z;
-    const int group = p.num_heads / p.num_kv_heads;
-    const int first_head = kvh * group + tile * 8 * NT, heads = min(8 * NT, group - tile * 8 * NT);
-    const int hi_key = held_position(p, b), lo_key = first_visible_key(max(hi_key, 0), p.window, p.chunk);
-    // the pages of this block that hold a key the token may see: those of the first tokens that stay visible, then the window's
-    const int begin_page = part * p.pages_per_block, end_page = min((part + 1) * p.pages_per_block, hi_key < 0 ? 0 : hi_key / FRB_PAGE + 1);
-    const int first_page = max(begin_page, lo_key / FRB_PAGE);
-    const int kept = max(0, min(end_page, kept_runs(p.keep_first, FRB_PAGE, lo_key / FRB_PAGE)) - begin_page);
-    const int num_pages = kept + max(0, end_page - first_page);
-    if (num_pages <= 0) return;                   // the join skips these blocks
-    const auto number_of = [&](int n) { return n < kept ? begin_page + n : first_page + n - kept; };
-    const int* table = p.page_table + (size_t)p.seq_slot[b] * p.max_pages;
-    // the store's page of the run's page n; -1 behind the run's end and for one that the table does not have
-    const auto page_of = [&](int n) {
-        if (n >= num_pages) return -1;
-        const int page = table[number_of(n)];
-        return page < p.num_pages ? page : -1;
-    };
-    const int vh = kvh / (p.num_kv_heads / p.v_heads);
-
-    if (threadIdx.x == 0) {
-        for (int w = 0; w < D8_WARPS; ++w) { bar_init(&full_k[w], 1); bar_init(&full_v[w], 1); }
-        failed = 0;
-        bar_init_fence();
+    __device__ __forceinline__ WarpTiles(uint8_t* base, uint64_t* bars, int warp) {
+        keys = base + (size_t)warp * (K_TILE + V_TILE);
+        values = keys + K_TILE;
+        key_scales = reinterpret_cast<float*>(base + (size_t)D8_WARPS * (K_TILE + V_TILE) + (size_t)warp * 2 * SCALES);
+        value_scales = key_scales + FRB_PAGE;
+        keys_full = bars + 2 * warp;
+        values_full = bars + 2 * warp + 1;
+        keys_parity = values_parity = 0;
+        keys_out = values_out = false;
     }
-    __syncthreads();
-
-    const auto ask_keys = [&](int page) {
-        bar_expect(&full_k[warp], K_TILE + SCALES);
-        load_2d(k_tile, &map_k, 0, (page * p.num_kv_heads + kvh) * FRB_PAGE, &full_k[warp]);
-        load_row_of_scales(k_scale, p.k_scales + ((size_t)page * p.num_kv_heads + kvh) * FRB_PAGE, &full_k[warp]);
-    };
-    const auto ask_values = [&](int page) {
-        bar_expect(&full_v[warp], V_TILE + SCALES);
-        load_2d(v_tile, &map_v, 0, (page * p.v_heads + vh) * FRB_PAGE, &full_v[warp]);
-        load_row_of_scales(v_scale, p.v_scales + ((size_t)page * p.v_heads + vh) * FRB_PAGE, &full_v[warp]);
-    };
-
-    // Copies in flight at any time: the keys and the values of page `page`.  The run's page n is this warp's for n = warp, warp +
-    // D8_WARPS, ...; pages that the table does not have are passed over.
-    int n = warp, page = -1;
-    const auto next_page = [&](int from) {                  // the warp's first page from the run's page `from` on
-        n = from;
-        for (page = -1; n < num_pages && page < 0; n += page < 0 ? D8_WARPS : 0) page = page_of(n);
-    };
-    const int newest = kept + hi_key / FRB_PAGE - first_page;       // the page that the kernel before this one writes to
-    bool waited = !p.early;
-    if (waited) wait_for_previous_kernel();
-    next_page(warp);
-    if (page >= 0 && (waited || n != newest) && lane == 0) { ask_keys(page); ask_values(page); }
-    if (!waited) {
-        wait_for_previous_kernel();
-        if (page >= 0 && n == newest && lane == 0) { ask_keys(page); ask_values(page); }
-    }
-
-    // the queries: head g of a tile, entries as the keys' words have them
-    uint32_t q[NT][K_STEPS * K_WORDS][2];
-    float s_scale[NT][2], slope2[NT][2];                     // heads 2 t and 2 t + 1: scores to units of log2, or for a cap to units of the cap
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const bf16* row = p.q + ((size_t)b * p.num_heads + first_head + 8 * j + g) * HD;
-        float x[K_STEPS * K_WORDS][4];
-        float top = 0.f;
-#pragma unroll
-        for (int s = 0; s < K_STEPS; ++s)
-#pragma unroll
-            for (int w = 0; w < K_WORDS; ++w) {
-                const float4 v = 8 * j + g < heads ? load4<bf16>(row + (4 * s + t) * KU + 4 * w) : make_float4(0.f, 0.f, 0.f, 0.f);
-                float (&to)[4] = x[s * K_WORDS + w];
-                to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to[e]));
-            }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = max(exponent_of(top), -100);           // |q| 2^(14 - e) < 2^15
-        const float factor = power_of_two(14 - min(e, 127));
-        const float unit = power_of_two(min(e, 127) - 14) * (p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f);
-#pragma unroll
-        for (int i = 0; i < K_STEPS * K_WORDS; ++i) {
-            const bool plain = CODES == FRB_E4M3;
-            q[j][i][0] = pack_f16(x[i][0] * factor, x[i][plain ? 1 : 2] * factor);
-            q[j][i][1] = pack_f16(x[i][plain ? 2 : 1] * factor, x[i][3] * factor);
+    // page kvh-th (or vh-th) head of the store's page `page`; called by all lanes
+    __device__ __forceinline__ void ask_keys(const Decode8Params& p, const CUtensorMap* map, int page, int kvh, int lane) {
+        if (lane == 0) {
+            bar_expect(keys_full, K_TILE + SCALES);
+            load_2d(keys, map, 0, (page * p.num_kv_heads + kvh) * FRB_PAGE, keys_full);
+            load_row_of_scales(key_scales, p.k_scales + ((size_t)page * p.num_kv_heads + kvh) * FRB_PAGE, keys_full);
         }
-        s_scale[j][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
-        s_scale[j][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-            slope2[j][c] = p.slopes && 8 * j + 2 * t + c < heads ? p.slopes[first_head + 8 * j + 2 * t + c] * 1.4426950408889634f : 0.f;
+        keys_out = true;
     }
-    const float cap2 = p.softcap > 0.f ? p.softcap * 1.4426950408889634f : 0.f;
-
-    float row_max[NT][2], row_sum[NT][2], unit[NT][2], inverse[NT][2];
-    float o[NT][MT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) { row_max[j][c] = -INFINITY; row_sum[j][c] = 0.f; unit[j][c] = 0.f; inverse[j][c] = 0.f; }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][i][e] = 0.f;
+    __device__ __forceinline__ void ask_values(const Decode8Params& p, const CUtensorMap* map, int page, int vh, int lane) {
+        if (lane == 0) {
+            bar_expect(values_full, V_TILE + SCALES);
+            load_2d(values, map, 0, (page * p.v_heads + vh) * FRB_PAGE, values_full);
+            load_row_of_scales(value_scales, p.v_scales + ((size_t)page * p.v_heads + vh) * FRB_PAGE, values_full);
+        }
+        values_out = true;
     }
-
-    uint32_t k_parity = 0, v_parity = 0;
-    bool keys_out = page >= 0, values_out = page >= 0;      // a copy is in flight
-    bool cleared = false;                                   // this warp wrote into its tiles
-    while (page >= 0) {
-        const int key_base = number_of(n) * FRB_PAGE;
-        const bool edge = key_base < lo_key || key_base + FRB_PAGE - 1 > hi_key;
-        next_page(n + D8_WARPS);                            // the next one's number is there when its copy is asked for
-        if (!__all_sync(0xffffffffu, bar_wait(&full_k[warp], k_parity, &failed))) break;
-        k_parity ^= 1;
+    __device__ __forceinline__ bool wait_keys(int* failed) {
+        if (!__all_sync(0xffffffffu, bar_wait(keys_full, keys_parity, failed))) return false;
+        keys_parity ^= 1;
         keys_out = false;
-        float s[NT][4][4];
+        return true;
+    }
+    __device__ __forceinline__ bool wait_values(int* failed) {
+        if (!__all_sync(0xffffffffu, bar_wait(values_full, values_parity, failed))) return false;
+        values_parity ^= 1;
+        values_out = false;
+        return true;
+    }
+    // a warp that gave up leaves only when the copies that it asked for have landed (or a second limit has passed)
+    __device__ __forceinline__ void leave() {
+        int again = 0;
+        if (keys_out) bar_wait(keys_full, keys_parity, &again);
+        if (values_out) bar_wait(values_full, values_parity, &again);
+    }
+};
+
+// Up to 8 NT query heads of one key head and what they have added up.  Lane 4 g + t holds, of head 2 t + c (c = 0, 1) of each tile of
+// eight, the dimensions VB g .. VB g + VB - 1 of the output.
+template <int HD, int VD, int NT, int CODES>
+struct HeadTile {
+    static constexpr int KU = HD % 64 == 0 ? 16 : 8, K_STEPS = HD / (4 * KU), K_WORDS = KU / 4;     // a lane's bytes of a key at a time
+    static constexpr int VB = VD / 8, MT = VD / 16;                                                // a lane's bytes of a value; output tiles
+    uint32_t q[NT][K_STEPS * K_WORDS][2];
+    float s_scale[NT][2], slope2[NT][2];        // scores to units of log2, or for a cap to units of the cap
+    float row_max[NT][2], row_sum[NT][2];       // row_sum: of the lane's own keys
+    float unit[NT][2], inverse[NT][2];          // U and 1 / U
+    float o[NT][MT][4];
+    float corr[NT][2];                          // what the sums before the present page are multiplied by
+    bool grew;
+
+    __device__ __forceinline__ void begin() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {                       // sixteen keys: rows g and g + 8 of the tile
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) { row_max[j][c] = -INFINITY; row_sum[j][c] = 0.f; unit[j][c] = 0.f; inverse[j][c] = 0.f; }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][i][e] = 0.f;
+        }
+    }
+
+    // heads first_head .. first_head + heads - 1 of row b
+    __device__ __forceinline__ void load_queries(const Decode8Params& p, int b, int first_head, int heads, int g, int t) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const bf16* row = p.q + ((size_t)b * p.num_heads + first_head + 8 * j + g) * HD;
+            float x[K_STEPS * K_WORDS][4];
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < K_STEPS; ++s)
+#pragma unroll
+                for (int w = 0; w < K_WORDS; ++w) {
+                    const float4 v = 8 * j + g < heads ? load4<bf16>(row + (4 * s + t) * KU + 4 * w) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    float (&to)[4] = x[s * K_WORDS + w];
+                    to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to[e]));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = min(max(exponent_of(top), -100), 127);           // |q| 2^(14 - e) < 2^15
+            const float factor = power_of_two(14 - e);
+            const float back = power_of_two(e - 14) * (p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f);
+#pragma unroll
+            for (int i = 0; i < K_STEPS * K_WORDS; ++i) {
+                constexpr bool plain = CODES == FRB_E4M3;
+                q[j][i][0] = pack_f16(x[i][0] * factor, x[i][plain ? 1 : 2] * factor);
+                q[j][i][1] = pack_f16(x[i][plain ? 2 : 1] * factor, x[i][3] * factor);
+            }
+            s_scale[j][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+            s_scale[j][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                slope2[j][c] = p.slopes && 8 * j + 2 * t + c < heads ? p.slopes[first_head + 8 * j + 2 * t + c] * 1.4426950408889634f : 0.f;
+        }
+    }
+
+    // The scores of a page whose first key is key_base, in units of log2: s[j][i][e] belongs to key 16 i + key_of_row(g) (+ 8 for e > 1)
+    // and head 2 t + (e & 1) of tile j.
+    __device__ __forceinline__ void scores(const Decode8Params& p, float (&s)[NT][4][4], const uint8_t* tile, const float* scales, int key_base, int hi_key,
+                                           int g, int t) {
+        const float cap2 = p.softcap * 1.4426950408889634f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
             const int k0 = 16 * i + key_of_row<VD>(g), k1 = k0 + 8;
 #pragma unroll
             for (int j = 0; j < NT; ++j)
@@ -302,7 +320,7 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int e = 0; e < 4; ++e) s[j][i][e] = 0.f;
 #pragma unroll
             for (int step = 0; step < K_STEPS; ++step) {
-                const Words<KU> a = row_words<HD, KU>(k_tile, k0, (4 * step + t) * KU), c = row_words<HD, KU>(k_tile, k1, (4 * step + t) * KU);
+                const Words<KU> a = row_words<HD, KU>(tile, k0, (4 * step + t) * KU), c = row_words<HD, KU>(tile, k1, (4 * step + t) * KU);
 #pragma unroll
                 for (int w = 0; w < K_WORDS; ++w) {
                     uint32_t a0, a1, a2, a3;
@@ -312,7 +330,7 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     for (int j = 0; j < NT; ++j) mma_f16(s[j][i], a0, a1, a2, a3, q[j][step * K_WORDS + w][0], q[j][step * K_WORDS + w][1]);
                 }
             }
-            const float ks0 = k_scale[k0], ks1 = k_scale[k1];
+            const float ks0 = scales[k0], ks1 = scales[k1];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -323,21 +341,23 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     s[j][i][e] = fmaf(slope2[j][e & 1], (float)(key_base + (e < 2 ? k0 : k1) - hi_key), score);
                 }
         }
-        __syncwarp();
-        if (page >= 0 && lane == 0) ask_keys(page);          // this page's keys are no longer needed
-        keys_out = page >= 0;
-        // only the pages at the window's edge, behind the first tokens and of the token itself hold keys it may not see
-        if (edge) {
+    }
+
+    // Keys that the token may not see get no weight.
+    __device__ __forceinline__ void hide(const Decode8Params& p, float (&s)[NT][4][4], int key_base, int lo_key, int hi_key, int g) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+            for (int e = 0; e < 4; e += 2)
+                if (!key_visible(key_base + 16 * i + key_of_row<VD>(g) + 4 * e, lo_key, hi_key, p.keep_first)) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!key_visible(key_base + 16 * i + key_of_row<VD>(g) + (e < 2 ? 0 : 8), lo_key, hi_key, p.keep_first))
-                            s[j][i][e] = -INFINITY;
-        }
-        float page_max[NT][2];
+                    for (int j = 0; j < NT; ++j) s[j][i][e] = s[j][i][e + 1] = -INFINITY;
+                }
+    }
+
+    // The running maximum follows the page's.
+    __device__ __forceinline__ void raise(const float (&s)[NT][4][4]) {
+        grew = false;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -347,34 +367,17 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(s[j][i][c], s[j][i][c + 2]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                page_max[j][c] = top;
-            }
-        float corr[NT][2];
-        bool grew = false;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
                 corr[j][c] = 1.f;
-                if (page_max[j][c] > row_max[j][c] + D8_RAISE) {      // also on the warp's first page
-                    corr[j][c] = exp2_of(row_max[j][c] - page_max[j][c]);
-                    row_max[j][c] = page_max[j][c];
+                if (top > row_max[j][c] + D8_RAISE) {                 // also on the first page
+                    corr[j][c] = exp2_of(row_max[j][c] - top);
+                    row_max[j][c] = top;
                     grew = true;
                 }
             }
-        if (!__all_sync(0xffffffffu, bar_wait(&full_v[warp], v_parity, &failed))) break;
-        v_parity ^= 1;
-        values_out = false;
-        if (edge) {
-            // whatever lies in the places of keys that the token may not see (their weight is zero, but zero times NaN is not)
-            for (int k = 0; k < FRB_PAGE; ++k)
-                if (!key_visible(key_base + k, lo_key, hi_key, p.keep_first)) {
-                    if (4 * lane < VD) *reinterpret_cast<uint32_t*>(v_tile + k * VD + 4 * lane) = 0u;
-                    if (lane == 0) v_scale[k] = 0.f;
-                }
-            cleared = true;
-            __syncwarp();
-        }
+    }
+
+    // Adds the page's values, weighted.
+    __device__ __forceinline__ void add_values(float (&s)[NT][4][4], const uint8_t* tile, const float* scales, int g, int t) {
         float top_w[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -383,7 +386,7 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int k0 = 16 * i + key_of_row<VD>(g);
-            const float vs0 = v_scale[k0], vs1 = v_scale[k0 + 8];
+            const float vs0 = scales[k0], vs1 = scales[k0 + 8];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -426,8 +429,8 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 b1[j] = transposed_8x8(pack_f16(s[j][i][2] * inverse[j][0], s[j][i][3] * inverse[j][1]));
             }
             const int ka = 16 * i + key_of_row<VD>(2 * t), kb = 16 * i + key_of_row<VD>(2 * t + 1);
-            const Words<VB> va = row_words<VD, VB>(v_tile, ka, VB * g), vb = row_words<VD, VB>(v_tile, kb, VB * g);
-            const Words<VB> vc = row_words<VD, VB>(v_tile, ka + 8, VB * g), vd = row_words<VD, VB>(v_tile, kb + 8, VB * g);
+            const Words<VB> va = row_words<VD, VB>(tile, ka, VB * g), vb = row_words<VD, VB>(tile, kb, VB * g);
+            const Words<VB> vc = row_words<VD, VB>(tile, ka + 8, VB * g), vd = row_words<VD, VB>(tile, kb + 8, VB * g);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {                  // rows g and g + 8: dimensions VB g + 2 m and + 1
                 uint32_t a0, a1, a2, a3;
@@ -437,42 +440,124 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int j = 0; j < NT; ++j) mma_f16(o[j][m], a0, a1, a2, a3, b0[j], b1[j]);
             }
         }
-        if (cleared) {                                      // ordinary stores into the tile, before a copy writes there again
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            cleared = false;
+    }
+
+    // The sums over all of the warp's keys.
+    __device__ __forceinline__ void end() {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) row_sum[j][c] += __shfl_xor_sync(0xffffffffu, row_sum[j][c], d);
+    }
+
+    // Head 8 j + 2 t + c's output entries VB g .. + VB - 1 to `row`, four or two at a time.
+    __device__ __forceinline__ void store_entries(float* row, int j, int c, int g) const {
+        if (MT % 2 == 0) {
+#pragma unroll
+            for (int m = 0; m < MT; m += 2)
+                *reinterpret_cast<float4*>(row + VB * g + 2 * m) = make_float4(o[j][m][c] * unit[j][c], o[j][m][c + 2] * unit[j][c],
+                                                                               o[j][m + 1][c] * unit[j][c], o[j][m + 1][c + 2] * unit[j][c]);
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                *reinterpret_cast<float2*>(row + VB * g + 2 * m) = make_float2(o[j][m][c] * unit[j][c], o[j][m][c + 2] * unit[j][c]);
         }
-        __syncwarp();
-        if (page >= 0 && lane == 0) ask_values(page);
-        values_out = page >= 0;
     }
-    // a warp that gave up leaves only when the copies that it asked for have landed (or a second limit has passed)
-    if (keys_out || values_out) {
-        int again = 0;
-        if (keys_out) bar_wait(&full_k[warp], k_parity, &again);
-        if (values_out) bar_wait(&full_v[warp], v_parity, &again);
-        failed = 1;
+};
+
+// Whatever lies in the places of keys that the token may not see (their weight is zero, but zero times NaN is not; int8 has no NaN).
+template <int VD, int CODES>
+__device__ __forceinline__ void clear_hidden(const Decode8Params& p, uint8_t* tile, float* scales, int key_base, int lo_key, int hi_key, int lane) {
+    if (CODES == FRB_E4M3)
+        for (int i = lane; i < FRB_PAGE * VD / 16; i += 32)
+            if (!key_visible(key_base + i / (VD / 16), lo_key, hi_key, p.keep_first)) reinterpret_cast<uint4*>(tile)[i] = make_uint4(0, 0, 0, 0);
+    for (int k = lane; k < FRB_PAGE; k += 32)
+        if (!key_visible(key_base + k, lo_key, hi_key, p.keep_first)) scales[k] = 0.f;
+    __syncwarp();
+}
+
+template <int HD, int VD>
+__device__ __forceinline__ uint8_t* begin_block(uint8_t* dynamic, uint64_t* bars, int* failed) {
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * D8_WARPS; ++i) bar_init(&bars[i], 1);
+        *failed = 0;
+        bar_init_fence();
     }
+    return reinterpret_cast<uint8_t*>(((uintptr_t)dynamic + 1023) & ~(uintptr_t)1023);
+}
+
+// ----------------------------------------------------------------------------- chunks: four pages of a key head a block
+
+// grid (chunk, key head and tile of query heads, sequence).
+template <int HD, int VD, int NT, int CODES>
+__global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(NT))
+attention_decode_8bit_chunks_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Params p) {
+    // as attention_decode_tma: the copies of every page but the sequence's last go out before the kernel before this one has ended
+    let_next_kernel_start();
+    typedef WarpTiles<HD, VD> Tiles;
+    constexpr int O_STRIDE = VD + 4;
+    static_assert(NT * 8 * O_STRIDE * 4 <= Tiles::K_TILE + Tiles::V_TILE, "a warp's partial result fits into its pages");
+    extern __shared__ uint8_t dynamic[];
+    __shared__ uint64_t bars[2 * D8_WARPS];
+    __shared__ float sm_m[D8_WARPS][8 * NT], sm_l[D8_WARPS][8 * NT];
+    __shared__ int failed;
+    const int chunk = blockIdx.x, kvh = blockIdx.y / p.head_tiles, tile = blockIdx.y - kvh * p.head_tiles, b = blockIdx.z;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const Sight sight = sight_of(p, b);
+    if (chunk * D8_CHUNK_PAGES >= sight.count) {
+        wait_for_previous_kernel();               // (were all blocks to leave without, the kernel after this one would not wait for it either)
+        return;
+    }
+    uint8_t* base = begin_block<HD, VD>(dynamic, bars, &failed);
+    Tiles tiles(base, bars, warp);
+    const int n = chunk * D8_CHUNK_PAGES + warp, number = sight.number(n);
+    int page = n < sight.count ? p.page_table[(size_t)p.seq_slot[b] * p.max_pages + number] : -1;
+    if (page >= p.num_pages) page = -1;
+    const int group = p.num_heads / p.num_kv_heads, first_head = kvh * group + tile * 8 * NT, heads = min(8 * NT, group - tile * 8 * NT);
+    __syncthreads();
+    const bool ahead = page >= 0 && p.early && number != sight.hi_key / FRB_PAGE;       // the kernel before this one writes to the last page
+    const int vh = kvh / (p.num_kv_heads / p.v_heads);
+    if (ahead) { tiles.ask_keys(p, &map_k, page, kvh, lane); tiles.ask_values(p, &map_v, page, vh, lane); }
+    wait_for_previous_kernel();
+    if (page >= 0 && !ahead) { tiles.ask_keys(p, &map_k, page, kvh, lane); tiles.ask_values(p, &map_v, page, vh, lane); }
+
+    HeadTile<HD, VD, NT, CODES> rows;
+    rows.begin();
+    bool ok = true;
+    if (page >= 0) {
+        const int key_base = number * FRB_PAGE;
+        const bool edge = key_base < sight.lo_key || key_base + FRB_PAGE - 1 > sight.hi_key;
+        rows.load_queries(p, b, first_head, heads, g, t);
+        float s[NT][4][4];
+        ok = tiles.wait_keys(&failed);
+        if (ok) {
+            rows.scores(p, s, tiles.keys, tiles.key_scales, key_base, sight.hi_key, g, t);
+            if (edge) rows.hide(p, s, key_base, sight.lo_key, sight.hi_key, g);
+            rows.raise(s);
+            ok = tiles.wait_values(&failed);
+        }
+        if (ok) {
+            if (edge) clear_hidden<VD, CODES>(p, tiles.values, tiles.value_scales, key_base, sight.lo_key, sight.hi_key, lane);
+            rows.add_values(s, tiles.values, tiles.value_scales, g, t);
+        }
+        rows.end();
+    }
+    if (!ok) { tiles.leave(); failed = 1; }
     __syncthreads();
     if (failed) {
         if (threadIdx.x == 0) *p.status = D8_STATUS_WAIT;
         return;
     }
-    float* mine = reinterpret_cast<float*>(k_tile);          // [8 NT heads][O_STRIDE]
+    float* mine = reinterpret_cast<float*>(tiles.keys);          // [8 NT heads][O_STRIDE]
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) row_sum[j][c] += __shfl_xor_sync(0xffffffffu, row_sum[j][c], d);
-            float* row = mine + (8 * j + 2 * t + c) * O_STRIDE;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                row[VB * g + 2 * m] = o[j][m][c] * unit[j][c];
-                row[VB * g + 2 * m + 1] = o[j][m][c + 2] * unit[j][c];
-            }
-            if (g == 0) { sm_m[warp][8 * j + 2 * t + c] = row_max[j][c]; sm_l[warp][8 * j + 2 * t + c] = row_sum[j][c]; }
+            rows.store_entries(mine + (8 * j + 2 * t + c) * O_STRIDE, j, c, g);
+            if (g == 0) { sm_m[warp][8 * j + 2 * t + c] = rows.row_max[j][c]; sm_l[warp][8 * j + 2 * t + c] = rows.row_sum[j][c]; }
         }
-    }
     __syncthreads();
     for (int idx = threadIdx.x; idx < heads * VD; idx += D8_THREADS) {
         const int r = idx / VD, d = idx - r * VD;
@@ -485,86 +570,331 @@ attention_decode_8bit_kernel(const __grid_constant__ CUtensorMap map_k, const __
             if (sm_l[w][r] != 0.f) {                        // a warp that had no page wrote zeros and no maximum
                 const float f = exp2f(sm_m[w][r] - top);
                 sum += sm_l[w][r] * f;
-                acc += reinterpret_cast<const float*>(tiles + (size_t)w * (K_TILE + V_TILE))[r * O_STRIDE + d] * f;
+                acc += reinterpret_cast<const float*>(base + (size_t)w * (Tiles::K_TILE + Tiles::V_TILE))[r * O_STRIDE + d] * f;
             }
         }
-        const size_t row = ((size_t)b * p.num_heads + first_head + r) * p.parts + part;
+        const size_t row = ((size_t)b * p.num_heads + first_head + r) * p.max_chunks + chunk;
         p.part_o[row * VD + d] = acc;
         if (d == 0) { p.part_ml[row * 2] = top; p.part_ml[row * 2 + 1] = sum; }
     }
 }
 
-// Entry d of the joined output of one (sequence, head): partial results 0 .. kept - 1, then first .. last, in that order, eight at a
-// time (all of their loads before the first use).  A partial result without a key (maximum -inf, sum 0) adds nothing; without any the
-// output is zero, with a sink or not.
-template <int VD>
-__device__ __forceinline__ float joined_8bit(const float* __restrict__ part_ml, const float* __restrict__ part_o, size_t row0, int kept,
-                                             int first, int last, int d, float sink2) {
-    constexpr int AT_ONCE = 8;
-    float top = -INFINITY, sum = 0.f, acc = 0.f;
-    const int end = kept + last - first;
-    for (int c0 = 0; c0 <= end; c0 += AT_ONCE) {
-        float2 ml[AT_ONCE];
-        float o[AT_ONCE];
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            const int c = run_at(min(c0 + u, end), kept, first);
-            ml[u] = *reinterpret_cast<const float2*>(part_ml + (row0 + c) * 2);
-            o[u] = part_o[(row0 + c) * VD + d];
-        }
-        float group_top = top;
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-            if (c0 + u <= end) group_top = fmaxf(group_top, ml[u].x);
-        const float keep = sum == 0.f ? 0.f : exp2f(top - group_top);
-        sum *= keep;
-        acc *= keep;
-        top = group_top;
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-            if (c0 + u <= end && ml[u].y != 0.f) {
-                const float f = exp2f(ml[u].x - top);
-                sum += ml[u].y * f;
-                acc += o[u] * f;
-            }
-    }
-    if (sum == 0.f) return 0.f;
-    if (sink2 > -INFINITY) {                              // a sink: a term of the denominator without a value
-        const float top_all = fmaxf(top, sink2);
-        const float keep = exp2f(top - top_all);
-        sum = sum * keep + exp2f(sink2 - top_all);
-        acc *= keep;
-    }
-    return acc / sum;
+// ----------------------------------------------------------------------------- pieces: a warp a piece of the line of pages
+
+// Whether row b is the row before it once more (the same token of the same sequence, as a recorded step repeats its last one).
+__device__ __forceinline__ bool repeats(const Decode8Params& p, int b) {
+    return b > 0 && p.seq_slot[b] == p.seq_slot[b - 1] && p.seq_pos[b] == p.seq_pos[b - 1];
 }
 
-// grid (output head, sequence), a thread per value entry.
+__device__ __forceinline__ int times_repeated(const Decode8Params& p, int b) {       // of a row that repeats none: itself and its repetitions
+    int n = 1;
+    while (b + n < p.num_seqs && repeats(p, b + n)) ++n;
+    return n;
+}
+
+// A row's pages in the line, for one key head: each page as many times as the row is repeated, so that a piece's pages are done for all of
+// those rows alike and repeated rows come out the same to the last bit.  Zero for a row that repeats another.
+__device__ __forceinline__ int places_of(const Decode8Params& p, int b) {
+    return b >= p.num_seqs || repeats(p, b) ? 0 : sight_of(p, b).count * times_repeated(p, b);
+}
+
+// A run: the pages [begin, end) in sight of one key head's, for one row (none where a piece lies within the repetitions of a page).  Its
+// partial result is number `room` of the (row, head)'s; the first run's warp also leaves the number of all of them, in the last place's sum.
+struct Run {
+    Sight sight;
+    int row, slot, kvh, first_head, heads, begin, end, room;
+    int runs;                  // not zero: the number to leave
+};
+
+// The runs of a piece, one after the other; all lanes of a warp alike.
+struct RunOrder {
+    int at, piece_end, length;         // places in the line; of a piece
+    int seq, times, copy;              // the row, how often it is there, which one is next
+    int before, places;                // places before the row, and of one of its key heads
+
+    __device__ __forceinline__ bool next(const Decode8Params& p, Run& run, int per_tile) {
+        if (at >= piece_end) return false;
+        if (copy == times) {                                                  // on to the next key head, or the next row that has pages
+            copy = 0;
+            at = min(piece_end, before + ((at - before) / places + 1) * places);
+            if (at < piece_end && at == before + p.num_kv_heads * p.head_tiles * places) {
+                before = at;
+                seq += times;
+                while (seq < p.num_seqs && (places = places_of(p, seq)) == 0) ++seq;
+                if (seq >= p.num_seqs) at = piece_end;                        // (not with tables that stay as they are)
+                else times = times_repeated(p, seq);
+            }
+            if (at >= piece_end) return false;
+        }
+        const int pair = (at - before) / places, pair_at = before + pair * places, run_end = min(piece_end, pair_at + places);
+        const int group = p.num_heads / p.num_kv_heads, tile = pair % p.head_tiles;
+        run.sight = sight_of(p, seq);
+        run.row = seq + copy;
+        run.slot = p.seq_slot[seq];
+        run.kvh = pair / p.head_tiles;
+        run.first_head = run.kvh * group + tile * per_tile;
+        run.heads = min(per_tile, group - tile * per_tile);
+        run.begin = (at - pair_at + times - 1) / times;
+        run.end = (run_end - pair_at + times - 1) / times;
+        run.room = at / length - pair_at / length;
+        run.runs = at == pair_at ? (pair_at + places - 1) / length - pair_at / length + 1 : 0;
+        ++copy;
+        return true;
+    }
+};
+
+#define D8_MIN_ROOM 5          // partial results that a line cut into pieces needs room for, per (sequence, head)
+
+template <int HD, int VD, int NT, int CODES>
+__global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(NT))
+attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Params p) {
+    let_next_kernel_start();
+    typedef WarpTiles<HD, VD> Tiles;
+    extern __shared__ uint8_t dynamic[];
+    __shared__ uint64_t bars[2 * D8_WARPS];
+    __shared__ int sums[D8_WARPS], tops[D8_WARPS];
+    __shared__ Run runs[D8_WARPS][2];
+    __shared__ int failed;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int heads_in_line = p.num_kv_heads * p.head_tiles;
+    uint8_t* base = begin_block<HD, VD>(dynamic, bars, &failed);
+
+    // The line's length, and that of a piece: a warp's share, at least as many places that a key head's pages lie in no more pieces than there
+    // is room for partial results (less one, where their number is left).
+    int total = 0, longest = 0;
+    for (int b = threadIdx.x; b < p.num_seqs; b += D8_THREADS) {
+        const int places = places_of(p, b);
+        total += places;
+        longest = max(longest, places);
+    }
+    if (warp * 32 < p.num_seqs) {
+        total = __reduce_add_sync(0xffffffffu, total);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+    }
+    if (lane == 0) { sums[warp] = total; tops[warp] = longest; }
+    __syncthreads();
+    total = longest = 0;
+#pragma unroll
+    for (int w = 0; w < D8_WARPS; ++w) { total += sums[w]; longest = max(longest, tops[w]); }
+    total *= heads_in_line;
+    RunOrder order;
+    order.length = max(1, max((total + p.pieces - 1) / p.pieces, (longest + p.max_chunks - 4) / (p.max_chunks - 3)));
+    // neighbouring pieces go to different SMs: warps without a piece are then spread over all of them
+    order.at = (int)min((long long)total, (long long)(warp * (int)gridDim.x + (int)blockIdx.x) * order.length);
+    order.piece_end = min(total - order.at, order.length) + order.at;
+    // the row that the piece begins in
+    order.seq = order.before = order.places = 0;
+    for (int b0 = 0, upto = 0; b0 < p.num_seqs && order.at < total; b0 += 32) {
+        const int own = heads_in_line * places_of(p, b0 + lane);
+        int to = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int left = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += left;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, order.at >= upto + to - own && order.at < upto + to);
+        if (here) {
+            const int found = __ffs(here) - 1;
+            order.seq = b0 + found;
+            order.before = upto + __shfl_sync(0xffffffffu, to - own, found);
+            order.places = __shfl_sync(0xffffffffu, own, found) / heads_in_line;
+            break;
+        }
+        upto += __shfl_sync(0xffffffffu, to, 31);
+    }
+    if (order.places == 0) order.at = order.piece_end;
+    order.copy = 0;
+    order.times = order.at < order.piece_end ? times_repeated(p, order.seq) : 0;
+
+    Tiles tiles(base, bars, warp);
+    const int v_share = p.num_kv_heads / p.v_heads;
+    // the store's page of a run's page n; -1 for one that the table, or the run, does not have
+    const auto page_of = [&](const Run& run, int n) {
+        if (n >= run.end) return -1;
+        const int page = p.page_table[(size_t)run.slot * p.max_pages + run.sight.number(n)];
+        return page < p.num_pages ? page : -1;
+    };
+    const auto next_run = [&](int to) {                     // the next run as runs[warp][to]
+        Run found;
+        const bool more = order.next(p, found, 8 * NT);
+        __syncwarp();
+        if (lane == 0) runs[warp][to] = found;
+        __syncwarp();
+        return more;
+    };
+    int now = 0;
+    bool more = next_run(now);
+    int n = 0, page = -1;
+    if (more) {
+        const Run& run = runs[warp][now];
+        n = run.begin;
+        page = page_of(run, n);
+        if (page >= 0 && p.early && run.sight.number(n) != run.sight.hi_key / FRB_PAGE) {      // the kernel before this one writes to the last page
+            tiles.ask_keys(p, &map_k, page, run.kvh, lane);
+            tiles.ask_values(p, &map_v, page, run.kvh / v_share, lane);
+        }
+    }
+    wait_for_previous_kernel();
+    if (page >= 0 && !tiles.keys_out) {
+        tiles.ask_keys(p, &map_k, page, runs[warp][now].kvh, lane);
+        tiles.ask_values(p, &map_v, page, runs[warp][now].kvh / v_share, lane);
+    }
+
+    HeadTile<HD, VD, NT, CODES> rows;
+    bool ok = true, fresh = true;
+    while (more) {
+        const Run& run = runs[warp][now];
+        const int key_base = run.sight.number(n) * FRB_PAGE, lo_key = run.sight.lo_key, hi_key = run.sight.hi_key;
+        const bool edge = key_base < lo_key || key_base + FRB_PAGE - 1 > hi_key, last = n + 1 >= run.end, there = page >= 0;
+        if (fresh) {
+            rows.begin();
+            rows.load_queries(p, run.row, run.first_head, run.heads, g, t);
+        }
+        // the page after this one: its number is there when its copy is asked for
+        const int next = last ? now ^ 1 : now;
+        if (last) more = next_run(next);
+        n = last ? runs[warp][next].begin : n + 1;
+        page = more ? page_of(runs[warp][next], n) : -1;
+        float s[NT][4][4];
+        if (there) {
+            ok = tiles.wait_keys(&failed);
+            if (!ok) break;
+            rows.scores(p, s, tiles.keys, tiles.key_scales, key_base, hi_key, g, t);
+        }
+        __syncwarp();
+        if (page >= 0) tiles.ask_keys(p, &map_k, page, runs[warp][next].kvh, lane);        // this page's keys are no longer needed
+        if (there) {
+            // only the pages at the window's edge, behind the first tokens and of the token itself hold keys it may not see
+            if (edge) rows.hide(p, s, key_base, lo_key, hi_key, g);
+            rows.raise(s);
+            ok = tiles.wait_values(&failed);
+            if (!ok) break;
+            if (edge) clear_hidden<VD, CODES>(p, tiles.values, tiles.value_scales, key_base, lo_key, hi_key, lane);
+            rows.add_values(s, tiles.values, tiles.value_scales, g, t);
+            // ordinary stores into the tile come before a copy that writes there again
+            if (edge) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (page >= 0) tiles.ask_values(p, &map_v, page, runs[warp][next].kvh / v_share, lane);
+        if (last) {
+            rows.end();
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int head = 8 * j + 2 * t + c;
+                    if (head >= run.heads) continue;
+                    const size_t row = ((size_t)run.row * p.num_heads + run.first_head + head) * p.max_chunks + run.room;
+                    rows.store_entries(p.part_o + row * VD, j, c, g);
+                    if (g == 0) {
+                        *reinterpret_cast<float2*>(p.part_ml + row * 2) = make_float2(rows.row_max[j][c], rows.row_sum[j][c]);
+                        if (run.runs > 0) p.part_ml[(row + p.max_chunks - 1) * 2 + 1] = (float)run.runs;           // (the first run: room 0)
+                    }
+                }
+        }
+        fresh = last;
+        now = next;
+    }
+    if (!ok) {
+        tiles.leave();
+        failed = 1;
+        if (lane == 0) *p.status = D8_STATUS_WAIT;
+    }
+}
+
+// ----------------------------------------------------------------------------- the join
+
+struct Joined { float top, sum, acc; };       // maximum (units of log2), sum and unnormalised output entry of some partial results
+
+__device__ __forceinline__ void add_joined(Joined& a, const Joined& b) {
+    if (b.sum == 0.f) return;                     // no key (a sum that is not a number is none of these)
+    if (a.sum == 0.f) { a = b; return; }
+    const float top = fmaxf(a.top, b.top), fa = exp2f(a.top - top), fb = exp2f(b.top - top);
+    a.top = top;
+    a.sum = a.sum * fa + b.sum * fb;
+    a.acc = a.acc * fa + b.acc * fb;
+}
+
+// Entry d of the partial results share, share + shares, ... of `count`, in that order, eight at a time (all of their loads before the first use).
 template <int VD>
-__global__ void __launch_bounds__(VD) attention_decode_8bit_join_kernel(Decode8Params p) {
-    after_previous_kernel();
-    __shared__ float scratch[32];
-    const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-    const int pos = held_position(p, b), keys_per_part = p.pages_per_block * FRB_PAGE;
-    const int heads = p.lam ? p.num_heads / 2 : p.num_heads;
+__device__ __forceinline__ Joined joined_parts(const Decode8Params& p, size_t row0, int count, int d, int share, int shares) {
+    constexpr int AT_ONCE = 8;
+    Joined all = {-INFINITY, 0.f, 0.f};
+    for (int c0 = share; c0 < count; c0 += AT_ONCE * shares) {
+        Joined part[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int c = min(c0 + u * shares, count - 1);
+            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (row0 + c) * 2);
+            part[u] = {ml.x, c0 + u * shares < count ? ml.y : 0.f, p.part_o[(row0 + c) * VD + d]};
+        }
+        float top = all.top;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) top = fmaxf(top, part[u].sum != 0.f ? part[u].top : -INFINITY);
+        const float keep = all.sum == 0.f ? 0.f : exp2f(all.top - top);
+        all.top = top;
+        all.sum *= keep;
+        all.acc *= keep;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+            if (part[u].sum != 0.f) {
+                const float f = exp2f(part[u].top - top);
+                all.sum += part[u].sum * f;
+                all.acc += part[u].acc * f;
+            }
+    }
+    return all;
+}
+
+#define D8_JOIN_THREADS 512
+
+// grid (output heads / heads a block, sequence); a thread per value entry of a head, and `shares` times that where there are few heads.
+// A (sequence, head) without any key gives zeros, with a sink or not.
+template <int VD>
+__global__ void __launch_bounds__(D8_JOIN_THREADS) attention_decode_8bit_join_kernel(Decode8Params p, int shares) {
+    let_next_kernel_start();
+    __shared__ Joined others[D8_JOIN_THREADS];
+    __shared__ float squares[D8_JOIN_THREADS / 32];
+    const int heads = p.lam ? p.num_heads / 2 : p.num_heads, b = blockIdx.y;
+    const int per_block = blockDim.x / (VD * shares), local = threadIdx.x / VD, d = threadIdx.x - local * VD, share = local % shares;
+    const int head = blockIdx.x * per_block + local / shares;
+    const Sight sight = sight_of(p, b);                        // from the step's tables, which were there before the kernel before this one began
+    wait_for_previous_kernel();
+    if (sight.cut && threadIdx.x == 0) atomicExch(p.status, D8_STATUS_TOO_LONG);               // keys were left out
+    const auto joined = [&](int query_head) {
+        Joined all = {-INFINITY, 0.f, 0.f};
+        if (sight.count > 0 && head < heads) {
+            const size_t row0 = ((size_t)b * p.num_heads + query_head) * p.max_chunks;
+            const int count = p.pieces > 0 ? (int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1] : (sight.count + D8_CHUNK_PAGES - 1) / D8_CHUNK_PAGES;
+            all = joined_parts<VD>(p, row0, min(count, p.max_chunks), d, share, shares);
+        }
+        if (shares > 1) {
+            __syncthreads();                                   // (read from an earlier call)
+            others[threadIdx.x] = all;
+            __syncthreads();
+            all = others[threadIdx.x - share * VD];
+            for (int s = 1; s < shares; ++s) add_joined(all, others[threadIdx.x + (s - share) * VD]);
+        }
+        return all;
+    };
     bf16* out = p.out + ((size_t)b * heads + head) * VD + d;
-    if (pos < 0) { *out = __float2bfloat16_rn(0.f); return; }
-    const int lo_key = first_visible_key(pos, p.window, p.chunk);
-    const int last = min(pos / keys_per_part, p.parts - 1), first = min(lo_key / keys_per_part, last);
-    const int kept = kept_runs(p.keep_first, keys_per_part, first);
-    if (pos / keys_per_part >= p.parts && d == 0) atomicExch(p.status, D8_STATUS_TOO_LONG);   // keys were left out
     if (p.lam) {
-        const int group = p.num_heads / p.num_kv_heads, g = head / group;
-        const size_t row1 = ((size_t)b * p.num_heads + (size_t)(2 * g) * group + (head - g * group)) * p.parts;
-        const size_t row2 = row1 + (size_t)group * p.parts;
-        const float a1 = joined_8bit<VD>(p.part_ml, p.part_o, row1, kept, first, last, d, -INFINITY);
-        const float a2 = joined_8bit<VD>(p.part_ml, p.part_o, row2, kept, first, last, d, -INFINITY);
-        const float o = a1 - *p.lam * a2;
-        const float ss = block_sum<VD>(o * o, scratch);
-        *out = __float2bfloat16_rn(o / sqrtf(ss / (float)VD + p.diff_eps) * p.diff_factor);
+        const int group = p.num_heads / p.num_kv_heads, pair = head / group, first = 2 * pair * group + (head - pair * group);
+        const Joined one = joined(first), two = joined(first + group);
+        const float o = (one.sum == 0.f ? 0.f : one.acc / one.sum) - *p.lam * (two.sum == 0.f ? 0.f : two.acc / two.sum);
+        const float part = warp_sum(o * o);
+        if ((threadIdx.x & 31) == 0) squares[threadIdx.x >> 5] = part;
+        __syncthreads();
+        float ss = 0.f;
+#pragma unroll
+        for (int w = 0; w < VD / 32; ++w) ss += squares[local * (VD / 32) + w];
+        if (share == 0 && head < heads) *out = __float2bfloat16_rn(o / sqrtf(ss / (float)VD + p.diff_eps) * p.diff_factor);
         return;
     }
-    *out = __float2bfloat16_rn(joined_8bit<VD>(p.part_ml, p.part_o, ((size_t)b * p.num_heads + head) * p.parts, kept, first, last, d,
-                                               p.sinks ? p.sinks[head] * 1.4426950408889634f : -INFINITY));
+    Joined all = joined(head);
+    if (share != 0 || head >= heads) return;
+    if (p.sinks && all.sum != 0.f) add_joined(all, {p.sinks[head] * 1.4426950408889634f, 1.f, 0.f});      // a term of the denominator without a value
+    *out = __float2bfloat16_rn(all.sum == 0.f ? 0.f : all.acc / all.sum);
 }
 
 // A map over rows of `row` one-byte codes, boxes of 64 rows with the swizzle of the row's size.
@@ -582,20 +912,22 @@ static bool map_code_rows(CUtensorMap* map, const void* base, uint64_t rows, int
 }
 
 template <int HD, int VD, int NT, int CODES>
-static void launch_decode_8bit(const CUtensorMap& map_k, const CUtensorMap& map_v, const Decode8Params& p, dim3 grid, cudaStream_t stream) {
-    const size_t smem = (size_t)D8_WARPS * (FRB_PAGE * (HD + VD) + 8 * FRB_PAGE) + 1024;
-    auto kernel = attention_decode_8bit_kernel<HD, VD, NT, CODES>;
+static void launch_decode_8bit(const CUtensorMap& map_k, const CUtensorMap& map_v, const Decode8Params& p, cudaStream_t stream) {
+    const size_t smem = (size_t)WarpTiles<HD, VD>::BYTES + 1024;
+    const bool pieces = p.pieces > 0;
+    auto kernel = pieces ? attention_decode_8bit_pieces_kernel<HD, VD, NT, CODES> : attention_decode_8bit_chunks_kernel<HD, VD, NT, CODES>;
+    const dim3 grid = pieces ? dim3((p.pieces + D8_WARPS - 1) / D8_WARPS) : dim3(p.max_chunks, p.num_kv_heads * p.head_tiles, p.num_seqs);
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    launch_dependent_resident(p.early ? (NT == 1 ? 3 : 2) : 1, kernel, grid, dim3(D8_THREADS), smem, stream, map_k, map_v, p);
+    launch_dependent_resident(p.early ? D8_RESIDENT(NT) : 1, kernel, grid, dim3(D8_THREADS), smem, stream, map_k, map_v, p);
 }
 
-// max_chunks: chunks of 256 keys of the longest sequence; part_o and part_ml hold ceil(max_chunks / chunks_per_block) partial results per
-// (sequence, head).  num_pages: pages of the store.  status: one int on the device.
+// max_chunks: chunks of 256 keys of the longest sequence (or more); part_o and part_ml hold as many partial results per (sequence, head).
+// num_pages: pages of the store.  max_pieces: 0, or into how many pieces (warps) the work is cut, whatever its size.  status: one int on the device.
 FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales,
                                       int codes, int num_pages, const int* page_table, int num_slots, int max_pages, const int* seq_pos,
                                       const int* seq_slot, float* part_o, float* part_ml, void* out, int num_seqs, int num_heads,
                                       int num_kv_heads, int v_heads, int head_dim, int v_dim, float scale, int window, int chunk,
-                                      int keep_first, int max_chunks, int chunks_per_block, const float* slopes, const float* sinks,
+                                      int keep_first, int max_chunks, int max_pieces, const float* slopes, const float* sinks,
                                       float softcap, const float* lam, float diff_eps, float diff_factor, int* status,
                                       cudaStream_t stream) {
     if (num_seqs == 0) return 0;
@@ -606,7 +938,7 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
                   num_pages, num_slots, max_pages);
     FRB_CHECK_ARG((long long)num_pages * num_kv_heads * FRB_PAGE < (1ll << 31), "attention_decode_8bit: %d pages of %d heads exceed a tensor map's rows",
                   num_pages, num_kv_heads);
-    FRB_CHECK_ARG(chunks_per_block >= 1 && max_chunks >= 1, "attention_decode_8bit: %d chunks, %d per block", max_chunks, chunks_per_block);
+    FRB_CHECK_ARG(max_chunks >= 1 && max_chunks < (1 << 23) && max_pieces >= 0 && max_pieces <= (1 << 24), "attention_decode_8bit: %d chunks, %d pieces", max_chunks, max_pieces);
     FRB_CHECK_ARG(window >= 0 && chunk >= 0 && keep_first >= 0 && !(keep_first > 0 && chunk > 0),
                   "attention_decode_8bit: a window of %d, chunks of %d, %d first tokens", window, chunk, keep_first);
     FRB_CHECK_ARG(!lam || (num_kv_heads == 2 * v_heads && !sinks), "attention_decode_8bit: two maps per head need two key heads a value head and no sinks");
@@ -621,21 +953,30 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
     p.part_o = part_o; p.part_ml = part_ml; p.out = (bf16*)out; p.slopes = slopes; p.sinks = sinks; p.lam = lam; p.status = status;
     p.scale = scale; p.softcap = softcap > 0.f ? softcap : 0.f; p.diff_eps = diff_eps; p.diff_factor = diff_factor; p.window = window;
     p.chunk = chunk; p.keep_first = window > 0 ? keep_first : 0; p.max_pages = max_pages; p.num_slots = num_slots; p.num_pages = num_pages;
-    p.num_heads = num_heads; p.num_kv_heads = num_kv_heads; p.v_heads = v_heads; p.parts = (max_chunks + chunks_per_block - 1) / chunks_per_block;
-    p.pages_per_block = chunks_per_block * D8_CHUNK_PAGES; p.head_tiles = head_tiles;
+    p.num_heads = num_heads; p.num_kv_heads = num_kv_heads; p.v_heads = v_heads; p.num_seqs = num_seqs; p.max_chunks = max_chunks;
+    p.head_tiles = head_tiles;
+    // Chunks where two waves of blocks hold all that there may be, or where a key head's partial results have no room for pieces.  (Measured
+    // on a B200 with 8 key heads of 128, microseconds of both kernels, chunks | pieces: CHOICE)
+    const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks, resident = (long long)D8_RESIDENT(per_block / 8) * frb_sm_count();
+    const bool by_piece = max_chunks >= D8_MIN_ROOM && chunks > 2 * resident && chunks * D8_CHUNK_PAGES < (1ll << 30);
+    p.pieces = max_pieces > 0 ? (max_chunks >= D8_MIN_ROOM && chunks * D8_CHUNK_PAGES < (1ll << 30) ? max_pieces : 0) : by_piece ? (int)resident * D8_WARPS : 0;
     static const int early = [] { const char* v = getenv("FIELDRUN_B200_ATTENTION_EARLY"); return !(v && v[0] == '0'); }();
     p.early = early;
     CUtensorMap map_k, map_v;
     FRB_CHECK_ARG(map_code_rows(&map_k, k_codes, (uint64_t)num_pages * num_kv_heads * FRB_PAGE, head_dim) &&
                   map_code_rows(&map_v, v_codes, (uint64_t)num_pages * v_heads * FRB_PAGE, v_dim),
                   "attention_decode_8bit: head_dim %d with value heads of %d: cuTensorMapEncodeTiled failed or is not available", head_dim, v_dim);
-    const dim3 grid(p.parts, num_kv_heads * head_tiles, num_seqs), join_grid(lam ? num_heads / 2 : num_heads, num_seqs);
+    const int out_heads = lam ? num_heads / 2 : num_heads;
+    // the join: blocks of up to D8_JOIN_THREADS threads, on one head each while that leaves SMs idle
+    const int most_rows = D8_JOIN_THREADS / v_dim, shares = (long long)out_heads * num_seqs <= 4 * frb_sm_count() && max_chunks > 8 ? (most_rows < 4 ? most_rows : 4) : 1;
+    const int heads_a_block = shares > 1 ? 1 : (out_heads < most_rows ? out_heads : most_rows);
+    const dim3 join_grid((out_heads + heads_a_block - 1) / heads_a_block, num_seqs), join_block(v_dim * shares * heads_a_block);
 #define FRB_LAUNCH_DECODE8(HD, VD)                                                                                                  \
-    if (per_block == 8 && codes == FRB_E4M3) launch_decode_8bit<HD, VD, 1, FRB_E4M3>(map_k, map_v, p, grid, stream);                \
-    else if (per_block == 8) launch_decode_8bit<HD, VD, 1, FRB_INT8>(map_k, map_v, p, grid, stream);                                \
-    else if (codes == FRB_E4M3) launch_decode_8bit<HD, VD, 2, FRB_E4M3>(map_k, map_v, p, grid, stream);                             \
-    else launch_decode_8bit<HD, VD, 2, FRB_INT8>(map_k, map_v, p, grid, stream);                                                    \
-    launch_dependent(attention_decode_8bit_join_kernel<VD>, join_grid, dim3(VD), 0, stream, p)
+    if (per_block == 8 && codes == FRB_E4M3) launch_decode_8bit<HD, VD, 1, FRB_E4M3>(map_k, map_v, p, stream);                \
+    else if (per_block == 8) launch_decode_8bit<HD, VD, 1, FRB_INT8>(map_k, map_v, p, stream);                                \
+    else if (codes == FRB_E4M3) launch_decode_8bit<HD, VD, 2, FRB_E4M3>(map_k, map_v, p, stream);                             \
+    else launch_decode_8bit<HD, VD, 2, FRB_INT8>(map_k, map_v, p, stream);                                                    \
+    launch_dependent(attention_decode_8bit_join_kernel<VD>, join_grid, join_block, 0, stream, p, shares)
     FRB_8BIT_SIZES("attention_decode_8bit", head_dim, v_dim, FRB_LAUNCH_DECODE8);
 #undef FRB_LAUNCH_DECODE8
     FRB_RETURN_LAUNCH("attention_decode_8bit");

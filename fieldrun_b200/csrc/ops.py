@@ -1723,30 +1723,55 @@ def attention_pair_tc(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
 CACHE_8BIT_TYPES = {torch.float8_e4m3fn: 0, torch.int8: 1}      # types of the codes (FRB_E4M3, FRB_INT8)
 
 
-def _want_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor, *others) -> int:
-    """Checks a store of 8-bit pages against itself and that it and the other tensors lie on the current device; the codes' type."""
-    if k_pages.dtype not in CACHE_8BIT_TYPES or v_pages.dtype != k_pages.dtype:
+def _store_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor) -> tuple:
+    """A store of 8-bit pages checked against itself: the codes' type, pages, key heads and entries, value heads and entries."""
+    codes, k_shape, v_shape = CACHE_8BIT_TYPES.get(k_pages.dtype), k_pages.shape, v_pages.shape
+    if codes is None or v_pages.dtype is not k_pages.dtype:
         raise KernelError(f"8-bit pages hold float8_e4m3fn or int8, keys and values alike: found {k_pages.dtype} and {v_pages.dtype}")
-    _want(k_scales, torch.float32, "the keys' scales")
-    _want(v_scales, torch.float32, "the values' scales")
-    for pages, scales, what in ((k_pages, k_scales, "keys"), (v_pages, v_scales, "values")):
-        if pages.dim() != 4 or pages.shape[2] != PAGE or tuple(scales.shape) != tuple(pages.shape[:3]):
-            raise KernelError(f"8-bit {what} of shape {list(pages.shape)} with scales of {list(scales.shape)}: pages are "
+    if k_scales.dtype is not torch.float32 or v_scales.dtype is not torch.float32:
+        _want(k_scales, torch.float32, "the keys' scales")
+        _want(v_scales, torch.float32, "the values' scales")
+    for shape, scales, what in ((k_shape, k_scales, "keys"), (v_shape, v_scales, "values")):
+        if len(shape) != 4 or shape[2] != PAGE or scales.shape != shape[:3]:
+            raise KernelError(f"8-bit {what} of shape {list(shape)} with scales of {list(scales.shape)}: pages are "
                               f"[pages, heads, {PAGE}, entries], scales [pages, heads, {PAGE}]")
-    if k_pages.shape[0] != v_pages.shape[0]:
-        raise KernelError(f"{k_pages.shape[0]} pages of keys and {v_pages.shape[0]} of values")
-    device = k_pages.device
-    for t in (k_scales, v_pages, v_scales, *others):
-        if t is not None and t.device != device:
-            raise KernelError(f"tensors on {device} and {t.device} in one call")
-    if device.type == "cuda" and device.index != torch.cuda.current_device():
-        raise KernelError(f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    return CACHE_8BIT_TYPES[k_pages.dtype]
+    pages, k_heads, _, head_dim = k_shape
+    v_count, v_heads, _, v_dim = v_shape
+    if pages != v_count:
+        raise KernelError(f"{pages} pages of keys and {v_count} of values")
+    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
+        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
+    return codes, pages, k_heads, head_dim, v_heads, v_dim
 
 
-def _want_ints(tensors: dict) -> None:
-    for what, t in tensors.items():
-        _want(t, torch.int32, what)
+def _want_heads(store: tuple, kv_heads: int, head_dim: int, v_heads: int, v_dim: int) -> None:
+    if store[2:] != (kv_heads, head_dim, v_heads, v_dim):
+        raise KernelError(f"8-bit pages of {store[2]} key heads of {store[3]} and {store[4]} value heads of {store[5]} for {kv_heads} key heads of "
+                          f"{head_dim} and {v_heads} value heads of {v_dim}")
+
+
+def _addresses(*tensors: Optional[torch.Tensor]) -> list:
+    """The tensors' addresses (as :func:`_ptr`), all of them on the current device."""
+    index, found = None, []
+    for t in tensors:
+        if t is None:
+            found.append(None)
+            continue
+        place = t.get_device()
+        if place != index or not t.is_contiguous():
+            _ptr(t)                                                    # a tensor on the host or in pieces
+            if index is None:
+                index = _DEVICE() if _DEVICE is not None else torch.cuda.current_device()
+            if place != index:
+                raise KernelError(f"a tensor on {t.device} while the current device is cuda:{index}")
+        found.append(t.data_ptr())
+    return found
+
+
+def _want_ints(what: str, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.dtype is not torch.int32:
+            raise KernelError(f"{what} must be torch.int32, found {t.dtype}")
 
 
 def qkv_prepare_8bit(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
@@ -1762,47 +1787,44 @@ def qkv_prepare_8bit(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k_weig
     not exist (a table entry of -1) leaves the store as it was.  Queries come out in bfloat16.  Head sizes: ``MMA_HEAD_SIZES``."""
     v_dim = int(v_dim or head_dim)
     num_v_heads = num_kv_heads if num_v_heads is None else int(num_v_heads)
-    codes = _want_8bit(k_pages, k_scales, v_pages, v_scales, qkv, q_weight, k_weight, cos_table, sin_table, tok_pos, tok_slot, page_table, q_out, bias)
+    store = _store_8bit(k_pages, k_scales, v_pages, v_scales)
+    _want_heads(store, num_kv_heads, head_dim, num_v_heads, v_dim)
     if (q_weight is None) != (k_weight is None):
         raise KernelError("q and k norm weights come together or not at all")
-    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
-        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
-    tokens = qkv.shape[0]
-    row = (num_heads + num_kv_heads) * head_dim + (0 if values_from_keys else num_v_heads * v_dim)
-    if qkv.dim() != 2 or qkv.shape[1] != row:
-        raise KernelError(f"projected rows of shape {list(qkv.shape)}, not [tokens, {row}]")
-    if tuple(k_pages.shape[1:]) != (num_kv_heads, PAGE, head_dim) or tuple(v_pages.shape[1:]) != (num_v_heads, PAGE, v_dim):
-        raise KernelError(f"8-bit pages of {list(k_pages.shape[1:])} and {list(v_pages.shape[1:])} for {num_kv_heads} key heads of {head_dim} "
-                          f"and {num_v_heads} value heads of {v_dim}")
-    _want(q_out, torch.bfloat16, "queries")
-    if q_out.numel() != tokens * num_heads * head_dim:
-        raise KernelError(f"{q_out.numel()} query entries for {tokens} tokens of {num_heads} heads of {head_dim}")
-    _want_ints({"positions": tok_pos, "slots": tok_slot, "the page table": page_table})
+    q_width = num_heads * head_dim
+    row = q_width + num_kv_heads * head_dim + (0 if values_from_keys else num_v_heads * v_dim)
+    qkv_shape = qkv.shape
+    tokens = qkv_shape[0]
+    if qkv_shape != (tokens, row):
+        raise KernelError(f"projected rows of shape {list(qkv_shape)}, not [tokens, {row}]")
+    if q_out.dtype is not torch.bfloat16 or q_out.numel() != tokens * q_width:
+        raise KernelError(f"{q_out.numel()} query entries of {q_out.dtype} for {tokens} tokens of {num_heads} heads of {head_dim} in bfloat16")
+    _want_ints("positions, slots and page table", tok_pos, tok_slot, page_table)
     if tok_pos.numel() != tokens or tok_slot.numel() != tokens or page_table.dim() != 2:
-        raise KernelError(f"{tok_pos.numel()} positions and {tok_slot.numel()} slots for {tokens} tokens")
+        raise KernelError(f"{tok_pos.numel()} positions, {tok_slot.numel()} slots and a page table of shape {list(page_table.shape)} for {tokens} tokens")
     wdtype = torch.float32
     if q_weight is not None:
         wdtype = q_weight.dtype
-        widths = (head_dim, head_dim) if per_head else (num_heads * head_dim, num_kv_heads * head_dim)
-        if k_weight.dtype != wdtype or (q_weight.numel(), k_weight.numel()) != widths:
+        widths = (head_dim, head_dim) if per_head else (q_width, num_kv_heads * head_dim)
+        if k_weight.dtype is not wdtype or q_weight.numel() != widths[0] or k_weight.numel() != widths[1]:
             raise KernelError(f"q and k norm weights of {q_weight.numel()} and {k_weight.numel()} entries ({wdtype}, {k_weight.dtype}), not {widths}")
     if bias is not None:
         _want(bias, torch.float32, "the projections' bias")
         if bias.numel() != row:
             raise KernelError(f"a bias of {bias.numel()} entries for rows of {row}")
+    table_positions = 0
     if rotary_dim:
         if cos_table is None or sin_table is None:
             raise KernelError("rotary tables are missing")
+        table_positions = cos_table.shape[0]
         for table in (cos_table, sin_table):
-            _want(table, torch.float32, "rotary tables")
-            if table.dim() != 2 or table.shape[1] != rotary_dim // 2 or table.shape[0] != cos_table.shape[0]:
-                raise KernelError(f"a rotary table of shape {list(table.shape)} for {rotary_dim} rotated entries")
-    _call("frb_qkv_prepare_8bit", _ptr(qkv), _code(qkv.dtype), _ptr(q_weight), _ptr(k_weight), _code(wdtype), float(eps),
-          _ptr(cos_table), _ptr(sin_table), cos_table.shape[0] if cos_table is not None else 0, _ptr(tok_pos), _ptr(tok_slot),
-          _ptr(page_table), page_table.shape[0], page_table.shape[1], _ptr(q_out), _ptr(k_pages), _ptr(k_scales), _ptr(v_pages),
-          _ptr(v_scales), codes, k_pages.shape[0], tokens, num_heads, num_kv_heads, num_v_heads, head_dim, v_dim, rotary_dim,
-          int(interleaved), int(per_head), int(tables_final), _ptr(bias), float(q_temp[0]) if q_temp else 0.0,
-          int(q_temp[1]) if q_temp else 1, int(values_from_keys))
+            if table.dtype is not torch.float32 or table.shape != (table_positions, rotary_dim // 2):
+                raise KernelError(f"a rotary table of shape {list(table.shape)} ({table.dtype}) for {rotary_dim} rotated entries in float32")
+    at = _addresses(qkv, q_weight, k_weight, cos_table, sin_table, tok_pos, tok_slot, page_table, q_out, k_pages, k_scales, v_pages, v_scales, bias)
+    _call("frb_qkv_prepare_8bit", at[0], _code(qkv.dtype), at[1], at[2], _code(wdtype), float(eps), at[3], at[4], table_positions, at[5], at[6],
+          at[7], *page_table.shape, *at[8:13], store[0], store[1], tokens, num_heads, num_kv_heads, num_v_heads, head_dim, v_dim, rotary_dim,
+          int(interleaved), int(per_head), int(tables_final), at[13], float(q_temp[0]) if q_temp else 0.0, int(q_temp[1]) if q_temp else 1,
+          int(values_from_keys))
 
 
 def cache_read_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,
@@ -1811,75 +1833,68 @@ def cache_read_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torc
     """Pages of a cache of 8-bit pages as bfloat16 pages in the layout of the prompt kernels: ``keys[n]`` and ``values[n]`` (transposed,
     [heads, entries, 64]) are page number ``page_index[n]`` of sequence ``page_seq[n]``, code times scale rounded once.  Sequence b is
     slot ``seq_slot[b]`` and holds ``seq_start[b] + seq_q_len[b]`` tokens; places behind them, and pages that the table does not have, become zero."""
-    codes = _want_8bit(k_pages, k_scales, v_pages, v_scales, page_table, page_seq, page_index, seq_slot, seq_start, seq_q_len, keys, values)
-    _want_ints({"the page table": page_table, "pages' sequences": page_seq, "pages' numbers": page_index, "slots": seq_slot,
-                "positions": seq_start, "new tokens": seq_q_len})
+    codes, pages, kv_heads, head_dim, v_heads, v_dim = _store_8bit(k_pages, k_scales, v_pages, v_scales)
+    _want_ints("the page table, sequences, page numbers, slots and lengths", page_table, page_seq, page_index, seq_slot, seq_start, seq_q_len)
     _want(keys, torch.bfloat16, "keys read back")
     _want(values, torch.bfloat16, "values read back")
-    kv_heads, head_dim, v_heads, v_dim = k_pages.shape[1], k_pages.shape[3], v_pages.shape[1], v_pages.shape[3]
-    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
-        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
-    count = page_seq.numel()
-    if page_index.numel() != count or tuple(keys.shape) != (count, kv_heads, PAGE, head_dim) or tuple(values.shape) != (count, v_heads, v_dim, PAGE):
+    count, seqs = page_seq.numel(), seq_slot.numel()
+    if page_index.numel() != count or keys.shape != (count, kv_heads, PAGE, head_dim) or values.shape != (count, v_heads, v_dim, PAGE):
         raise KernelError(f"{count} sequences and {page_index.numel()} numbers of pages with keys of shape {list(keys.shape)} and values of "
                           f"{list(values.shape)}")
-    if seq_start.numel() != seq_slot.numel() or seq_q_len.numel() != seq_slot.numel() or page_table.dim() != 2:
-        raise KernelError(f"{seq_slot.numel()} slots with {seq_start.numel()} positions and {seq_q_len.numel()} numbers of new tokens")
-    _call("frb_cache_read_8bit", _ptr(k_pages), _ptr(k_scales), _ptr(v_pages), _ptr(v_scales), codes, k_pages.shape[0], _ptr(page_table),
-          page_table.shape[0], page_table.shape[1], _ptr(page_seq), _ptr(page_index), count, _ptr(seq_slot), _ptr(seq_start), _ptr(seq_q_len),
-          seq_slot.numel(), _ptr(keys), _ptr(values), kv_heads, v_heads, head_dim, v_dim)
+    if seq_start.numel() != seqs or seq_q_len.numel() != seqs or page_table.dim() != 2:
+        raise KernelError(f"{seqs} slots with {seq_start.numel()} positions and {seq_q_len.numel()} numbers of new tokens, a page table of shape "
+                          f"{list(page_table.shape)}")
+    at = _addresses(k_pages, k_scales, v_pages, v_scales, page_table, page_seq, page_index, seq_slot, seq_start, seq_q_len, keys, values)
+    _call("frb_cache_read_8bit", *at[:4], codes, pages, at[4], *page_table.shape, at[5], at[6], count, *at[7:10], seqs, at[10], at[11], kv_heads,
+          v_heads, head_dim, v_dim)
 
 
 def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor,
                           page_table: torch.Tensor, seq_pos: torch.Tensor, seq_slot: torch.Tensor, part_o: torch.Tensor,
                           part_ml: torch.Tensor, out: torch.Tensor, *, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
-                          window: Optional[int], max_chunks: int, chunks_per_block: Optional[int] = None,
+                          window: Optional[int], max_chunks: int, pieces: Optional[int] = None,
                           slopes: Optional[torch.Tensor] = None, chunk: Optional[int] = None, sinks: Optional[torch.Tensor] = None,
                           softcap: Optional[float] = None, v_dim: Optional[int] = None, keep_first: int = 0, maps: int = 1,
                           difference: Optional[dict] = None) -> None:
     """As :func:`attention_decode_tma` over 8-bit pages (see :func:`qkv_prepare_8bit`), for every head size of ``MMA_HEAD_SIZES`` and
-    groups of any size; queries and output are bfloat16.  ``part_o`` and ``part_ml`` (float32) hold a partial result per (sequence, head,
-    run of ``chunks_per_block`` chunks): ``[sequences, heads, max_chunks, v_dim]`` and ``[..., 2]`` always suffice.  A sequence
-    at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
+    groups of any size; queries and output are bfloat16.  ``max_chunks``: chunks of 256 keys of the longest sequence, or more; ``part_o`` and
+    ``part_ml`` (float32) have room for ``[sequences, heads, max_chunks, v_dim]`` and ``[..., 2]``.  ``pieces``: into how many
+    pieces the step's pages are cut where they are more than fit at once (default: as many as warps are resident).  Where a sequence is cut
+    then depends on the others, a matter of rounding; neighbouring rows of one slot and position come out the same to the last bit
+    if their queries are the same.  A sequence at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
     v_dim = int(v_dim or head_dim)
-    codes = _want_8bit(k_pages, k_scales, v_pages, v_scales, q, page_table, seq_pos, seq_slot, part_o, part_ml, out, slopes, sinks,
-                       difference["lam"] if difference is not None else None)
+    store = _store_8bit(k_pages, k_scales, v_pages, v_scales)
     if maps < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or num_kv_heads % maps:
         raise KernelError(f"{num_heads} heads over {num_kv_heads} key heads with {maps} maps")
-    if (head_dim, v_dim) not in MMA_HEAD_SIZES:
-        raise KernelError(f"8-bit pages of key heads of {head_dim} with value heads of {v_dim}; known: {sorted(MMA_HEAD_SIZES)}")
-    if tuple(k_pages.shape[1:]) != (num_kv_heads, PAGE, head_dim) or tuple(v_pages.shape[1:]) != (num_kv_heads // maps, PAGE, v_dim):
-        raise KernelError(f"8-bit pages of {list(k_pages.shape[1:])} and {list(v_pages.shape[1:])} for {num_kv_heads} key heads of {head_dim} "
-                          f"and {num_kv_heads // maps} value heads of {v_dim}")
-    _want(q, torch.bfloat16, "queries")
-    _want(out, torch.bfloat16, "the attention output")
-    _want(part_o, torch.float32, "partial outputs")
-    _want(part_ml, torch.float32, "partial maxima and sums")
+    _want_heads(store, num_kv_heads, head_dim, num_kv_heads // maps, v_dim)
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16 or part_o.dtype is not torch.float32 or part_ml.dtype is not torch.float32:
+        raise KernelError(f"queries and outputs are bfloat16, partial results float32: found {q.dtype}, {out.dtype}, {part_o.dtype} and {part_ml.dtype}")
     _want_slopes(slopes, num_heads)
     _want_slopes(sinks, num_heads)
-    _want_ints({"the page table": page_table, "positions": seq_pos, "slots": seq_slot})
+    _want_ints("the page table, positions and slots", page_table, seq_pos, seq_slot)
     seqs = q.shape[0]
-    lam, eps, factor = _difference_args(difference, maps)
+    if difference is not None and maps != 2:
+        raise KernelError(f"the difference of {maps} maps")
     heads_out = num_heads // 2 if difference is not None else num_heads
     if q.numel() != seqs * num_heads * head_dim or out.numel() != seqs * heads_out * v_dim:
         raise KernelError(f"queries of shape {list(q.shape)} and an output of {list(out.shape)} for {num_heads} heads of {head_dim} and {v_dim}")
     if seq_pos.numel() != seqs or seq_slot.numel() != seqs or page_table.dim() != 2:
-        raise KernelError(f"{seq_pos.numel()} positions and {seq_slot.numel()} slots for {seqs} sequences")
-    if window is not None and window < 0 or chunk is not None and chunk < 0 or keep_first < 0:
+        raise KernelError(f"{seq_pos.numel()} positions, {seq_slot.numel()} slots and a page table of shape {list(page_table.shape)} for {seqs} sequences")
+    window, chunk, keep_first = int(window or 0), int(chunk or 0), int(keep_first or 0)
+    if window < 0 or chunk < 0 or keep_first < 0:
         raise KernelError(f"a window of {window}, chunks of {chunk}, {keep_first} first tokens")
-    if max_chunks < 1 or (chunks_per_block is not None and chunks_per_block < 1):
-        raise KernelError(f"{max_chunks} chunks, {chunks_per_block} per block")
-    if chunks_per_block is None:
-        _ptr(q)                                                         # refuses a tensor on the host before the device is asked
-        chunks_per_block = decode_chunks_per_block(seqs, num_kv_heads, max_chunks, sm_count(q.device))
-    rows = seqs * num_heads * -(-max_chunks // chunks_per_block)
+    if max_chunks < 1 or (pieces is not None and pieces < 1):
+        raise KernelError(f"{max_chunks} chunks, {pieces} pieces")
+    at = _addresses(q, k_pages, k_scales, v_pages, v_scales, page_table, seq_pos, seq_slot, part_o, part_ml, out, slopes, sinks)
+    rows = seqs * num_heads * max_chunks
     if part_o.numel() < rows * v_dim or part_ml.numel() < rows * 2:
         raise KernelError(f"room for {part_o.numel()} partial outputs and {part_ml.numel()} maxima and sums, {rows * v_dim} and {rows * 2} are needed")
-    _call("frb_attention_decode_8bit", _ptr(q), _ptr(k_pages), _ptr(k_scales), _ptr(v_pages), _ptr(v_scales), codes, k_pages.shape[0],
-          _ptr(page_table), page_table.shape[0], page_table.shape[1], _ptr(seq_pos), _ptr(seq_slot), _ptr(part_o), _ptr(part_ml), _ptr(out),
-          seqs, num_heads, num_kv_heads, num_kv_heads // maps, head_dim, v_dim, float(scale), int(window or 0), int(chunk or 0),
-          int(keep_first or 0), max_chunks, int(chunks_per_block), _ptr(slopes), _ptr(sinks), float(softcap or 0.0), lam, eps, factor,
-          _ptr(tc_status(q.device)))
+    lam, eps, factor = _difference_args(difference, maps)
+    if lam is not None:
+        _addresses(difference["lam"])
+    _call("frb_attention_decode_8bit", *at[:5], store[0], store[1], at[5], *page_table.shape, *at[6:11], seqs, num_heads, num_kv_heads,
+          num_kv_heads // maps, head_dim, v_dim, float(scale), window, chunk, keep_first, max_chunks, int(pieces or 0), at[11], at[12],
+          float(softcap or 0.0), lam, eps, factor, _ptr(tc_status(q.device)))
 
 
 def wait_probe(device, limit_cycles: int = 100_000) -> int:

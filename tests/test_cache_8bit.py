@@ -47,13 +47,13 @@ def test_what_writing_refuses():
         ops.qkv_prepare_8bit(*args, **options)
     for at, value, match in [
             (0, torch.zeros(3, 6 * 64 - 4), "projected rows of shape"), (1, torch.ones(128), "come together"),
-            (4, None, "rotary tables are missing"), (5, torch.zeros(9, 8), "a rotary table of shape"), (4, torch.zeros(9, 16).double(), "must be torch.float32"),
-            (6, ints(3).long(), "positions must be torch.int32"), (7, ints(2), "2 slots for 3 tokens"), (8, ints(8), "positions and"),
-            (9, torch.zeros(3, 128), "queries must be torch.bfloat16"), (9, torch.zeros(3, 64, dtype=torch.bfloat16), "query entries"),
+            (4, None, "rotary tables are missing"), (5, torch.zeros(9, 8), "a rotary table of shape"), (4, torch.zeros(9, 16).double(), "torch.float64"),
+            (6, ints(3).long(), "must be torch.int32"), (7, ints(2), "2 slots and a page table"), (8, ints(8), "3 slots and a page table"),
+            (9, torch.zeros(3, 128), "query entries of torch.float32"), (9, torch.zeros(3, 64, dtype=torch.bfloat16), "query entries"),
             (10, torch.zeros(3, 2, PAGE, 64), "float8_e4m3fn or int8"), (10, k.to(E4M3), "keys and values alike"), (10, k[:2], "with scales of"),
             (11, ks.double(), "the keys' scales must be"), (11, ks[:, :1], "with scales of"), (12, v[:, :, :32], "pages are"),
-            ("head_dim", 48, "known:"), ("num_heads", 3, "projected rows of shape"), ("num_kv_heads", 1, "projected rows of shape"),
-            ("bias", torch.zeros(6), "a bias of 6"), ("bias", torch.zeros(6 * 64).double(), "must be torch.float32"), ("v_dim", 128, "projected rows")]:
+            ("head_dim", 48, "8-bit pages of 2 key heads of 64"), ("num_heads", 3, "projected rows of shape"), ("num_kv_heads", 1, "for 1 key heads"),
+            ("bias", torch.zeros(6), "a bias of 6"), ("bias", torch.zeros(6 * 64).double(), "must be torch.float32"), ("v_dim", 128, "value heads of 128")]:
         refuses(ops.qkv_prepare_8bit, args, options, at, value, match)
     refuses(ops.qkv_prepare_8bit, (args[0], torch.ones(64), torch.ones(128), *args[3:]), options, "per_head", False, "norm weights of 64 and 128")
     refuses(ops.qkv_prepare_8bit, (*args[:12], *store(pages=4)[2:]), options, "per_head", False, "3 pages of keys and 4 of values")
@@ -84,15 +84,15 @@ def test_what_attention_refuses():
     with pytest.raises(ops.KernelError, match=HOST):
         ops.attention_decode_8bit(*args, **options)
     for at, value, match in [
-            (0, torch.zeros(3, 6 * 64), "queries must be"), (0, torch.zeros(3, 5 * 64, dtype=torch.bfloat16), "queries of shape"), (1, k.float(), "float8"),
-            (2, ks[:1], "with scales of"), (3, v.to(INT8), "keys and values alike"), (5, ints(5, 4).long(), "the page table must be"), (5, ints(20), "positions and"),
-            (6, ints(2), "2 positions"), (7, ints(4), "4 slots"), (8, torch.zeros(3 * 6 * 64 - 1), "room for"), (9, torch.zeros(35), "room for"),
-            (8, torch.zeros(3 * 6 * 64).double(), "must be torch.float32"), (10, torch.zeros(3, 6 * 64), "the attention output must be"),
+            (0, torch.zeros(3, 6 * 64), "queries and outputs are bfloat16"), (0, torch.zeros(3, 5 * 64, dtype=torch.bfloat16), "queries of shape"), (1, k.float(), "float8"),
+            (2, ks[:1], "with scales of"), (3, v.to(INT8), "keys and values alike"), (5, ints(5, 4).long(), "the page table, positions and slots must be"), (5, ints(20), "slots and a page table"),
+            (6, ints(2), "2 positions"), (7, ints(4), "4 slots"), (8, torch.zeros(3 * 6 * 64).double(), "partial results float32"),
+            (10, torch.zeros(3, 6 * 64), "outputs are bfloat16"),
             (10, torch.zeros(3, 64, dtype=torch.bfloat16), "an output of"), ("num_heads", 5, "5 heads over 2"), ("num_kv_heads", 3, "8-bit pages of"),
-            ("head_dim", 80, "known:"), ("v_dim", 128, "8-bit pages of"), ("maps", 3, "with 3 maps"), ("max_chunks", 0, "0 chunks"), ("chunks_per_block", 0, "0 per block"),
+            ("head_dim", 80, "key heads of 80"), ("v_dim", 128, "8-bit pages of"), ("maps", 3, "with 3 maps"), ("max_chunks", 0, "0 chunks"), ("pieces", 0, "0 pieces"),
             ("window", -1, "a window of -1"), ("keep_first", -1, "-1 first tokens"), ("slopes", torch.zeros(2), "2 numbers for 6 heads"),
             ("sinks", torch.zeros(6).double(), "must be torch.float32"), ("difference", dict(lam=torch.zeros(1), eps=0.1, factor=1.0), "the difference of 1 maps")]:
-        refuses(ops.attention_decode_8bit, args, {**options, "chunks_per_block": 1} if at != "chunks_per_block" else options, at, value, match)
+        refuses(ops.attention_decode_8bit, args, options, at, value, match)
 
 
 def test_entry_points_refuse_sizes_by_a_message():

@@ -344,10 +344,10 @@ MASKS = [dict(window=1), dict(window=64), dict(window=65), dict(window=300), dic
 
 
 @pytest.mark.parametrize("options", MASKS, ids=lambda o: "-".join(f"{k}{v}" for k, v in o.items()))
-@pytest.mark.parametrize("per_block", [None, 1, 3])
-def test_attention_masks(options, per_block):
-    Attended([0, 63, 64, 200, 999, 1300, 511], INT8, heads=12, kv_heads=4, dim=64, chunks_per_block=per_block, **options).run().check()
-    Attended([1300, 40, 1023], E4M3, heads=10, kv_heads=1, dim=128, chunks_per_block=per_block, **options).run().check()
+@pytest.mark.parametrize("pieces", [None, 1, 3, 29, 1000])
+def test_attention_masks(options, pieces):
+    Attended([0, 63, 64, 200, 999, 1300, 511], INT8, heads=12, kv_heads=4, dim=64, pieces=pieces, **options).run().check()
+    Attended([1300, 40, 1023], E4M3, heads=10, kv_heads=1, dim=128, pieces=pieces, **options).run().check()
 
 
 def test_attention_scores_with_everything():
@@ -367,8 +367,8 @@ def test_attention_of_two_maps(dim, v_dim, heads, kv_heads, dtype):
 
 
 def test_attention_long_sequences_and_the_split():
-    for per_block in (None, 1, 5, 8, 64):
-        Attended([16000, 3, 9000], E4M3, heads=12, kv_heads=2, dim=128, chunks_per_block=per_block).run().check()
+    for pieces in (None, 1, 5, 8, 64, 1776):
+        Attended([16000, 3, 9000], E4M3, heads=12, kv_heads=2, dim=128, pieces=pieces).run().check()
 
 
 def test_attention_sharp_scores():
@@ -477,6 +477,23 @@ def test_attention_of_sequences_and_pages_that_are_not_there():
     assert (a.out == 0).all()
 
 
+def test_attention_refuses_too_little_room_and_tensors_in_pieces():
+    a = Attended([100, 700], E4M3, heads=6, kv_heads=2, dim=64, pieces=1)
+    for name, value in (("part_o", a.part_o[:-1]), ("part_ml", a.part_ml[:-1])):
+        kept = getattr(a, name)
+        setattr(a, name, value)
+        with pytest.raises(ops.KernelError, match="room for"):
+            a.run()
+        setattr(a, name, kept)
+    kept, a.out = a.out, a.out.t().contiguous().t()
+    with pytest.raises(ops.KernelError, match="not contiguous"):
+        a.run()
+    a.out = kept
+    a.q = a.q.cpu()
+    with pytest.raises(ops.KernelError, match="a CPU tensor"):
+        a.run()
+
+
 def test_attention_more_keys_than_the_launch_is_sized_for_are_reported():
     a = Attended([100, 1000], E4M3, heads=6, kv_heads=2, dim=64)
     a.options["max_chunks"] = 2
@@ -486,14 +503,30 @@ def test_attention_more_keys_than_the_launch_is_sized_for_are_reported():
     a.run().check()
 
 
-def test_attention_twice_is_the_same_bits_and_a_sequence_does_not_depend_on_the_others():
-    a = Attended([2000, 300, 64], INT8, heads=12, kv_heads=2, dim=128, chunks_per_block=2).run()
-    first = a.out.clone()
-    a.run()
-    assert torch.equal(a.out, first)
-    a.positions, a.slots, a.q, a.out = [300], a.slots[1:2].contiguous(), a.q[1:2].contiguous(), a.out[1:2].clone()
-    a.run()
-    assert torch.equal(a.out, first[1:2])
+def test_attention_twice_is_the_same_bits():
+    for lengths in ([2000, 300, 64], [9000] * 20):
+        a = Attended(lengths, INT8, heads=12, kv_heads=2, dim=128).run()
+        first = a.out.clone()
+        a.run()
+        assert torch.equal(a.out, first)
+
+
+@pytest.mark.parametrize("pieces", [None, 1, 7, 40, 5000])
+@pytest.mark.parametrize("times", [2, 3, 9])
+def test_attention_of_repeated_rows_is_the_same_bits(times, pieces):
+    # a recorded step repeats its last row; here rows in the middle are repeated, too, among them one without tokens
+    for lengths, heads, kv_heads, options in (([700, 64, 5000, -1, 333], 12, 2, {}), ([6000, 4000], 6, 6, dict(window=3000, keep_first=70)), ([20000], 20, 1, {})):
+        counts = [1 + (i % 2) * (times - 1) for i in range(len(lengths) - 1)] + [times]
+        a = Attended(lengths, E4M3, heads=heads, kv_heads=kv_heads, dim=64, pieces=pieces, **options)
+        index = torch.tensor([i for i, n in enumerate(counts) for _ in range(n)], device=DEV)
+        a.positions = [lengths[int(i)] for i in index]
+        a.q, a.slots, a.out = a.q[index].contiguous(), a.slots[index].contiguous(), a.out[index].contiguous()
+        a.part_o, a.part_ml = (x.reshape(len(lengths), -1)[index].reshape(-1).contiguous() for x in (a.part_o, a.part_ml))
+        a.run()
+        for i in range(len(lengths)):
+            rows = a.out[index == i]
+            assert torch.equal(rows, rows[:1].expand_as(rows))
+        a.check()
 
 
 def test_attention_beyond_32_bits():
