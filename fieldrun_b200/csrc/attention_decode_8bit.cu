@@ -7,9 +7,13 @@
 // What bounds it is the cache's bytes, dim + vdim + 8 a key and head.  They are half of the bfloat16 cache's, so everything a warp does
 // with a key has to take half the time: the products are laid out with the keys as the rows of an MMA (S^T = K Q^T and O^T = V^T P^T,
 // m16n8k16), where up to eight query heads of a key head fill the columns; with the heads as rows half of every MMA, of the
-// accumulators and of the exponentials would belong to rows that do not exist.  Codes become float16 in registers, which is exact for
-// both types; the queries are brought to float16 by a power of two per head (exact down to 2^-29 of a head's largest entry); a
-// key's scale multiplies its scores, a value's scale its weight.
+// accumulators and of the exponentials would belong to rows that do not exist.  A key's scale multiplies its scores, a value's its weight.
+//
+// Scores: int8 codes go into the tensor cores as they are (m16n8k32, 32-bit integer sums), the queries in two parts of 8 bits, q = h 256 + l in
+// units of 1/32512 of the head's largest entry (errors of up to 2^-16 of it).  e4m3 codes become float16 in registers, which is exact; the
+// queries are brought to float16 by a power of two per head (exact down to 2^-29 of a head's largest entry).  (The products of e4m3
+// codes are no instruction of their own for single warps: with them, and the queries in two e4m3 parts, 32 sequences of 4,096 keys took 71
+// us, with float16 58.)  The values' codes, of either type, become float16, since the weights need its range and precision.
 //
 // Weights: p_j = 2^(s_j - m) with m a running maximum that follows a page's only beyond a margin.  The weight that multiplies codes is
 // w_j = p_j vs_j, rounded to float16 after division by a unit U per head, a power of two that follows the largest w seen: w / U is at most
@@ -35,7 +39,9 @@
 
 #define D8_WARPS 4
 #define D8_THREADS (32 * D8_WARPS)
-#define D8_RESIDENT(NT) ((NT) == 1 ? 3 : 2)     // blocks that an SM holds
+// Blocks that an SM holds: their pages fill its shared memory (heads of 128: 203 of 227 KB) or their registers its file (128 a thread
+// for the smaller heads, 168).
+#define D8_RESIDENT(HD, VD, NT) ((NT) == 2 ? 2 : (HD) + (VD) <= 128 ? 4 : 3)
 #define D8_CHUNK_PAGES 4               // a chunk is 256 keys
 #define D8_RAISE 8.0f                  // the running maximum follows a page's maximum only beyond this margin (in units of log2)
 #define D8_STATUS_WAIT 7               // a wait gave up
@@ -92,15 +98,22 @@ __device__ __forceinline__ Sight sight_of(const Decode8Params& p, int b) {
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same over 32 int8 codes of k
+__device__ __forceinline__ void mma_int8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 
@@ -160,11 +173,22 @@ __device__ __forceinline__ Words<BYTES> row_words(const uint8_t* tile, int r, in
     return v;
 }
 
-// Four codes of a key as two float16 pairs (entries 0 1 | 2 3 for e4m3, 0 2 | 1 3 for int8: the queries are paired alike).
+// Four query entries as two registers beside the registers of four codes of a key.  e4m3: float16 pairs, of entries below 2^15.  int8, of
+// entries of up to 32512: the codes of the two parts.
 template <int CODES>
-__device__ __forceinline__ void key_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if (CODES == FRB_E4M3) halves_of_e4m3(w, lo, hi);
-    else { lo = half_of_int8(w); hi = half_of_int8(w >> 8); }
+__device__ __forceinline__ void query_words(const float (&x)[4], uint32_t& first, uint32_t& second) {
+    if (CODES == FRB_E4M3) {
+        first = pack_f16(x[0], x[1]);
+        second = pack_f16(x[2], x[3]);
+    } else {
+        first = second = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int n = __float2int_rn(x[e]), h = (n + 128) >> 8;
+            first |= ((uint32_t)h & 0xffu) << (8 * e);
+            second |= ((uint32_t)(n - 256 * h) & 0xffu) << (8 * e);
+        }
+    }
 }
 
 // Entries 2 n and 2 n + 1 (n = 0, 1) of four codes of two keys: entry 2 n of both as `even`, entry 2 n + 1 as `odd`.
@@ -250,25 +274,27 @@ template <int HD, int VD, int NT, int CODES>
 struct HeadTile {
     static constexpr int KU = HD % 64 == 0 ? 16 : 8, K_STEPS = HD / (4 * KU), K_WORDS = KU / 4;     // a lane's bytes of a key at a time
     static constexpr int VB = VD / 8, MT = VD / 16;                                                // a lane's bytes of a value; output tiles
-    uint32_t q[NT][K_STEPS * K_WORDS][2];
+    uint32_t q[NT][2][K_STEPS * K_WORDS];       // two registers for every word of a key (query_words)
     float s_scale[NT][2], slope2[NT][2];        // scores to units of log2, or for a cap to units of the cap
-    float row_max[NT][2], row_sum[NT][2];       // row_sum: of the lane's own keys
-    float unit[NT][2], inverse[NT][2];          // U and 1 / U
+    float gain[NT][2];                          // what scores() gives, to units of log2
+    float row_max[NT][2], limit[NT][2], row_sum[NT][2];       // units of log2; a score beyond `limit` raises the maximum; row_sum: of the lane's own keys
+    float inverse[NT][2];                       // 1 / U; 0 while there is no weight
     float o[NT][MT][4];
-    float corr[NT][2];                          // what the sums before the present page are multiplied by
-    bool grew;
 
     __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) { row_max[j][c] = -INFINITY; row_sum[j][c] = 0.f; unit[j][c] = 0.f; inverse[j][c] = 0.f; }
+            for (int c = 0; c < 2; ++c) { row_max[j][c] = limit[j][c] = -INFINITY; row_sum[j][c] = 0.f; inverse[j][c] = 0.f; }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][i][e] = 0.f;
         }
     }
+
+    // scores are what the products give times the scales, no more (and the scale keeps their order)
+    static __device__ __forceinline__ bool plain(const Decode8Params& p) { return p.softcap == 0.f && !p.slopes && p.scale > 0.f; }
 
     // heads first_head .. first_head + heads - 1 of row b
     __device__ __forceinline__ void load_queries(const Decode8Params& p, int b, int first_head, int heads, int g, int t) {
@@ -277,6 +303,7 @@ struct HeadTile {
             const bf16* row = p.q + ((size_t)b * p.num_heads + first_head + 8 * j + g) * HD;
             float x[K_STEPS * K_WORDS][4];
             float top = 0.f;
+            bool bad = false;
 #pragma unroll
             for (int s = 0; s < K_STEPS; ++s)
 #pragma unroll
@@ -285,61 +312,128 @@ struct HeadTile {
                     float (&to)[4] = x[s * K_WORDS + w];
                     to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(to[e]));
+                    for (int e = 0; e < 4; ++e) { top = fmaxf(top, fabsf(to[e])); bad |= !(fabsf(to[e]) < INFINITY); }
                 }
+            bad = ((__ballot_sync(0xffffffffu, bad) >> (4 * g)) & 15u) != 0;            // the head has an entry that is not finite: so are its scores
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = min(max(exponent_of(top), -100), 127);           // |q| 2^(14 - e) < 2^15
-            const float factor = power_of_two(14 - e);
-            const float back = power_of_two(e - 14) * (p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f);
+            float factor, back;
+            if (CODES == FRB_E4M3) {
+                const int e = min(max(exponent_of(top), -100), 127);       // |q| 2^(14 - e) < 2^15
+                factor = power_of_two(14 - e);
+                back = power_of_two(e - 14);
+            } else {
+                top = fmaxf(top, 1e-30f);
+                factor = 32512.f / top;
+                back = top * (1.f / 32512.f);
+            }
 #pragma unroll
             for (int i = 0; i < K_STEPS * K_WORDS; ++i) {
-                constexpr bool plain = CODES == FRB_E4M3;
-                q[j][i][0] = pack_f16(x[i][0] * factor, x[i][plain ? 1 : 2] * factor);
-                q[j][i][1] = pack_f16(x[i][plain ? 2 : 1] * factor, x[i][3] * factor);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) x[i][d] *= factor;
+                query_words<CODES>(x[i], q[j][0][i], q[j][1][i]);
             }
+            back *= p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f;
+            if (bad) back = __uint_as_float(0x7fc00000u);
             s_scale[j][0] = __shfl_sync(0xffffffffu, back, 8 * t);
             s_scale[j][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) gain[j][c] = plain(p) ? s_scale[j][c] : 1.f;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 slope2[j][c] = p.slopes && 8 * j + 2 * t + c < heads ? p.slopes[first_head + 8 * j + 2 * t + c] * 1.4426950408889634f : 0.f;
         }
     }
 
-    // The scores of a page whose first key is key_base, in units of log2: s[j][i][e] belongs to key 16 i + key_of_row(g) (+ 8 for e > 1)
-    // and head 2 t + (e & 1) of tile j.
-    __device__ __forceinline__ void scores(const Decode8Params& p, float (&s)[NT][4][4], const uint8_t* tile, const float* scales, int key_base, int hi_key,
-                                           int g, int t) {
-        const float cap2 = p.softcap * 1.4426950408889634f;
+    // The products of the queries with the keys of 16-key tiles i0 and i0 + 1 of a page (two at a time: the one's sums do not wait for the
+    // other's), in units of s_scale: s[j][i][e] belongs to key 16 i + key_of_row(g) (+ 8 for e > 1) and head 2 t + (e & 1) of tile j.
+    __device__ __forceinline__ void products(float (&s)[NT][4][4], const uint8_t* tile, int i0, int g, int t) {
+        Words<KU> a[2][K_STEPS], c[2][K_STEPS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k0 = 16 * i + key_of_row<VD>(g), k1 = k0 + 8;
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[j][i][e] = 0.f;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int step = 0; step < K_STEPS; ++step) {
-                const Words<KU> a = row_words<HD, KU>(tile, k0, (4 * step + t) * KU), c = row_words<HD, KU>(tile, k1, (4 * step + t) * KU);
-#pragma unroll
-                for (int w = 0; w < K_WORDS; ++w) {
-                    uint32_t a0, a1, a2, a3;
-                    key_halves<CODES>(a.w[w], a0, a2);
-                    key_halves<CODES>(c.w[w], a1, a3);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) mma_f16(s[j][i], a0, a1, a2, a3, q[j][step * K_WORDS + w][0], q[j][step * K_WORDS + w][1]);
-                }
+                const int k0 = 16 * (i0 + i) + key_of_row<VD>(g);
+                a[i][step] = row_words<HD, KU>(tile, k0, (4 * step + t) * KU);
+                c[i][step] = row_words<HD, KU>(tile, k0 + 8, (4 * step + t) * KU);
             }
-            const float ks0 = scales[k0], ks1 = scales[k1];
+        if (CODES == FRB_E4M3) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][i0 + i][e] = 0.f;
+#pragma unroll
+            for (int n = 0; n < K_STEPS * K_WORDS; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t a0, a1, a2, a3;
+                    halves_of_e4m3(a[i][n / K_WORDS].w[n % K_WORDS], a0, a2);
+                    halves_of_e4m3(c[i][n / K_WORDS].w[n % K_WORDS], a1, a3);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mma_f16(s[j][i0 + i], a0, a1, a2, a3, q[j][0][n], q[j][1][n]);
+                }
+        } else {
+            int sum[2][NT][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[i][j][e] = 0;
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                for (int n = 0; n < K_STEPS * K_WORDS; n += 2)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            const Words<KU>&top = a[i][n / K_WORDS], &low = c[i][n / K_WORDS];
+                            mma_int8(sum[i][j], top.w[n % K_WORDS], low.w[n % K_WORDS], top.w[n % K_WORDS + 1], low.w[n % K_WORDS + 1], q[j][part][n],
+                                     q[j][part][n + 1]);
+                        }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (part == 0) sum[i][j][e] *= 256;
+                            else s[j][i0 + i][e] = (float)sum[i][j][e];
+                        }
+            }
+        }
+    }
+
+    // The scores of a page whose first key is key_base; times `gain` they are in units of log2.
+    __device__ __forceinline__ void scores(const Decode8Params& p, float (&s)[NT][4][4], const uint8_t* tile, const float* scales, int key_base, int hi_key,
+                                           int g, int t) {
+        products(s, tile, 0, g, t);
+        products(s, tile, 2, g, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k0 = 16 * i + key_of_row<VD>(g);
+            const float ks0 = scales[k0], ks1 = scales[k0 + 8];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float scaled = s[j][i][e] * (s_scale[j][e & 1] * (e < 2 ? ks0 : ks1));
-                    // (the cap's minimum would turn NaN into a number)
-                    const float score = cap2 > 0.f && scaled == scaled ? capped_score2(scaled, 1.f, cap2) : scaled;
-                    s[j][i][e] = fmaf(slope2[j][e & 1], (float)(key_base + (e < 2 ? k0 : k1) - hi_key), score);
-                }
+                for (int e = 0; e < 4; ++e) s[j][i][e] *= e < 2 ? ks0 : ks1;
+        }
+        if (!plain(p)) {
+            const float cap2 = p.softcap * 1.4426950408889634f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float scaled = s[j][i][e] * s_scale[j][e & 1];
+                        // (the cap's minimum would turn NaN into a number)
+                        const float score = cap2 > 0.f && scaled == scaled ? capped_score2(scaled, 1.f, cap2) : scaled;
+                        s[j][i][e] = fmaf(slope2[j][e & 1], (float)(key_base + 16 * i + key_of_row<VD>(g) + (e < 2 ? 0 : 8) - hi_key), score);
+                    }
         }
     }
 
@@ -355,34 +449,54 @@ struct HeadTile {
                 }
     }
 
-    // The running maximum follows the page's.
+    // The running maximum follows the page's.  That is rare, so that the lanes first only ask one another whether any has a reason.
     __device__ __forceinline__ void raise(const float (&s)[NT][4][4]) {
-        grew = false;
+        float top[NT][2];
+        bool reason = false;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float top = s[j][0][c];
+                top[j][c] = s[j][0][c];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(s[j][i][c], s[j][i][c + 2]));
+                for (int i = 0; i < 4; ++i) top[j][c] = fmaxf(top[j][c], fmaxf(s[j][i][c], s[j][i][c + 2]));
+                top[j][c] *= gain[j][c];
+                reason |= top[j][c] > limit[j][c];                        // also on the first page
+            }
+        if (!__any_sync(0xffffffffu, reason)) return;
+        float corr[NT][2];
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top[j][c] = fmaxf(top[j][c], __shfl_xor_sync(0xffffffffu, top[j][c], d));
                 corr[j][c] = 1.f;
-                if (top > row_max[j][c] + D8_RAISE) {                 // also on the first page
-                    corr[j][c] = exp2_of(row_max[j][c] - top);
-                    row_max[j][c] = top;
-                    grew = true;
+                if (top[j][c] > limit[j][c]) {
+                    corr[j][c] = exp2_of(row_max[j][c] - top[j][c]);
+                    row_max[j][c] = top[j][c];
+                    limit[j][c] = top[j][c] + D8_RAISE;
+                    row_sum[j][c] *= corr[j][c];
                 }
+            }
+        rescale(corr);
+    }
+
+    __device__ __forceinline__ void rescale(const float (&corr)[NT][2]) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                o[j][i][0] *= corr[j][0]; o[j][i][1] *= corr[j][1];
+                o[j][i][2] *= corr[j][0]; o[j][i][3] *= corr[j][1];
             }
     }
 
     // Adds the page's values, weighted.
     __device__ __forceinline__ void add_values(float (&s)[NT][4][4], const uint8_t* tile, const float* scales, int g, int t) {
-        float top_w[NT][2];
+        float top[NT][2];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) { row_sum[j][c] *= corr[j][c]; top_w[j][c] = 0.f; }
+        for (int j = 0; j < NT; ++j) top[j][0] = top[j][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int k0 = 16 * i + key_of_row<VD>(g);
@@ -391,34 +505,34 @@ struct HeadTile {
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float weight = exp2_of(s[j][i][e] - row_max[j][e & 1]);
+                    const float weight = exp2_of(fmaf(s[j][i][e], gain[j][e & 1], -row_max[j][e & 1]));
                     row_sum[j][e & 1] += weight;
                     s[j][i][e] = weight * (e < 2 ? vs0 : vs1);
-                    top_w[j][e & 1] = fmaxf(top_w[j][e & 1], s[j][i][e]);
+                    top[j][e & 1] = fmaxf(top[j][e & 1], s[j][i][e]);
                 }
         }
+        // the unit follows the largest weight times scale; rare, too
+        bool reason = false;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) top_w[j][c] = fmaxf(top_w[j][c], __shfl_xor_sync(0xffffffffu, top_w[j][c], d));
-                if (top_w[j][c] * inverse[j][c] > 32768.f || (unit[j][c] == 0.f && top_w[j][c] > 0.f)) {
-                    const int e = min(max(exponent_of(top_w[j][c]) - 7, -119), 119);
-                    corr[j][c] *= unit[j][c] * power_of_two(-e);
-                    unit[j][c] = power_of_two(e);
-                    inverse[j][c] = power_of_two(-e);
-                    grew = true;
-                }
-            }
-        if (__any_sync(0xffffffffu, grew)) {
+            for (int c = 0; c < 2; ++c) reason |= top[j][c] * inverse[j][c] > 32768.f || (inverse[j][c] == 0.f && top[j][c] > 0.f);
+        if (__any_sync(0xffffffffu, reason)) {
+            float corr[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    o[j][i][0] *= corr[j][0]; o[j][i][1] *= corr[j][1];
-                    o[j][i][2] *= corr[j][0]; o[j][i][3] *= corr[j][1];
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top[j][c] = fmaxf(top[j][c], __shfl_xor_sync(0xffffffffu, top[j][c], d));
+                    corr[j][c] = 1.f;
+                    if (top[j][c] * inverse[j][c] > 32768.f || (inverse[j][c] == 0.f && top[j][c] > 0.f)) {
+                        const int e = min(max(exponent_of(top[j][c]) - 7, -119), 119);
+                        corr[j][c] = inverse[j][c] == 0.f ? 0.f : power_of_two(-e) / inverse[j][c];
+                        inverse[j][c] = power_of_two(-e);
+                    }
                 }
+            rescale(corr);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -454,15 +568,14 @@ struct HeadTile {
 
     // Head 8 j + 2 t + c's output entries VB g .. + VB - 1 to `row`, four or two at a time.
     __device__ __forceinline__ void store_entries(float* row, int j, int c, int g) const {
+        const float unit = inverse[j][c] == 0.f ? 0.f : 1.f / inverse[j][c];          // a power of two
         if (MT % 2 == 0) {
 #pragma unroll
             for (int m = 0; m < MT; m += 2)
-                *reinterpret_cast<float4*>(row + VB * g + 2 * m) = make_float4(o[j][m][c] * unit[j][c], o[j][m][c + 2] * unit[j][c],
-                                                                               o[j][m + 1][c] * unit[j][c], o[j][m + 1][c + 2] * unit[j][c]);
+                *reinterpret_cast<float4*>(row + VB * g + 2 * m) = make_float4(o[j][m][c] * unit, o[j][m][c + 2] * unit, o[j][m + 1][c] * unit, o[j][m + 1][c + 2] * unit);
         } else {
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-                *reinterpret_cast<float2*>(row + VB * g + 2 * m) = make_float2(o[j][m][c] * unit[j][c], o[j][m][c + 2] * unit[j][c]);
+            for (int m = 0; m < MT; ++m) *reinterpret_cast<float2*>(row + VB * g + 2 * m) = make_float2(o[j][m][c] * unit, o[j][m][c + 2] * unit);
         }
     }
 };
@@ -485,14 +598,15 @@ __device__ __forceinline__ uint8_t* begin_block(uint8_t* dynamic, uint64_t* bars
         *failed = 0;
         bar_init_fence();
     }
-    return reinterpret_cast<uint8_t*>(((uintptr_t)dynamic + 1023) & ~(uintptr_t)1023);
+    // an offset into the array, not an address made from a number: what is read from it is then known to be shared memory
+    return dynamic + ((1024u - (smem_addr(dynamic) & 1023u)) & 1023u);
 }
 
 // ----------------------------------------------------------------------------- chunks: four pages of a key head a block
 
 // grid (chunk, key head and tile of query heads, sequence).
 template <int HD, int VD, int NT, int CODES>
-__global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(NT))
+__global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(HD, VD, NT))
 attention_decode_8bit_chunks_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Params p) {
     // as attention_decode_tma: the copies of every page but the sequence's last go out before the kernel before this one has ended
     let_next_kernel_start();
@@ -646,7 +760,7 @@ struct RunOrder {
 #define D8_MIN_ROOM 5          // partial results that a line cut into pieces needs room for, per (sequence, head)
 
 template <int HD, int VD, int NT, int CODES>
-__global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(NT))
+__global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(HD, VD, NT))
 attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Decode8Params p) {
     let_next_kernel_start();
     typedef WarpTiles<HD, VD> Tiles;
@@ -747,8 +861,8 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
         const int key_base = run.sight.number(n) * FRB_PAGE, lo_key = run.sight.lo_key, hi_key = run.sight.hi_key;
         const bool edge = key_base < lo_key || key_base + FRB_PAGE - 1 > hi_key, last = n + 1 >= run.end, there = page >= 0;
         if (fresh) {
-            rows.begin();
             rows.load_queries(p, run.row, run.first_head, run.heads, g, t);
+            rows.begin();
         }
         // the page after this one: its number is there when its copy is asked for
         const int next = last ? now ^ 1 : now;
@@ -815,22 +929,28 @@ __device__ __forceinline__ void add_joined(Joined& a, const Joined& b) {
     a.acc = a.acc * fa + b.acc * fb;
 }
 
-// Entry d of the partial results share, share + shares, ... of `count`, in that order, eight at a time (all of their loads before the first use).
+// Entry d of the partial results share, share + shares, ... of those that there are, in that order, eight at a time (all of their loads
+// before the first use, and the first eight's before their number is known: places without one are read and not used).
 template <int VD>
-__device__ __forceinline__ Joined joined_parts(const Decode8Params& p, size_t row0, int count, int d, int share, int shares) {
+__device__ __forceinline__ Joined joined_parts(const Decode8Params& p, size_t row0, int chunks, int d, int share, int shares) {
     constexpr int AT_ONCE = 8;
     Joined all = {-INFINITY, 0.f, 0.f};
+    int count = p.max_chunks;
     for (int c0 = share; c0 < count; c0 += AT_ONCE * shares) {
         Joined part[AT_ONCE];
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
-            const int c = min(c0 + u * shares, count - 1);
+            const int c = min(c0 + u * shares, p.max_chunks - 1);
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (row0 + c) * 2);
-            part[u] = {ml.x, c0 + u * shares < count ? ml.y : 0.f, p.part_o[(row0 + c) * VD + d]};
+            part[u] = {ml.x, ml.y, p.part_o[(row0 + c) * VD + d]};
         }
+        if (c0 == share) count = p.pieces > 0 ? min((int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1], p.max_chunks) : chunks;
         float top = all.top;
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) top = fmaxf(top, part[u].sum != 0.f ? part[u].top : -INFINITY);
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (c0 + u * shares >= count) part[u] = {-INFINITY, 0.f, 0.f};
+            top = fmaxf(top, part[u].sum != 0.f ? part[u].top : -INFINITY);
+        }
         const float keep = all.sum == 0.f ? 0.f : exp2f(all.top - top);
         all.top = top;
         all.sum *= keep;
@@ -864,9 +984,8 @@ __global__ void __launch_bounds__(D8_JOIN_THREADS) attention_decode_8bit_join_ke
     const auto joined = [&](int query_head) {
         Joined all = {-INFINITY, 0.f, 0.f};
         if (sight.count > 0 && head < heads) {
-            const size_t row0 = ((size_t)b * p.num_heads + query_head) * p.max_chunks;
-            const int count = p.pieces > 0 ? (int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1] : (sight.count + D8_CHUNK_PAGES - 1) / D8_CHUNK_PAGES;
-            all = joined_parts<VD>(p, row0, min(count, p.max_chunks), d, share, shares);
+            const int chunks = (sight.count + D8_CHUNK_PAGES - 1) / D8_CHUNK_PAGES;
+            all = joined_parts<VD>(p, ((size_t)b * p.num_heads + query_head) * p.max_chunks, chunks, d, share, shares);
         }
         if (shares > 1) {
             __syncthreads();                                   // (read from an earlier call)
@@ -918,7 +1037,7 @@ static void launch_decode_8bit(const CUtensorMap& map_k, const CUtensorMap& map_
     auto kernel = pieces ? attention_decode_8bit_pieces_kernel<HD, VD, NT, CODES> : attention_decode_8bit_chunks_kernel<HD, VD, NT, CODES>;
     const dim3 grid = pieces ? dim3((p.pieces + D8_WARPS - 1) / D8_WARPS) : dim3(p.max_chunks, p.num_kv_heads * p.head_tiles, p.num_seqs);
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    launch_dependent_resident(p.early ? D8_RESIDENT(NT) : 1, kernel, grid, dim3(D8_THREADS), smem, stream, map_k, map_v, p);
+    launch_dependent_resident(p.early ? D8_RESIDENT(HD, VD, NT) : 1, kernel, grid, dim3(D8_THREADS), smem, stream, map_k, map_v, p);
 }
 
 // max_chunks: chunks of 256 keys of the longest sequence (or more); part_o and part_ml hold as many partial results per (sequence, head).
@@ -957,7 +1076,7 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
     p.head_tiles = head_tiles;
     // Chunks where two waves of blocks hold all that there may be, or where a key head's partial results have no room for pieces.  (Measured
     // on a B200 with 8 key heads of 128, microseconds of both kernels, chunks | pieces: CHOICE)
-    const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks, resident = (long long)D8_RESIDENT(per_block / 8) * frb_sm_count();
+    const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks, resident = (long long)D8_RESIDENT(head_dim, v_dim, per_block / 8) * frb_sm_count();
     const bool by_piece = max_chunks >= D8_MIN_ROOM && chunks > 2 * resident && chunks * D8_CHUNK_PAGES < (1ll << 30);
     p.pieces = max_pieces > 0 ? (max_chunks >= D8_MIN_ROOM && chunks * D8_CHUNK_PAGES < (1ll << 30) ? max_pieces : 0) : by_piece ? (int)resident * D8_WARPS : 0;
     static const int early = [] { const char* v = getenv("FIELDRUN_B200_ATTENTION_EARLY"); return !(v && v[0] == '0'); }();
@@ -976,7 +1095,7 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
     else if (per_block == 8) launch_decode_8bit<HD, VD, 1, FRB_INT8>(map_k, map_v, p, stream);                                \
     else if (codes == FRB_E4M3) launch_decode_8bit<HD, VD, 2, FRB_E4M3>(map_k, map_v, p, stream);                             \
     else launch_decode_8bit<HD, VD, 2, FRB_INT8>(map_k, map_v, p, stream);                                                    \
-    launch_dependent(attention_decode_8bit_join_kernel<VD>, join_grid, join_block, 0, stream, p, shares)
+    launch_dependent_resident(early ? 4 : 1, attention_decode_8bit_join_kernel<VD>, join_grid, join_block, 0, stream, p, shares)
     FRB_8BIT_SIZES("attention_decode_8bit", head_dim, v_dim, FRB_LAUNCH_DECODE8);
 #undef FRB_LAUNCH_DECODE8
     FRB_RETURN_LAUNCH("attention_decode_8bit");

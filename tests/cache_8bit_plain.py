@@ -48,19 +48,20 @@ def numbers(codes):
 
 def attend(q, k, v, position, *, scale, group, maps=1, window=None, chunk=None, keep_first=0, slopes=None, sinks=None, softcap=None):
     """One token's attention in float64: q [heads, dim], k [kv_heads, keys, dim], v [v_heads, keys, vdim] (the sequence's rows from key 0
-    on).  Returns out [heads, vdim] (each map's own), the same with |v|, the largest weight times value of every head, and the largest
-    sum |q k| scale: what bounds on the error are made of."""
+    on).  Returns out [heads, vdim] (each map's own), the same with |v|, the largest weight times value of every head, the largest
+    sum |q k| scale, and the largest |q| times the largest sum |k| times scale: what bounds on the error are made of."""
     keys = np.arange(position + 1)
     lo = max(0, position - window + 1) if window else 0
     if chunk:
         lo = max(lo, position // chunk * chunk)
     seen = keys[(keys >= lo) | (keys < keep_first)]
     heads, vdim = q.shape[0], v.shape[-1]
-    out, size, top, reach = np.zeros((heads, vdim)), np.zeros((heads, vdim)), np.zeros(heads), np.zeros(heads)
+    out, size, top, reach, span = np.zeros((heads, vdim)), np.zeros((heads, vdim)), np.zeros(heads), np.zeros(heads), np.zeros(heads)
     for h in range(heads):
         kv = h // group
         s = k[kv][seen] @ q[h] * scale
         reach[h] = (np.abs(k[kv][seen]) @ np.abs(q[h])).max() * scale
+        span[h] = np.abs(q[h]).max() * np.abs(k[kv][seen]).sum(-1).max() * scale
         if softcap:
             s = softcap * np.tanh(s / softcap)
         if slopes is not None:
@@ -71,7 +72,7 @@ def attend(q, k, v, position, *, scale, group, maps=1, window=None, chunk=None, 
         rows = v[kv // maps][seen]
         out[h], size[h] = p @ rows / total, p @ np.abs(rows) / total
         top[h] = (p * np.abs(rows).max(-1)).max() / total
-    return out, size, top, reach
+    return out, size, top, reach, span
 
 
 def difference(out, lam, heads, kv_heads, eps, factor):
@@ -81,15 +82,18 @@ def difference(out, lam, heads, kv_heads, eps, factor):
     return o / np.sqrt((o * o).mean(-1, keepdims=True) + eps) * factor
 
 
-def output_bound(want, size, top, reach, position, *, dim, group, maps=1, softcap=None, slopes=None, lam=None, eps=None, factor=None,
+def output_bound(want, size, top, reach, span, position, *, dim, group, codes, maps=1, softcap=None, slopes=None, lam=None, eps=None, factor=None,
                  rounding=2.0 ** -11):
     """What one token's output (bfloat16) may be off by, and the value itself with two maps' difference taken; ``rounding``: of a weight.
 
-    Scores: exact products (float16 of 11 bits and codes of 8, or bfloat16) added in float32, up to 2^-23 of the terms' size a step, and a few
-    roundings of the score itself, of a slope's product and of a cap; twice that is the relative error of a weight over the sum.
+    Scores: exact products added in float32 (or integers), up to 2^-23 of the terms' size a step, and a few roundings of the score itself, of a
+    slope's product and of a cap; twice that is the relative error of a weight over the sum.  With ``codes`` (the type, for single
+    tokens) the queries are rounded: int8 to 16 bits, half a unit of 1/32512 of the head's largest entry; float8_e4m3fn to float16, half of
+    whose smallest step is 2^-25 in units in which the largest entry is 2^14 or more.
     Weights: their rounding, the hardware's exponential, sums of position + 1 terms in float32; a weight below 2^-22 of the largest has an
     absolute error instead.  Then the output's own rounding."""
-    score = 2.0 ** -23 * (dim + 16) * reach + (2.0 ** -20 * softcap if softcap else 0.0)
+    rounded = {None: 0.0, torch.int8: 0.5 / 32512, torch.float8_e4m3fn: 2.0 ** -39}[codes]
+    score = 2.0 ** -23 * (dim + 16) * reach + rounded * 1.001 * span + (2.0 ** -20 * softcap if softcap else 0.0)
     if slopes is not None:
         score = score + 2.0 ** -22 * slopes * position
     weight = rounding + 2.0 ** -16 + (position + 1) * 2.0 ** -26 + 4 * score[:, None]

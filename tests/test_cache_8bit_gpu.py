@@ -313,12 +313,12 @@ class Attended:
                 assert (got[i] == 0).all()
                 continue
             q = self.q[i].double().cpu().numpy().reshape(self.heads, self.dim)
-            want, size, top, reach = plain.attend(q, self.rows_of(i, self.k, self.ks), self.rows_of(i, self.v, self.vs), position,
+            want, size, top, reach, span = plain.attend(q, self.rows_of(i, self.k, self.ks), self.rows_of(i, self.v, self.vs), position,
                                                   scale=o["scale"], group=self.heads // self.kv_heads, maps=self.maps, window=o["window"],
                                                   chunk=o.get("chunk"), keep_first=o.get("keep_first", 0), softcap=o.get("softcap"), **arrays)
             d = o.get("difference")
             more = dict(lam=float(d["lam"].double()), eps=d["eps"], factor=d["factor"]) if d else {}
-            want, bound = plain.output_bound(want, size, top, reach, position, dim=self.dim, group=self.heads // self.kv_heads, maps=self.maps,
+            want, bound = plain.output_bound(want, size, top, reach, span, position, dim=self.dim, codes=self.dtype, group=self.heads // self.kv_heads, maps=self.maps,
                                              softcap=o.get("softcap"), slopes=arrays["slopes"], **more)
             off = np.abs(got[i] - want)
             assert np.isfinite(got[i]).all() and (off <= bound).all(), (i, position, float((off / bound).max()))
@@ -470,7 +470,7 @@ def test_attention_of_sequences_and_pages_that_are_not_there():
     keep[2 * PAGE:3 * PAGE] = keep[5 * PAGE:6 * PAGE] = False
     keep[701:] = False
     k, v = a.rows_of(0, a.k, a.ks)[:, keep], a.rows_of(0, a.v, a.vs)[:, keep]
-    want, size, _, _ = plain.attend(q, k, v, int(keep.sum()) - 1, scale=0.125, group=3)
+    want, size, *_ = plain.attend(q, k, v, int(keep.sum()) - 1, scale=0.125, group=3)
     assert (np.abs(got.double().cpu().numpy().reshape(6, 64) - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * size).all()
     a.table[row] = -1
     a.run()

@@ -69,11 +69,11 @@ class Checker:
             places = range(n) if n <= 12 else sorted({0, 1, n // 3, n // 2, n - 2, n - 1})
             for place in places:
                 pos = start + place
-                want, size, top, reach = plain.attend(q[at + place], k, v, pos, scale=part.softmax_scale, group=group, maps=part.maps,
+                want, size, top, reach, span = plain.attend(q[at + place], k, v, pos, scale=part.softmax_scale, group=group, maps=part.maps,
                                                       window=int(part.window) if part.window else None, chunk=part.chunk, keep_first=part.keep_first,
                                                       slopes=slopes, sinks=sinks, softcap=part.softcap)
                 # prompts: weights in bfloat16 (2^-8); the softmax's sum is of the unrounded ones
-                want, bound = plain.output_bound(want, size, top, reach, pos, dim=part.head_dim, group=part.num_heads // part.num_kv_heads,
+                want, bound = plain.output_bound(want, size, top, reach, span, pos, dim=part.head_dim, codes=None if prompt else line.keys.dtype, group=part.num_heads // part.num_kv_heads,
                                                  maps=part.maps, softcap=part.softcap, slopes=slopes, rounding=2.0 ** -8 if prompt else 2.0 ** -11,
                                                  **(dict(lam=float(part.lam.double()), eps=part.diff_eps, factor=1 - part.diff) if part.maps == 2 else {}))
                 if gates is not None:
