@@ -44,8 +44,12 @@ __device__ __forceinline__ uint32_t four_codes(float4 x, float factor, int codes
             : "=r"(out) : "f"(a), "f"(b), "f"(c), "f"(d));
         return out;
     }
-    const auto code = [](float v) { return (uint32_t)max(-127, min(127, __float2int_rn(v))) & 0xffu; };
-    return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
+    uint32_t out;                     // (products of up to 127 (1 + 2^-23): none is rounded to another code than -127 .. 127)
+    asm("{\n\t.reg .b32 upper;\n\t"
+        "cvt.pack.sat.s8.s32.b32 upper, %4, %3, 0;\n\t"
+        "cvt.pack.sat.s8.s32.b32 %0, %2, %1, upper;\n\t}"
+        : "=r"(out) : "r"(__float2int_rn(a)), "r"(__float2int_rn(b)), "r"(__float2int_rn(c)), "r"(__float2int_rn(d)));
+    return out;
 }
 
 // The codes of two halves of a register as float16 pairs: every code of either type is a float16 number.

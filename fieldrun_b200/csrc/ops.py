@@ -75,7 +75,7 @@ _SIGNATURES = {
     "frb_expert_gemm_tc": "pipippppiipiiipif",
     "frb_gather_rows_bf16": "pppii",
     "frb_attention_prefill_tc": "pippipippipppppiiifippipf" "iiii",
-    "frb_qkv_prepare_8bit": "pippif" "ppi" "pppii" "ppppp" "ii" "iiiiiiiii" "i" "pfi" "i",
+    "frb_qkv_prepare_8bit": "pippif" "ppi" "pppii" "ppppp" "ii" "iiiiiiiii" "i" "pfi" "ip",
     "frb_cache_read_8bit": "ppppi" "ipii" "ppi" "pppi" "pp" "iiii",
     "frb_attention_decode_8bit": "pppppi" "ipii" "pp" "ppp" "iiiiii" "f" "iii" "ii" "pp" "f" "pff" "p",
     "frb_attention_pair_tc": "pippi" "pippi" "ppppp" "iiiifiif" "pffp",
@@ -1533,6 +1533,7 @@ _WAIT_CODES = {
     6: "expert products: the MMA thread waiting for the epilogue to have read the accumulators",
     4: "one-token attention: waiting for a page's copy",
     7: "one-token attention over 8-bit pages: waiting for a page's copy",
+    9: "rows for 8-bit pages: waiting for a row's copy",
     8: "one-token attention over 8-bit pages: a sequence has more keys than the launch was sized for (max_chunks); keys were left out",
     5: "one-token attention: a sequence has more keys than the launch was sized for (max_chunks); keys were left out",
     21: "weight stream: the producer waiting for a free stage",
@@ -1824,7 +1825,7 @@ def qkv_prepare_8bit(qkv: torch.Tensor, q_weight: Optional[torch.Tensor], k_weig
     _call("frb_qkv_prepare_8bit", at[0], _code(qkv.dtype), at[1], at[2], _code(wdtype), float(eps), at[3], at[4], table_positions, at[5], at[6],
           at[7], *page_table.shape, *at[8:13], store[0], store[1], tokens, num_heads, num_kv_heads, num_v_heads, head_dim, v_dim, rotary_dim,
           int(interleaved), int(per_head), int(tables_final), at[13], float(q_temp[0]) if q_temp else 0.0, int(q_temp[1]) if q_temp else 1,
-          int(values_from_keys))
+          int(values_from_keys), _ptr(tc_status(qkv.device)))
 
 
 def cache_read_8bit(k_pages: torch.Tensor, k_scales: torch.Tensor, v_pages: torch.Tensor, v_scales: torch.Tensor, page_table: torch.Tensor,

@@ -110,14 +110,14 @@ def test_entry_points_refuse_sizes_by_a_message():
     assert lib.frb_cache_read_8bit(*[None] * 4, 5, 1, None, 1, 1, None, None, 1, None, None, None, 1, None, None, 1, 1, 64, 64, None) == -1
     assert b"codes of type 5" in lib.frb_last_error()
     assert lib.frb_qkv_prepare_8bit(None, 0, None, None, 0, 1e-6, None, None, 0, None, None, None, 1, 1, *[None] * 5, 0, 1, 1, 2, 2, 2, 64, 64, 31, 0, 0, 0,
-                                    None, 0.0, 1, 0, None) == -1
+                                    None, 0.0, 1, 0, None, None) == -1
     assert b"rotary_dim 31" in lib.frb_last_error()
     assert lib.frb_qkv_prepare_8bit(4, 0, None, None, 0, 1e-6, None, None, 0, None, None, None, 1, 1, *[None] * 5, 0, 1, 1, 2, 2, 2, 64, 64, 0, 0, 0, 0,
-                                    None, 0.0, 1, 0, None) == -1
-    assert b"whole group of four" in lib.frb_last_error()
+                                    None, 0.0, 1, 0, None, None) == -1
+    assert b"rows start on 16 bytes" in lib.frb_last_error()
     assert lib.frb_qkv_prepare_8bit(None, 0, None, None, 0, 1e-6, None, None, 0, None, None, None, 1, 1, *[None] * 5, 0, 1, 1, 900, 2, 2, 64, 64, 0, 0, 0, 0,
-                                    None, 0.0, 1, 0, None) == -1
-    assert b"more than 256 warps" in lib.frb_last_error()
+                                    None, 0.0, 1, 0, None, None) == -1
+    assert b"more than 200 KB" in lib.frb_last_error()
 
 
 # ------------------------------------------------------------------------------------------------ pages and tables
