@@ -43,6 +43,7 @@
 // for the smaller heads, 168).
 #define D8_RESIDENT(HD, VD, NT) ((NT) == 2 ? 2 : (HD) + (VD) <= 128 ? 4 : 3)
 #define D8_CHUNK_PAGES 4               // a chunk is 256 keys
+#define D8_LEAD 2                      // pages that a run costs as much time as, beside its own
 #define D8_RAISE 8.0f                  // the running maximum follows a page's maximum only beyond this margin (in units of log2)
 #define D8_STATUS_WAIT 7               // a wait gave up
 #define D8_STATUS_TOO_LONG 8           // a sequence has more keys than the launch was sized for
@@ -706,10 +707,13 @@ __device__ __forceinline__ int times_repeated(const Decode8Params& p, int b) {  
     return n;
 }
 
-// A row's pages in the line, for one key head: each page as many times as the row is repeated, so that a piece's pages are done for all of
-// those rows alike and repeated rows come out the same to the last bit.  Zero for a row that repeats another.
+// A row's places in the line, for one key head: D8_LEAD in front, since a run costs time beside its pages, and its pages, all of them as many
+// times as the row is repeated, so that a piece's pages are done for all of those rows alike and repeated rows come out the same to the
+// last bit.  Zero for a row that repeats another or has no pages.
 __device__ __forceinline__ int places_of(const Decode8Params& p, int b) {
-    return b >= p.num_seqs || repeats(p, b) ? 0 : sight_of(p, b).count * times_repeated(p, b);
+    if (b >= p.num_seqs || repeats(p, b)) return 0;
+    const int count = sight_of(p, b).count;
+    return count > 0 ? (count + D8_LEAD) * times_repeated(p, b) : 0;
 }
 
 // A run: the pages [begin, end) in sight of one key head's, for one row (none where a piece lies within the repetitions of a page).  Its
@@ -727,10 +731,28 @@ struct RunOrder {
     int before, places;                // places before the row, and of one of its key heads
 
     __device__ __forceinline__ bool next(const Decode8Params& p, Run& run, int per_tile) {
-        if (at >= piece_end) return false;
-        if (copy == times) {                                                  // on to the next key head, or the next row that has pages
+        for (;;) {
+            if (at >= piece_end) return false;
+            const int pair = (at - before) / places, pair_at = before + pair * places, pages_at = pair_at + D8_LEAD * times;
+            const int run_end = min(piece_end, pair_at + places);
+            if (copy < times && run_end > pages_at) {
+                const int group = p.num_heads / p.num_kv_heads, tile = pair % p.head_tiles;
+                run.sight = sight_of(p, seq);
+                run.row = seq + copy;
+                run.slot = p.seq_slot[seq];
+                run.kvh = pair / p.head_tiles;
+                run.first_head = run.kvh * group + tile * per_tile;
+                run.heads = min(per_tile, group - tile * per_tile);
+                run.begin = (max(at - pages_at, 0) + times - 1) / times;
+                run.end = (run_end - pages_at + times - 1) / times;
+                run.room = at / length - pages_at / length;                   // (the piece's number, and that of the first with pages)
+                run.runs = run.room == 0 ? (pair_at + places - 1) / length - pages_at / length + 1 : 0;
+                ++copy;
+                return true;
+            }
+            // on to the next key head, or the next row that has pages
             copy = 0;
-            at = min(piece_end, before + ((at - before) / places + 1) * places);
+            at = run_end;
             if (at < piece_end && at == before + p.num_kv_heads * p.head_tiles * places) {
                 before = at;
                 seq += times;
@@ -738,22 +760,7 @@ struct RunOrder {
                 if (seq >= p.num_seqs) at = piece_end;                        // (not with tables that stay as they are)
                 else times = times_repeated(p, seq);
             }
-            if (at >= piece_end) return false;
         }
-        const int pair = (at - before) / places, pair_at = before + pair * places, run_end = min(piece_end, pair_at + places);
-        const int group = p.num_heads / p.num_kv_heads, tile = pair % p.head_tiles;
-        run.sight = sight_of(p, seq);
-        run.row = seq + copy;
-        run.slot = p.seq_slot[seq];
-        run.kvh = pair / p.head_tiles;
-        run.first_head = run.kvh * group + tile * per_tile;
-        run.heads = min(per_tile, group - tile * per_tile);
-        run.begin = (at - pair_at + times - 1) / times;
-        run.end = (run_end - pair_at + times - 1) / times;
-        run.room = at / length - pair_at / length;
-        run.runs = at == pair_at ? (pair_at + places - 1) / length - pair_at / length + 1 : 0;
-        ++copy;
-        return true;
     }
 };
 
@@ -779,7 +786,7 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
     for (int b = threadIdx.x; b < p.num_seqs; b += D8_THREADS) {
         const int places = places_of(p, b);
         total += places;
-        longest = max(longest, places);
+        longest = max(longest, places);                     // (more than its pages: the lead in front counts, too)
     }
     if (warp * 32 < p.num_seqs) {
         total = __reduce_add_sync(0xffffffffu, total);
