@@ -70,6 +70,7 @@ struct Decode8Params {
     int max_chunks;            // partial results that there is room for per (sequence, head); a sequence has at most four times as many pages
     int head_tiles;            // tiles of query heads per key head
     int pieces;                // warps that the line of pages is cut for; 0: chunks
+    int whole;                 // a key head's pages are one piece's, since there is no room for partial results
     int early;                 // copies go out before the kernel before this one has ended (0: FIELDRUN_B200_ATTENTION_EARLY=0)
 };
 
@@ -730,12 +731,13 @@ struct RunOrder {
     int seq, times, copy;              // the row, how often it is there, which one is next
     int before, places;                // places before the row, and of one of its key heads
 
+    // (Cut between key heads only, a piece has those that begin in it.)
     __device__ __forceinline__ bool next(const Decode8Params& p, Run& run, int per_tile) {
         for (;;) {
             if (at >= piece_end) return false;
             const int pair = (at - before) / places, pair_at = before + pair * places, pages_at = pair_at + D8_LEAD * times;
-            const int run_end = min(piece_end, pair_at + places);
-            if (copy < times && run_end > pages_at) {
+            const int run_end = p.whole ? pair_at + places : min(piece_end, pair_at + places);
+            if (copy < times && run_end > pages_at && !(p.whole && at != pair_at)) {
                 const int group = p.num_heads / p.num_kv_heads, tile = pair % p.head_tiles;
                 run.sight = sight_of(p, seq);
                 run.row = seq + copy;
@@ -747,6 +749,7 @@ struct RunOrder {
                 run.end = (run_end - pages_at + times - 1) / times;
                 run.room = at / length - pages_at / length;                   // (the piece's number, and that of the first with pages)
                 run.runs = run.room == 0 ? (pair_at + places - 1) / length - pages_at / length + 1 : 0;
+                if (p.whole) run.room = run.runs = 0;
                 ++copy;
                 return true;
             }
@@ -764,7 +767,7 @@ struct RunOrder {
     }
 };
 
-#define D8_MIN_ROOM 5          // partial results that a line cut into pieces needs room for, per (sequence, head)
+#define D8_MIN_ROOM 4          // partial results that a line cut anywhere needs room for, per (sequence, head)
 
 template <int HD, int VD, int NT, int CODES>
 __global__ void __launch_bounds__(D8_THREADS, D8_RESIDENT(HD, VD, NT))
@@ -799,7 +802,8 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
     for (int w = 0; w < D8_WARPS; ++w) { total += sums[w]; longest = max(longest, tops[w]); }
     total *= heads_in_line;
     RunOrder order;
-    order.length = max(1, max((total + p.pieces - 1) / p.pieces, (longest + p.max_chunks - 4) / (p.max_chunks - 3)));
+    order.length = max(1, (total + p.pieces - 1) / p.pieces);
+    if (!p.whole) order.length = max(order.length, (longest + p.max_chunks - 3) / (p.max_chunks - 2));
     // neighbouring pieces go to different SMs: warps without a piece are then spread over all of them
     order.at = (int)min((long long)total, (long long)(warp * (int)gridDim.x + (int)blockIdx.x) * order.length);
     order.piece_end = min(total - order.at, order.length) + order.at;
@@ -951,7 +955,7 @@ __device__ __forceinline__ Joined joined_parts(const Decode8Params& p, size_t ro
             const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (row0 + c) * 2);
             part[u] = {ml.x, ml.y, p.part_o[(row0 + c) * VD + d]};
         }
-        if (c0 == share) count = p.pieces > 0 ? min((int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1], p.max_chunks) : chunks;
+        if (c0 == share) count = p.whole ? 1 : p.pieces > 0 ? min((int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1], p.max_chunks) : chunks;
         float top = all.top;
 #pragma unroll
         for (int u = 0; u < AT_ONCE; ++u) {
@@ -1081,11 +1085,13 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
     p.chunk = chunk; p.keep_first = window > 0 ? keep_first : 0; p.max_pages = max_pages; p.num_slots = num_slots; p.num_pages = num_pages;
     p.num_heads = num_heads; p.num_kv_heads = num_kv_heads; p.v_heads = v_heads; p.num_seqs = num_seqs; p.max_chunks = max_chunks;
     p.head_tiles = head_tiles;
-    // Chunks where two waves of blocks hold all that there may be, or where a key head's partial results have no room for pieces.  (Measured
-    // on a B200 with 8 key heads of 128, microseconds of both kernels, chunks | pieces: CHOICE)
-    const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks, resident = (long long)D8_RESIDENT(head_dim, v_dim, per_block / 8) * frb_sm_count();
-    const bool by_piece = max_chunks >= D8_MIN_ROOM && chunks > 2 * resident && chunks * D8_CHUNK_PAGES < (1ll << 30);
-    p.pieces = max_pieces > 0 ? (max_chunks >= D8_MIN_ROOM && chunks * D8_CHUNK_PAGES < (1ll << 30) ? max_pieces : 0) : by_piece ? (int)resident * D8_WARPS : 0;
+    // Chunks where two waves of blocks hold all that there may be.  (Measured on a B200 with 8 key heads of 128, microseconds of both
+    // kernels, chunks | pieces: CHOICE)
+    const int resident = D8_RESIDENT(head_dim, v_dim, per_block / 8) * frb_sm_count();
+    const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks;
+    const bool countable = chunks * D8_CHUNK_PAGES < (1ll << 30);
+    p.pieces = !countable ? 0 : max_pieces > 0 ? max_pieces : chunks > 2ll * resident ? resident * D8_WARPS : 0;
+    p.whole = p.pieces > 0 && max_chunks < D8_MIN_ROOM;
     static const int early = [] { const char* v = getenv("FIELDRUN_B200_ATTENTION_EARLY"); return !(v && v[0] == '0'); }();
     p.early = early;
     CUtensorMap map_k, map_v;
@@ -1107,3 +1113,5 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
 #undef FRB_LAUNCH_DECODE8
     FRB_RETURN_LAUNCH("attention_decode_8bit");
 }
+
+FRB_API int frb_attention_decode_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_attention_decode_8bit, packed, stream); }

@@ -522,3 +522,7 @@ FRB_API int frb_cache_read_8bit(const void* k_codes, const float* k_scales, cons
 #undef FRB_LAUNCH_READ8
     FRB_RETURN_LAUNCH("cache_read_8bit");
 }
+
+FRB_API int frb_qkv_prepare_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_qkv_prepare_8bit, packed, stream); }
+
+FRB_API int frb_cache_read_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_cache_read_8bit, packed, stream); }

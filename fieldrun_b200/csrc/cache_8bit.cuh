@@ -10,6 +10,9 @@
 
 #include <cuda_fp16.h>
 
+#include <cstring>
+#include <tuple>
+
 #include "common.cuh"
 
 // Types of the codes.
@@ -95,3 +98,23 @@ __device__ __forceinline__ float4 four_values(uint32_t w, float scale, int codes
         else if (head_dim == 128 && v_dim == 128) { LAUNCH(128, 128); }                                                       \
         else { frb_set_error("%s: head_dim %d with value heads of %d is not built", what, head_dim, v_dim); return -1; }      \
     } while (0)
+
+// Calls an entry point with its arguments read one after another from `packed`, each at its type's alignment, as they lie in a C struct of
+// them.  (A call of thirty arguments costs the interpreter four microseconds argument by argument and one as a struct.)
+template <typename... Args>
+inline int call_packed(int (*entry)(Args...), const void* packed, cudaStream_t stream) {
+    size_t at = 0;
+    const auto next = [&](auto* type) {
+        typedef std::remove_pointer_t<decltype(type)> T;
+        if constexpr (std::is_same_v<T, cudaStream_t>) return stream;             // the last one
+        else {
+            at = (at + alignof(T) - 1) / alignof(T) * alignof(T);
+            T value;
+            memcpy(&value, static_cast<const char*>(packed) + at, sizeof(T));
+            at += sizeof(T);
+            return value;
+        }
+    };
+    const std::tuple<Args...> args{next(static_cast<Args*>(nullptr))...};         // (braces: from the first to the last)
+    return std::apply(entry, args);
+}

@@ -7,6 +7,7 @@ be built or loaded, or a tensor is not on a CUDA device, the call raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -100,6 +101,11 @@ _SIGNATURES = {
 _CTYPE = {"p": _P, "i": _I, "f": _F, "l": _L}
 
 
+# Entry points that also take their arguments as one C struct (``<name>_packed``), for which the interpreter needs a quarter of the time.
+_PACKED = {name: struct.Struct("@" + _SIGNATURES[name].replace("p", "P"))
+           for name in ("frb_qkv_prepare_8bit", "frb_cache_read_8bit", "frb_attention_decode_8bit")}
+
+
 class KernelError(RuntimeError):
     pass
 
@@ -148,6 +154,10 @@ def prepare(groups) -> None:
             fn = getattr(lib, name)
             fn.restype = _I
             fn.argtypes = [_CTYPE[c] for c in _SIGNATURES[name]] + [_P]
+            if name in _PACKED:
+                fn = getattr(lib, name + "_packed")
+                fn.restype = _I
+                fn.argtypes = [ctypes.c_char_p, _P]
             _FUNCTIONS[name] = fn
         _LIBS[group], _LIB_PATHS[group] = lib, paths[group]
 
@@ -272,7 +282,11 @@ def _call(name: str, *args) -> None:
     global _LAUNCHES
     fn = _FUNCTIONS.get(name)
     if fn is None:
-        fn = getattr(library(_GROUP_OF[name]), name)
+        library(_GROUP_OF[name])
+        fn = _FUNCTIONS.get(name) or getattr(library(_GROUP_OF[name]), name)
+    packer = _PACKED.get(name)
+    if packer is not None:
+        args = (packer.pack(*args),)
     if _TIMINGS is not None:
         with timed(name[4:]):
             status = fn(*args, _stream())
@@ -1756,7 +1770,7 @@ def _addresses(*tensors: Optional[torch.Tensor]) -> list:
     index, found = None, []
     for t in tensors:
         if t is None:
-            found.append(None)
+            found.append(0)
             continue
         place = t.get_device()
         if place != index or not t.is_contiguous():
@@ -1890,9 +1904,10 @@ def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torc
     rows = seqs * num_heads * max_chunks
     if part_o.numel() < rows * v_dim or part_ml.numel() < rows * 2:
         raise KernelError(f"room for {part_o.numel()} partial outputs and {part_ml.numel()} maxima and sums, {rows * v_dim} and {rows * 2} are needed")
-    lam, eps, factor = _difference_args(difference, maps)
-    if lam is not None:
-        _addresses(difference["lam"])
+    lam, eps, factor = 0, 0.0, 0.0
+    if difference is not None:
+        _want(difference["lam"], torch.float32, "lambda")
+        (lam,), eps, factor = _addresses(difference["lam"]), float(difference["eps"]), float(difference["factor"])
     _call("frb_attention_decode_8bit", *at[:5], store[0], store[1], at[5], *page_table.shape, *at[6:11], seqs, num_heads, num_kv_heads,
           num_kv_heads // maps, head_dim, v_dim, float(scale), window, chunk, keep_first, max_chunks, int(pieces or 0), at[11], at[12],
           float(softcap or 0.0), lam, eps, factor, _ptr(tc_status(q.device)))

@@ -371,6 +371,20 @@ def test_attention_long_sequences_and_the_split():
         Attended([16000, 3, 9000], E4M3, heads=12, kv_heads=2, dim=128, pieces=pieces).run().check()
 
 
+@pytest.mark.parametrize("chunks", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("pieces", [None, 1, 7, 200])
+def test_attention_many_short_sequences(chunks, pieces):
+    # partial results have little room or none: the line is cut between key heads only, or into few pieces a head
+    positions = [-1 if i % 11 == 5 else (257 * i * i + 63 * (i % 3)) % (256 * chunks) for i in range(90)]
+    a = Attended(positions, E4M3, heads=24, kv_heads=12, dim=64, pieces=pieces, max_chunks=chunks).run().check()
+    index = [0, 1, 1, 1, 40, 41, 41, 89, 89]                       # with rows repeated
+    a.positions = [positions[i] for i in index]
+    a.q, a.slots, a.out = a.q[index].contiguous(), a.slots[index].contiguous(), a.out[index].contiguous()
+    a.run().check()
+    assert torch.equal(a.out[1], a.out[2]) and torch.equal(a.out[2], a.out[3]) and torch.equal(a.out[5], a.out[6]) and torch.equal(a.out[7], a.out[8])
+    Attended(positions[:40], INT8, heads=18, kv_heads=1, dim=128, pieces=pieces, max_chunks=chunks, window=150, keep_first=70).run().check()
+
+
 def test_attention_sharp_scores():
     # one key has nearly all the weight, at any place, and scores of hundreds: the running maximum moves by much
     for seed in range(4):
