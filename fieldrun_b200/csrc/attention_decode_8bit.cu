@@ -74,12 +74,6 @@ struct Decode8Params {
     int early;                 // copies go out before the kernel before this one has ended (0: FIELDRUN_B200_ATTENTION_EARLY=0)
 };
 
-// The position that the kernels work with: none (-1) for a slot that does not exist.
-__device__ __forceinline__ int held_position(const Decode8Params& p, int b) {
-    const int slot = p.seq_slot[b];
-    return slot >= 0 && slot < p.num_slots ? min(p.seq_pos[b], p.max_pages * FRB_PAGE - 1) : -1;
-}
-
 // The pages that hold a key which a sequence's token may see: those of the first tokens that stay visible, then the window's.
 struct Sight {
     int lo_key, hi_key, kept, first_page, count;
@@ -87,9 +81,10 @@ struct Sight {
     __device__ __forceinline__ int number(int n) const { return n < kept ? n : first_page + n - kept; }     // the n-th one's place in the sequence
 };
 
-__device__ __forceinline__ Sight sight_of(const Decode8Params& p, int b) {
+// of a token at `position` of `slot`; a slot that does not exist has none
+__device__ __forceinline__ Sight sight_from(const Decode8Params& p, int slot, int position) {
     Sight s;
-    s.hi_key = held_position(p, b);
+    s.hi_key = slot >= 0 && slot < p.num_slots ? min(position, p.max_pages * FRB_PAGE - 1) : -1;
     s.lo_key = first_visible_key(max(s.hi_key, 0), p.window, p.chunk);
     s.first_page = s.lo_key / FRB_PAGE;
     s.kept = kept_runs(p.keep_first, FRB_PAGE, s.first_page);
@@ -98,6 +93,8 @@ __device__ __forceinline__ Sight sight_of(const Decode8Params& p, int b) {
     s.count = s.cut ? D8_CHUNK_PAGES * p.max_chunks : pages;
     return s;
 }
+
+__device__ __forceinline__ Sight sight_of(const Decode8Params& p, int b) { return sight_from(p, p.seq_slot[b], p.seq_pos[b]); }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm(
@@ -717,6 +714,25 @@ __device__ __forceinline__ int places_of(const Decode8Params& p, int b) {
     return count > 0 ? (count + D8_LEAD) * times_repeated(p, b) : 0;
 }
 
+// The same of 32 rows, b0 on, a lane each; both loads of every row at once.
+__device__ __forceinline__ int places_of_rows(const Decode8Params& p, int b0, int lane) {
+    const int b = b0 + lane;
+    const bool there = b < p.num_seqs;
+    const int slot = there ? p.seq_slot[b] : -1, position = there ? p.seq_pos[b] : -1;
+    const bool beside = lane == 0 ? b0 > 0 : lane == 31 && b + 1 < p.num_seqs;             // the rows around these
+    const int other = lane == 0 ? b0 - 1 : b + 1, other_slot = beside ? p.seq_slot[other] : -1, other_position = beside ? p.seq_pos[other] : -1;
+    const int left_slot = __shfl_up_sync(0xffffffffu, slot, 1), left_position = __shfl_up_sync(0xffffffffu, position, 1);
+    const bool repeat = there && (lane > 0 ? slot == left_slot && position == left_position : beside && slot == other_slot && position == other_position);
+    const unsigned repeats_left = __ballot_sync(0xffffffffu, repeat);
+    const int next_slot = __shfl_sync(0xffffffffu, other_slot, 31), next_position = __shfl_sync(0xffffffffu, other_position, 31);
+    const int count = there && !repeat ? sight_from(p, slot, position).count : 0;
+    if (count == 0) return 0;
+    const unsigned behind = lane < 31 ? repeats_left >> (lane + 1) : 0u;
+    int times = __ffs(~behind);
+    if (lane + times == 32 && b0 + 32 < p.num_seqs && slot == next_slot && position == next_position) times = times_repeated(p, b);
+    return (count + D8_LEAD) * times;
+}
+
 // A run: the pages [begin, end) in sight of one key head's, for one row (none where a piece lies within the repetitions of a page).  Its
 // partial result is number `room` of the (row, head)'s; the first run's warp also leaves the number of all of them, in the last place's sum.
 struct Run {
@@ -767,6 +783,7 @@ struct RunOrder {
     }
 };
 
+#define D8_ROW_GROUPS 64       // (two for a lane)
 #define D8_MIN_ROOM 4          // partial results that a line cut anywhere needs room for, per (sequence, head)
 
 template <int HD, int VD, int NT, int CODES>
@@ -776,31 +793,46 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
     typedef WarpTiles<HD, VD> Tiles;
     extern __shared__ uint8_t dynamic[];
     __shared__ uint64_t bars[2 * D8_WARPS];
-    __shared__ int sums[D8_WARPS], tops[D8_WARPS];
+    __shared__ int sums[D8_ROW_GROUPS], tops[D8_WARPS];
     __shared__ Run runs[D8_WARPS][2];
     __shared__ int failed;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int heads_in_line = p.num_kv_heads * p.head_tiles;
     uint8_t* base = begin_block<HD, VD>(dynamic, bars, &failed);
 
-    // The line's length, and that of a piece: a warp's share, at least as many places that a key head's pages lie in no more pieces than there
-    // is room for partial results (less one, where their number is left).
-    int total = 0, longest = 0;
-    for (int b = threadIdx.x; b < p.num_seqs; b += D8_THREADS) {
-        const int places = places_of(p, b);
-        total += places;
-        longest = max(longest, places);                     // (more than its pages: the lead in front counts, too)
+    // The line's length, from those of its rows in up to D8_ROW_GROUPS groups.
+    const int group_steps = (p.num_seqs + 32 * D8_ROW_GROUPS - 1) / (32 * D8_ROW_GROUPS), groups = (p.num_seqs + 32 * group_steps - 1) / (32 * group_steps);
+    int longest = 0;
+    for (int i = warp; i < groups; i += D8_WARPS) {
+        int sum = 0;
+        for (int s = 0; s < group_steps; ++s) {
+            const int places = places_of_rows(p, 32 * (i * group_steps + s), lane);
+            sum += places;
+            longest = max(longest, places);                 // (more than its pages: the lead in front counts, too)
+        }
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) sums[i] = sum;
     }
-    if (warp * 32 < p.num_seqs) {
-        total = __reduce_add_sync(0xffffffffu, total);
-        longest = __reduce_max_sync(0xffffffffu, longest);
-    }
-    if (lane == 0) { sums[warp] = total; tops[warp] = longest; }
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) tops[warp] = longest;
     __syncthreads();
-    total = longest = 0;
+    longest = 0;
 #pragma unroll
-    for (int w = 0; w < D8_WARPS; ++w) { total += sums[w]; longest = max(longest, tops[w]); }
-    total *= heads_in_line;
+    for (int w = 0; w < D8_WARPS; ++w) longest = max(longest, tops[w]);
+    // a lane has two groups
+    const int even = 2 * lane < groups ? heads_in_line * sums[2 * lane] : 0, both = even + (2 * lane + 1 < groups ? heads_in_line * sums[2 * lane + 1] : 0);
+    const auto upto_lane = [&](int own) {                   // the lanes' sum up to and with this one
+        int to = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int left = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += left;
+        }
+        return to;
+    };
+    const int to_both = upto_lane(both), total = __shfl_sync(0xffffffffu, to_both, 31);
+    // A piece is a warp's share, at least as many places that a key head's pages lie in no more pieces than there is room for partial results
+    // (less one, where their number is left).
     RunOrder order;
     order.length = max(1, (total + p.pieces - 1) / p.pieces);
     if (!p.whole) order.length = max(order.length, (longest + p.max_chunks - 3) / (p.max_chunks - 2));
@@ -809,23 +841,24 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
     order.piece_end = min(total - order.at, order.length) + order.at;
     // the row that the piece begins in
     order.seq = order.before = order.places = 0;
-    for (int b0 = 0, upto = 0; b0 < p.num_seqs && order.at < total; b0 += 32) {
-        const int own = heads_in_line * places_of(p, b0 + lane);
-        int to = own;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int left = __shfl_up_sync(0xffffffffu, to, o);
-            if (lane >= o) to += left;
+    if (order.at < total) {
+        const int pair = __ffs(__ballot_sync(0xffffffffu, order.at < to_both)) - 1;
+        int upto = __shfl_sync(0xffffffffu, to_both - both, pair);
+        const int first = __shfl_sync(0xffffffffu, even, pair), second = order.at >= upto + first;
+        if (second) upto += first;
+        const int b_end = min(p.num_seqs, (2 * pair + second + 1) * 32 * group_steps);
+        for (int b0 = (2 * pair + second) * 32 * group_steps; b0 < b_end; b0 += 32) {
+            const int own = heads_in_line * places_of_rows(p, b0, lane), to = upto_lane(own);
+            const unsigned here = __ballot_sync(0xffffffffu, order.at < upto + to);
+            if (here) {
+                const int found = __ffs(here) - 1;
+                order.seq = b0 + found;
+                order.before = upto + __shfl_sync(0xffffffffu, to - own, found);
+                order.places = __shfl_sync(0xffffffffu, own, found) / heads_in_line;
+                break;
+            }
+            upto += __shfl_sync(0xffffffffu, to, 31);
         }
-        const unsigned here = __ballot_sync(0xffffffffu, order.at >= upto + to - own && order.at < upto + to);
-        if (here) {
-            const int found = __ffs(here) - 1;
-            order.seq = b0 + found;
-            order.before = upto + __shfl_sync(0xffffffffu, to - own, found);
-            order.places = __shfl_sync(0xffffffffu, own, found) / heads_in_line;
-            break;
-        }
-        upto += __shfl_sync(0xffffffffu, to, 31);
     }
     if (order.places == 0) order.at = order.piece_end;
     order.copy = 0;
@@ -929,102 +962,148 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
 
 // ----------------------------------------------------------------------------- the join
 
-struct Joined { float top, sum, acc; };       // maximum (units of log2), sum and unnormalised output entry of some partial results
+// Maximum (units of log2), sum and unnormalised output entries of some partial results; a lane has N entries side by side.
+template <int N>
+struct Joined {
+    float top = -INFINITY, sum = 0.f, acc[N] = {};
+    __device__ __forceinline__ void add(float other_top, float other_sum, const float (&other)[N]) {
+        if (other_sum == 0.f) return;                 // no key (a sum that is not a number is none of these)
+        const float both = fmaxf(top, other_top), fa = sum == 0.f ? 0.f : exp2f(top - both), fb = exp2f(other_top - both);
+        top = both;
+        sum = sum * fa + other_sum * fb;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = acc[e] * fa + other[e] * fb;
+    }
+};
 
-__device__ __forceinline__ void add_joined(Joined& a, const Joined& b) {
-    if (b.sum == 0.f) return;                     // no key (a sum that is not a number is none of these)
-    if (a.sum == 0.f) { a = b; return; }
-    const float top = fmaxf(a.top, b.top), fa = exp2f(a.top - top), fb = exp2f(b.top - top);
-    a.top = top;
-    a.sum = a.sum * fa + b.sum * fb;
-    a.acc = a.acc * fa + b.acc * fb;
+template <int N>
+__device__ __forceinline__ void load_entries(const float* from, float (&to)[N]) {
+    if constexpr (N == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(from);
+        to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+    } else if constexpr (N == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(from);
+        to[0] = v.x; to[1] = v.y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) to[e] = from[e];
+    }
 }
 
-// Entry d of the partial results share, share + shares, ... of those that there are, in that order, eight at a time (all of their loads
-// before the first use, and the first eight's before their number is known: places without one are read and not used).
-template <int VD>
-__device__ __forceinline__ Joined joined_parts(const Decode8Params& p, size_t row0, int chunks, int d, int share, int shares) {
-    constexpr int AT_ONCE = 8;
-    Joined all = {-INFINITY, 0.f, 0.f};
+// The partial results share, share + shares, ... of a (row, head) in that order: a lane weighs one of 32, then the warp adds their entries.
+// The first entries are asked for before the number of partial results is known: places without one are read and not used.
+template <int N>
+__device__ __forceinline__ Joined<N> joined_parts(const Decode8Params& p, size_t row0, int chunks, int lane, int share, int shares) {
+    constexpr int AT_ONCE = 4, VD = 32 * N;
+    Joined<N> all;
+    const float* entries = p.part_o + row0 * VD + N * lane;
+    float first[AT_ONCE][N];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u)
+        if (share + u * shares < p.max_chunks) load_entries<N>(entries + (size_t)(share + u * shares) * VD, first[u]);
     int count = p.max_chunks;
-    for (int c0 = share; c0 < count; c0 += AT_ONCE * shares) {
-        Joined part[AT_ONCE];
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            const int c = min(c0 + u * shares, p.max_chunks - 1);
-            const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (row0 + c) * 2);
-            part[u] = {ml.x, ml.y, p.part_o[(row0 + c) * VD + d]};
-        }
+    for (int c0 = share; c0 < count; c0 += 32 * shares) {
+        const int mine = c0 + lane * shares;
+        const float2 ml = mine < p.max_chunks ? *reinterpret_cast<const float2*>(p.part_ml + (row0 + mine) * 2) : make_float2(0.f, 0.f);
         if (c0 == share) count = p.whole ? 1 : p.pieces > 0 ? min((int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1], p.max_chunks) : chunks;
-        float top = all.top;
-#pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-            if (c0 + u * shares >= count) part[u] = {-INFINITY, 0.f, 0.f};
-            top = fmaxf(top, part[u].sum != 0.f ? part[u].top : -INFINITY);
-        }
-        const float keep = all.sum == 0.f ? 0.f : exp2f(all.top - top);
+        const bool has = mine < count && ml.y != 0.f;
+        const unsigned some = __ballot_sync(0xffffffffu, has);
+        if (some == 0) continue;
+        const float top = fmaxf(all.top, warp_max(has ? ml.x : -INFINITY)), keep = all.sum == 0.f ? 0.f : exp2f(all.top - top);
+        const float weight = has ? exp2f(ml.x - top) : 0.f;
         all.top = top;
-        all.sum *= keep;
-        all.acc *= keep;
+        all.sum = all.sum * keep + warp_sum(has ? ml.y * weight : 0.f);
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-            if (part[u].sum != 0.f) {
-                const float f = exp2f(part[u].top - top);
-                all.sum += part[u].sum * f;
-                all.acc += part[u].acc * f;
+        for (int e = 0; e < N; ++e) all.acc[e] *= keep;
+        const int here = 32 - __clz(some);
+#pragma unroll 2
+        for (int u0 = 0; u0 < here; u0 += AT_ONCE) {
+            float part[AT_ONCE][N];
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                if (c0 == share && u0 == 0) {
+#pragma unroll
+                    for (int e = 0; e < N; ++e) part[u][e] = first[u][e];
+                } else if (u0 + u < here) load_entries<N>(entries + (size_t)(c0 + (u0 + u) * shares) * VD, part[u]);
             }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const float f = __shfl_sync(0xffffffffu, weight, u0 + u);
+                if (some >> (u0 + u) & 1)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) all.acc[e] += part[u][e] * f;
+            }
+        }
     }
     return all;
 }
 
-#define D8_JOIN_THREADS 512
+#define D8_JOIN_WARPS 8
 
-// grid (output heads / heads a block, sequence); a thread per value entry of a head, and `shares` times that where there are few heads.
-// A (sequence, head) without any key gives zeros, with a sink or not.
+// grid (8 / shares output heads, sequence): `shares` warps a (sequence, head), a lane VD / 32 entries side by side.  What bounds it is latency, or for many
+// sequences the partial results' bytes.  A (sequence, head) without any key gives zeros, with a sink or not.
 template <int VD>
-__global__ void __launch_bounds__(D8_JOIN_THREADS) attention_decode_8bit_join_kernel(Decode8Params p, int shares) {
+__global__ void __launch_bounds__(32 * D8_JOIN_WARPS) attention_decode_8bit_join_kernel(Decode8Params p, int shares) {
     let_next_kernel_start();
-    __shared__ Joined others[D8_JOIN_THREADS];
-    __shared__ float squares[D8_JOIN_THREADS / 32];
-    const int heads = p.lam ? p.num_heads / 2 : p.num_heads, b = blockIdx.y;
-    const int per_block = blockDim.x / (VD * shares), local = threadIdx.x / VD, d = threadIdx.x - local * VD, share = local % shares;
-    const int head = blockIdx.x * per_block + local / shares;
+    constexpr int N = VD / 32;
+    __shared__ Joined<N> others[D8_JOIN_WARPS][32];
+    const int heads = p.lam ? p.num_heads / 2 : p.num_heads, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int share = warp % shares, head = (blockIdx.x * D8_JOIN_WARPS + warp) / shares;
     const Sight sight = sight_of(p, b);                        // from the step's tables, which were there before the kernel before this one began
     wait_for_previous_kernel();
     if (sight.cut && threadIdx.x == 0) atomicExch(p.status, D8_STATUS_TOO_LONG);               // keys were left out
     const auto joined = [&](int query_head) {
-        Joined all = {-INFINITY, 0.f, 0.f};
+        Joined<N> all;
         if (sight.count > 0 && head < heads) {
             const int chunks = (sight.count + D8_CHUNK_PAGES - 1) / D8_CHUNK_PAGES;
-            all = joined_parts<VD>(p, ((size_t)b * p.num_heads + query_head) * p.max_chunks, chunks, d, share, shares);
+            all = joined_parts<N>(p, ((size_t)b * p.num_heads + query_head) * p.max_chunks, chunks, lane, share, shares);
         }
         if (shares > 1) {
             __syncthreads();                                   // (read from an earlier call)
-            others[threadIdx.x] = all;
+            others[warp][lane] = all;
             __syncthreads();
-            all = others[threadIdx.x - share * VD];
-            for (int s = 1; s < shares; ++s) add_joined(all, others[threadIdx.x + (s - share) * VD]);
+            if (share == 0)
+                for (int s = 1; s < shares; ++s) all.add(others[warp + s][lane].top, others[warp + s][lane].sum, others[warp + s][lane].acc);
         }
         return all;
     };
-    bf16* out = p.out + ((size_t)b * heads + head) * VD + d;
+    float result[N];
     if (p.lam) {
         const int group = p.num_heads / p.num_kv_heads, pair = head / group, first = 2 * pair * group + (head - pair * group);
-        const Joined one = joined(first), two = joined(first + group);
-        const float o = (one.sum == 0.f ? 0.f : one.acc / one.sum) - *p.lam * (two.sum == 0.f ? 0.f : two.acc / two.sum);
-        const float part = warp_sum(o * o);
-        if ((threadIdx.x & 31) == 0) squares[threadIdx.x >> 5] = part;
-        __syncthreads();
-        float ss = 0.f;
+        const Joined<N> one = joined(first), two = joined(first + group);
+        float squares = 0.f;
 #pragma unroll
-        for (int w = 0; w < VD / 32; ++w) ss += squares[local * (VD / 32) + w];
-        if (share == 0 && head < heads) *out = __float2bfloat16_rn(o / sqrtf(ss / (float)VD + p.diff_eps) * p.diff_factor);
-        return;
+        for (int e = 0; e < N; ++e) {
+            result[e] = (one.sum == 0.f ? 0.f : one.acc[e] / one.sum) - *p.lam * (two.sum == 0.f ? 0.f : two.acc[e] / two.sum);
+            squares += result[e] * result[e];
+        }
+        const float rms = sqrtf(warp_sum(squares) / (float)VD + p.diff_eps);
+#pragma unroll
+        for (int e = 0; e < N; ++e) result[e] = result[e] / rms * p.diff_factor;
+    } else {
+        Joined<N> all = joined(head);
+        if (p.sinks && all.sum != 0.f && head < heads) {
+            const float nothing[N] = {};
+            all.add(p.sinks[head] * 1.4426950408889634f, 1.f, nothing);      // a term of the denominator without a value
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) result[e] = all.sum == 0.f ? 0.f : all.acc[e] / all.sum;
     }
-    Joined all = joined(head);
     if (share != 0 || head >= heads) return;
-    if (p.sinks && all.sum != 0.f) add_joined(all, {p.sinks[head] * 1.4426950408889634f, 1.f, 0.f});      // a term of the denominator without a value
-    *out = __float2bfloat16_rn(all.sum == 0.f ? 0.f : all.acc / all.sum);
+    bf16* out = p.out + ((size_t)b * heads + head) * VD + N * lane;
+    if constexpr (N % 2 == 0) {
+        uint32_t two[N / 2];
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(result[e], result[e + 1]);
+            two[e / 2] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        if constexpr (N == 4) *reinterpret_cast<uint2*>(out) = make_uint2(two[0], two[1]);
+        else *reinterpret_cast<uint32_t*>(out) = two[0];
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = __float2bfloat16_rn(result[e]);
+    }
 }
 
 // A map over rows of `row` one-byte codes, boxes of 64 rows with the swizzle of the row's size.
@@ -1073,8 +1152,8 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
                   "attention_decode_8bit: a window of %d, chunks of %d, %d first tokens", window, chunk, keep_first);
     FRB_CHECK_ARG(!lam || (num_kv_heads == 2 * v_heads && !sinks), "attention_decode_8bit: two maps per head need two key heads a value head and no sinks");
     const auto aligned = [](const void* ptr, uintptr_t bytes) { return ((uintptr_t)ptr & (bytes - 1)) == 0; };
-    FRB_CHECK_ARG(aligned(q, 8) && aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_scales, 16) && aligned(v_scales, 16) && aligned(part_ml, 8),
-                  "attention_decode_8bit: queries start on 8 bytes, codes and scales on 16");
+    FRB_CHECK_ARG(aligned(q, 8) && aligned(k_codes, 16) && aligned(v_codes, 16) && aligned(k_scales, 16) && aligned(v_scales, 16) && aligned(part_o, 16) && aligned(part_ml, 8) && aligned(out, 8),
+                  "attention_decode_8bit: queries, maxima and outputs start on 8 bytes, codes, scales and partial outputs on 16");
     const int group = num_heads / num_kv_heads, per_block = group <= 8 ? 8 : 16, head_tiles = (group + per_block - 1) / per_block;
     FRB_CHECK_ARG(num_seqs <= 65535 && (long long)num_kv_heads * head_tiles <= 65535, "attention_decode_8bit: %d sequences of %d heads exceed the grid",
                   num_seqs, num_heads);
@@ -1099,10 +1178,10 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
                   map_code_rows(&map_v, v_codes, (uint64_t)num_pages * v_heads * FRB_PAGE, v_dim),
                   "attention_decode_8bit: head_dim %d with value heads of %d: cuTensorMapEncodeTiled failed or is not available", head_dim, v_dim);
     const int out_heads = lam ? num_heads / 2 : num_heads;
-    // the join: blocks of up to D8_JOIN_THREADS threads, on one head each while that leaves SMs idle
-    const int most_rows = D8_JOIN_THREADS / v_dim, shares = (long long)out_heads * num_seqs <= 4 * frb_sm_count() && max_chunks > 8 ? (most_rows < 4 ? most_rows : 4) : 1;
-    const int heads_a_block = shares > 1 ? 1 : (out_heads < most_rows ? out_heads : most_rows);
-    const dim3 join_grid((out_heads + heads_a_block - 1) / heads_a_block, num_seqs), join_block(v_dim * shares * heads_a_block);
+    // the join: more warps a (sequence, head) while that leaves SMs idle and each has some partial results
+    int shares = 1;
+    while (shares < D8_JOIN_WARPS && (long long)out_heads * num_seqs * shares <= 6 * frb_sm_count() && max_chunks >= 8 * shares) shares *= 2;
+    const dim3 join_grid((out_heads * shares + D8_JOIN_WARPS - 1) / D8_JOIN_WARPS, num_seqs), join_block(32 * D8_JOIN_WARPS);
 #define FRB_LAUNCH_DECODE8(HD, VD)                                                                                                  \
     if (per_block == 8 && codes == FRB_E4M3) launch_decode_8bit<HD, VD, 1, FRB_E4M3>(map_k, map_v, p, stream);                \
     else if (per_block == 8) launch_decode_8bit<HD, VD, 1, FRB_INT8>(map_k, map_v, p, stream);                                \

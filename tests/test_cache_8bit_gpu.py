@@ -508,6 +508,16 @@ def test_attention_refuses_too_little_room_and_tensors_in_pieces():
         a.run()
 
 
+@pytest.mark.parametrize("name", ["part_o", "part_ml", "out", "q", "ks", "vs", "k", "v"])
+def test_attention_refuses_tensors_off_their_boundaries(name):
+    a = Attended([100, 700], E4M3, heads=6, kv_heads=2, dim=64)
+    held = getattr(a, name)
+    wide = torch.empty(held.numel() + 1, dtype=held.dtype, device=DEV)
+    setattr(a, name, wide[1:].view(held.shape))
+    with pytest.raises(ops.KernelError, match="start on"):
+        a.run()
+
+
 def test_attention_more_keys_than_the_launch_is_sized_for_are_reported():
     a = Attended([100, 1000], E4M3, heads=6, kv_heads=2, dim=64)
     a.options["max_chunks"] = 2
