@@ -993,7 +993,7 @@ __device__ __forceinline__ void load_entries(const float* from, float (&to)[N]) 
 // The partial results share, share + shares, ... of a (row, head) in that order: a lane weighs one of 32, then the warp adds their entries.
 // The first entries are asked for before the number of partial results is known: places without one are read and not used.
 template <int N>
-__device__ __forceinline__ Joined<N> joined_parts(const Decode8Params& p, size_t row0, int chunks, int lane, int share, int shares) {
+__device__ __forceinline__ Joined<N> joined_parts(const Decode8Params& p, size_t row0, int pages, int lane, int share, int shares) {
     constexpr int AT_ONCE = 4, VD = 32 * N;
     Joined<N> all;
     const float* entries = p.part_o + row0 * VD + N * lane;
@@ -1005,7 +1005,8 @@ __device__ __forceinline__ Joined<N> joined_parts(const Decode8Params& p, size_t
     for (int c0 = share; c0 < count; c0 += 32 * shares) {
         const int mine = c0 + lane * shares;
         const float2 ml = mine < p.max_chunks ? *reinterpret_cast<const float2*>(p.part_ml + (row0 + mine) * 2) : make_float2(0.f, 0.f);
-        if (c0 == share) count = p.whole ? 1 : p.pieces > 0 ? min((int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1], p.max_chunks) : chunks;
+        if (c0 == share) count = p.whole ? min(pages, 1) : p.pieces == 0 ? (pages + D8_CHUNK_PAGES - 1) / D8_CHUNK_PAGES
+                               : pages > 0 ? min((int)p.part_ml[(row0 + p.max_chunks - 1) * 2 + 1], p.max_chunks) : 0;
         const bool has = mine < count && ml.y != 0.f;
         const unsigned some = __ballot_sync(0xffffffffu, has);
         if (some == 0) continue;
@@ -1016,7 +1017,7 @@ __device__ __forceinline__ Joined<N> joined_parts(const Decode8Params& p, size_t
 #pragma unroll
         for (int e = 0; e < N; ++e) all.acc[e] *= keep;
         const int here = 32 - __clz(some);
-#pragma unroll 2
+#pragma unroll 1
         for (int u0 = 0; u0 < here; u0 += AT_ONCE) {
             float part[AT_ONCE][N];
 #pragma unroll
@@ -1043,21 +1044,20 @@ __device__ __forceinline__ Joined<N> joined_parts(const Decode8Params& p, size_t
 // grid (8 / shares output heads, sequence): `shares` warps a (sequence, head), a lane VD / 32 entries side by side.  What bounds it is latency, or for many
 // sequences the partial results' bytes.  A (sequence, head) without any key gives zeros, with a sink or not.
 template <int VD>
-__global__ void __launch_bounds__(32 * D8_JOIN_WARPS) attention_decode_8bit_join_kernel(Decode8Params p, int shares) {
-    let_next_kernel_start();
+__global__ void __launch_bounds__(32 * D8_JOIN_WARPS, 3) attention_decode_8bit_join_kernel(Decode8Params p, int shares_log2) {
     constexpr int N = VD / 32;
     __shared__ Joined<N> others[D8_JOIN_WARPS][32];
     const int heads = p.lam ? p.num_heads / 2 : p.num_heads, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int share = warp % shares, head = (blockIdx.x * D8_JOIN_WARPS + warp) / shares;
+    const int shares = 1 << shares_log2, share = warp & (shares - 1), head = (int)(blockIdx.x * D8_JOIN_WARPS + warp) >> shares_log2;
     const Sight sight = sight_of(p, b);                        // from the step's tables, which were there before the kernel before this one began
     wait_for_previous_kernel();
+    // (The kernel after this one starts no earlier: were it attention once more, its blocks would take the SMs' room unevenly while pieces are
+    // still being done; 32 sequences of 4,096 keys took 59 us, with this 54.)
+    let_next_kernel_start();
     if (sight.cut && threadIdx.x == 0) atomicExch(p.status, D8_STATUS_TOO_LONG);               // keys were left out
     const auto joined = [&](int query_head) {
         Joined<N> all;
-        if (sight.count > 0 && head < heads) {
-            const int chunks = (sight.count + D8_CHUNK_PAGES - 1) / D8_CHUNK_PAGES;
-            all = joined_parts<N>(p, ((size_t)b * p.num_heads + query_head) * p.max_chunks, chunks, lane, share, shares);
-        }
+        if (head < heads) all = joined_parts<N>(p, ((size_t)b * p.num_heads + query_head) * p.max_chunks, sight.count, lane, share, shares);
         if (shares > 1) {
             __syncthreads();                                   // (read from an earlier call)
             others[warp][lane] = all;
@@ -1086,8 +1086,9 @@ __global__ void __launch_bounds__(32 * D8_JOIN_WARPS) attention_decode_8bit_join
             const float nothing[N] = {};
             all.add(p.sinks[head] * 1.4426950408889634f, 1.f, nothing);      // a term of the denominator without a value
         }
+        const float inverse = all.sum == 0.f ? 0.f : 1.f / all.sum;
 #pragma unroll
-        for (int e = 0; e < N; ++e) result[e] = all.sum == 0.f ? 0.f : all.acc[e] / all.sum;
+        for (int e = 0; e < N; ++e) result[e] = all.sum == 0.f ? 0.f : all.acc[e] * inverse;
     }
     if (share != 0 || head >= heads) return;
     bf16* out = p.out + ((size_t)b * heads + head) * VD + N * lane;
@@ -1179,15 +1180,15 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
                   "attention_decode_8bit: head_dim %d with value heads of %d: cuTensorMapEncodeTiled failed or is not available", head_dim, v_dim);
     const int out_heads = lam ? num_heads / 2 : num_heads;
     // the join: more warps a (sequence, head) while that leaves SMs idle and each has some partial results
-    int shares = 1;
-    while (shares < D8_JOIN_WARPS && (long long)out_heads * num_seqs * shares <= 6 * frb_sm_count() && max_chunks >= 8 * shares) shares *= 2;
-    const dim3 join_grid((out_heads * shares + D8_JOIN_WARPS - 1) / D8_JOIN_WARPS, num_seqs), join_block(32 * D8_JOIN_WARPS);
+    int shares_log2 = 0;
+    while ((1 << shares_log2) < D8_JOIN_WARPS && ((long long)out_heads * num_seqs << shares_log2) <= 6 * frb_sm_count() && max_chunks >= 8 << shares_log2) ++shares_log2;
+    const dim3 join_grid(((out_heads << shares_log2) + D8_JOIN_WARPS - 1) / D8_JOIN_WARPS, num_seqs), join_block(32 * D8_JOIN_WARPS);
 #define FRB_LAUNCH_DECODE8(HD, VD)                                                                                                  \
     if (per_block == 8 && codes == FRB_E4M3) launch_decode_8bit<HD, VD, 1, FRB_E4M3>(map_k, map_v, p, stream);                \
     else if (per_block == 8) launch_decode_8bit<HD, VD, 1, FRB_INT8>(map_k, map_v, p, stream);                                \
     else if (codes == FRB_E4M3) launch_decode_8bit<HD, VD, 2, FRB_E4M3>(map_k, map_v, p, stream);                             \
     else launch_decode_8bit<HD, VD, 2, FRB_INT8>(map_k, map_v, p, stream);                                                    \
-    launch_dependent_resident(early ? 4 : 1, attention_decode_8bit_join_kernel<VD>, join_grid, join_block, 0, stream, p, shares)
+    launch_dependent_resident(early ? 4 : 1, attention_decode_8bit_join_kernel<VD>, join_grid, join_block, 0, stream, p, shares_log2)
     FRB_8BIT_SIZES("attention_decode_8bit", head_dim, v_dim, FRB_LAUNCH_DECODE8);
 #undef FRB_LAUNCH_DECODE8
     FRB_RETURN_LAUNCH("attention_decode_8bit");
