@@ -30,7 +30,10 @@
 //   length, a warp's each, about as many as warps are resident.  A warp runs through its piece without waiting for any other: the
 //   next page's keys are asked for as soon as the present page's scores are done and its values as soon as they are multiplied, also from
 //   one key head or sequence to the next, where the warp leaves a partial result.  Sequences of unequal lengths need no more time than
-//   their pages, and there is no last wave of a few blocks.
+//   their pages, and there is no last wave of a few blocks.  Where a head has room for too few partial results, cut between key heads only.
+//
+// Measured on a B200, 48 heads on 8 key heads of 128: 32 sequences of 4,096 keys 54 us (e4m3; 277 MB, 5.1 TB/s; 52 of them the pieces, issue slots 35 %
+// busy, 9 to 10 warps an SM; pages of bfloat16 take 92 us), one of 131,072 keys 54 us (int8), one of 2,048 keys 6.5 us.
 //
 // Every wait on an mbarrier gives up after about a second and sets `status`; the warps then wait (with the same limit) for the copies
 // that are in flight and return.
@@ -1132,14 +1135,15 @@ static void launch_decode_8bit(const CUtensorMap& map_k, const CUtensorMap& map_
 }
 
 // max_chunks: chunks of 256 keys of the longest sequence (or more); part_o and part_ml hold as many partial results per (sequence, head).
-// num_pages: pages of the store.  max_pieces: 0, or into how many pieces (warps) the work is cut, whatever its size.  status: one int on the device.
+// num_pages: pages of the store.  max_pieces: 0, or into how many pieces (warps) the work is cut, whatever its size.  pages_final: every page but a
+// sequence's newest was written by kernels that had ended when the kernel before this one began.  status: one int on the device.
 FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales,
                                       int codes, int num_pages, const int* page_table, int num_slots, int max_pages, const int* seq_pos,
                                       const int* seq_slot, float* part_o, float* part_ml, void* out, int num_seqs, int num_heads,
                                       int num_kv_heads, int v_heads, int head_dim, int v_dim, float scale, int window, int chunk,
                                       int keep_first, int max_chunks, int max_pieces, const float* slopes, const float* sinks,
-                                      float softcap, const float* lam, float diff_eps, float diff_factor, int* status,
-                                      cudaStream_t stream) {
+                                      float softcap, const float* lam, float diff_eps, float diff_factor, int pages_final,
+                                      int* status, cudaStream_t stream) {
     if (num_seqs == 0) return 0;
     FRB_CHECK_ARG(num_seqs > 0 && num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0 && v_heads > 0 && num_kv_heads % v_heads == 0,
                   "attention_decode_8bit: %d sequences, %d heads over %d key heads and %d value heads", num_seqs, num_heads, num_kv_heads, v_heads);
@@ -1165,15 +1169,18 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
     p.chunk = chunk; p.keep_first = window > 0 ? keep_first : 0; p.max_pages = max_pages; p.num_slots = num_slots; p.num_pages = num_pages;
     p.num_heads = num_heads; p.num_kv_heads = num_kv_heads; p.v_heads = v_heads; p.num_seqs = num_seqs; p.max_chunks = max_chunks;
     p.head_tiles = head_tiles;
-    // Chunks where two waves of blocks hold all that there may be.  (Measured on a B200 with 8 key heads of 128, microseconds of both
-    // kernels, chunks | pieces: CHOICE)
+    // Chunks where two waves of blocks hold all that there may be.  Measured on a B200 with 48 heads on 8 key heads of 128, sequences x keys, microseconds
+    // with the join, chunks | pieces: 64 blocks (1 x 2048) 6.5 | 17.0; 256 (1 x 8192) 10.0 | 16.5; 512 (4 x 4096) 18.0 | 17.5, (8 x 2048) 17.8 | 19.0;
+    // 1,024 (8 x 4096) 25.7 | 21.3; 2,048 (8 x 8192) 40.9 | 31.2, (128 x 512, cut between key heads) 44.9 | 37.2; 4,096 (32 x 4096) 69.9 | 53.7,
+    // (1 x 131072) 78.9 | 53.6; 8,192 blocks with a page each (1024 x 40) 142 | 76.  Heads of 64: 1,024 (8 x 4096) 16.3 | 17.5, 2,048 (8 x 8192)
+    // 24.3 | 21.1, (128 x 512) 27.0 | 31.9, 4,096 (32 x 4096) 40.0 | 35.2.
     const int resident = D8_RESIDENT(head_dim, v_dim, per_block / 8) * frb_sm_count();
     const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks;
     const bool countable = chunks * D8_CHUNK_PAGES < (1ll << 30);
     p.pieces = !countable ? 0 : max_pieces > 0 ? max_pieces : chunks > 2ll * resident ? resident * D8_WARPS : 0;
     p.whole = p.pieces > 0 && max_chunks < D8_MIN_ROOM;
     static const int early = [] { const char* v = getenv("FIELDRUN_B200_ATTENTION_EARLY"); return !(v && v[0] == '0'); }();
-    p.early = early;
+    p.early = early && pages_final;
     CUtensorMap map_k, map_v;
     FRB_CHECK_ARG(map_code_rows(&map_k, k_codes, (uint64_t)num_pages * num_kv_heads * FRB_PAGE, head_dim) &&
                   map_code_rows(&map_v, v_codes, (uint64_t)num_pages * v_heads * FRB_PAGE, v_dim),

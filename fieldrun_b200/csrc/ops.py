@@ -78,7 +78,7 @@ _SIGNATURES = {
     "frb_attention_prefill_tc": "pippipippipppppiiifippipf" "iiii",
     "frb_qkv_prepare_8bit": "pippif" "ppi" "pppii" "ppppp" "ii" "iiiiiiiii" "i" "pfi" "ip",
     "frb_cache_read_8bit": "ppppi" "ipii" "ppi" "pppi" "pp" "iiii",
-    "frb_attention_decode_8bit": "pppppi" "ipii" "pp" "ppp" "iiiiii" "f" "iii" "ii" "pp" "f" "pff" "p",
+    "frb_attention_decode_8bit": "pppppi" "ipii" "pp" "ppp" "iiiiii" "f" "iii" "ii" "pp" "f" "pff" "ip",
     "frb_attention_pair_tc": "pippi" "pippi" "ppppp" "iiiifiif" "pffp",
     "frb_dyt_rows": "ppppp" "ppp" "pp" "iii" "p" "pppp" "pll",
     "frb_stream_copies": "pip" "pp" "ppppp" "ip" "ppp" "ppp" "pip" "iii",
@@ -1870,13 +1870,15 @@ def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torc
                           window: Optional[int], max_chunks: int, pieces: Optional[int] = None,
                           slopes: Optional[torch.Tensor] = None, chunk: Optional[int] = None, sinks: Optional[torch.Tensor] = None,
                           softcap: Optional[float] = None, v_dim: Optional[int] = None, keep_first: int = 0, maps: int = 1,
-                          difference: Optional[dict] = None) -> None:
+                          difference: Optional[dict] = None, pages_final: bool = True) -> None:
     """As :func:`attention_decode_tma` over 8-bit pages (see :func:`qkv_prepare_8bit`), for every head size of ``MMA_HEAD_SIZES`` and
     groups of any size; queries and output are bfloat16.  ``max_chunks``: chunks of 256 keys of the longest sequence, or more; ``part_o`` and
     ``part_ml`` (float32) have room for ``[sequences, heads, max_chunks, v_dim]`` and ``[..., 2]``.  ``pieces``: into how many
     pieces the step's pages are cut where they are more than fit at once (default: as many as warps are resident).  Where a sequence is cut
     then depends on the others, a matter of rounding; neighbouring rows of one slot and position come out the same to the last bit
-    if their queries are the same.  A sequence at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
+    if their queries are the same.  ``pages_final``: every page but a sequence's newest was written by kernels that had
+    ended when the kernel before this one began, as in a step of one token a sequence (those pages are asked for ahead of that kernel's
+    end); False right behind a call that wrote more than that.  A sequence at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
     v_dim = int(v_dim or head_dim)
     store = _store_8bit(k_pages, k_scales, v_pages, v_scales)
     if maps < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or num_kv_heads % maps:
@@ -1907,10 +1909,12 @@ def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torc
     lam, eps, factor = 0, 0.0, 0.0
     if difference is not None:
         _want(difference["lam"], torch.float32, "lambda")
+        if difference["lam"].numel() != 1:
+            raise KernelError(f"lambda has {difference['lam'].numel()} entries, not one")
         (lam,), eps, factor = _addresses(difference["lam"]), float(difference["eps"]), float(difference["factor"])
     _call("frb_attention_decode_8bit", *at[:5], store[0], store[1], at[5], *page_table.shape, *at[6:11], seqs, num_heads, num_kv_heads,
           num_kv_heads // maps, head_dim, v_dim, float(scale), window, chunk, keep_first, max_chunks, int(pieces or 0), at[11], at[12],
-          float(softcap or 0.0), lam, eps, factor, _ptr(tc_status(q.device)))
+          float(softcap or 0.0), lam, eps, factor, int(pages_final), _ptr(tc_status(q.device)))
 
 
 def wait_probe(device, limit_cycles: int = 100_000) -> int:

@@ -9,7 +9,8 @@ arithmetic it stands for.  Cases: ``experts_tc`` (prompt-sized expert products o
 per expert, as in a step of 16k prompt tokens),
 ``experts_stream`` (decode-sized expert products: the persistent TMA-fed stream; ``experts_stream_mma``: the kernel that
 loads weights into registers, kept for inner sizes that are no multiple of 64), ``attention_decode`` (pages by TMA),
-``attention_decode_mma`` (pages loaded into registers), ``attention_prefill``
+``attention_decode_mma`` (pages loaded into registers), ``attention_decode_8bit`` (pages of e4m3 codes; ``..._int8``: int8; ``..._long``: one sequence
+of 131,072 keys), ``cache_8bit_write`` (rows of a prompt of 2,048 tokens into 8-bit pages) and ``cache_8bit_read`` (512 pages read back), ``attention_prefill``
 (mma.sync tiles of 16 queries), ``attention_prefill_tc`` (tcgen05 tiles of 128 queries; ``attention_prefill_tc_long``: one prompt of 16,384 tokens),
 ``latent_attention_prefill`` (attention over shared key rows of 512 + 64 entries, tcgen05; ``latent_attention_prefill_mma``: the
 mma.sync kernel), ``latent_attention_decode`` and ``latent_attention_decode_small`` (single tokens in chunks of keys, with the join; ``..._mma``: the mma.sync kernel),
@@ -154,6 +155,56 @@ def attention(kind: str, launches: int) -> dict:
         ops.tc_status_check(dev)
     flops = 4 * HEADS * HEAD_DIM * context * (context + 1) // 2
     return {"case": f"attention_{kind}", "ms": round(ms, 4), "tokens": context, "tflops": round(flops / ms / 1e9, 2)}
+
+
+def cache_8bit(kind: str, launches: int) -> dict:
+    dtype = torch.int8 if kind.endswith("int8") else torch.float8_e4m3fn
+    if kind == "write":
+        batch, context = 1, 2048
+    elif kind == "read":
+        batch, context = 1, 32768
+    else:
+        batch, context = (1, 131072) if kind.endswith("long") else (32, 4096)
+    pages_per = context // 64
+    pages = batch * pages_per
+    k, v = (torch.randint(-60, 60, (pages, KV_HEADS, 64, HEAD_DIM), dtype=torch.int8, device=DEV).view(dtype) for _ in range(2))
+    ks, vs = (torch.rand(pages, KV_HEADS, 64, device=DEV) * 0.01 for _ in range(2))
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).view(batch, pages_per).contiguous()
+    slots = torch.arange(batch, dtype=torch.int32, device=DEV)
+    code_bytes = 2 * (k.numel() + ks.numel() * 4)
+    if kind == "write":
+        wide = (HEADS + 2 * KV_HEADS) * HEAD_DIM
+        qkv = [torch.randn(context, wide, device=DEV) for _ in range(3)]
+        q_norm, k_norm = torch.ones(HEADS * HEAD_DIM, device=DEV), torch.ones(KV_HEADS * HEAD_DIM, device=DEV)
+        cos, sin = torch.rand(context, 32, device=DEV), torch.rand(context, 32, device=DEV)
+        positions = torch.arange(context, dtype=torch.int32, device=DEV)
+        zeros = torch.zeros_like(positions)
+        q = torch.empty(context, HEADS * HEAD_DIM, dtype=torch.bfloat16, device=DEV)
+        turn = iter(range(1 << 30))
+        launch = lambda: ops.qkv_prepare_8bit(qkv[next(turn) % 3], q_norm, k_norm, 1e-6, cos, sin, positions, zeros, table, q, k, ks,
+                                              v, vs, num_heads=HEADS, num_kv_heads=KV_HEADS, head_dim=HEAD_DIM, rotary_dim=64, interleaved=False)
+        moved = qkv[0].numel() * 4 + q.numel() * 2 + code_bytes
+    elif kind == "read":
+        keys = torch.empty(pages, KV_HEADS, 64, HEAD_DIM, dtype=torch.bfloat16, device=DEV)
+        values = torch.empty(pages, KV_HEADS, HEAD_DIM, 64, dtype=torch.bfloat16, device=DEV)
+        seqs, numbers = torch.zeros(pages, dtype=torch.int32, device=DEV), torch.arange(pages, dtype=torch.int32, device=DEV)
+        start, new = torch.full((1,), context - 64, dtype=torch.int32, device=DEV), torch.full((1,), 64, dtype=torch.int32, device=DEV)
+        launch = lambda: ops.cache_read_8bit(k, ks, v, vs, table, seqs, numbers, slots, start, new, keys, values)
+        moved = code_bytes + 4 * keys.numel()
+    else:
+        q = torch.randn(batch, HEADS * HEAD_DIM, device=DEV).to(torch.bfloat16)
+        out = torch.empty_like(q)
+        positions = torch.full((batch,), context - 1, dtype=torch.int32, device=DEV)
+        chunks = context // ops.ATTENTION_CHUNK
+        part_o = torch.empty(batch, HEADS, chunks, HEAD_DIM, dtype=torch.float32, device=DEV)
+        part_ml = torch.empty(batch, HEADS, chunks, 2, dtype=torch.float32, device=DEV)
+        launch = lambda: ops.attention_decode_8bit(q, k, ks, v, vs, table, positions, slots, part_o, part_ml, out, num_heads=HEADS,
+                                                   num_kv_heads=KV_HEADS, head_dim=HEAD_DIM, scale=HEAD_DIM ** -0.5, window=None, max_chunks=chunks)
+        moved = code_bytes
+    ms = _time_recorded(launch, launches)
+    ops.tc_status_check(torch.device(DEV))
+    return {"case": ("cache_8bit_" if kind in ("write", "read") else "") + kind, "ms": round(ms, 4), "batch": batch, "context": context,
+            "gb_per_s": round(moved / ms / 1e6, 1)}
 
 
 LATENT_HEADS, LATENT_RANK, LATENT_ROT = 16, 512, 64
@@ -764,6 +815,11 @@ CASES = {
     "experts_stream_mma": lambda n: experts("stream_mma", n),
     "attention_decode": lambda n: attention("decode", n),
     "attention_decode_mma": lambda n: attention("decode_mma", n),
+    "attention_decode_8bit": lambda n: cache_8bit("attention_decode_8bit", n),
+    "attention_decode_8bit_int8": lambda n: cache_8bit("attention_decode_8bit_int8", n),
+    "attention_decode_8bit_long": lambda n: cache_8bit("attention_decode_8bit_long", n),
+    "cache_8bit_write": lambda n: cache_8bit("write", n),
+    "cache_8bit_read": lambda n: cache_8bit("read", n),
     "attention_prefill": lambda n: attention("prefill", n),
     "attention_prefill_tc": lambda n: attention("prefill_tc", n),
     "attention_prefill_tc_long": lambda n: attention("prefill_tc_long", n),

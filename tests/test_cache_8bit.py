@@ -99,13 +99,13 @@ def test_entry_points_refuse_sizes_by_a_message():
     # the C entry points' own checks, which come before anything is launched
     lib = ops.library("cache8")
     assert lib.frb_attention_decode_8bit(*[None] * 5, 0, 1, None, 1, 1, *[None] * 5, 1, 6, 4, 2, 64, 64, 0.1, 0, 0, 0, 1, 1, None, None, 0.0, None, 0.0, 0.0,
-                                         None, None) == -1
+                                         1, None, None) == -1
     assert b"6 heads over 4 key heads" in lib.frb_last_error()
     assert lib.frb_attention_decode_8bit(*[None] * 5, 0, 1, None, 1, 1, *[None] * 5, 70_000, 4, 4, 4, 64, 64, 0.1, 0, 0, 0, 1, 1, None, None, 0.0, None, 0.0, 0.0,
-                                         None, None) == -1
+                                         1, None, None) == -1
     assert b"exceed the grid" in lib.frb_last_error()
     assert lib.frb_attention_decode_8bit(*[None] * 5, 0, 1 << 24, None, 1, 1, *[None] * 5, 1, 4, 4, 4, 64, 64, 0.1, 0, 0, 0, 1, 1, None, None, 0.0, None, 0.0, 0.0,
-                                         None, None) == -1
+                                         1, None, None) == -1
     assert b"exceed a tensor map's rows" in lib.frb_last_error()
     assert lib.frb_cache_read_8bit(*[None] * 4, 5, 1, None, 1, 1, None, None, 1, None, None, None, 1, None, None, 1, 1, 64, 64, None) == -1
     assert b"codes of type 5" in lib.frb_last_error()

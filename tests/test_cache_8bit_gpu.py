@@ -617,3 +617,39 @@ def test_recorded_and_on_another_stream():
     torch.cuda.synchronize()
     assert all(torch.equal(x, t.view(torch.uint8)) for x, t in zip(want, (w3.k, w3.vs, w3.q, a3.out)))
     assert torch.equal(keys, read[0]) and torch.equal(values, read[1])
+
+
+def test_rows_written_and_attended_one_after_the_other():
+    # a prompt's rows and a token's attention over them, nothing in between: the attention waits for all of its pages
+    tokens, heads, kv_heads, dim = 300, 12, 4, 64
+    gen = generator(31)
+    table = torch.randperm(5, generator=gen, device=DEV).to(torch.int32).view(1, 5)
+    positions, zeros = torch.arange(tokens, dtype=torch.int32, device=DEV), torch.zeros(tokens, dtype=torch.int32, device=DEV)
+    qkv = [torch.randn(tokens, (heads + 2 * kv_heads) * dim, generator=gen, device=DEV) for _ in range(20)]
+    results = []
+    for wait in (True, False):
+        for rows in qkv:
+            k, v = (torch.full((5, kv_heads, PAGE, dim), 3, dtype=torch.int8, device=DEV) for _ in range(2))
+            ks, vs = (torch.full((5, kv_heads, PAGE), 9.0, device=DEV) for _ in range(2))
+            q = torch.empty(tokens, heads * dim, dtype=torch.bfloat16, device=DEV)
+            part_o, part_ml = torch.empty(heads, 2, dim, device=DEV), torch.empty(heads, 2, 2, device=DEV)
+            last, out = torch.randn(1, heads * dim, generator=generator(5), device=DEV).to(torch.bfloat16), torch.empty(1, heads * dim, dtype=torch.bfloat16, device=DEV)
+            position = ints([tokens - 1])
+            torch.cuda.synchronize()
+            ops.qkv_prepare_8bit(rows, None, None, 1e-6, None, None, positions, zeros, table, q, k, ks, v, vs, num_heads=heads, num_kv_heads=kv_heads,
+                                 head_dim=dim, rotary_dim=0, interleaved=False)
+            if wait:
+                torch.cuda.synchronize()
+            ops.attention_decode_8bit(last, k, ks, v, vs, table, position, zeros[:1], part_o, part_ml, out, num_heads=heads, num_kv_heads=kv_heads,
+                                      head_dim=dim, scale=dim ** -0.5, window=None, max_chunks=2, pages_final=wait)
+            ops.tc_status_check(out.device)
+            results.append(out)
+    for a, b in zip(results, results[len(qkv):]):
+        assert torch.equal(a, b)
+
+
+def test_attention_refuses_a_lambda_without_an_entry():
+    a = Attended([100, 70], E4M3, heads=8, kv_heads=4, dim=64, maps=2)
+    a.options["difference"]["lam"] = torch.empty(0, device=DEV)
+    with pytest.raises(ops.KernelError, match="lambda"):
+        a.run()

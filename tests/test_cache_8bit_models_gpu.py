@@ -31,7 +31,7 @@ def vocabulary(config):
     return config.get("vocab_size") or config["vocab"]
 
 
-class Checker:
+class Watched:
     """Compares every attention of the steps run inside with float64 over the rows of the cache (codes times scales; for prompts rounded to
     bfloat16, as they are read back)."""
 
@@ -91,7 +91,7 @@ def test_every_attention_of_a_model(design, name, cache_dtype, monkeypatch):
     lm, config = model(design, name, cache_dtype)
     engine = lm.engine
     engine.record_steps = False
-    checker = Checker(monkeypatch)
+    watched = Watched(monkeypatch)
     rng = np.random.default_rng(3)
     draw = lambda n: rng.integers(0, vocabulary(config), size=n).tolist()
     slots = [engine.new_sequence() for _ in range(4)]
@@ -101,7 +101,7 @@ def test_every_attention_of_a_model(design, name, cache_dtype, monkeypatch):
     engine.step(slots[1:], [draw(130), draw(66), draw(64)])          # prompts that go on
     engine.step(slots, [draw(1) for _ in slots])
     engine.check()
-    assert {p for p, *_ in checker.seen} == {True, False}
+    assert {p for p, *_ in watched.seen} == {True, False}
 
 
 @pytest.mark.parametrize("cache_dtype", ["int8", "float8_e4m3fn"])
