@@ -286,7 +286,10 @@ def _call(name: str, *args) -> None:
         fn = _FUNCTIONS.get(name) or getattr(library(_GROUP_OF[name]), name)
     packer = _PACKED.get(name)
     if packer is not None:
-        args = (packer.pack(*args),)
+        try:
+            args = (packer.pack(*args),)
+        except struct.error as error:
+            raise KernelError(f"{name}: {error}") from None
     if _TIMINGS is not None:
         with timed(name[4:]):
             status = fn(*args, _stream())

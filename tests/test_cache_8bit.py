@@ -120,6 +120,21 @@ def test_entry_points_refuse_sizes_by_a_message():
     assert b"more than 200 KB" in lib.frb_last_error()
 
 
+def test_arguments_in_one_struct():
+    # the packed entry points read what the ordinary ones get: the same refusals, and numbers beyond 32 bits are an error
+    lib = ops.library("cache8")
+    attend = [0] * 5 + [0, 1, 0, 1, 1] + [0] * 5 + [1, 6, 4, 2, 64, 64, 0.1, 0, 0, 0, 1, 1, 0, 0, 0.0, 0, 0.0, 0.0, 1, 0]
+    read = [0] * 4 + [5, 1, 0, 1, 1, 0, 0, 1, 0, 0, 0, 1, 0, 0, 1, 1, 64, 64]
+    write = [0, 0, 0, 0, 0, 1e-6, 0, 0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 0, 0, 1, 1, 2, 2, 2, 64, 64, 31, 0, 0, 0, 0, 0.0, 1, 0, 0]
+    for name, args, message in (("frb_attention_decode_8bit", attend, b"6 heads over 4 key heads"), ("frb_cache_read_8bit", read, b"codes of type 5"),
+                                ("frb_qkv_prepare_8bit", write, b"rotary_dim 31")):
+        assert getattr(lib, name + "_packed")(ops._PACKED[name].pack(*args), None) == -1
+        assert message in lib.frb_last_error()
+    attend[22] = 1 << 31
+    with pytest.raises(ops.KernelError, match="frb_attention_decode_8bit"):
+        ops._call("frb_attention_decode_8bit", *attend)
+
+
 # ------------------------------------------------------------------------------------------------ pages and tables
 
 @pytest.mark.parametrize("codes,dtype", [("int8", INT8), ("float8_e4m3fn", E4M3)])

@@ -385,6 +385,29 @@ def test_attention_many_short_sequences(chunks, pieces):
     Attended(positions[:40], INT8, heads=18, kv_heads=1, dim=128, pieces=pieces, max_chunks=chunks, window=150, keep_first=70).run().check()
 
 
+@pytest.mark.parametrize("chunks,pieces", [(1, None), (1, 50), (4, None), (4, 3000)])
+def test_attention_thousands_of_sequences(chunks, pieces):
+    # more rows than 64 groups of 32
+    positions = [-1 if i % 7 == 3 else (i * 37) % 130 + (600 if chunks == 4 and i % 97 == 0 else 0) for i in range(2500)]
+    Attended(positions, E4M3, heads=2, kv_heads=1, dim=32, pieces=pieces, max_chunks=chunks).run().check()
+
+
+@pytest.mark.parametrize("chunks,pieces", [(1, 9), (4, 1), (4, 333), (12, 40), (12, None)])
+def test_attention_of_a_row_repeated_many_times(chunks, pieces):
+    # over the bounds of 32 rows, at the end and in the middle
+    lengths = [256 * chunks - 5, 100, -1, 70]
+    counts = [3, 69, 1, 60]
+    a = Attended(lengths, INT8, heads=12, kv_heads=6, dim=64, pieces=pieces, max_chunks=chunks)
+    index = torch.tensor([i for i, n in enumerate(counts) for _ in range(n)], device=DEV)
+    a.positions = [lengths[int(i)] for i in index]
+    a.q, a.slots, a.out = a.q[index].contiguous(), a.slots[index].contiguous(), a.out[index].contiguous()
+    a.part_o, a.part_ml = (x.reshape(len(lengths), -1)[index].reshape(-1).contiguous() for x in (a.part_o, a.part_ml))
+    a.run().check()
+    for i in range(len(lengths)):
+        rows = a.out[index == i]
+        assert torch.equal(rows, rows[:1].expand_as(rows))
+
+
 def test_attention_sharp_scores():
     # one key has nearly all the weight, at any place, and scores of hundreds: the running maximum moves by much
     for seed in range(4):
