@@ -38,6 +38,7 @@
 // Every wait on an mbarrier gives up after about a second and sets `status`; the warps then wait (with the same limit) for the copies
 // that are in flight and return.
 #include "cache_8bit.cuh"
+#include "step_rows.h"
 #include "tma.cuh"
 
 #define D8_WARPS 4
@@ -722,8 +723,9 @@ __device__ __forceinline__ int places_of_rows(const Decode8Params& p, int b0, in
     const int b = b0 + lane;
     const bool there = b < p.num_seqs;
     const int slot = there ? p.seq_slot[b] : -1, position = there ? p.seq_pos[b] : -1;
-    const bool beside = lane == 0 ? b0 > 0 : lane == 31 && b + 1 < p.num_seqs;             // the rows around these
-    const int other = lane == 0 ? b0 - 1 : b + 1, other_slot = beside ? p.seq_slot[other] : -1, other_position = beside ? p.seq_pos[other] : -1;
+    const int other = row_beside(b0, lane, p.num_seqs);
+    const bool beside = other >= 0;
+    const int other_slot = beside ? p.seq_slot[other] : -1, other_position = beside ? p.seq_pos[other] : -1;
     const int left_slot = __shfl_up_sync(0xffffffffu, slot, 1), left_position = __shfl_up_sync(0xffffffffu, position, 1);
     const bool repeat = there && (lane > 0 ? slot == left_slot && position == left_position : beside && slot == other_slot && position == other_position);
     const unsigned repeats_left = __ballot_sync(0xffffffffu, repeat);
@@ -804,7 +806,8 @@ attention_decode_8bit_pieces_kernel(const __grid_constant__ CUtensorMap map_k, c
     uint8_t* base = begin_block<HD, VD>(dynamic, bars, &failed);
 
     // The line's length, from those of its rows in up to D8_ROW_GROUPS groups.
-    const int group_steps = (p.num_seqs + 32 * D8_ROW_GROUPS - 1) / (32 * D8_ROW_GROUPS), groups = (p.num_seqs + 32 * group_steps - 1) / (32 * group_steps);
+    const RowGroups in_groups = row_groups(p.num_seqs, D8_ROW_GROUPS);
+    const int group_steps = in_groups.steps, groups = in_groups.count;
     int longest = 0;
     for (int i = warp; i < groups; i += D8_WARPS) {
         int sum = 0;
