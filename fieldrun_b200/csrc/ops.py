@@ -1873,15 +1873,15 @@ def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torc
                           window: Optional[int], max_chunks: int, pieces: Optional[int] = None,
                           slopes: Optional[torch.Tensor] = None, chunk: Optional[int] = None, sinks: Optional[torch.Tensor] = None,
                           softcap: Optional[float] = None, v_dim: Optional[int] = None, keep_first: int = 0, maps: int = 1,
-                          difference: Optional[dict] = None, pages_final: bool = True) -> None:
+                          difference: Optional[dict] = None, pages_final: bool = False) -> None:
     """As :func:`attention_decode_tma` over 8-bit pages (see :func:`qkv_prepare_8bit`), for every head size of ``MMA_HEAD_SIZES`` and
     groups of any size; queries and output are bfloat16.  ``max_chunks``: chunks of 256 keys of the longest sequence, or more; ``part_o`` and
     ``part_ml`` (float32) have room for ``[sequences, heads, max_chunks, v_dim]`` and ``[..., 2]``.  ``pieces``: into how many
     pieces the step's pages are cut where they are more than fit at once (default: as many as warps are resident).  Where a sequence is cut
     then depends on the others, a matter of rounding; neighbouring rows of one slot and position come out the same to the last bit
-    if their queries are the same.  ``pages_final``: every page but a sequence's newest was written by kernels that had
-    ended when the kernel before this one began, as in a step of one token a sequence (those pages are asked for ahead of that kernel's
-    end); False right behind a call that wrote more than that.  A sequence at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
+    if their queries are the same.  ``pages_final`` (a promise): every page but a sequence's newest was written by kernels that had
+    ended when the kernel before this one began, as in a step of one token a sequence; those pages are then asked for ahead of that kernel's
+    end.  Without it every page is read after the kernel before this one.  A sequence at a negative position holds no token and gets zeros; a page that the table does not have (-1) holds no keys."""
     v_dim = int(v_dim or head_dim)
     store = _store_8bit(k_pages, k_scales, v_pages, v_scales)
     if maps < 1 or num_kv_heads < 1 or num_heads % num_kv_heads or num_kv_heads % maps:

@@ -289,6 +289,7 @@ class GQAAttention(Mixer):
             part_ml = ctx.buffer("attention.part_ml", (ctx.num_seqs, self.q_heads, chunks, 2), torch.float32)
             ops.attention_decode_8bit(q, line.keys, line.key_scales, line.values, line.value_scales, line.page_table, ctx.seq_start,
                                       ctx.seq_slot, part_o, part_ml, out, max_chunks=chunks,
+                                      pages_final=True,       # this step wrote one row a sequence, into its newest page
                                       difference=difference if self.maps == 2 else None, **common)
             if gate is not None:
                 ops.head_gate(out, gate, self.num_heads, self.value_dim)

@@ -199,7 +199,8 @@ def cache_8bit(kind: str, launches: int) -> dict:
         part_o = torch.empty(batch, HEADS, chunks, HEAD_DIM, dtype=torch.float32, device=DEV)
         part_ml = torch.empty(batch, HEADS, chunks, 2, dtype=torch.float32, device=DEV)
         launch = lambda: ops.attention_decode_8bit(q, k, ks, v, vs, table, positions, slots, part_o, part_ml, out, num_heads=HEADS,
-                                                   num_kv_heads=KV_HEADS, head_dim=HEAD_DIM, scale=HEAD_DIM ** -0.5, window=None, max_chunks=chunks)
+                                                   num_kv_heads=KV_HEADS, head_dim=HEAD_DIM, scale=HEAD_DIM ** -0.5, window=None, max_chunks=chunks,
+                                                   pages_final=True)
         moved = code_bytes
     ms = _time_recorded(launch, launches)
     ops.tc_status_check(torch.device(DEV))

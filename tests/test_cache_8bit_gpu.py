@@ -676,3 +676,33 @@ def test_attention_refuses_a_lambda_without_an_entry():
     a.options["difference"]["lam"] = torch.empty(0, device=DEV)
     with pytest.raises(ops.KernelError, match="lambda"):
         a.run()
+
+
+@pytest.mark.parametrize("tokens,pieces", [(300, None), (300, 7), (2000, None)])
+def test_a_prompt_written_and_attended_without_a_word(tokens, pieces):
+    # as above with no option given: attention reads what the kernel right before it wrote
+    heads, kv_heads, dim = 12, 4, 64
+    gen = generator(33)
+    pages = -(-tokens // PAGE)
+    table = torch.randperm(pages, generator=gen, device=DEV).to(torch.int32).view(1, pages)
+    positions, zeros, position = torch.arange(tokens, dtype=torch.int32, device=DEV), torch.zeros(tokens, dtype=torch.int32, device=DEV), ints([tokens - 1])
+    last = torch.randn(1, heads * dim, generator=gen, device=DEV).to(torch.bfloat16)
+    chunks = -(-tokens // 256)
+    part_o, part_ml = torch.empty(heads, chunks, dim, device=DEV), torch.empty(heads, chunks, 2, device=DEV)
+    for _ in range(10):
+        rows = torch.randn(tokens, (heads + 2 * kv_heads) * dim, generator=gen, device=DEV)
+        results = []
+        for wait in (True, False):
+            k, v = (torch.full((pages, kv_heads, PAGE, dim), 3, dtype=torch.int8, device=DEV) for _ in range(2))
+            ks, vs = (torch.full((pages, kv_heads, PAGE), 9.0, device=DEV) for _ in range(2))
+            q, out = torch.empty(tokens, heads * dim, dtype=torch.bfloat16, device=DEV), torch.empty(1, heads * dim, dtype=torch.bfloat16, device=DEV)
+            torch.cuda.synchronize()
+            ops.qkv_prepare_8bit(rows, None, None, 1e-6, None, None, positions, zeros, table, q, k, ks, v, vs, num_heads=heads, num_kv_heads=kv_heads,
+                                 head_dim=dim, rotary_dim=0, interleaved=False)
+            if wait:
+                torch.cuda.synchronize()
+            ops.attention_decode_8bit(last, k, ks, v, vs, table, position, zeros[:1], part_o, part_ml, out, num_heads=heads, num_kv_heads=kv_heads,
+                                      head_dim=dim, scale=dim ** -0.5, window=None, max_chunks=chunks, pieces=pieces)
+            ops.tc_status_check(out.device)
+            results.append(out)
+        assert torch.equal(*results)
