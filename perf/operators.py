@@ -386,6 +386,7 @@ def _own_attend(s, q):
                               s["out"], num_heads=q_heads, num_kv_heads=k_heads, head_dim=dim, v_dim=vdim, scale=dim ** -0.5,
                               window=case["window"] or None, chunk=case["chunk"] or None, keep_first=case["keep_first"],
                               max_chunks=s["max_chunks"], slopes=s["slopes"], sinks=s["sinks"], softcap=case["softcap"] or None, maps=maps,
+                              pages_final=True,               # at most one row a sequence was just written, into its newest page
                               difference=dict(lam=s["lam"], eps=DIFF_EPS, factor=DIFF_FACTOR) if maps == 2 else None)
 
 
