@@ -9,11 +9,11 @@
 // m16n8k16), where up to eight query heads of a key head fill the columns; with the heads as rows half of every MMA, of the
 // accumulators and of the exponentials would belong to rows that do not exist.  A key's scale multiplies its scores, a value's its weight.
 //
-// Scores: int8 codes go into the tensor cores as they are (m16n8k32, 32-bit integer sums), the queries in two parts of 8 bits, q = h 256 + l in
-// units of 1/32512 of the head's largest entry (errors of up to 2^-16 of it).  e4m3 codes become float16 in registers, which is exact; the
-// queries are brought to float16 by a power of two per head (exact down to 2^-29 of a head's largest entry).  (The products of e4m3
-// codes are no instruction of their own for single warps: with them, and the queries in two e4m3 parts, 32 sequences of 4,096 keys took 71
-// us, with float16 58.)  The values' codes, of either type, become float16, since the weights need its range and precision.
+// Scores: codes of either type become float16 in registers, which is exact, and the queries are brought to float16 by a power of two per head
+// (exact down to 2^-29 of a head's largest entry): what a score loses is lost in float32 sums.  (int8 codes multiplied as they are, by queries in two
+// parts of 8 bits, take 55 us for 32 sequences of 4,096 keys where this takes 57, but round every query entry to 2^-16 of the head's largest: where
+// that one meets keys of zero and is 1,000 times the others, outputs are off by 4 per cent.  The products of e4m3 codes are no instruction of
+// their own for single warps: with them, and the queries in two e4m3 parts, the same sequences took 71 us, with float16 58.)
 //
 // Weights: p_j = 2^(s_j - m) with m a running maximum that follows a page's only beyond a margin.  The weight that multiplies codes is
 // w_j = p_j vs_j, rounded to float16 after division by a unit U per head, a power of two that follows the largest w seen: w / U is at most
@@ -107,13 +107,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// the same over 32 int8 codes of k
-__device__ __forceinline__ void mma_int8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 __device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -176,22 +169,23 @@ __device__ __forceinline__ Words<BYTES> row_words(const uint8_t* tile, int r, in
     return v;
 }
 
-// Four query entries as two registers beside the registers of four codes of a key.  e4m3: float16 pairs, of entries below 2^15.  int8, of
-// entries of up to 32512: the codes of the two parts.
+// Four codes of a key as two float16 pairs, and four query entries as the pairs that they are multiplied with.  e4m3: entries 0, 1 and 2, 3;
+// int8: 0, 2 and 1, 3, as the bytes' places make them.
 template <int CODES>
-__device__ __forceinline__ void query_words(const float (&x)[4], uint32_t& first, uint32_t& second) {
+__device__ __forceinline__ void key_halves(uint32_t w, uint32_t& first, uint32_t& second) {
     if (CODES == FRB_E4M3) {
-        first = pack_f16(x[0], x[1]);
-        second = pack_f16(x[2], x[3]);
+        halves_of_e4m3(w, first, second);
     } else {
-        first = second = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int n = __float2int_rn(x[e]), h = (n + 128) >> 8;
-            first |= ((uint32_t)h & 0xffu) << (8 * e);
-            second |= ((uint32_t)(n - 256 * h) & 0xffu) << (8 * e);
-        }
+        first = half_of_int8(w);
+        second = half_of_int8(w >> 8);
     }
+}
+
+template <int CODES>
+__device__ __forceinline__ void query_halves(const float (&x)[4], uint32_t& first, uint32_t& second) {
+    constexpr int NEXT = CODES == FRB_E4M3 ? 1 : 2;
+    first = pack_f16(x[0], x[NEXT]);
+    second = pack_f16(x[3 - NEXT], x[3]);
 }
 
 // Entries 2 n and 2 n + 1 (n = 0, 1) of four codes of two keys: entry 2 n of both as `even`, entry 2 n + 1 as `odd`.
@@ -277,7 +271,7 @@ template <int HD, int VD, int NT, int CODES>
 struct HeadTile {
     static constexpr int KU = HD % 64 == 0 ? 16 : 8, K_STEPS = HD / (4 * KU), K_WORDS = KU / 4;     // a lane's bytes of a key at a time
     static constexpr int VB = VD / 8, MT = VD / 16;                                                // a lane's bytes of a value; output tiles
-    uint32_t q[NT][2][K_STEPS * K_WORDS];       // two registers for every word of a key (query_words)
+    uint32_t q[NT][2][K_STEPS * K_WORDS];       // two registers for every word of a key (query_halves)
     float s_scale[NT][2], slope2[NT][2];        // scores to units of log2, or for a cap to units of the cap
     float gain[NT][2];                          // what scores() gives, to units of log2
     float row_max[NT][2], limit[NT][2], row_sum[NT][2];       // units of log2; a score beyond `limit` raises the maximum; row_sum: of the lane's own keys
@@ -320,21 +314,14 @@ struct HeadTile {
             bad = ((__ballot_sync(0xffffffffu, bad) >> (4 * g)) & 15u) != 0;            // the head has an entry that is not finite: so are its scores
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            float factor, back;
-            if (CODES == FRB_E4M3) {
-                const int e = min(max(exponent_of(top), -100), 127);       // |q| 2^(14 - e) < 2^15
-                factor = power_of_two(14 - e);
-                back = power_of_two(e - 14);
-            } else {
-                top = fmaxf(top, 1e-30f);
-                factor = 32512.f / top;
-                back = top * (1.f / 32512.f);
-            }
+            const int e = min(max(exponent_of(top), -100), 127);           // |q| 2^(14 - e) < 2^15
+            const float factor = power_of_two(14 - e);
+            float back = power_of_two(e - 14);
 #pragma unroll
             for (int i = 0; i < K_STEPS * K_WORDS; ++i) {
 #pragma unroll
                 for (int d = 0; d < 4; ++d) x[i][d] *= factor;
-                query_words<CODES>(x[i], q[j][0][i], q[j][1][i]);
+                query_halves<CODES>(x[i], q[j][0][i], q[j][1][i]);
             }
             back *= p.softcap > 0.f ? p.scale / p.softcap : p.scale * 1.4426950408889634f;
             if (bad) back = __uint_as_float(0x7fc00000u);
@@ -360,54 +347,22 @@ struct HeadTile {
                 a[i][step] = row_words<HD, KU>(tile, k0, (4 * step + t) * KU);
                 c[i][step] = row_words<HD, KU>(tile, k0 + 8, (4 * step + t) * KU);
             }
-        if (CODES == FRB_E4M3) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[j][i0 + i][e] = 0.f;
+                for (int e = 0; e < 4; ++e) s[j][i0 + i][e] = 0.f;
 #pragma unroll
-            for (int n = 0; n < K_STEPS * K_WORDS; ++n)
+        for (int n = 0; n < K_STEPS * K_WORDS; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t a0, a1, a2, a3;
-                    halves_of_e4m3(a[i][n / K_WORDS].w[n % K_WORDS], a0, a2);
-                    halves_of_e4m3(c[i][n / K_WORDS].w[n % K_WORDS], a1, a3);
+            for (int i = 0; i < 2; ++i) {
+                uint32_t a0, a1, a2, a3;
+                key_halves<CODES>(a[i][n / K_WORDS].w[n % K_WORDS], a0, a2);
+                key_halves<CODES>(c[i][n / K_WORDS].w[n % K_WORDS], a1, a3);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) mma_f16(s[j][i0 + i], a0, a1, a2, a3, q[j][0][n], q[j][1][n]);
-                }
-        } else {
-            int sum[2][NT][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sum[i][j][e] = 0;
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-#pragma unroll
-                for (int n = 0; n < K_STEPS * K_WORDS; n += 2)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            const Words<KU>&top = a[i][n / K_WORDS], &low = c[i][n / K_WORDS];
-                            mma_int8(sum[i][j], top.w[n % K_WORDS], low.w[n % K_WORDS], top.w[n % K_WORDS + 1], low.w[n % K_WORDS + 1], q[j][part][n],
-                                     q[j][part][n + 1]);
-                        }
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (part == 0) sum[i][j][e] *= 256;
-                            else s[j][i0 + i][e] = (float)sum[i][j][e];
-                        }
+                for (int j = 0; j < NT; ++j) mma_f16(s[j][i0 + i], a0, a1, a2, a3, q[j][0][n], q[j][1][n]);
             }
-        }
     }
 
     // The scores of a page whose first key is key_base; times `gain` they are in units of log2.

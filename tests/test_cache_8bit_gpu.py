@@ -706,3 +706,27 @@ def test_a_prompt_written_and_attended_without_a_word(tokens, pieces):
             ops.tc_status_check(out.device)
             results.append(out)
         assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("ratio", [2.0 ** 7, 2.0 ** 10, 2.0 ** 12, 2.0 ** 20])
+@pytest.mark.parametrize("dim,heads,kv_heads,pieces", [(128, 12, 2, None), (128, 10, 1, 5), (64, 12, 4, 9), (96, 12, 2, None), (32, 4, 4, None)])
+def test_attention_scores_beside_a_large_query_entry(dim, heads, kv_heads, pieces, ratio, dtype):
+    # one entry of every query head is `ratio` times the largest of the others, and the keys are zero there: what it
+    # multiplies is nothing, and the other entries count to their last bit
+    a = Attended([900, 70], dtype, heads=heads, kv_heads=kv_heads, dim=dim, pieces=pieces, q_size=4.0, k_spread=0.0, seed=41)
+    q = a.q.view(2, heads, dim)
+    for head in range(heads):
+        place = (7 * (head // (heads // kv_heads)) + 3) % dim                # the heads of a key head share the place
+        q[:, head, place] = 0.0
+        q[:, head, place] = ratio * q[:, head].abs().amax(-1)
+        a.k.view(torch.uint8)[:, head // (heads // kv_heads), :, place] = 0
+    a.run()
+    got = a.out.double().cpu().numpy().reshape(2, heads, a.v_dim)
+    for i, position in enumerate(a.positions):
+        want, size, top, reach, _ = plain.attend(a.q[i].double().cpu().numpy().reshape(heads, dim), a.rows_of(i, a.k, a.ks), a.rows_of(i, a.v, a.vs),
+                                                 position, scale=dim ** -0.5, group=heads // kv_heads)
+        # queries as they are: no term for their rounding (and none for their largest entry)
+        want, bound = plain.output_bound(want, size, top, reach, 0.0, position, dim=dim, group=heads // kv_heads, codes=None)
+        off = np.abs(got[i] - want)
+        assert (off <= bound).all(), (i, float((off / bound).max()))
