@@ -8,7 +8,7 @@ the host (for decisions) and on the device (for the kernels).
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 import torch
@@ -90,6 +90,14 @@ def _tiles_of(q_lens: Sequence[int], rows: int) -> tuple[list[int], list[int]]:
             seqs.append(b)
             firsts.append(q0)
     return seqs, firsts
+
+
+class SightPortion(NamedTuple):
+    """Some neighbouring sequences of a step, and the cache pages that their new tokens may see; int32 on the device."""
+    first_seq: int
+    end_seq: int
+    page_seq: torch.Tensor               # the sequence (of the step) of each page
+    page_index: torch.Tensor             # and its number there
 
 
 class StepContext:
@@ -198,16 +206,17 @@ class StepContext:
             kept[key] = total
         return kept[key]
 
-    def pages_in_sight(self, window: Optional[int], chunk: Optional[int], keep_first: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """The cache pages that the new tokens may see (those that :meth:`visible_pages` counts), sequence by sequence: the sequence
-        of each (of the step) and its number there, and a table [sequences, pages] of each one's place in that list, -1 elsewhere; int32 on
-        the device.  For steps of prompts only, as :meth:`token_chunks`."""
-        kept = self.__dict__.setdefault("_pages_in_sight", {})
-        key = (window, chunk, keep_first)
+    def sight_portions(self, window: Optional[int], chunk: Optional[int], keep_first: int,
+                       most: Optional[int] = None) -> tuple[list[SightPortion], torch.Tensor]:
+        """The cache pages that the new tokens may see (those that :meth:`visible_pages` counts), sequence by sequence, in portions of whole
+        sequences with at most ``most`` pages each, or of one sequence that has more; and a table [sequences, pages] (int32 on the
+        device) of each page's place in its portion, -1 elsewhere.  For steps of prompts only, as :meth:`token_chunks`."""
+        kept = self.__dict__.setdefault("_sight_portions", {})
+        key = (window, chunk, keep_first, most)
         if key not in kept:
             pages = [-(-(start + n) // PAGE_TOKENS) for start, n in zip(self.seq_starts, self.seq_q_lens)]
             table = np.full((self.num_seqs, max(pages)), -1, dtype=np.int32)
-            seqs, numbers, count = [], [], 0
+            seqs, numbers, total, bounds = [], [], 0, [(0, 0)]         # of each portion: the first sequence, and pages before it
             for b, (start, n) in enumerate(zip(self.seq_starts, self.seq_q_lens)):
                 if n == 0:
                     continue
@@ -216,13 +225,23 @@ class StepContext:
                     low = max(low, start // chunk * chunk)
                 first = low // PAGE_TOKENS
                 own = np.concatenate([np.arange(min(-(-(keep_first if window else 0) // PAGE_TOKENS), first)), np.arange(first, pages[b])])
-                table[b, own] = np.arange(count, count + len(own))
+                if most is not None and bounds[-1][1] < total and total + len(own) - bounds[-1][1] > most:
+                    bounds.append((b, total))
+                place = total - bounds[-1][1]
+                table[b, own] = np.arange(place, place + len(own))
                 seqs.append(np.full(len(own), b))
                 numbers.append(own)
-                count += len(own)
+                total += len(own)
             flat = torch.from_numpy(np.concatenate([*seqs, *numbers, table.reshape(-1)]).astype(np.int32)).to(self.device)
-            kept[key] = (flat[:count], flat[count:2 * count], flat[2 * count:].view(table.shape))
+            ends = bounds[1:] + [(self.num_seqs, total)]
+            portions = [SightPortion(b0, b1, flat[at:to], flat[total + at:total + to]) for (b0, at), (b1, to) in zip(bounds, ends)]
+            kept[key] = (portions, flat[2 * total:].view(table.shape))
         return kept[key]
+
+    def pages_in_sight(self, window: Optional[int], chunk: Optional[int], keep_first: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """:meth:`sight_portions` as one: the sequence of each page (of the step), its number there, and the table."""
+        (whole,), table = self.sight_portions(window, chunk, keep_first)
+        return whole.page_seq, whole.page_index, table
 
     @property
     def seq_rows(self) -> torch.Tensor:
@@ -231,11 +250,18 @@ class StepContext:
             self._seq_rows = torch.arange(self.num_seqs, dtype=torch.int32, device=self.device)
         return self._seq_rows
 
-    def query_tiles(self, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    def query_tiles(self, rows: int, portion: Optional[SightPortion] = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Tiles of ``rows`` consecutive new tokens that never span two sequences: (sequence of each tile,
-        first row of each tile among its sequence's new tokens), on the device."""
+        first row of each tile among its sequence's new tokens), on the device; of all sequences or of a portion's."""
         if rows not in self._tiles:
             seqs, firsts = _tiles_of(self.seq_q_lens, rows)
             both = torch.tensor([seqs, firsts], dtype=torch.int32).to(self.device)
             self._tiles[rows] = (both[0].contiguous(), both[1].contiguous())
-        return self._tiles[rows]
+        if portion is None:
+            return self._tiles[rows]
+        count = [sum(-(-n // rows) for n in self.seq_q_lens[:b]) for b in (portion.first_seq, portion.end_seq)]
+        return tuple(t[count[0]:count[1]] for t in self._tiles[rows])
+
+    def tokens_of(self, portion: SightPortion) -> slice:
+        """The new tokens of a portion's sequences."""
+        return slice(sum(self.seq_q_lens[:portion.first_seq]), sum(self.seq_q_lens[:portion.end_seq]))

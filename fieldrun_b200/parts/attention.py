@@ -60,6 +60,9 @@ TC_ATTENTION_MIN_QUERIES = 64       # a step whose longest run of new tokens is 
 # launch is 12 us of the host's time more, which a small layer's step of a few dozen tokens waits for.
 F32_TC_KEYS = 3072
 F32_TC_SCRATCH = 1 << 28           # floats that the parts of the pages in sight may take (a gigabyte: 128,000 tokens of MiniMax-M2's layer)
+# Bytes that a step's pages of a cache in 8 bits may take as bfloat16 pages (a gigabyte: 262,144 tokens of MiniMax-M2's layer).  Sequences that take more
+# together come in portions, one after another through the same room; one that takes more by itself gets what it takes.
+READ_BACK_BYTES = 1 << 30
 
 
 class GQAAttention(Mixer):
@@ -282,7 +285,6 @@ class GQAAttention(Mixer):
                       scale=self.softmax_scale, window=self.window, slopes=self.slopes, chunk=self.chunk, sinks=self.sinks,
                       softcap=self.softcap, keep_first=self.keep_first, maps=self.maps)
         difference = dict(lam=self.lam, eps=self.diff_eps, factor=1.0 - self.diff)
-        both = self.softcap is not None and self.slopes is not None     # the tcgen05 kernel has either, not both
         if self.codes and ctx.is_decode:
             chunks = (ctx.max_kv_len + ops.ATTENTION_CHUNK - 1) // ops.ATTENTION_CHUNK
             part_o = ctx.buffer("attention.part_o", (ctx.num_seqs, self.q_heads, chunks, self.value_dim), torch.float32)
@@ -294,16 +296,32 @@ class GQAAttention(Mixer):
             if gate is not None:
                 ops.head_gate(out, gate, self.num_heads, self.value_dim)
             return
-        keys, values, table, seq_slot, tok_slot = line.keys, line.values, line.page_table, ctx.seq_slot, ctx.tok_slot
-        if self.codes:
-            # the pages in sight as bfloat16 pages of the step's own: sequence b of the step is row b of their table
-            page_seq, page_index, table = ctx.pages_in_sight(self.window, self.chunk, self.keep_first)
-            keys = ctx.buffer("attention.keys", (page_seq.numel(), self.k_heads, PAGE_TOKENS, self.head_dim), torch.bfloat16)
-            values = ctx.buffer("attention.values", (page_seq.numel(), self.num_kv_heads, self.value_dim, PAGE_TOKENS), torch.bfloat16)
-            ops.cache_read_8bit(line.keys, line.key_scales, line.values, line.value_scales, line.page_table, page_seq, page_index,
-                                ctx.seq_slot, ctx.seq_start, ctx.seq_q_len, keys, values)
-            seq_slot, tok_slot = ctx.seq_rows, ctx.tok_seq
         maps_out = out if self.maps == 1 else ctx.buffer("attention.maps", (out.shape[0], self.maps * self.out_width), torch.float32)
+        if not self.codes:
+            done, gate = self._attend_pages(ctx, q, line.keys, line.values, line.page_table, ctx.seq_slot, ctx.tok_slot, out, maps_out, gate, None, common, difference)
+        else:
+            # the pages in sight as bfloat16 pages of the step's own, portion by portion: sequence b of the step is row b of their table
+            page_entries = PAGE_TOKENS * (self.k_heads * self.head_dim + self.num_kv_heads * self.value_dim)
+            portions, table = ctx.sight_portions(self.window, self.chunk, self.keep_first, max(1, READ_BACK_BYTES // (2 * page_entries)))
+            room = max(portion.page_seq.numel() for portion in portions)
+            all_keys = ctx.buffer("attention.keys", (room, self.k_heads, PAGE_TOKENS, self.head_dim), torch.bfloat16)
+            all_values = ctx.buffer("attention.values", (room, self.num_kv_heads, self.value_dim, PAGE_TOKENS), torch.bfloat16)
+            for portion in portions:
+                keys, values = all_keys[:portion.page_seq.numel()], all_values[:portion.page_seq.numel()]
+                ops.cache_read_8bit(line.keys, line.key_scales, line.values, line.value_scales, line.page_table, portion.page_seq, portion.page_index,
+                                    ctx.seq_slot, ctx.seq_start, ctx.seq_q_len, keys, values)
+                done, gate_left = self._attend_pages(ctx, q, keys, values, table, ctx.seq_rows, ctx.tok_seq, out, maps_out, gate,
+                                                     portion if len(portions) > 1 else None, common, difference)
+            gate = gate_left
+        if gate is not None:
+            ops.head_gate(out, gate, self.num_heads, self.value_dim)
+        if done is not out:
+            ops.map_difference(done, out, heads=self.num_heads, kv_heads=self.num_kv_heads, v_dim=self.value_dim, **difference)
+
+    def _attend_pages(self, ctx, q, keys, values, table, seq_slot, tok_slot, out, maps_out, gate, portion, common, difference):
+        """:meth:`attend` over pages in the model's dtype, of all of the step's sequences or of a portion's.  Returns where the result lies (``out``, or
+        ``maps_out`` where the difference of two maps is left to take) and the gates if they are left to apply."""
+        both = self.softcap is not None and self.slopes is not None     # the tcgen05 kernel has either, not both
         if self.tensor_cores and not both:
             if ctx.is_decode and self.num_heads // self.num_kv_heads <= 16:
                 chunks = (ctx.max_kv_len + ops.ATTENTION_CHUNK - 1) // ops.ATTENTION_CHUNK
@@ -313,26 +331,25 @@ class GQAAttention(Mixer):
                 decode = ops.attention_decode_tma if self.head_dim in ops.TC_ATTENTION_HEAD_DIMS else ops.attention_decode_mma
                 decode(q, keys, values, table, ctx.seq_start, seq_slot, part_o, part_ml, out,
                        max_chunks=chunks, difference=difference if self.maps == 2 else None, **common)
-                maps_out = out
-            elif self.head_dim in ops.TC_ATTENTION_HEAD_DIMS and ctx.max_q_len >= TC_ATTENTION_MIN_QUERIES:
+                return out, gate
+            if self.head_dim in ops.TC_ATTENTION_HEAD_DIMS and ctx.max_q_len >= TC_ATTENTION_MIN_QUERIES:
                 # prompts: 128 queries of one head per block, both products on tcgen05
-                tile_seq, tile_q0 = ctx.query_tiles(ops.TC_ATTENTION_QUERIES)
+                tile_seq, tile_q0 = ctx.query_tiles(ops.TC_ATTENTION_QUERIES, portion)
                 if self.maps == 2 and self.chunk is None and ops.attention_pair_takes(self.head_dim, self.value_dim):
                     # both maps, their difference and its norm in one kernel
                     ops.attention_pair_tc(q, keys, values, table, tile_seq, tile_q0, seq_slot, ctx.seq_start,
                                           ctx.seq_q_len, ctx.cu_q_len, out, heads=self.num_heads, v_heads=self.num_kv_heads,
                                           head_dim=self.head_dim, v_dim=self.value_dim, scale=self.softmax_scale, window=self.window,
                                           keep_first=self.keep_first, softcap=self.softcap, **difference)
-                    return
+                    return out, gate
                 ops.attention_prefill_tc(q, keys, values, table, tile_seq, tile_q0, seq_slot,
                                          ctx.seq_start, ctx.seq_q_len, ctx.cu_q_len, maps_out, **common)
             else:
-                tile_seq, tile_q0 = ctx.query_tiles(16)
+                tile_seq, tile_q0 = ctx.query_tiles(16, portion)
                 ops.attention_prefill_mma(q, keys, values, table, tile_seq, tile_q0, seq_slot,
                                           ctx.seq_start, ctx.seq_q_len, ctx.cu_q_len, maps_out, **common)
-            if gate is not None:
-                ops.head_gate(out, gate, self.num_heads, self.value_dim)
-        elif self.float32_token and ctx.is_decode and ops.attention_f32_token_takes(self.head_dim, self.value_dim, ctx.num_seqs):
+            return maps_out, gate
+        if self.float32_token and ctx.is_decode and ops.attention_f32_token_takes(self.head_dim, self.value_dim, ctx.num_seqs):
             # float32: one token a sequence in chunks of keys side by side, prompts in tiles of queries; the general kernel, a
             # block per token, keeps the head sizes neither takes
             chunks = (ctx.max_kv_len + ops.ATTENTION_CHUNK - 1) // ops.ATTENTION_CHUNK
@@ -355,9 +372,9 @@ class GQAAttention(Mixer):
                 ops.attention_f32_tiles(q, keys, values, table, tile_seq, tile_q0, seq_slot, ctx.seq_start,
                                         ctx.seq_q_len, ctx.cu_q_len, maps_out, gate=gate, **common)
         else:
-            ops.attention_generic(q, keys, values, table, ctx.tok_pos, tok_slot, maps_out, gate=gate, **common)
-        if maps_out is not out:
-            ops.map_difference(maps_out, out, heads=self.num_heads, kv_heads=self.num_kv_heads, v_dim=self.value_dim, **difference)
+            rows = slice(None) if portion is None else ctx.tokens_of(portion)
+            ops.attention_generic(q[rows], keys, values, table, ctx.tok_pos[rows], tok_slot[rows], maps_out[rows], gate=gate if gate is None else gate[rows], **common)
+        return maps_out, None
 
 
 register_part("mixer", "gqa_attention", GQAAttention, replace=True)

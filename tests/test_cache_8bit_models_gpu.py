@@ -176,3 +176,25 @@ def test_command_line_and_replay(tmp_path):
     assert proc.returncode == 0, proc.stderr[-2000:]
     logits = np.fromfile(os.path.join(out, "0.f32"), dtype="<f4")
     assert int(logits.argmax()) == want[0]
+
+
+@pytest.mark.parametrize("design,name", MODELS)
+def test_pages_read_back_in_portions_give_the_same_bits(design, name, monkeypatch):
+    # steps that mix prompts with single tokens over longer histories, the read-back in one portion and in several
+    from fieldrun_b200.parts import attention
+    logits, rooms = [], []
+    for most in (attention.READ_BACK_BYTES, 1 << 17):
+        monkeypatch.setattr(attention, "READ_BACK_BYTES", most)
+        lm, config = model(design, name, "int8")
+        engine = lm.engine
+        rng = np.random.default_rng(11)
+        draw = lambda n: rng.integers(0, vocabulary(config), size=n).tolist()
+        slots = [engine.new_sequence() for _ in range(6)]
+        out = [engine.step(slots, [draw(n) for n in (400, 9, 200, 1, 130, 333)])]
+        out.append(engine.step(slots, [draw(n) for n in (1, 1, 70, 1, 1, 1)]))
+        out.append(engine.step(slots, [draw(n) for n in (1, 1, 1, 5, 1, 1)]))
+        engine.check()
+        logits.append(torch.cat(out).cpu())
+        rooms.append(sum(engine.workspace.buffer(n, (0,), torch.bfloat16).untyped_storage().nbytes() for n in ("attention.keys", "attention.values")))
+    assert torch.isfinite(logits[0]).all() and torch.equal(*logits)
+    assert rooms[1] < rooms[0]
