@@ -17,7 +17,8 @@
 //
 // Weights: p_j = 2^(s_j - m) with m a running maximum that follows a page's only beyond a margin.  The weight that multiplies codes is
 // w_j = p_j vs_j, rounded to float16 after division by a unit U per head, a power of two that follows the largest w seen: w / U is at most
-// 2^15, and full precision (2^-11) reaches down to 2^-22 of the largest.  The sum of the p_j stays in float32.
+// 2^15, and full precision (2^-11) reaches down to 2^-22 of the largest so far.  U only grows: where the running maximum has risen since, the outputs
+// shrink and U does not, so that beside an early value row 10^7 times the others these have fewer digits.  The sum of the p_j stays in float32.
 //
 // A page of 64 keys is one warp's work: its keys and values come by TMA into tiles of the warp's own, each announced on an mbarrier of
 // the warp's own.  Which key a row of the score tile stands for, and which dimension a row of the output tile, is free; both are
@@ -33,7 +34,8 @@
 //   their pages, and there is no last wave of a few blocks.  Where a head has room for too few partial results, cut between key heads only.
 //
 // Measured on a B200, 48 heads on 8 key heads of 128: 32 sequences of 4,096 keys 54 us (e4m3; 277 MB, 5.1 TB/s; 52 of them the pieces, issue slots 35 %
-// busy, 9 to 10 warps an SM; pages of bfloat16 take 92 us), one of 131,072 keys 54 us (int8), one of 2,048 keys 6.5 us.
+// busy, 9 to 10 warps an SM; pages of bfloat16 take 92 us), one of 131,072 keys 58 us (int8, issue slots 50 %
+// busy), one of 2,048 keys 6.5 us.
 //
 // Every wait on an mbarrier gives up after about a second and sets `status`; the warps then wait (with the same limit) for the copies
 // that are in flight and return.
@@ -47,7 +49,7 @@
 // for the smaller heads, 168).
 #define D8_RESIDENT(HD, VD, NT) ((NT) == 2 ? 2 : (HD) + (VD) <= 128 ? 4 : 3)
 #define D8_CHUNK_PAGES 4               // a chunk is 256 keys
-#define D8_LEAD 2                      // pages that a run costs as much time as, beside its own (64 ragged sequences in windows: 0 64 us, 2 43 us)
+#define D8_LEAD 2                      // pages that a run costs as much time as, beside its own (64 ragged sequences in windows: 0 59 us, 2 47 us)
 #define D8_RAISE 8.0f                  // the running maximum follows a page's maximum only beyond this margin (in units of log2)
 #define D8_STATUS_WAIT 7               // a wait gave up
 #define D8_STATUS_TOO_LONG 8           // a sequence has more keys than the launch was sized for
@@ -1133,7 +1135,8 @@ FRB_API int frb_attention_decode_8bit(const void* q, const void* k_codes, const 
     // with the join, chunks | pieces: 64 blocks (1 x 2048) 6.5 | 17.0; 256 (1 x 8192) 10.0 | 16.5; 512 (4 x 4096) 18.0 | 17.5, (8 x 2048) 17.8 | 19.0;
     // 1,024 (8 x 4096) 25.7 | 21.3; 2,048 (8 x 8192) 40.9 | 31.2, (128 x 512, cut between key heads) 44.9 | 37.2; 4,096 (32 x 4096) 69.9 | 53.7,
     // (1 x 131072) 78.9 | 53.6; 8,192 blocks with a page each (1024 x 40) 142 | 76.  Heads of 64: 1,024 (8 x 4096) 16.3 | 17.5, 2,048 (8 x 8192)
-    // 24.3 | 21.1, (128 x 512) 27.0 | 31.9, 4,096 (32 x 4096) 40.0 | 35.2.
+    // 24.3 | 21.1, (128 x 512) 27.0 | 31.9, 4,096 (32 x 4096) 40.0 | 35.2.  The rule counts the blocks that there may be (max_chunks), not the pages that are in
+    // sight: it takes pieces for the 128 x 512 of heads of 64, and for a window far shorter than what max_chunks stands for.
     const int resident = D8_RESIDENT(head_dim, v_dim, per_block / 8) * frb_sm_count();
     const long long chunks = (long long)num_seqs * num_kv_heads * head_tiles * max_chunks;
     const bool countable = chunks * D8_CHUNK_PAGES < (1ll << 30);

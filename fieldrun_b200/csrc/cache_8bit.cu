@@ -204,7 +204,7 @@ __device__ __forceinline__ void write_queries_and_keys(const Write8Params& p, co
 // instructions, 115 a warp and 128 entries.  (Rows held in registers, eight spans a warp unrolled, took three times as many.)  Measured on a B200 with
 // MiniMax-M2's rows of 8,192 entries: 1 token 4.3 us, 64 tokens 4.5 us, a prompt of 2,048 31 us (3.1 TB/s; issue slots 46 % busy, the loads of norm
 // weights and angles the largest stall).
-// LEAN: rows and weights in float32, no bias.
+// LEAN: rows and weights in float32, no bias.  (The other form, for everything else, spills 68 to 108 bytes a thread; it was not timed.)
 template <int HD, int VD, int THREADS, int RESIDENT, bool LEAN>
 __global__ void __launch_bounds__(THREADS, RESIDENT) qkv_prepare_8bit_kernel(Write8Params p) {
     let_next_kernel_start();
@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(THREADS, RESIDENT) qkv_prepare_8bit_kernel(Wri
     }
 }
 
-// Up to this many tokens a block has a warp for every two spans, up to 32; beyond, as many blocks as are resident take the tokens in turn.
+// Up to this many tokens (two for each of a B200's 148 SMs) a block has a warp for every two spans, up to 32; beyond, as many blocks as are resident take
+// the tokens in turn.
 #define WRITE8_FEW_TOKENS 296
 
 FRB_API int frb_qkv_prepare_8bit(const void* qkv, int in_dtype, const void* q_weight, const void* k_weight, int weight_dtype, float eps,
