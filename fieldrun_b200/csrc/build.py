@@ -37,6 +37,7 @@ GROUPS: dict[str, tuple[str, ...]] = {
     "streams": ("experts_stream.cu", "experts_mma.cu", "rows_f32.cu"),
     "experts": ("routing.cu", "experts_generic.cu"),
     "products": ("experts_tc.cu",),
+    "products8": ("linear_8bit.cu", "products_8bit.cu", "rows_8bit.cu"),
     "products32": ("products_f32.cu",),
     "recurrent": ("gla.cu", "gla_chunks.cu"),
     "scans": ("scans.cu", "state_space_chunks.cu"),

@@ -1,0 +1,124 @@
+// The operators on 8-bit weights, each one call: a linear layer, a gated feed-forward block, routed experts.  The kernels are in
+// rows_8bit.cu and products_8bit.cu; what passes between them lies in the caller's scratch.
+#include "cache_8bit.cuh"          // call_packed
+#include "products_8bit.cuh"
+
+using namespace frb_products8;
+
+// Runs of the scratch, each from a 256-byte boundary on.
+struct Scratch {
+    char* base;
+    long long at = 0;
+    explicit Scratch(void* p) : base((char*)p) {}
+    template <typename T> T* take(long long count) {
+        T* here = reinterpret_cast<T*>(base + at);
+        at += (count * (long long)sizeof(T) + 255) / 256 * 256;
+        return here;
+    }
+};
+
+#define FRB_TRY(call)                         \
+    do {                                      \
+        const int status_ = (call);           \
+        if (status_ != 0) return status_;     \
+    } while (0)
+
+// out [T, F] = x [T, K] W^T; W as codes [F up to 16][K up to 128] with scales [F up to 16].  scratch: T (K up to 128) + 4 T bytes, each run
+// up to 256.
+FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void* w, const float* w_scale, int F, void* out, int out_type, void* scratch,
+                            long long scratch_bytes, int* status, cudaStream_t stream) {
+    if (T == 0) return 0;
+    Scratch s(scratch);
+    int8_t* codes = s.take<int8_t>((long long)T * up_to(K, FRB_8BIT_KBLOCK));
+    float* scales = s.take<float>(T);
+    FRB_CHECK_ARG(s.at <= scratch_bytes, "linear in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
+    FRB_TRY(rows_codes(x, x_type, T, K, nullptr, 1, codes, scales, stream));
+    Product p = {};
+    p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K;
+    p.x = codes; p.x_scale = scales; p.rows = T; p.out = out; p.out_type = out_type; p.status = status;
+    return product(p, stream);
+}
+
+// The two products of gated units over rows of codes: hidden [N, I] float32, then y [N, d].
+static int unit(const int8_t* codes, const float* scales, int N, int d, int I, int experts, const Lists& lists, const void* w_in, const float* in_scale,
+                const void* w_down, const float* down_scale, int gate, float limit, float* hidden, int8_t* hidden_codes, float* hidden_scales, void* y,
+                int y_type, int* status, cudaStream_t stream) {
+    Product p = {};
+    p.w = w_in; p.w_scale = in_scale; p.experts = experts; p.parts = 2; p.F = I; p.K = d;
+    p.x = codes; p.x_scale = scales; p.rows = N; p.lists = lists; p.out = hidden; p.out_type = FRB_F32; p.gate = gate; p.limit = limit; p.status = status;
+    FRB_TRY(product(p, stream));
+    FRB_TRY(rows_codes(hidden, FRB_F32, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
+    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I;
+    p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y; p.out_type = y_type;
+    return product(p, stream);
+}
+
+// h = act(x Wg^T) * (x Wu^T) in float32, rounded to codes row by row, out [T, d] = h Wd^T.  w_in: codes [2][I up to 16][d up to 128] (gate, up),
+// w_down: [d up to 16][I up to 128].
+FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* w_in, const float* in_scale, int I, const void* w_down,
+                           const float* down_scale, int gate, float limit, void* out, int out_type, void* scratch, long long scratch_bytes, int* status,
+                           cudaStream_t stream) {
+    if (T == 0) return 0;
+    FRB_CHECK_ARG(gate == FRB_GATE_SILU || gate == FRB_GATE_GELU_TANH, "gated block in 8 bits: activation %d", gate);
+    Scratch s(scratch);
+    int8_t* codes = s.take<int8_t>((long long)T * up_to(d, FRB_8BIT_KBLOCK));
+    float* scales = s.take<float>(T);
+    float* hidden = s.take<float>((long long)T * I);
+    int8_t* hidden_codes = s.take<int8_t>((long long)T * up_to(I, FRB_8BIT_KBLOCK));
+    float* hidden_scales = s.take<float>(T);
+    FRB_CHECK_ARG(s.at <= scratch_bytes, "gated block in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
+    FRB_TRY(rows_codes(x, x_type, T, d, nullptr, 1, codes, scales, stream));
+    return unit(codes, scales, T, d, I, 1, Lists{}, w_in, in_scale, w_down, down_scale, gate, limit, hidden, hidden_codes, hidden_scales, out, out_type,
+                status, stream);
+}
+
+// The experts' outputs y [N, d] (float32, in the order of the lists) for T tokens that were given their rows already: row_of_assign [T, top_k].
+// scratch as for frb_experts_8bit without lists and y.
+FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int top_k, const int* row_of_assign, const int* tile_expert, const int* tile_row0,
+                                 const int* num_tiles, const int* offsets, int max_tiles, int tile_rows, const void* w_in, const float* in_scale, int experts,
+                                 int I, const void* w_down, const float* down_scale, float limit, float* y, void* scratch, long long scratch_bytes, int* status,
+                                 cudaStream_t stream) {
+    if (T == 0) return 0;
+    FRB_CHECK_ARG((long long)T * top_k < (1ll << 31), "experts in 8 bits: %d tokens of %d experts", T, top_k);
+    const int N = T * top_k;
+    Scratch s(scratch);
+    int8_t* codes = s.take<int8_t>((long long)N * up_to(d, FRB_8BIT_KBLOCK));
+    float* scales = s.take<float>(N);
+    float* hidden = s.take<float>((long long)N * I);
+    int8_t* hidden_codes = s.take<int8_t>((long long)N * up_to(I, FRB_8BIT_KBLOCK));
+    float* hidden_scales = s.take<float>(N);
+    FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
+    FRB_TRY(rows_codes(x, x_type, T, d, row_of_assign, top_k, codes, scales, stream));
+    const Lists lists = {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows};
+    return unit(codes, scales, N, d, I, experts, lists, w_in, in_scale, w_down, down_scale, FRB_GATE_SILU, limit, hidden, hidden_codes, hidden_scales, y,
+                FRB_F32, status, stream);
+}
+
+// out [T, d] = sum over r of weights[t, r] * unit of expert ids[t, r] on x[t].  w_in: codes [experts][2][I up to 16][d up to 128], w_down:
+// [experts][d up to 16][I up to 128].
+FRB_API int frb_experts_8bit(const void* x, int x_type, int T, int d, int top_k, const int* ids, const float* weights, const void* w_in,
+                             const float* in_scale, int experts, int I, const void* w_down, const float* down_scale, float limit, int tile_rows, void* out,
+                             int out_type, void* scratch, long long scratch_bytes, int* status, cudaStream_t stream) {
+    if (T == 0) return 0;
+    FRB_CHECK_ARG((long long)T * top_k < (1ll << 31), "experts in 8 bits: %d tokens of %d experts", T, top_k);
+    FRB_CHECK_ARG(experts >= 1 && experts <= 8192, "experts in 8 bits: %d experts are outside 1..8192", experts);
+    FRB_CHECK_ARG(tile_rows >= 1, "experts in 8 bits: tiles of %d rows", tile_rows);
+    const int N = T * top_k, max_tiles = N / tile_rows + (experts < N ? experts : N);
+    Scratch s(scratch);
+    int* offsets = s.take<int>(experts + 1);
+    int* row_of_assign = s.take<int>(N);
+    int* tile_expert = s.take<int>(max_tiles);
+    int* tile_row0 = s.take<int>(max_tiles);
+    int* num_tiles = s.take<int>(1);
+    float* y = s.take<float>((long long)N * d);
+    FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, more are needed", scratch_bytes);
+    FRB_TRY(plan(ids, T, top_k, experts, tile_rows, offsets, row_of_assign, tile_expert, tile_row0, num_tiles, stream));
+    FRB_TRY(frb_expert_rows_8bit(x, x_type, T, d, top_k, row_of_assign, tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows, w_in, in_scale,
+                                 experts, I, w_down, down_scale, limit, y, s.base + s.at, scratch_bytes - s.at, status, stream));
+    return combine(y, weights, row_of_assign, T, top_k, d, out, out_type, stream);
+}
+
+FRB_API int frb_linear_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_linear_8bit, packed, stream); }
+FRB_API int frb_gated_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_gated_8bit, packed, stream); }
+FRB_API int frb_expert_rows_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_expert_rows_8bit, packed, stream); }
+FRB_API int frb_experts_8bit_packed(const void* packed, cudaStream_t stream) { return call_packed(frb_experts_8bit, packed, stream); }

@@ -79,6 +79,11 @@ _SIGNATURES = {
     "frb_qkv_prepare_8bit": "pippif" "ppi" "pppii" "ppppp" "ii" "iiiiiiiii" "i" "pfi" "ip",
     "frb_cache_read_8bit": "ppppi" "ipii" "ppi" "pppi" "pp" "iiii",
     "frb_attention_decode_8bit": "pppppi" "ipii" "pp" "ppp" "iiiiii" "f" "iii" "ii" "pp" "f" "pff" "ip",
+    "frb_rows_8bit": "piii" "pi" "pp",
+    "frb_linear_8bit": "piii" "ppi" "pi" "plp",
+    "frb_gated_8bit": "piii" "ppi" "pp" "if" "pi" "plp",
+    "frb_expert_rows_8bit": "piiii" "pppppii" "ppii" "pp" "f" "p" "plp",
+    "frb_experts_8bit": "piiii" "pp" "ppii" "pp" "fi" "pi" "plp",
     "frb_attention_pair_tc": "pippi" "pippi" "ppppp" "iiiifiif" "pffp",
     "frb_dyt_rows": "ppppp" "ppp" "pp" "iii" "p" "pppp" "pll",
     "frb_stream_copies": "pip" "pp" "ppppp" "ip" "ppp" "ppp" "pip" "iii",
@@ -103,7 +108,8 @@ _CTYPE = {"p": _P, "i": _I, "f": _F, "l": _L}
 
 # Entry points that also take their arguments as one C struct (``<name>_packed``), for which the interpreter needs a quarter of the time.
 _PACKED = {name: struct.Struct("@" + _SIGNATURES[name].replace("p", "P"))
-           for name in ("frb_qkv_prepare_8bit", "frb_cache_read_8bit", "frb_attention_decode_8bit")}
+           for name in ("frb_qkv_prepare_8bit", "frb_cache_read_8bit", "frb_attention_decode_8bit", "frb_linear_8bit", "frb_gated_8bit",
+                        "frb_expert_rows_8bit", "frb_experts_8bit")}
 
 
 class KernelError(RuntimeError):
@@ -127,6 +133,7 @@ _ENTRY_GROUPS = {
     "experts": ("frb_router_topk", "frb_expert_plan", "frb_expert_combine", "frb_expert_gemm_generic", "frb_route_plan_small",
                 "frb_router_small", "frb_router_logits", "frb_scaled_rows"),
     "products": ("frb_expert_gemm_tc", "frb_gather_rows_bf16"),
+    "products8": ("frb_rows_8bit", "frb_linear_8bit", "frb_gated_8bit", "frb_expert_rows_8bit", "frb_experts_8bit"),
     "products32": ("frb_weight_scales", "frb_split_rows", "frb_products_f32"),
     "recurrent": ("frb_gla_scan", "frb_gla_chunks"),
     "scans": ("frb_causal_conv", "frb_softplus_bias", "frb_selective_scan", "frb_gated_recurrence", "frb_state_space_scan", "frb_state_space_chunks", "frb_group_rms_norm",
@@ -221,7 +228,7 @@ def _stream() -> int:
 
 
 _LAUNCHES = 0
-_KERNELS_PER_CALL = {"frb_gated_delta_rule": 2, "frb_gated_recurrence": 2, "frb_sample_floor": 3, "frb_argmax_rows": 2, "frb_expert_plan": 3, "frb_attention_decode_mma": 2, "frb_attention_decode_tma": 2, "frb_attention_f32_token": 2, "frb_attention_decode_8bit": 2, "frb_gla_chunks": 3, "frb_state_space_chunks": 3, "frb_delta_chunks": 4, "frb_products_f32": 2, "frb_attention_f32_tc": 2}
+_KERNELS_PER_CALL = {"frb_gated_delta_rule": 2, "frb_gated_recurrence": 2, "frb_sample_floor": 3, "frb_argmax_rows": 2, "frb_expert_plan": 3, "frb_attention_decode_mma": 2, "frb_attention_decode_tma": 2, "frb_attention_f32_token": 2, "frb_attention_decode_8bit": 2, "frb_linear_8bit": 2, "frb_gated_8bit": 4, "frb_expert_rows_8bit": 4, "frb_experts_8bit": 6, "frb_gla_chunks": 3, "frb_state_space_chunks": 3, "frb_delta_chunks": 4, "frb_products_f32": 2, "frb_attention_f32_tc": 2}
 
 
 def launches() -> int:
@@ -1617,6 +1624,11 @@ _WAIT_CODES = {
     26: "latent attention: the softmax waiting for the scores",
     27: "latent attention: the correction waiting for the page before",
     28: "latent attention: the epilogue waiting for the last page",
+    121: "8-bit products: the producer waiting for a free stage",
+    122: "8-bit products: the producer waiting for its last stages",
+    123: "8-bit products: the MMA warp waiting for sums to have been read",
+    124: "8-bit products: the MMA warp waiting for a loaded stage",
+    125: "8-bit products: the epilogue waiting for finished sums",
     99: "the wait probe, whose wait is meant to run out",
 }
 
@@ -1918,6 +1930,187 @@ def attention_decode_8bit(q: torch.Tensor, k_pages: torch.Tensor, k_scales: torc
     _call("frb_attention_decode_8bit", *at[:5], store[0], store[1], at[5], *page_table.shape, *at[6:11], seqs, num_heads, num_kv_heads,
           num_kv_heads // maps, head_dim, v_dim, float(scale), window, chunk, keep_first, max_chunks, int(pieces or 0), at[11], at[12],
           float(softcap or 0.0), lam, eps, factor, int(pages_final), _ptr(tc_status(q.device)))
+
+
+# ------------------------------------------------------------------------------------------------ products in 8-bit integers
+
+EIGHT_BIT_KBLOCK = 128          # a row of codes is filled up with zeros to a multiple of this many entries
+EIGHT_BIT_ROWS = 16             # the rows of a weight of codes to a multiple of this many
+EIGHT_BIT_MOST_INNER = 131072   # 127^2 times as many stay below 2^31
+GATES_8BIT = {"silu": 0, "gelu_tanh": 1}
+EXPERT_TILES_8BIT = (8, 16, 32, 64, 128, 256)      # rows of one expert that a tile may take
+
+
+def _up(n: int, step: int) -> int:
+    return -(-n // step) * step
+
+
+def weight_8bit_shape(experts: int, parts: int, features: int, inner: int) -> tuple[int, int, int, int]:
+    """The shape of a weight's codes; its scales have the first three sizes."""
+    return experts, parts, _up(features, EIGHT_BIT_ROWS), _up(inner, EIGHT_BIT_KBLOCK)
+
+
+def rows_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> None:
+    """Rows of float32 or bfloat16 [rows, inner] as int8 ``codes`` [rows, inner up to 128] and float32 ``scales`` [rows]:
+    scale = max |x| / 127, code = 127 x / max |x| rounded half to even (exactly: a value in the middle goes to the even code), the
+    entries behind the row zero.  A row whose largest entry is below 2^-96 is stored as zeros with scale zero; one with an
+    entry that is not finite as zeros with scale NaN, so that every product with it is NaN."""
+    if x.dim() != 2 or not 1 <= x.shape[1] <= EIGHT_BIT_MOST_INNER:
+        raise KernelError(f"rows of shape {list(x.shape)}: 8-bit rows are [rows, 1 to {EIGHT_BIT_MOST_INNER} entries]")
+    rows, inner = x.shape
+    _want(codes, torch.int8, "codes of rows")
+    _want(scales, torch.float32, "scales of rows")
+    if codes.shape != (rows, _up(inner, EIGHT_BIT_KBLOCK)) or scales.shape != (rows,):
+        raise KernelError(f"codes of shape {list(codes.shape)} with scales of {list(scales.shape)} for {rows} rows of {inner} entries: codes are "
+                          f"[{rows}, {_up(inner, EIGHT_BIT_KBLOCK)}], scales [{rows}]")
+    at = _addresses(x, codes, scales)
+    _call("frb_rows_8bit", at[0], _code(x.dtype), rows, inner, None, 1, at[1], at[2])
+
+
+def weight_8bit(*parts: torch.Tensor, codes: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """A weight's rows (one or two matrices [features, inner], gate and up; float32 or bfloat16) as codes [1, parts, features up to 16,
+    inner up to 128] with scales [1, parts, features up to 16], as the products take them: every row as :func:`rows_8bit` stores it.  ``codes``
+    and ``scales``: one expert's places in larger tensors (filled with zeros where no weights go)."""
+    features, inner = parts[0].shape if parts[0].dim() == 2 else (0, 0)
+    if not 1 <= len(parts) <= 2 or features < 1 or any(part.shape != (features, inner) for part in parts):
+        raise KernelError(f"weights of shapes {[list(part.shape) for part in parts]}: one matrix, or gate and up of one shape")
+    shape = weight_8bit_shape(1, len(parts), features, inner)
+    if codes is None:
+        codes = torch.zeros(shape, dtype=torch.int8, device=parts[0].device)
+        scales = torch.zeros(shape[:3], dtype=torch.float32, device=parts[0].device)
+    if codes.shape != shape or scales is None or scales.shape != shape[:3]:
+        raise KernelError(f"codes of shape {list(codes.shape)}, not {list(shape)}, for {len(parts)} matrices of {features} x {inner}")
+    for part, part_codes, part_scales in zip(parts, codes[0], scales[0]):
+        rows_8bit(part, part_codes[:features], part_scales[:features])
+    return codes, scales
+
+
+def _weight_8bit_of(what: str, codes: torch.Tensor, scales: torch.Tensor, experts: Optional[int], parts: int, features: int, inner: int) -> None:
+    shape = codes.shape
+    if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
+        raise KernelError(f"{what}: codes are int8 and scales float32, found {codes.dtype} and {scales.dtype}")
+    if len(shape) != 4 or shape[1] != parts or shape[2] != -(-features // 16) * 16 or shape[3] != -(-inner // 128) * 128 or shape[0] < 1 \
+            or (experts is not None and shape[0] != experts) or scales.shape != shape[:3]:
+        wanted = list(weight_8bit_shape(experts or 1, parts, features, inner))
+        raise KernelError(f"{what}: codes of shape {list(shape)} with scales of {list(scales.shape)}, not {wanted if experts else ['experts'] + wanted[1:]} "
+                          f"with scales of the first three sizes")
+
+
+def _rows_in_and_out(x: torch.Tensor, out: torch.Tensor, features: Optional[int]) -> tuple[int, int, int]:
+    if x.dim() != 2 or out.dim() != 2 or x.shape[0] != out.shape[0] or not 1 <= x.shape[1] <= EIGHT_BIT_MOST_INNER or out.shape[1] < 1 \
+            or (features is not None and out.shape[1] != features):
+        raise KernelError(f"rows of shape {list(x.shape)} with results of {list(out.shape)}")
+    return x.shape[0], x.shape[1], out.shape[1]
+
+
+def _scratch_8bit(scratch: Optional[torch.Tensor], need: int, device) -> torch.Tensor:
+    if scratch is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    if scratch.dtype is not torch.uint8 or scratch.numel() < need:
+        raise KernelError(f"{scratch.numel()} entries of {scratch.dtype} as scratch: {need} bytes (uint8) are needed")
+    return scratch
+
+
+def linear_8bit_scratch(rows: int, inner: int) -> int:
+    """Bytes of scratch that :func:`linear_8bit` needs."""
+    return _up(rows * _up(inner, EIGHT_BIT_KBLOCK), 256) + _up(4 * rows, 256)
+
+
+def linear_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, *, scratch: Optional[torch.Tensor] = None) -> None:
+    """out [T, F] = x [T, K] W^T in 8-bit integers: the tokens' rows (float32 or bfloat16) are rounded to codes as :func:`rows_8bit` does,
+    W is codes [1, 1, F up to 16, K up to 128] with scales (:func:`weight_8bit`), sums are exact, and out (float32 or bfloat16) is
+    scale of the token * scale of the channel * sum.  A row's results depend on that row alone, to the last bit.  ``scratch``: uint8 of
+    :func:`linear_8bit_scratch` bytes, for the call's own use."""
+    rows, inner, features = _rows_in_and_out(x, out, None)
+    _weight_8bit_of("linear_8bit", codes, scales, 1, 1, features, inner)
+    scratch = _scratch_8bit(scratch, linear_8bit_scratch(rows, inner), x.device)
+    at = _addresses(x, codes, scales, out, scratch)
+    _call("frb_linear_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], features, at[3], _code(out.dtype), at[4], scratch.numel(),
+          _ptr(tc_status(x.device)))
+
+
+def gated_8bit_scratch(rows: int, inner: int, width: int) -> int:
+    """Bytes of scratch that :func:`gated_8bit` needs."""
+    return linear_8bit_scratch(rows, inner) + _up(4 * rows * width, 256) + linear_8bit_scratch(rows, width)
+
+
+def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor, out: torch.Tensor, *,
+               width: int, activation: str = "silu", gate_limit: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
+    """A gated feed-forward block in 8-bit integers: h = act(x W_gate^T) * (x W_up^T) with ``activation`` silu or gelu_tanh (``gate_limit`` > 0:
+    the clamped gate, as in the expert products), out [T, d] = h W_down^T.  Both products are as in :func:`linear_8bit`; h is made in float32
+    and rounded to codes row by row.  ``in_codes`` [1, 2, width up to 16, d up to 128] (gate, up), ``down_codes`` [1, 1, d up to 16, width up to 128]."""
+    rows, inner, _ = _rows_in_and_out(x, out, x.shape[-1])
+    if not 1 <= width <= EIGHT_BIT_MOST_INNER or activation not in GATES_8BIT or gate_limit < 0.0 or (gate_limit > 0.0 and activation != "silu"):
+        raise KernelError(f"gated_8bit: a width of {width}, activation {activation!r} and a gate limit of {gate_limit}")
+    _weight_8bit_of("gated_8bit, gate and up", in_codes, in_scales, 1, 2, width, inner)
+    _weight_8bit_of("gated_8bit, down", down_codes, down_scales, 1, 1, inner, width)
+    scratch = _scratch_8bit(scratch, gated_8bit_scratch(rows, inner, width), x.device)
+    at = _addresses(x, in_codes, in_scales, down_codes, down_scales, out, scratch)
+    _call("frb_gated_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], width, at[3], at[4], GATES_8BIT[activation], float(gate_limit), at[5],
+          _code(out.dtype), at[6], scratch.numel(), _ptr(tc_status(x.device)))
+
+
+def expert_tile_rows_8bit(assignments: int, experts: int) -> int:
+    """Rows of a tile of the 8-bit expert products: most experts' rows fit one."""
+    return next((t for t in EXPERT_TILES_8BIT if t * experts >= 1.3 * assignments), EXPERT_TILES_8BIT[-1])
+
+
+def expert_rows_8bit_scratch(tokens: int, top_k: int, inner: int, width: int) -> int:
+    """Bytes of scratch that :func:`expert_rows_8bit` needs."""
+    return gated_8bit_scratch(tokens * top_k, inner, width)
+
+
+def experts_8bit_scratch(tokens: int, top_k: int, experts: int, inner: int, width: int) -> int:
+    """Bytes of scratch that :func:`experts_8bit` needs."""
+    n = tokens * top_k
+    tiles = n // expert_tile_rows_8bit(n, experts) + min(experts, n)
+    return (_up(4 * (experts + 1), 256) + _up(4 * n, 256) + 2 * _up(4 * tiles, 256) + 256 + _up(4 * n * inner, 256)
+            + expert_rows_8bit_scratch(tokens, top_k, inner, width))
+
+
+def expert_rows_8bit(x: torch.Tensor, row_of_assign: torch.Tensor, lists: tuple, max_tiles: int, tile_rows: int, in_codes: torch.Tensor,
+                     in_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor, y: torch.Tensor, *, width: int,
+                     gate_limit: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
+    """The gated blocks (:func:`gated_8bit`) of a step's experts: ``y[row_of_assign[t * top_k + r]]`` (float32 [T * top_k, d]) becomes the block
+    of token t's expert of rank r on x[t].  ``lists`` = (tile_expert, tile_row0, num_tiles, offsets) as :func:`expert_plan` makes them with tiles of
+    ``tile_rows`` (a value of ``EXPERT_TILES_8BIT``); ``in_codes`` [E, 2, width up to 16, d up to 128], ``down_codes`` [E, 1, d up to 16, width up to 128]."""
+    if x.dim() != 2 or x.shape[0] < 1 or row_of_assign.numel() % x.shape[0] or y.shape != (row_of_assign.numel(), x.shape[1]):
+        raise KernelError(f"rows of shape {list(x.shape)} with {row_of_assign.numel()} rows of experts and results of {list(y.shape)}")
+    tokens, inner = x.shape
+    top_k = row_of_assign.numel() // tokens
+    if tile_rows not in EXPERT_TILES_8BIT or max_tiles < 1 or not 1 <= width <= EIGHT_BIT_MOST_INNER or gate_limit < 0.0 or not 1 <= top_k <= 128:
+        raise KernelError(f"expert_rows_8bit: {max_tiles} tiles of {tile_rows} rows, a width of {width}, {top_k} experts a token, a gate limit of {gate_limit}")
+    _want(y, torch.float32, "expert outputs")
+    _want_ints("lists of the experts' rows", row_of_assign, *lists)
+    _weight_8bit_of("expert_rows_8bit, gate and up", in_codes, in_scales, None, 2, width, inner)
+    _weight_8bit_of("expert_rows_8bit, down", down_codes, down_scales, in_codes.shape[0], 1, inner, width)
+    if lists[0].numel() < max_tiles or lists[1].numel() < max_tiles or lists[2].numel() != 1 or lists[3].numel() != in_codes.shape[0] + 1:
+        raise KernelError(f"expert_rows_8bit: lists of {[t.numel() for t in lists]} entries for {max_tiles} tiles of {in_codes.shape[0]} experts")
+    scratch = _scratch_8bit(scratch, expert_rows_8bit_scratch(tokens, top_k, inner, width), x.device)
+    at = _addresses(x, row_of_assign, *lists, in_codes, in_scales, down_codes, down_scales, y, scratch)
+    _call("frb_expert_rows_8bit", at[0], _code(x.dtype), tokens, inner, top_k, *at[1:6], max_tiles, tile_rows, at[6], at[7], in_codes.shape[0], width,
+          at[8], at[9], float(gate_limit), at[10], at[11], scratch.numel(), _ptr(tc_status(x.device)))
+
+
+def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor,
+                 down_scales: torch.Tensor, out: torch.Tensor, *, width: int, gate_limit: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
+    """Routed experts in 8-bit integers: out[t] = sum over r of ``weights[t, r]`` * (gated block of expert ``ids[t, r]`` on x[t]), the
+    blocks as :func:`expert_rows_8bit` computes them, their sum in float32 in the order of r, rounded once to out's type.  ``ids`` int32 and
+    ``weights`` float32 [T, top_k]; an id that names no expert (-1) adds nothing."""
+    tokens, inner, _ = _rows_in_and_out(x, out, x.shape[-1])
+    if ids.dim() != 2 or ids.shape[0] != tokens or weights.shape != ids.shape or not 1 <= ids.shape[1] <= 128:
+        raise KernelError(f"ids of shape {list(ids.shape)} and weights of {list(weights.shape)} for {tokens} tokens (1 to 128 experts each)")
+    _want_ints("the experts' ids", ids)
+    _want(weights, torch.float32, "the experts' weights")
+    if not 1 <= width <= EIGHT_BIT_MOST_INNER or gate_limit < 0.0:
+        raise KernelError(f"experts_8bit: a width of {width} and a gate limit of {gate_limit}")
+    _weight_8bit_of("experts_8bit, gate and up", in_codes, in_scales, None, 2, width, inner)
+    experts, top_k = in_codes.shape[0], ids.shape[1]
+    _weight_8bit_of("experts_8bit, down", down_codes, down_scales, experts, 1, inner, width)
+    scratch = _scratch_8bit(scratch, experts_8bit_scratch(tokens, top_k, experts, inner, width), x.device)
+    at = _addresses(x, ids, weights, in_codes, in_scales, down_codes, down_scales, out, scratch)
+    _call("frb_experts_8bit", at[0], _code(x.dtype), tokens, inner, top_k, at[1], at[2], at[3], at[4], experts, width, at[5], at[6], float(gate_limit),
+          expert_tile_rows_8bit(tokens * top_k, experts), at[7], _code(out.dtype), at[8], scratch.numel(), _ptr(tc_status(x.device)))
 
 
 def wait_probe(device, limit_cycles: int = 100_000) -> int:

@@ -1,0 +1,252 @@
+// Rows as 8-bit codes with a scale, and what routed experts need around their products: lists of each expert's rows, and the sum over
+// a token's experts.
+#include "products_8bit.cuh"
+
+namespace frb_products8 {
+
+// ----------------------------------------------------------------------------- rows as codes
+
+#define RC_KEPT 4                      // runs of 8 entries that a thread keeps in registers; what is beyond is read a second time (from L1)
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int left, bool whole, float (&v)[8]) {
+    if (whole) {
+        const float4 a = load4(p), b = load4(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
+}
+template <>
+__device__ __forceinline__ void load8<bf16>(const bf16* p, int left, bool whole, float (&v)[8]) {
+    if (whole) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
+}
+
+// The magnitude's bits order like the magnitudes, with infinities and NaN above all numbers.
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    return top;
+}
+
+// 127 x / a rounded half to even, exactly: x * (127 / a) in float32 is off by less than 127 * 2^-22.4 = 2.3e-5, so a product farther than
+// 1e-4 from the middle of two codes is on the right side; a nearer one is made again in 64 bits, where 127 x is exact and a quotient of
+// numbers of 31 and 24 bits that is not a middle is farther from one than the division's rounding (2^-25 against 2^-46).
+__device__ __forceinline__ int code_of(float x, float factor, float top) {
+    const float v = x * factor, r = rintf(v);
+    if (fabsf(fabsf(v - r) - 0.5f) > 1e-4f) return (int)r;
+    return (int)rint((double)x * 127.0 / (double)top);
+}
+
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float factor, float top) {
+    if (factor == 0.f) return make_uint2(0u, 0u);
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w[h] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[h] |= ((uint32_t)code_of(v[4 * h + i], factor, top) & 0xffu) << (8 * i);
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// A block takes a row at a time.  Bound by memory where there are many rows, by two trips to it and the block's maximum where there are
+// few.  `places`: row t goes to the rows places[t * copies + c] of the result (negative: nowhere), else to row t.
+template <typename T, int BLOCK>
+__global__ void __launch_bounds__(BLOCK)
+rows_8bit_kernel(const T* __restrict__ x, int rows, int K, int KP, const int* __restrict__ places, int copies, int8_t* __restrict__ codes,
+                 float* __restrict__ scales, int whole_rows) {
+    __shared__ uint32_t warp_top[2][BLOCK / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    wait_for_previous_kernel();
+    let_next_kernel_start();           // after the wait: the kernel after this one may read ahead what kernels before this one wrote
+    int turn = 0;
+    for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+        const T* src = x + (size_t)row * K;
+        float kept[RC_KEPT][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < RC_KEPT; ++j) {
+            const int k = (j * BLOCK + threadIdx.x) * 8;
+            if (k < K) { load8(src + k, K - k, whole_rows, kept[j]); }
+            else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) kept[j][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < RC_KEPT; ++j) top = top_of(kept[j], top);
+        for (int k = (RC_KEPT * BLOCK + threadIdx.x) * 8; k < K; k += BLOCK * 8) {
+            float v[8];
+            load8(src + k, K - k, whole_rows, v);
+            top = top_of(v, top);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) warp_top[turn][warp] = top;
+        __syncthreads();               // (two sets of maxima in turn: a warp that is ahead writes the other)
+        top = __reduce_max_sync(0xffffffffu, lane < BLOCK / 32 ? warp_top[turn][lane] : 0u);
+        const float a = __uint_as_float(top);
+        float factor = 0.f, scale = 0.f;
+        if (top >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
+        else if (a >= FRB_8BIT_SMALLEST_ROW) { factor = __fdiv_rn(127.f, a); scale = __fdiv_rn(a, 127.f); }
+        const int first = places ? 0 : row, count = places ? copies : 1;
+        const auto put = [&](int k, uint2 c) {
+            for (int i = 0; i < count; ++i) {
+                const int to = places ? places[(size_t)row * copies + i] : first;
+                if (to >= 0) *reinterpret_cast<uint2*>(codes + (size_t)to * KP + k) = c;
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < RC_KEPT; ++j) {
+            const int k = (j * BLOCK + threadIdx.x) * 8;
+            if (k < KP) put(k, codes_of(kept[j], factor, a));
+        }
+        for (int k = (RC_KEPT * BLOCK + threadIdx.x) * 8; k < KP; k += BLOCK * 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+            if (k < K) load8(src + k, K - k, whole_rows, v);
+            put(k, codes_of(v, factor, a));
+        }
+        if (threadIdx.x < count) {
+            const int to = places ? places[(size_t)row * copies + threadIdx.x] : first;
+            if (to >= 0) scales[to] = scale;
+        }
+    }
+}
+
+int rows_codes(const void* x, int x_type, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream) {
+    if (rows == 0) return 0;
+    FRB_CHECK_ARG(K >= 1 && K <= FRB_8BIT_MOST_INNER, "rows in 8 bits: %d entries are outside 1..%d", K, FRB_8BIT_MOST_INNER);
+    FRB_CHECK_ARG(copies >= 1 && copies <= 128, "rows in 8 bits: %d places a row are outside 1..128", copies);
+    FRB_CHECK_ARG(((uintptr_t)codes & 15) == 0, "rows in 8 bits: codes start on 16 bytes");
+    const int KP = up_to(K, FRB_8BIT_KBLOCK);
+    // 16-byte loads where every row starts on 16 bytes and is a whole number of runs of 8 entries
+    const int whole = K % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    const dim3 grid((unsigned)(rows < (1 << 20) ? rows : 1 << 20));
+    FRB_DISPATCH_DTYPE(x_type, T, {
+        if (K <= 128 * 8 * RC_KEPT && rows > 2 * frb_sm_count())
+            launch_dependent(rows_8bit_kernel<T, 128>, grid, dim3(128), 0, stream, (const T*)x, rows, K, KP, places, copies, (int8_t*)codes, scales, whole);
+        else
+            launch_dependent(rows_8bit_kernel<T, 512>, grid, dim3(512), 0, stream, (const T*)x, rows, K, KP, places, copies, (int8_t*)codes, scales, whole);
+    });
+    FRB_RETURN_LAUNCH("rows_8bit");
+}
+
+// ----------------------------------------------------------------------------- lists of the experts' rows
+
+#define PLAN_THREADS 1024
+
+// One block counts the assignments of every expert, gives each expert its run of rows and its tiles, and every assignment a row of its
+// expert's run.  Which of them comes first there is left to chance: every row's results depend on that row alone.  An id that
+// names no expert gets the row -1: nothing is computed for it and nothing added.
+__global__ void __launch_bounds__(PLAN_THREADS)
+plan_kernel(const int* __restrict__ ids, int assignments, int experts, int tile_rows, int* __restrict__ offsets, int* __restrict__ row_of_assign,
+            int* __restrict__ tile_expert, int* __restrict__ tile_row0, int* __restrict__ num_tiles) {
+    extern __shared__ int next_row[];                       // [experts]: counts, then each expert's next row
+    __shared__ int warp_rows[32], warp_tiles[32], rows_before, tiles_before;
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e < experts; e += PLAN_THREADS) next_row[e] = 0;
+    if (threadIdx.x == 0) { rows_before = 0; tiles_before = 0; }
+    __syncthreads();
+    for (int a = threadIdx.x; a < assignments; a += PLAN_THREADS) {
+        const int e = ids[a];
+        if ((unsigned)e < (unsigned)experts) atomicAdd(&next_row[e], 1);
+    }
+    __syncthreads();
+    for (int base = 0; base < experts; base += PLAN_THREADS) {
+        const int e = base + threadIdx.x;
+        const int count = e < experts ? next_row[e] : 0, tiles = (count + tile_rows - 1) / tile_rows;
+        int rows_to = count, tiles_to = tiles;              // sums up to and with this expert
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int r = __shfl_up_sync(0xffffffffu, rows_to, o), t = __shfl_up_sync(0xffffffffu, tiles_to, o);
+            if (lane >= o) { rows_to += r; tiles_to += t; }
+        }
+        if (lane == 31) { warp_rows[warp] = rows_to; warp_tiles[warp] = tiles_to; }
+        __syncthreads();
+        int row = rows_before + rows_to - count, tile = tiles_before + tiles_to - tiles;
+        for (int w = 0; w < warp; ++w) { row += warp_rows[w]; tile += warp_tiles[w]; }
+        __syncthreads();                                    // all have read the sums before
+        if (threadIdx.x == PLAN_THREADS - 1) { rows_before = row + count; tiles_before = tile + tiles; }
+        if (e < experts) {
+            offsets[e] = row;
+            next_row[e] = row;
+            for (int i = 0; i < tiles; ++i) { tile_expert[tile + i] = e; tile_row0[tile + i] = row + i * tile_rows; }
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) { offsets[experts] = rows_before; num_tiles[0] = tiles_before; }
+    for (int a = threadIdx.x; a < assignments; a += PLAN_THREADS) {
+        const int e = ids[a];
+        row_of_assign[a] = (unsigned)e < (unsigned)experts ? atomicAdd(&next_row[e], 1) : -1;
+    }
+}
+
+int plan(const int* ids, int tokens, int top_k, int experts, int tile_rows, int* offsets, int* row_of_assign, int* tile_expert, int* tile_row0,
+         int* num_tiles, cudaStream_t stream) {
+    launch_dependent(plan_kernel, dim3(1), dim3(PLAN_THREADS), (size_t)experts * sizeof(int), stream, ids, tokens * top_k, experts, tile_rows, offsets,
+                     row_of_assign, tile_expert, tile_row0, num_tiles);
+    FRB_RETURN_LAUNCH("experts_8bit");
+}
+
+// ----------------------------------------------------------------------------- the sum over a token's experts
+
+// out[t] = sum over r of weights[t, r] * y[row_of_assign[t, r]] in the order of r, in float32 and rounded once; a rank without a row adds nothing.
+template <typename OutT, int V>
+__global__ void __launch_bounds__(256)
+combine_8bit_kernel(const float* __restrict__ y, const float* __restrict__ weights, const int* __restrict__ row_of_assign, int top_k, int width,
+                    OutT* __restrict__ out) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    const size_t t = blockIdx.x;
+    const int c = (blockIdx.y * 256 + threadIdx.x) * V;
+    if (c >= width) return;
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    for (int r = 0; r < top_k; ++r) {
+        const int row = row_of_assign[t * top_k + r];
+        if (row < 0) continue;
+        const float w = weights[t * top_k + r];
+        const float* src = y + (size_t)row * width + c;
+        if constexpr (V == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            sum[0] += w * v.x; sum[1] += w * v.y; sum[2] += w * v.z; sum[3] += w * v.w;
+        } else {
+            sum[0] += w * src[0];
+        }
+    }
+    if constexpr (V == 4) store4(out + t * width + c, make_float4(sum[0], sum[1], sum[2], sum[3]));
+    else out[t * width + c] = from_f32<OutT>(sum[0]);
+}
+
+int combine(const float* y, const float* weights, const int* row_of_assign, int tokens, int top_k, int width, void* out, int out_type,
+            cudaStream_t stream) {
+    const bool fours = width % 4 == 0 && (((uintptr_t)y | (uintptr_t)out) & 15) == 0;
+    const dim3 grid((unsigned)tokens, (unsigned)((width + (fours ? 1023 : 255)) / (fours ? 1024 : 256)));
+    FRB_CHECK_ARG(grid.y <= 65535, "experts in 8 bits: a width of %d exceeds the grid", width);
+    FRB_DISPATCH_DTYPE(out_type, OutT, {
+        if (fours) launch_dependent(combine_8bit_kernel<OutT, 4>, grid, dim3(256), 0, stream, y, weights, row_of_assign, top_k, width, (OutT*)out);
+        else launch_dependent(combine_8bit_kernel<OutT, 1>, grid, dim3(256), 0, stream, y, weights, row_of_assign, top_k, width, (OutT*)out);
+    });
+    FRB_RETURN_LAUNCH("experts_8bit");
+}
+
+}  // namespace frb_products8
+
+// Rows of x [rows, K] (float32 or bfloat16) as codes [.., K up to 128] and scales; row t goes to places[t * copies + c], or to row t.
+FRB_API int frb_rows_8bit(const void* x, int x_type, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream) {
+    return frb_products8::rows_codes(x, x_type, rows, K, places, copies, codes, scales, stream);
+}
