@@ -23,42 +23,41 @@ struct Scratch {
         if (status_ != 0) return status_;     \
     } while (0)
 
-// out [T, F] = x [T, K] W^T; W as codes [F up to 16][K up to 128] with scales [F up to 16].  scratch: T (K up to 128) + 4 T bytes, each run
-// up to 256.
-FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void* w, const float* w_scale, int F, void* out, int out_type, void* scratch,
-                            long long scratch_bytes, int* status, cudaStream_t stream) {
+// Rows and the product that reads them: one launch where the product rounds them itself, else rows as codes in the scratch first.  The kernel
+// that makes those lets the product start only after its own wait, so that the weights, whoever wrote them, are complete by then.
+static int rows_and_product(Product& p, const void* x, int x_type, int8_t* codes, float* scales, bool weights_final, cudaStream_t stream) {
+    if (!p.lists.tile_expert && tokens_fit(p.rows, p.K)) {
+        p.x = x; p.x_type = x_type; p.x_scale = nullptr; p.weights_final = weights_final;
+        return product(p, stream);
+    }
+    FRB_TRY(rows_codes(x, x_type, p.rows, p.K, nullptr, 1, codes, scales, stream));
+    p.x = codes; p.x_scale = scales; p.weights_final = true;
+    return product(p, stream);
+}
+
+// out [T, F] = x [T, K] W^T; W as codes [F up to 16][K up to 128] with scales [F up to 16].  weights_final: they were complete before the kernel
+// before this call began.  scratch: T (K up to 128) + 4 T bytes, each run up to 256.
+FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void* w, const float* w_scale, int F, void* out, int out_type,
+                            int weights_final, void* scratch, long long scratch_bytes, int* status, cudaStream_t stream) {
     if (T == 0) return 0;
+    FRB_CHECK_ARG(K >= 1 && K <= FRB_8BIT_MOST_INNER, "linear in 8 bits: %d entries are outside 1..%d", K, FRB_8BIT_MOST_INNER);
     Scratch s(scratch);
     int8_t* codes = s.take<int8_t>((long long)T * up_to(K, FRB_8BIT_KBLOCK));
     float* scales = s.take<float>(T);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "linear in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
-    FRB_TRY(rows_codes(x, x_type, T, K, nullptr, 1, codes, scales, stream));
     Product p = {};
-    p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K;
-    p.x = codes; p.x_scale = scales; p.rows = T; p.out = out; p.out_type = out_type; p.status = status;
-    return product(p, stream);
-}
-
-// The two products of gated units over rows of codes: hidden [N, I] float32, then y [N, d].
-static int unit(const int8_t* codes, const float* scales, int N, int d, int I, int experts, const Lists& lists, const void* w_in, const float* in_scale,
-                const void* w_down, const float* down_scale, int gate, float limit, float* hidden, int8_t* hidden_codes, float* hidden_scales, void* y,
-                int y_type, int* status, cudaStream_t stream) {
-    Product p = {};
-    p.w = w_in; p.w_scale = in_scale; p.experts = experts; p.parts = 2; p.F = I; p.K = d;
-    p.x = codes; p.x_scale = scales; p.rows = N; p.lists = lists; p.out = hidden; p.out_type = FRB_F32; p.gate = gate; p.limit = limit; p.status = status;
-    FRB_TRY(product(p, stream));
-    FRB_TRY(rows_codes(hidden, FRB_F32, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
-    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I;
-    p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y; p.out_type = y_type;
-    return product(p, stream);
+    p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K; p.rows = T; p.out = out; p.out_type = out_type; p.status = status;
+    return rows_and_product(p, x, x_type, codes, scales, weights_final != 0, stream);
 }
 
 // h = act(x Wg^T) * (x Wu^T) in float32, rounded to codes row by row, out [T, d] = h Wd^T.  w_in: codes [2][I up to 16][d up to 128] (gate, up),
 // w_down: [d up to 16][I up to 128].
 FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* w_in, const float* in_scale, int I, const void* w_down,
-                           const float* down_scale, int gate, float limit, void* out, int out_type, void* scratch, long long scratch_bytes, int* status,
-                           cudaStream_t stream) {
+                           const float* down_scale, int gate, float limit, void* out, int out_type, int weights_final, void* scratch,
+                           long long scratch_bytes, int* status, cudaStream_t stream) {
     if (T == 0) return 0;
+    FRB_CHECK_ARG(d >= 1 && d <= FRB_8BIT_MOST_INNER && I >= 1 && I <= FRB_8BIT_MOST_INNER, "gated block in 8 bits: %d entries, %d between, outside 1..%d", d, I,
+                  FRB_8BIT_MOST_INNER);
     FRB_CHECK_ARG(gate == FRB_GATE_SILU || gate == FRB_GATE_GELU_TANH, "gated block in 8 bits: activation %d", gate);
     Scratch s(scratch);
     int8_t* codes = s.take<int8_t>((long long)T * up_to(d, FRB_8BIT_KBLOCK));
@@ -67,9 +66,12 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     int8_t* hidden_codes = s.take<int8_t>((long long)T * up_to(I, FRB_8BIT_KBLOCK));
     float* hidden_scales = s.take<float>(T);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "gated block in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
-    FRB_TRY(rows_codes(x, x_type, T, d, nullptr, 1, codes, scales, stream));
-    return unit(codes, scales, T, d, I, 1, Lists{}, w_in, in_scale, w_down, down_scale, gate, limit, hidden, hidden_codes, hidden_scales, out, out_type,
-                status, stream);
+    Product p = {};
+    p.w = w_in; p.w_scale = in_scale; p.experts = 1; p.parts = 2; p.F = I; p.K = d; p.rows = T; p.out = hidden; p.out_type = FRB_F32; p.gate = gate;
+    p.limit = limit; p.status = status;
+    FRB_TRY(rows_and_product(p, x, x_type, codes, scales, weights_final != 0, stream));
+    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.out = out; p.out_type = out_type;
+    return rows_and_product(p, hidden, FRB_F32, hidden_codes, hidden_scales, true, stream);     // (the first product waited before it let this one start)
 }
 
 // The experts' outputs y [N, d] (float32, in the order of the lists) for T tokens that were given their rows already: row_of_assign [T, top_k].
@@ -89,9 +91,14 @@ FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int to
     float* hidden_scales = s.take<float>(N);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
     FRB_TRY(rows_codes(x, x_type, T, d, row_of_assign, top_k, codes, scales, stream));
-    const Lists lists = {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows};
-    return unit(codes, scales, N, d, I, experts, lists, w_in, in_scale, w_down, down_scale, FRB_GATE_SILU, limit, hidden, hidden_codes, hidden_scales, y,
-                FRB_F32, status, stream);
+    Product p = {};
+    p.w = w_in; p.w_scale = in_scale; p.experts = experts; p.parts = 2; p.F = I; p.K = d; p.rows = N; p.x = codes; p.x_scale = scales;
+    p.lists = {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows};
+    p.out = hidden; p.out_type = FRB_F32; p.gate = FRB_GATE_SILU; p.limit = limit; p.status = status; p.weights_final = true;
+    FRB_TRY(product(p, stream));
+    FRB_TRY(rows_codes(hidden, FRB_F32, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
+    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y;
+    return product(p, stream);
 }
 
 // out [T, d] = sum over r of weights[t, r] * unit of expert ids[t, r] on x[t].  w_in: codes [experts][2][I up to 16][d up to 128], w_down:

@@ -80,8 +80,8 @@ _SIGNATURES = {
     "frb_cache_read_8bit": "ppppi" "ipii" "ppi" "pppi" "pp" "iiii",
     "frb_attention_decode_8bit": "pppppi" "ipii" "pp" "ppp" "iiiiii" "f" "iii" "ii" "pp" "f" "pff" "ip",
     "frb_rows_8bit": "piii" "pi" "pp",
-    "frb_linear_8bit": "piii" "ppi" "pi" "plp",
-    "frb_gated_8bit": "piii" "ppi" "pp" "if" "pi" "plp",
+    "frb_linear_8bit": "piii" "ppi" "pi" "i" "plp",
+    "frb_gated_8bit": "piii" "ppi" "pp" "if" "pi" "i" "plp",
     "frb_expert_rows_8bit": "piiii" "pppppii" "ppii" "pp" "f" "p" "plp",
     "frb_experts_8bit": "piiii" "pp" "ppii" "pp" "fi" "pi" "plp",
     "frb_attention_pair_tc": "pippi" "pippi" "ppppp" "iiiifiif" "pffp",
@@ -1629,6 +1629,7 @@ _WAIT_CODES = {
     123: "8-bit products: the MMA warp waiting for sums to have been read",
     124: "8-bit products: the MMA warp waiting for a loaded stage",
     125: "8-bit products: the epilogue waiting for finished sums",
+    126: "8-bit products: the MMA warp waiting for the tokens' codes",
     99: "the wait probe, whose wait is meant to run out",
 }
 
@@ -2016,17 +2017,19 @@ def linear_8bit_scratch(rows: int, inner: int) -> int:
     return _up(rows * _up(inner, EIGHT_BIT_KBLOCK), 256) + _up(4 * rows, 256)
 
 
-def linear_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, *, scratch: Optional[torch.Tensor] = None) -> None:
+def linear_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, *, weights_final: bool = False,
+                scratch: Optional[torch.Tensor] = None) -> None:
     """out [T, F] = x [T, K] W^T in 8-bit integers: the tokens' rows (float32 or bfloat16) are rounded to codes as :func:`rows_8bit` does,
     W is codes [1, 1, F up to 16, K up to 128] with scales (:func:`weight_8bit`), sums are exact, and out (float32 or bfloat16) is
-    scale of the token * scale of the channel * sum.  A row's results depend on that row alone, to the last bit.  ``scratch``: uint8 of
-    :func:`linear_8bit_scratch` bytes, for the call's own use."""
+    scale of the token * scale of the channel * sum.  A row's results depend on that row alone, to the last bit.  ``weights_final`` (a promise):
+    codes and scales were complete before the kernel before this call in the stream began, so that they may be read while that one still
+    runs.  ``scratch``: uint8 of :func:`linear_8bit_scratch` bytes, for the call's own use."""
     rows, inner, features = _rows_in_and_out(x, out, None)
     _weight_8bit_of("linear_8bit", codes, scales, 1, 1, features, inner)
     scratch = _scratch_8bit(scratch, linear_8bit_scratch(rows, inner), x.device)
     at = _addresses(x, codes, scales, out, scratch)
-    _call("frb_linear_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], features, at[3], _code(out.dtype), at[4], scratch.numel(),
-          _ptr(tc_status(x.device)))
+    _call("frb_linear_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], features, at[3], _code(out.dtype), int(weights_final), at[4],
+          scratch.numel(), _ptr(tc_status(x.device)))
 
 
 def gated_8bit_scratch(rows: int, inner: int, width: int) -> int:
@@ -2035,7 +2038,8 @@ def gated_8bit_scratch(rows: int, inner: int, width: int) -> int:
 
 
 def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor, out: torch.Tensor, *,
-               width: int, activation: str = "silu", gate_limit: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
+               width: int, activation: str = "silu", gate_limit: float = 0.0, weights_final: bool = False,
+               scratch: Optional[torch.Tensor] = None) -> None:
     """A gated feed-forward block in 8-bit integers: h = act(x W_gate^T) * (x W_up^T) with ``activation`` silu or gelu_tanh (``gate_limit`` > 0:
     the clamped gate, as in the expert products), out [T, d] = h W_down^T.  Both products are as in :func:`linear_8bit`; h is made in float32
     and rounded to codes row by row.  ``in_codes`` [1, 2, width up to 16, d up to 128] (gate, up), ``down_codes`` [1, 1, d up to 16, width up to 128]."""
@@ -2047,7 +2051,7 @@ def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor,
     scratch = _scratch_8bit(scratch, gated_8bit_scratch(rows, inner, width), x.device)
     at = _addresses(x, in_codes, in_scales, down_codes, down_scales, out, scratch)
     _call("frb_gated_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], width, at[3], at[4], GATES_8BIT[activation], float(gate_limit), at[5],
-          _code(out.dtype), at[6], scratch.numel(), _ptr(tc_status(x.device)))
+          _code(out.dtype), int(weights_final), at[6], scratch.numel(), _ptr(tc_status(x.device)))
 
 
 def expert_tile_rows_8bit(assignments: int, experts: int) -> int:

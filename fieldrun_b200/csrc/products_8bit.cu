@@ -12,10 +12,13 @@
 // Blocks stay for the whole launch and take the tiles in turn.  One thread copies k-blocks (rows of 128 bytes, swizzled) of the tokens'
 // and the weights' codes into a ring of stages with TMA, running ahead into the next tile; one thread issues the MMAs; the sums of a tile
 // lie in one half of the tensor memory while eight warps read the other half's out.  With few tokens the weights are the traffic: their
-// first stages are asked for before the kernel before this one has ended (it makes the tokens' codes; whatever wrote weights or lists had
-// ended before that one let this one start).
+// first stages are asked for before the kernel before this one has ended where that is safe (weights_final), and up to eight tokens are
+// rounded to codes by every block for itself, into shared memory, while its first weights are on their way: one launch instead of two.
 //
 // Every wait on an mbarrier gives up after about a second, records a code in `status` and lets the block leave through the common exit.
+#include <cmath>
+#include <type_traits>
+
 #include "products_8bit.cuh"
 #include "tcgen05.cuh"
 
@@ -28,6 +31,15 @@ namespace frb_products8 {
 #define P8_THREADS (64 + 32 * P8_EPILOGUE_WARPS)
 #define P8_MAX_STAGES 16
 #define P8_SMEM (220 * 1024)
+
+// The gates in one form, g' sigmoid(g' (a + b g'^2)) (u' + add): silu a = 1, b = 0; tanh-gelu, 0.5 g (1 + tanh(z)) = g sigmoid(2 z) with
+// z = sqrt(2 / pi) (g + 0.044715 g^3); the clamped gate a = 1.702, g' = min(g, L), u' = clamp(u, -L, L), add 1.  NaN stays NaN.  The hardware's
+// exponential and reciprocal are off by 2 units in the last place each; the value is rounded to 8 bits next.  (One short form for all
+// gates: 32 copies of three with exact divisions were 100 KB of instructions, and one token's unit waited 24 us for them to be fetched.)
+struct Gate {
+    float a, b;            // times -log2(e)
+    float limit, add;      // infinity and 0 without a limit
+};
 
 struct Params {
     Lists lists;
@@ -46,8 +58,10 @@ struct Params {
     int tmem_columns;
     int row_tiles;         // without lists: tiles of tokens
     int channel_tiles;
-    int gate;
-    float limit;
+    Gate gate;
+    const void* x;         // tokens as they are (kernels that round them themselves)
+    int K, whole_rows;     // their entries; whether every row starts on 16 bytes
+    int weights_final;
     int out_align;         // 2: rows of 32-byte multiples from a 32-byte boundary, 1: of 16, 0: neither
 };
 
@@ -105,17 +119,29 @@ __device__ __forceinline__ uint32_t first_blocks(uint64_t* bar) {
     return at;
 }
 
-// A box into this block's shared memory; the bytes count on the (first) block's barrier.
+// Boxes of the tokens' codes (coordinates: entry of a k-block, token, k-block) and of the weights' (entry, channel, part, k-block) into this
+// block's shared memory, k-block after k-block; the bytes count on the (first) block's barrier.
 template <int CTAS>
-__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void load_tokens_box(void* dst, const CUtensorMap* map, int row, int k_block, uint32_t bar) {
     if constexpr (CTAS == 2)
         asm volatile(
-            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(k_block) : "memory");
     else
         asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(k_block) : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void load_weights_box(void* dst, const CUtensorMap* map, int channel, int part, int k_block, uint32_t bar) {
+    if constexpr (CTAS == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(channel), "r"(part), "r"(k_block) : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(channel), "r"(part), "r"(k_block) : "memory");
 }
 
 template <int CTAS>
@@ -168,34 +194,94 @@ __device__ __forceinline__ void store16(bf16* at, const float (&v)[16], int left
     }
 }
 
-__device__ __forceinline__ float gated(float g, float u, int gate, float limit) {
-    if (limit <= 0.f && gate == FRB_GATE_GELU_TANH)
-        return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))) * u;
-    return paired_gate(g, u, limit);
+__device__ __forceinline__ float gated(float g, float u, const Gate& gate) {
+    g = g > gate.limit ? gate.limit : g;
+    u = u > gate.limit ? gate.limit : u;
+    u = u < -gate.limit ? -gate.limit : u;
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * fmaf(gate.b * g, g, gate.a)));
+    return __fdividef(g, 1.0f + e) * (u + gate.add);
 }
 
 // ----------------------------------------------------------------------------- the kernel
 
-template <int CTAS, int PARTS, typename OutT>
+#define P8_KEPT 8                      // runs of 8 entries of a token that a lane holds
+
+__host__ __device__ inline int warps_a_token(int tokens) { return tokens == 1 ? 8 : tokens == 2 ? 4 : tokens <= 4 ? 2 : 1; }
+
+// One to eight tokens rounded by the epilogue's warps: as many warps a row as there are for it.  Entry k of row r goes to k-block k / 128,
+// row r of its eight of 128 bytes, the 16-byte chunk that the swizzle has there; scales to `scales`.
+template <typename InT>
+__device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, uint8_t* codes, float* scales, uint32_t (*tops)[P8_EPILOGUE_WARPS]) {
+    const int per_row = warps_a_token(p.rows), row = ew / per_row, sub = ew % per_row;
+    const bool mine = row < p.rows;
+    const InT* src = (const InT*)p.x + (size_t)(mine ? row : 0) * p.K;
+    const int KP = p.k_blocks * FRB_8BIT_KBLOCK, step = per_row * 256;
+    const int first = (sub * 32 + lane) * 8;
+    Eight<InT> kept[P8_KEPT];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < P8_KEPT; ++j) {
+        const int k = first + j * step;
+        if (mine && k < p.K) kept[j].read(src + k, p.K - k, p.whole_rows);
+        else kept[j].clear();
+    }
+#pragma unroll
+    for (int j = 0; j < P8_KEPT; ++j) top = top_of(kept[j], top);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[0][ew] = top;
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * P8_EPILOGUE_WARPS) : "memory");
+    top = 0;
+    for (int i = 0; i < per_row; ++i) top = max(top, tops[0][ew - sub + i]);
+    float factor, scale;
+    bool check;
+    row_factor<InT>(top, factor, scale, check);
+    if (!mine) return;
+    const auto place = [&](int k) { return reinterpret_cast<uint2*>(codes + (k >> 7) * 1024 + row * 128 + ((((k >> 4) & 7) ^ row) << 4) + (k & 8)); };
+    uint32_t again = 0;                                       // one bit for each run of eight entries that slow_codes() decides
+#pragma unroll
+    for (int j = 0; j < P8_KEPT; ++j) {
+        const int k = first + j * step;
+        if (k >= KP) continue;
+        bool near;
+        *place(k) = codes_of(kept[j], factor, check, near);
+        again |= (uint32_t)near << j;
+    }
+#pragma unroll 1
+    for (int j = 0; again >> j; ++j) {
+        const int k = first + j * step;
+        if (again >> j & 1) *place(k) = slow_codes(src + k, p.K - k, factor, __uint_as_float(top));
+    }
+    if (sub == 0 && lane == 0) scales[row] = scale;
+}
+
+// InT int8_t: the tokens' codes come with the weights, stage by stage; otherwise they are rounded here (at most eight, CTAS 1, no lists).
+template <int CTAS, int PARTS, typename OutT, typename InT>
 __global__ void __launch_bounds__(P8_THREADS, 1)
 product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Params p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full_bar[P8_MAX_STAGES], empty_bar[P8_MAX_STAGES];
     __shared__ uint64_t sums_bar[2], read_bar[2];             // a half's sums are complete; the epilogue has read them
-    __shared__ uint32_t tmem_slot;
+    __shared__ uint64_t tokens_bar;
+    __shared__ uint32_t tmem_slot, token_tops[1][P8_EPILOGUE_WARPS];
+    __shared__ float token_scales[8];
     __shared__ int failed_flag;
+    constexpr bool ROUNDS = !std::is_same<InT, int8_t>::value;
     volatile int* failed = &failed_flag;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int side = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;   // which block of the pair (clusters are runs of two blocks)
-    uint8_t* ring = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const uint32_t x_bytes = (uint32_t)p.x_box * 128, block_bytes = x_bytes + (uint32_t)p.n_box * 128;
-    const uint32_t stage_bytes = block_bytes * p.per_stage;
+    uint8_t* tokens = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);          // ROUNDS: all k-blocks of eight tokens
+    uint8_t* ring = tokens + (ROUNDS ? p.k_blocks * 1024 : 0);
+    // a stage: its k-blocks of tokens, then its k-blocks of weights
+    const uint32_t x_bytes = (uint32_t)p.x_box * 128, w_bytes = (uint32_t)p.n_box * 128;
+    const uint32_t stage_x = ROUNDS ? 0 : x_bytes * p.per_stage, stage_bytes = stage_x + w_bytes * p.per_stage;
 
     if (threadIdx.x == 0) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+        if (!ROUNDS) asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
         for (int s = 0; s < p.stages; ++s) { bar_init(&full_bar[s], 1); bar_init(&empty_bar[s], 1); }
         for (int h = 0; h < 2; ++h) { bar_init(&sums_bar[h], 1); bar_init(&read_bar[h], P8_EPILOGUE_WARPS * CTAS); }
+        bar_init(&tokens_bar, P8_EPILOGUE_WARPS);
         failed_flag = 0;
         bar_init_fence();
     }
@@ -228,28 +314,19 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if (warp == 0) {
         if (lane == 0) {
             const auto barrier_at = [&](int s) { return CTAS == 2 ? first_blocks(&full_bar[s]) : smem_addr(&full_bar[s]); };
+            // (boxes that end behind the last k-block are filled with zeros there)
             const auto load_weights = [&](int s, int st, int expert, int channel) {
-                const int blocks = min(p.per_stage, p.k_blocks - st * p.per_stage);
-                if (side == 0) bar_expect(&full_bar[s], block_bytes * blocks * CTAS);
-                const uint32_t bar = barrier_at(s);
-                const int row = (expert * PARTS) * p.FP + channel;
-                for (int b = 0; b < blocks; ++b) {
-                    uint8_t* dst = ring + (size_t)s * stage_bytes + b * block_bytes + x_bytes;
-                    const int k = (st * p.per_stage + b) * FRB_8BIT_KBLOCK;
-                    if (PARTS == 1) load_box<CTAS>(dst, &map_w, k, row + side * p.n_box, bar);
-                    else if (CTAS == 2) load_box<CTAS>(dst, &map_w, k, row + side * p.FP, bar);
-                    else { load_box<CTAS>(dst, &map_w, k, row, bar); load_box<CTAS>(dst + p.n * 128, &map_w, k, row + p.FP, bar); }
-                }
+                if (side == 0) bar_expect(&full_bar[s], stage_bytes * CTAS);
+                const bool by_part = CTAS == 2 && PARTS == 2;  // of a pair, the first block brings the gate's rows and the second the up's
+                load_weights_box<CTAS>(ring + (size_t)s * stage_bytes + stage_x, &map_w, by_part ? channel : channel + side * p.n_box,
+                                       expert * PARTS + (by_part ? side : 0), st * p.per_stage, barrier_at(s));
             };
             const auto load_tokens = [&](int s, int st, int row0) {
-                const int blocks = min(p.per_stage, p.k_blocks - st * p.per_stage);
-                const uint32_t bar = barrier_at(s);
-                for (int b = 0; b < blocks; ++b)
-                    load_box<CTAS>(ring + (size_t)s * stage_bytes + b * block_bytes, &map_x, (st * p.per_stage + b) * FRB_8BIT_KBLOCK,
-                                   row0 + side * 128, bar);
+                if (!ROUNDS) load_tokens_box<CTAS>(ring + (size_t)s * stage_bytes, &map_x, row0 + side * 128, st * p.per_stage, barrier_at(s));
             };
             // The first stages' weights before the wait for the tokens' codes, then their tokens, then stage after stage.
             int row0, expert, channel, ahead = 0;
+            if (!p.weights_final) wait_for_previous_kernel();
             for (int item = first; item < items && ahead < p.stages; item += step) {
                 place(item, row0, expert, channel);
                 for (int st = 0; st < stages_per_item && ahead < p.stages; ++st) load_weights(ahead++, st, expert, channel);
@@ -288,6 +365,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             int s = 0, half = 0;
             uint32_t parity = 0, read_parity = 3;             // (one bit of the latter for each half)
             bool ok = true;
+            if (ROUNDS && first < items && !warp_wait(&tokens_bar, 0, failed)) { if (lane == 0) atomicExch(p.status, 126); ok = false; }
             for (int item = first; item < items && ok; item += step) {
                 if (!warp_wait(&read_bar[half], (read_parity >> half) & 1, failed)) { if (lane == 0) atomicExch(p.status, 123); break; }
                 read_parity ^= 1u << half;
@@ -299,8 +377,9 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     const int blocks = min(p.per_stage, p.k_blocks - st * p.per_stage);
                     if (elect_one()) {
                         for (int b = 0; b < blocks; ++b) {
-                            const uint64_t desc_x = tile_desc(ring_at + s * stage_bytes + b * block_bytes);
-                            const uint64_t desc_w = tile_desc(ring_at + s * stage_bytes + b * block_bytes + x_bytes);
+                            const uint64_t desc_x = ROUNDS ? tile_desc(smem_addr(tokens) + (st * p.per_stage + b) * 1024)
+                                                           : tile_desc(ring_at + s * stage_bytes + b * x_bytes);
+                            const uint64_t desc_w = tile_desc(ring_at + s * stage_bytes + stage_x + b * w_bytes);
 #pragma unroll
                             for (int k = 0; k < FRB_8BIT_KBLOCK / 32; ++k)           // 32 k per MMA: 32 bytes along the swizzled row
                                 i8_mma<CTAS>(sums, desc_x + 2 * k, desc_w + 2 * k, idesc, (st | b | k) != 0);
@@ -322,6 +401,13 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         OutT* out = (OutT*)p.out;
         wait_for_previous_kernel();
         let_next_kernel_start();
+        if (ROUNDS) {
+            if constexpr (ROUNDS) round_tokens<InT>(p, warp - 2, lane, tokens, token_scales, token_tops);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads what was written here
+            __syncwarp();
+            if (lane == 0) bar_arrive(&tokens_bar);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * P8_EPILOGUE_WARPS) : "memory");       // the scales are there
+        }
         int half = 0;
         uint32_t sums_parity = 0;                                 // one bit for each half
         for (int item = first; item < items; item += step) {
@@ -332,7 +418,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             const bool mine = within < rows && quarter * 32 + lane < p.x_box;
             const bool any = side * 128 + quarter * 32 < rows && quarter * 32 < p.x_box;
             const int row = row0 + within;
-            const float x_scale = mine ? p.x_scale[row] : 0.f;
+            const float x_scale = !mine ? 0.f : ROUNDS ? token_scales[within & 7] : p.x_scale[row];
             const float* w_scale = p.w_scale + (size_t)expert * PARTS * p.FP + channel;
             const int channels = min(p.n, p.F - channel);
             if (!__all_sync(0xffffffffu, bar_wait(&sums_bar[half], (sums_parity >> half) & 1, failed))) { if (lane == 0) atomicExch(p.status, 125); break; }
@@ -370,7 +456,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             v[i] = (float)(int)acc[h][0][i] * x_scale * scale[0][i];
-                            if (PARTS == 2) v[i] = gated(v[i], (float)(int)acc[h][PARTS - 1][i] * x_scale * scale[PARTS - 1][i], p.gate, p.limit);
+                            if (PARTS == 2) v[i] = gated(v[i], (float)(int)acc[h][PARTS - 1][i] * x_scale * scale[PARTS - 1][i], p.gate);
                         }
                         if (mine) store16(dst + c0, v, channels - c0, p.out_align);
                     }
@@ -398,18 +484,30 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 
 // ----------------------------------------------------------------------------- host side
 
-static bool map_codes(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+static bool map_of(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     EncodeFn fn = encoder();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {cols};
-    cuuint32_t box[2] = {FRB_8BIT_KBLOCK, box_rows};
-    cuuint32_t elem[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    cuuint32_t elem[4] = {1, 1, 1, 1};
+    return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct Shape { int ctas, n; };
+// Rows of codes as (entry of a k-block, row, k-block), `box_rows` rows and `blocks` k-blocks a box.
+static bool map_tokens(CUtensorMap* map, const void* base, uint64_t rows, uint64_t KP, uint32_t box_rows, uint32_t blocks) {
+    const cuuint64_t dims[3] = {128, rows, KP / 128}, strides[2] = {KP, 128};
+    const cuuint32_t box[3] = {128, box_rows, blocks};
+    return map_of(map, base, 3, dims, strides, box);
+}
+
+// Weights as (entry of a k-block, channel, part of any expert, k-block).
+static bool map_weights(CUtensorMap* map, const void* base, uint64_t parts, uint64_t FP, uint64_t KP, uint32_t box_rows, uint32_t box_parts, uint32_t blocks) {
+    const cuuint64_t dims[4] = {128, FP, parts, KP / 128}, strides[3] = {KP, FP * KP, 128};
+    const cuuint32_t box[4] = {128, box_rows, box_parts, blocks};
+    return map_of(map, base, 4, dims, strides, box);
+}
+
+// Whether the product rounds the tokens itself: up to eight that the warps hold in registers, and whose codes leave half of a block's
+// shared memory to the weights.  (Longer ones would be read twice, 10 us for eight tokens of 4,096 entries where a launch costs 3.)
+bool tokens_fit(int rows, int K) { return rows <= 8 && K <= 14336 && K <= warps_a_token(rows) * P8_KEPT * 256; }
 
 // Tokens that a block copies at a time: 128, or as many as a tile has where that is less.
 static int tokens_box(const Product& p, int ctas) {
@@ -417,25 +515,35 @@ static int tokens_box(const Product& p, int ctas) {
     return ctas == 2 || tile >= 128 ? 128 : up_to(tile, 8);
 }
 
-// The form of a tile: the one whose last block is done first.  A block's k-block takes the tensor core 2 clocks a column and brings
-// (tokens + its share of the weights' rows) * 128 bytes at about 50 bytes a clock and SM; a tile costs about 500 clocks besides.
+struct Shape { int ctas, n, per_stage, stages; };
+
+// The form of a tile and of a stage: the one whose last block is done first.  Clocks of a k-block: the tensor core's 2 a column, but at
+// least 128 (it reads 128 tokens' codes from shared memory, however many there are), or those of the copies at 45 bytes a clock and SM;
+// of a stage at least 350 (the round from one copy to the next through both barriers); of a tile some 500 besides.  A stage is 52 KB at most
+// and holds several k-blocks where tiles are narrow: a box of them reads runs of several hundred bytes of a row at once.  Measured with a
+// 4096 x 24576 weight and one token, us: 32 channels and 1 k-block 56, 2 41, 8 30; 48 and 8 23; 64 and 4 23; 96 and 1 27, 4 22; 128 and 2 25.
 static Shape choose(const Product& p, int sms) {
     const int k_blocks = up_to(p.K, FRB_8BIT_KBLOCK) / FRB_8BIT_KBLOCK;
-    Shape best = {1, 32};
+    const bool listed = p.lists.tile_expert, rounds = !p.x_scale;
+    Shape best = {};
     double best_cost = 1e300;
     for (int ctas = 1; ctas <= 2; ++ctas) {
-        const int tile_rows = p.lists.tile_expert ? p.lists.tile_rows : p.rows;
-        if (p.lists.tile_expert ? (tile_rows > 128) != (ctas == 2) : ctas == 2 && p.rows <= 128) continue;
-        const long long row_tiles = p.lists.tile_expert ? p.lists.max_tiles : (p.rows + 128 * ctas - 1) / (128 * ctas);
-        const int x_box = tokens_box(p, ctas);
+        if (listed ? (p.lists.tile_rows > 128) != (ctas == 2) : ctas == 2 && p.rows <= 128) continue;
+        const long long row_tiles = listed ? p.lists.max_tiles : (p.rows + 128 * ctas - 1) / (128 * ctas);
+        const int x_box = tokens_box(p, ctas), x_rows = rounds ? 0 : x_box;
+        const int ring = P8_SMEM - 1024 - (x_box < 128 ? 128 * 128 : 0) - (rounds ? k_blocks * 1024 : 0);
         for (int n = 16 * ctas; n * p.parts <= 256; n += 16 * ctas) {
-            if (p.parts == 2 && ctas == 1 && n % 16) continue;
-            const int columns = n * p.parts;
+            const int columns = n * p.parts, block = (x_rows + columns / ctas) * 128;
+            int per_stage = 1;
+            while (per_stage < 16 && per_stage < k_blocks && 2 * per_stage * block <= 52 * 1024 && 3 * 2 * per_stage * block <= ring) per_stage *= 2;
+            const int fit = ring / (block * per_stage), stages = fit < P8_MAX_STAGES ? fit : P8_MAX_STAGES;
+            if (stages < 2) continue;
+            const double math = 2.0 * columns > 128.0 ? 2.0 * columns : 128.0, feed = block / 45.0, both = per_stage * (math > feed ? math : feed);
             const long long items = row_tiles * ((p.F + n - 1) / n), workers = sms / ctas;
-            const double feed = (x_box + columns / ctas) * 128 / 50.0, math = 2.0 * columns;
-            const double cost = (double)((items + workers - 1) / workers) * (k_blocks * (feed > math ? feed : math) + 500.0) + 8.0 * columns;
-            if (cost < best_cost) { best_cost = cost; best = {ctas, n}; }
-            if (n - 16 * ctas >= p.F) break;
+            const double cost = (double)((items + workers - 1) / workers) * ((k_blocks + per_stage - 1) / per_stage * (both > 350.0 ? both : 350.0) + 500.0) +
+                                8.0 * columns;
+            if (cost < best_cost) { best_cost = cost; best = {ctas, n, per_stage, stages}; }
+            if (n >= p.F) break;
         }
     }
     return best;
@@ -446,30 +554,39 @@ int product(const Product& q, cudaStream_t stream) {
     const int KP = up_to(q.K, FRB_8BIT_KBLOCK), FP = up_to(q.F, FRB_8BIT_ROWS);
     FRB_CHECK_ARG(q.K >= 1 && q.K <= FRB_8BIT_MOST_INNER, "product in 8 bits: an inner size of %d is outside 1..%d", q.K, FRB_8BIT_MOST_INNER);
     FRB_CHECK_ARG(q.F >= 1 && q.experts >= 1 && (q.parts == 1 || q.parts == 2), "product in 8 bits: %d experts of %d x %d channels", q.experts, q.parts, q.F);
-    FRB_CHECK_ARG((((uintptr_t)q.w | (uintptr_t)q.x | (uintptr_t)q.w_scale) & 15) == 0, "product in 8 bits: codes and scales start on 16 bytes");
+    FRB_CHECK_ARG((((uintptr_t)q.w | (q.x_scale ? (uintptr_t)q.x : 0) | (uintptr_t)q.w_scale) & 15) == 0, "product in 8 bits: codes and scales start on 16 bytes");
     FRB_CHECK_ARG(!q.lists.tile_expert || (q.lists.tile_rows >= 1 && q.lists.tile_rows <= 128) || q.lists.tile_rows == 256,
                   "product in 8 bits: tiles of %d rows (at most 128, or 256)", q.lists.tile_rows);
-    const uint64_t w_rows = (uint64_t)q.experts * q.parts * FP;
-    FRB_CHECK_ARG(w_rows < (1ull << 31) - 512, "product in 8 bits: %d experts of %d channels exceed a tensor map's rows", q.experts, q.F);
+    FRB_CHECK_ARG(q.F < (1 << 30) && q.rows < (1 << 30) && q.experts < (1 << 30), "product in 8 bits: %d rows of %d channels and %d experts exceed a tensor map",
+                  q.rows, q.F, q.experts);
     const int sms = frb_sm_count();
+    const bool rounds = !q.x_scale;
+    FRB_CHECK_ARG(!rounds || (tokens_fit(q.rows, q.K) && !q.lists.tile_expert), "product in 8 bits: %d tokens of %d entries to round", q.rows, q.K);
     const Shape shape = choose(q, sms);
     const int ctas = shape.ctas;
+    FRB_CHECK_ARG(ctas != 0, "product in 8 bits: no form for %d rows of %d entries", q.rows, q.K);
     Params p;
     p.lists = q.lists; p.w_scale = q.w_scale; p.x_scale = q.x_scale; p.out = q.out; p.status = q.status;
-    p.rows = q.rows; p.F = q.F; p.FP = FP; p.k_blocks = KP / FRB_8BIT_KBLOCK; p.gate = q.gate; p.limit = q.limit;
+    p.rows = q.rows; p.F = q.F; p.FP = FP; p.k_blocks = KP / FRB_8BIT_KBLOCK; 
+    const float log2e = 1.4426950408889634f, slope = q.limit > 0.f ? FRB_CLAMPED_GATE_SLOPE : q.gate == FRB_GATE_GELU_TANH ? 1.5957691216057308f : 1.0f;
+    p.gate.a = -log2e * slope;
+    p.gate.b = q.limit <= 0.f && q.gate == FRB_GATE_GELU_TANH ? -log2e * slope * 0.044715f : 0.f;
+    p.gate.limit = q.limit > 0.f ? q.limit : INFINITY;
+    p.gate.add = q.limit > 0.f ? 1.f : 0.f;
     p.n = shape.n;
     p.columns = p.n * q.parts;
     p.x_box = tokens_box(q, ctas);
     p.n_box = p.columns / ctas;
     const int two = 2 * p.columns;
     p.tmem_columns = two <= 32 ? 32 : two <= 64 ? 64 : two <= 128 ? 128 : two <= 256 ? 256 : 512;
-    const int block_bytes = (p.x_box + p.n_box) * 128;
+    p.per_stage = shape.per_stage;
+    p.stages = shape.stages;
     // the A operand of an MMA is 128 rows, whatever was copied: the last stage's has to end inside the block's shared memory
-    const int beyond = p.x_box < 128 ? 128 * 128 : 0;
-    p.per_stage = 1;
-    while (p.per_stage < 8 && p.per_stage * 2 * block_bytes <= 24 * 1024 && p.per_stage * 2 <= p.k_blocks) p.per_stage *= 2;
-    p.stages = (P8_SMEM - 1024 - beyond) / (block_bytes * p.per_stage);
-    if (p.stages > P8_MAX_STAGES) p.stages = P8_MAX_STAGES;
+    const size_t smem = 1024 + (rounds ? p.k_blocks * 1024 : 0) + (size_t)p.stages * p.per_stage * ((rounds ? 0 : p.x_box) + p.n_box) * 128 +
+                        (p.x_box < 128 ? 128 * 128 : 0);
+    FRB_CHECK_ARG(p.stages >= 2 && p.stages <= P8_MAX_STAGES && smem <= P8_SMEM, "product in 8 bits: %d stages in %zu bytes", p.stages, smem);
+    p.x = q.x; p.K = q.K; p.weights_final = q.weights_final;
+    p.whole_rows = q.K % 8 == 0 && ((uintptr_t)q.x & 15) == 0;
     p.row_tiles = (q.rows + 128 * ctas - 1) / (128 * ctas);
     p.channel_tiles = (q.F + p.n - 1) / p.n;
     const long long most = (long long)(q.lists.tile_expert ? q.lists.max_tiles : p.row_tiles) * p.channel_tiles;
@@ -477,10 +594,10 @@ int product(const Product& q, cudaStream_t stream) {
     const int row_bytes = q.F * (q.out_type == FRB_F32 ? 4 : 2);
     p.out_align = row_bytes % 32 == 0 && ((uintptr_t)q.out & 31) == 0 ? 2 : row_bytes % 16 == 0 && ((uintptr_t)q.out & 15) == 0 ? 1 : 0;
     CUtensorMap map_x, map_w;
-    const uint32_t w_box = q.parts == 2 && ctas == 1 ? p.n : p.n_box;
-    FRB_CHECK_ARG(map_codes(&map_x, q.x, q.rows, KP, p.x_box) && map_codes(&map_w, q.w, w_rows, KP, w_box),
+    const int box_parts = ctas == 2 ? 1 : q.parts;
+    FRB_CHECK_ARG((rounds || map_tokens(&map_x, q.x, q.rows, KP, p.x_box, p.per_stage)) &&
+                      map_weights(&map_w, q.w, (uint64_t)q.experts * q.parts, FP, KP, p.n_box / box_parts, box_parts, p.per_stage),
                   "product in 8 bits: cuTensorMapEncodeTiled failed or is not available");
-    const size_t smem = (size_t)p.stages * p.per_stage * block_bytes + beyond + 1024;
     const long long workers = sms / ctas;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)((most < workers ? most : workers) * ctas));
@@ -495,15 +612,23 @@ int product(const Product& q, cudaStream_t stream) {
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-#define LAUNCH(CTAS, PARTS, OutT)                                                                                                     \
+#define LAUNCH(CTAS, PARTS, OutT, InT)                                                                                                \
     do {                                                                                                                              \
-        cudaFuncSetAttribute(product_8bit_kernel<CTAS, PARTS, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM);            \
-        cudaLaunchKernelEx(&config, product_8bit_kernel<CTAS, PARTS, OutT>, map_x, map_w, p);                                         \
+        cudaFuncSetAttribute(product_8bit_kernel<CTAS, PARTS, OutT, InT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM);       \
+        cudaLaunchKernelEx(&config, product_8bit_kernel<CTAS, PARTS, OutT, InT>, map_x, map_w, p);                                    \
     } while (0)
-    FRB_DISPATCH_DTYPE(q.out_type, OutT, {
-        if (ctas == 2) { if (q.parts == 2) LAUNCH(2, 2, OutT); else LAUNCH(2, 1, OutT); }
-        else { if (q.parts == 2) LAUNCH(1, 2, OutT); else LAUNCH(1, 1, OutT); }
-    });
+    FRB_CHECK_ARG(q.parts == 1 || q.out_type == FRB_F32, "product in 8 bits: gated units come out in float32");
+    if (q.parts == 2) {
+        if (rounds) { FRB_DISPATCH_DTYPE(q.x_type, InT, LAUNCH(1, 2, float, InT)); }
+        else if (ctas == 2) LAUNCH(2, 2, float, int8_t);
+        else LAUNCH(1, 2, float, int8_t);
+    } else {
+        FRB_DISPATCH_DTYPE(q.out_type, OutT, {
+            if (rounds) { FRB_DISPATCH_DTYPE(q.x_type, InT, LAUNCH(1, 1, OutT, InT)); }
+            else if (ctas == 2) LAUNCH(2, 1, OutT, int8_t);
+            else LAUNCH(1, 1, OutT, int8_t);
+        });
+    }
 #undef LAUNCH
     FRB_RETURN_LAUNCH("product_8bit");
 }

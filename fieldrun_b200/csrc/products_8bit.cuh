@@ -16,7 +16,7 @@
 #define FRB_8BIT_MOST_INNER 131072     // 127^2 entries of it stay below 2^31
 #define FRB_8BIT_SMALLEST_ROW 1.2621774e-29f      // 2^-96
 
-// Gates of a unit with two products in.
+// Gates of a unit with two products in: silu or tanh-gelu of the gate, times up; with a limit L > 0 the clamped gate.
 enum Frb8BitGate { FRB_GATE_SILU = 0, FRB_GATE_GELU_TANH = 1 };
 
 namespace frb_products8 {
@@ -39,9 +39,11 @@ struct Product {
     const float* w_scale;      // [experts][parts][F up to 16]
     int experts, parts;        // parts 2: gate and up
     int F, K;
-    const void* x;             // codes [rows][K up to 128]
+    const void* x;             // codes [rows][K up to 128], or (x_scale null) rows as they are, which the kernel rounds itself: tokens_fit()
     const float* x_scale;      // [rows]
+    int x_type;                // without x_scale
     int rows;
+    bool weights_final;        // the weights were complete before the kernel before this one began
     Lists lists;
     void* out;                 // [rows][F]
     int out_type;
@@ -57,6 +59,133 @@ int plan(const int* ids, int tokens, int top_k, int experts, int tile_rows, int*
 int combine(const float* y, const float* weights, const int* row_of_assign, int tokens, int top_k, int width, void* out, int out_type,
             cudaStream_t stream);
 // products_8bit.cu
+bool tokens_fit(int rows, int K);
 int product(const Product& p, cudaStream_t stream);
 
 }  // namespace frb_products8
+
+// ----------------------------------------------------------------------------- rows as codes, on the device
+
+#ifdef __CUDACC__
+namespace frb_products8 {
+
+// Eight neighbouring entries as they are stored.
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void read(const float* p, int left, bool whole) {
+        if (whole) {
+            const float4 a = load4(p), b = load4(p + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+    __device__ __forceinline__ float entry(int i) const { return v[i]; }
+};
+template <> struct Eight<bf16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void read(const bf16* p, int left, bool whole) {
+        if (whole) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(p);
+            w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
+            return;
+        }
+        const unsigned short* bits = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = (2 * i < left ? (uint32_t)bits[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)bits[2 * i + 1] << 16 : 0u);
+    }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0u; }
+    __device__ __forceinline__ float entry(int i) const { return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16); }
+};
+
+// The magnitude's bits order like the magnitudes, with infinities and NaN above all numbers.
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Eight<T>& v, uint32_t top) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v.entry(i)) & 0x7fffffffu);
+    return top;
+}
+
+// What a row's largest magnitude a (its bits) gives: the factor of its entries before they are rounded, the scale that is stored, and whether
+// a bfloat16 row's products with the factor have to be looked at for values in the middle of two codes.
+//
+// bfloat16: with the factor rounded up they need not, but for one row in 128.  Let x and a be integers of 8 bits, 127 x / (a 2^s) their quotient.  If
+// it is not a middle n + 1/2, it is at least 1 / (254 x) > 1.5e-5 of itself from one, and the factor's error (2^-23 of itself) takes it past none.
+// If it is one, (2 n + 1) a 2^s = 254 x; unless 127 divides a (a = 254), 127 divides 2 n + 1, so n = 63, and rounding up gives the even code, 64.
+template <typename T>
+__device__ __forceinline__ void row_factor(uint32_t top, float& factor, float& scale, bool& check) {
+    const float a = __uint_as_float(top);
+    factor = scale = 0.f;
+    check = sizeof(T) == 2 && (top >> 16 & 0x7f) == 126;
+    if (top >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
+    else if (a >= FRB_8BIT_SMALLEST_ROW) { factor = sizeof(T) == 4 ? __fdiv_rn(127.f, a) : __fdiv_ru(127.f, a); scale = __fdiv_rn(a, 127.f); }
+}
+
+#define FRB_8BIT_WHOLE 12582912.f      // 1.5 * 2^23: a number added to it is rounded to a whole one, whose lowest byte is the sum's
+#define FRB_8BIT_BORDER 0.49998f       // the factor is off by 2^-23 of itself at most, a product by 127 * 2^-23 < 1.6e-5
+
+// 127 x / a rounded half to even, for eight entries; `near`: one of them is so near to the middle of two codes that slow_codes() has to decide.  In a
+// row of bfloat16 that is to be checked an entry nearer than 1e-6 of itself to a middle is one, and was rounded up: an odd code goes back by one.
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool check, bool& near) {
+    near = false;
+    if (factor == 0.f) return make_uint2(0u, 0u);
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = fmaf(v.entry(i), factor, FRB_8BIT_WHOLE);
+    if (sizeof(T) == 2) {
+        if (check) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float r = t[i] - FRB_8BIT_WHOLE;
+                if (fmaf(fabsf(r), 1e-6f, fabsf(fmaf(v.entry(i), factor, -r))) >= 0.5f && (__float_as_uint(t[i]) & 1u)) t[i] -= copysignf(1.f, r);
+            }
+        }
+    } else {
+        float middle = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) middle = fmaxf(middle, fabsf(fmaf(v.entry(i), factor, FRB_8BIT_WHOLE - t[i])));
+        near = middle > FRB_8BIT_BORDER;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(t[i]);
+    return make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
+}
+
+// The code next to c (or c itself) that 127 x / a is nearest to, half to even, where it lies next to the middle of two codes.  Exact: with 127 x =
+// p + e and c a = q + f, both sums of two float32, the remainder against half of a is (p - q -+ a/2) + (e - f), where both differences in the
+// first bracket are of numbers within a factor of two of one another and so without rounding, and so is e - f: every term is a
+// whole multiple of x's last place, e below 2^7 and f below 2^15 of them (a is less than 2^8 times x, or its code were 0).
+__device__ __forceinline__ float decided_code(float x, float c, float a) {
+    if (a > 1.2676506e30f) { x *= 9.5367432e-7f; a *= 9.5367432e-7f; }               // above 2^100: times 2^-20, or 127 x would be infinite
+    const float p = 127.f * x, e = fmaf(127.f, x, -p), q = c * a, f = fmaf(c, a, -q), d = p - q;
+    const float toward = copysignf(1.f, d), over = toward * ((d - toward * (0.5f * a)) + (e - f));
+    return over > 0.f || (over == 0.f && ((int)c & 1)) ? c + toward : c;
+}
+
+// The codes of eight entries that stand at p, decided one after another.  (Few runs come here; the code is short, and the registers of those
+// that do not come are left alone.)
+template <typename T>
+__device__ __forceinline__ uint2 slow_codes(const T* p, int left, float factor, float top) {
+    unsigned long long codes = 0;
+#pragma unroll 1
+    for (int i = 0; i < 8 && i < left; ++i) {
+        const float x = to_f32(p[i]);
+        float t = fmaf(x, factor, FRB_8BIT_WHOLE);
+        if (fabsf(fmaf(x, factor, FRB_8BIT_WHOLE - t)) > FRB_8BIT_BORDER) t = FRB_8BIT_WHOLE + decided_code(x, t - FRB_8BIT_WHOLE, top);
+        codes |= (unsigned long long)(__float_as_uint(t) & 0xffu) << (8 * i);
+    }
+    return make_uint2((uint32_t)codes, (uint32_t)(codes >> 32));
+}
+
+}  // namespace frb_products8
+#endif

@@ -8,118 +8,87 @@ namespace frb_products8 {
 
 #define RC_KEPT 4                      // runs of 8 entries that a thread keeps in registers; what is beyond is read a second time (from L1)
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, bool whole, float (&v)[8]) {
-    if (whole) {
-        const float4 a = load4(p), b = load4(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
-}
-template <>
-__device__ __forceinline__ void load8<bf16>(const bf16* p, int left, bool whole, float (&v)[8]) {
-    if (whole) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
-}
-
-// The magnitude's bits order like the magnitudes, with infinities and NaN above all numbers.
-__device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    return top;
-}
-
-// 127 x / a rounded half to even, exactly: x * (127 / a) in float32 is off by less than 127 * 2^-22.4 = 2.3e-5, so a product farther than
-// 1e-4 from the middle of two codes is on the right side; a nearer one is made again in 64 bits, where 127 x is exact and a quotient of
-// numbers of 31 and 24 bits that is not a middle is farther from one than the division's rounding (2^-25 against 2^-46).
-__device__ __forceinline__ int code_of(float x, float factor, float top) {
-    const float v = x * factor, r = rintf(v);
-    if (fabsf(fabsf(v - r) - 0.5f) > 1e-4f) return (int)r;
-    return (int)rint((double)x * 127.0 / (double)top);
-}
-
-__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float factor, float top) {
-    if (factor == 0.f) return make_uint2(0u, 0u);
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        w[h] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[h] |= ((uint32_t)code_of(v[4 * h + i], factor, top) & 0xffu) << (8 * i);
-    }
-    return make_uint2(w[0], w[1]);
-}
-
-// A block takes a row at a time.  Bound by memory where there are many rows, by two trips to it and the block's maximum where there are
-// few.  `places`: row t goes to the rows places[t * copies + c] of the result (negative: nowhere), else to row t.
-template <typename T, int BLOCK>
-__global__ void __launch_bounds__(BLOCK)
+// A row is taken by PER_ROW threads, a block of 128 or 512 holds one or several.  Bound by memory where there are many rows, by two trips to it
+// and the row's maximum where there are few.  `places`: row t goes to the rows places[t * copies + c] of the result (negative: nowhere),
+// else to row t.
+template <typename T, int PER_ROW>
+__global__ void __launch_bounds__(PER_ROW < 128 ? 128 : PER_ROW, PER_ROW == 512 ? 2 : sizeof(T) == 4 ? 6 : 8)
 rows_8bit_kernel(const T* __restrict__ x, int rows, int K, int KP, const int* __restrict__ places, int copies, int8_t* __restrict__ codes,
                  float* __restrict__ scales, int whole_rows) {
+    constexpr int BLOCK = PER_ROW < 128 ? 128 : PER_ROW, AT_ONCE = BLOCK / PER_ROW;
     __shared__ uint32_t warp_top[2][BLOCK / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x % PER_ROW;
     wait_for_previous_kernel();
     let_next_kernel_start();           // after the wait: the kernel after this one may read ahead what kernels before this one wrote
     int turn = 0;
-    for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    for (int row = blockIdx.x * AT_ONCE + threadIdx.x / PER_ROW; row < rows; row += gridDim.x * AT_ONCE, turn ^= 1) {
         const T* src = x + (size_t)row * K;
-        float kept[RC_KEPT][8];
+        Eight<T> kept[RC_KEPT];
         uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < RC_KEPT; ++j) {
-            const int k = (j * BLOCK + threadIdx.x) * 8;
-            if (k < K) { load8(src + k, K - k, whole_rows, kept[j]); }
-            else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) kept[j][i] = 0.f;
-            }
+            const int k = (j * PER_ROW + me) * 8;
+            if (k < K) kept[j].read(src + k, K - k, whole_rows);
+            else kept[j].clear();
         }
 #pragma unroll
         for (int j = 0; j < RC_KEPT; ++j) top = top_of(kept[j], top);
-        for (int k = (RC_KEPT * BLOCK + threadIdx.x) * 8; k < K; k += BLOCK * 8) {
-            float v[8];
-            load8(src + k, K - k, whole_rows, v);
+        for (int k = (RC_KEPT * PER_ROW + me) * 8; k < K; k += PER_ROW * 8) {
+            Eight<T> v;
+            v.read(src + k, K - k, whole_rows);
             top = top_of(v, top);
         }
         top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) warp_top[turn][warp] = top;
-        __syncthreads();               // (two sets of maxima in turn: a warp that is ahead writes the other)
-        top = __reduce_max_sync(0xffffffffu, lane < BLOCK / 32 ? warp_top[turn][lane] : 0u);
+        if (PER_ROW > 32) {
+            if (lane == 0) warp_top[turn][warp] = top;
+            __syncthreads();           // (two sets of maxima in turn: a warp that is ahead writes the other)
+            top = __reduce_max_sync(0xffffffffu, lane < BLOCK / 32 ? warp_top[turn][lane] : 0u);
+        }
         const float a = __uint_as_float(top);
-        float factor = 0.f, scale = 0.f;
-        if (top >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
-        else if (a >= FRB_8BIT_SMALLEST_ROW) { factor = __fdiv_rn(127.f, a); scale = __fdiv_rn(a, 127.f); }
-        const int first = places ? 0 : row, count = places ? copies : 1;
+        float factor, scale;
+        bool check;
+        row_factor<T>(top, factor, scale, check);
+        uint2 made[RC_KEPT];
+        uint32_t again = 0;            // one bit for each run of eight entries that slow_codes() decides
+#pragma unroll
+        for (int j = 0; j < RC_KEPT; ++j) {
+            bool near;
+            made[j] = codes_of(kept[j], factor, check, near);
+            again |= (uint32_t)near << j;
+        }
+        const int count = places ? copies : 1;
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) {
+            const int to = places ? places[(size_t)row * copies + i] : row;
+            if (to < 0) continue;
+            int8_t* dst = codes + (size_t)to * KP;
+#pragma unroll
+            for (int j = 0; j < RC_KEPT; ++j) {
+                const int k = (j * PER_ROW + me) * 8;
+                if (k < KP) *reinterpret_cast<uint2*>(dst + k) = made[j];
+            }
+            if (me == 0) scales[to] = scale;
+        }
         const auto put = [&](int k, uint2 c) {
+#pragma unroll 1
             for (int i = 0; i < count; ++i) {
-                const int to = places ? places[(size_t)row * copies + i] : first;
+                const int to = places ? places[(size_t)row * copies + i] : row;
                 if (to >= 0) *reinterpret_cast<uint2*>(codes + (size_t)to * KP + k) = c;
             }
         };
-#pragma unroll
-        for (int j = 0; j < RC_KEPT; ++j) {
-            const int k = (j * BLOCK + threadIdx.x) * 8;
-            if (k < KP) put(k, codes_of(kept[j], factor, a));
+#pragma unroll 1
+        for (int j = 0; again >> j; ++j) {
+            const int k = (j * PER_ROW + me) * 8;
+            if (again >> j & 1) put(k, slow_codes(src + k, K - k, factor, a));
         }
-        for (int k = (RC_KEPT * BLOCK + threadIdx.x) * 8; k < KP; k += BLOCK * 8) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            if (k < K) load8(src + k, K - k, whole_rows, v);
-            put(k, codes_of(v, factor, a));
-        }
-        if (threadIdx.x < count) {
-            const int to = places ? places[(size_t)row * copies + threadIdx.x] : first;
-            if (to >= 0) scales[to] = scale;
+#pragma unroll 1
+        for (int k = (RC_KEPT * PER_ROW + me) * 8; k < KP; k += PER_ROW * 8) {
+            Eight<T> v;
+            if (k < K) v.read(src + k, K - k, whole_rows);
+            else v.clear();
+            bool near;
+            const uint2 c = codes_of(v, factor, check, near);
+            put(k, near ? slow_codes(src + k, K - k, factor, a) : c);
         }
     }
 }
@@ -127,18 +96,24 @@ rows_8bit_kernel(const T* __restrict__ x, int rows, int K, int KP, const int* __
 int rows_codes(const void* x, int x_type, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream) {
     if (rows == 0) return 0;
     FRB_CHECK_ARG(K >= 1 && K <= FRB_8BIT_MOST_INNER, "rows in 8 bits: %d entries are outside 1..%d", K, FRB_8BIT_MOST_INNER);
-    FRB_CHECK_ARG(copies >= 1 && copies <= 128, "rows in 8 bits: %d places a row are outside 1..128", copies);
+    FRB_CHECK_ARG(copies >= 1, "rows in 8 bits: %d places a row", copies);
     FRB_CHECK_ARG(((uintptr_t)codes & 15) == 0, "rows in 8 bits: codes start on 16 bytes");
     const int KP = up_to(K, FRB_8BIT_KBLOCK);
     // 16-byte loads where every row starts on 16 bytes and is a whole number of runs of 8 entries
     const int whole = K % 8 == 0 && ((uintptr_t)x & 15) == 0;
-    const dim3 grid((unsigned)(rows < (1 << 20) ? rows : 1 << 20));
+#define LAUNCH(PER_ROW)                                                                                                          \
+    do {                                                                                                                         \
+        const int at_once = PER_ROW < 128 ? 128 / PER_ROW : 1, blocks = (rows + at_once - 1) / at_once;                          \
+        launch_dependent(rows_8bit_kernel<T, PER_ROW>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),                  \
+                         dim3(PER_ROW < 128 ? 128 : PER_ROW), 0, stream, (const T*)x, rows, K, KP, places, copies, (int8_t*)codes, scales, whole); \
+    } while (0)
+    // as few threads a row as hold it in registers, where there are rows for every SM; else as many as there may be
     FRB_DISPATCH_DTYPE(x_type, T, {
-        if (K <= 128 * 8 * RC_KEPT && rows > 2 * frb_sm_count())
-            launch_dependent(rows_8bit_kernel<T, 128>, grid, dim3(128), 0, stream, (const T*)x, rows, K, KP, places, copies, (int8_t*)codes, scales, whole);
-        else
-            launch_dependent(rows_8bit_kernel<T, 512>, grid, dim3(512), 0, stream, (const T*)x, rows, K, KP, places, copies, (int8_t*)codes, scales, whole);
+        if (rows <= 2 * frb_sm_count() || K > 128 * 8 * RC_KEPT) LAUNCH(512);
+        else if (K > 32 * 8 * RC_KEPT) LAUNCH(128);
+        else LAUNCH(32);
     });
+#undef LAUNCH
     FRB_RETURN_LAUNCH("rows_8bit");
 }
 

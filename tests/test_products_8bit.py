@@ -104,17 +104,17 @@ def test_what_expert_rows_refuse():
 def test_entry_points_refuse_sizes_by_a_message():
     # the C entry points' own checks, which come before anything is launched
     lib = ops.library("products8")
-    assert lib.frb_linear_8bit(None, 0, 3, 100, None, None, 33, None, 0, None, ops.linear_8bit_scratch(3, 100) - 1, None, None) == -1
+    assert lib.frb_linear_8bit(None, 0, 3, 100, None, None, 33, None, 0, 0, None, ops.linear_8bit_scratch(3, 100) - 1, None, None) == -1
     assert b"are needed" in lib.frb_last_error()
-    assert lib.frb_linear_8bit(None, 0, 3, 131073, None, None, 33, None, 0, None, 1 << 40, None, None) == -1
+    assert lib.frb_linear_8bit(None, 0, 3, 131073, None, None, 33, None, 0, 0, None, 1 << 40, None, None) == -1
     assert b"131073 entries" in lib.frb_last_error()
-    assert lib.frb_gated_8bit(None, 0, 3, 100, None, None, 40, None, None, 0, 0.0, None, 0, None, ops.gated_8bit_scratch(3, 100, 40) - 1, None, None) == -1
+    assert lib.frb_gated_8bit(None, 0, 3, 100, None, None, 40, None, None, 0, 0.0, None, 0, 0, None, ops.gated_8bit_scratch(3, 100, 40) - 1, None, None) == -1
     assert b"are needed" in lib.frb_last_error()
-    assert lib.frb_gated_8bit(None, 0, 3, 100, None, None, 40, None, None, 2, 0.0, None, 0, None, 1 << 40, None, None) == -1
+    assert lib.frb_gated_8bit(None, 0, 3, 100, None, None, 40, None, None, 2, 0.0, None, 0, 0, None, 1 << 40, None, None) == -1
     assert b"activation 2" in lib.frb_last_error()
     assert lib.frb_experts_8bit(None, 0, 1 << 24, 100, 128, None, None, None, None, 5, 40, None, None, 0.0, 8, None, 0, None, 1 << 40, None, None) == -1
     assert b"16777216 tokens of 128 experts" in lib.frb_last_error()
     assert lib.frb_experts_8bit(None, 0, 3, 100, 2, None, None, None, None, 9000, 40, None, None, 0.0, 8, None, 0, None, 1 << 40, None, None) == -1
     assert b"9000 experts" in lib.frb_last_error()
     # nothing to do is no error
-    assert lib.frb_linear_8bit(None, 0, 0, 100, None, None, 33, None, 0, None, 0, None, None) == 0
+    assert lib.frb_linear_8bit(None, 0, 0, 100, None, None, 33, None, 0, 0, None, 0, None, None) == 0
