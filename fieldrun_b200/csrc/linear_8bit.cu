@@ -36,14 +36,18 @@ static int rows_and_product(Product& p, const void* x, int x_type, int8_t* codes
 }
 
 // out [T, F] = x [T, K] W^T; W as codes [F up to 16][K up to 128] with scales [F up to 16].  weights_final: they were complete before the kernel
-// before this call began.  scratch: T (K up to 128) + 4 T bytes, each run up to 256.
+// before this call began.  scratch: T (K up to 128) + 4 T bytes, each run up to 256, none where tokens_fit().
 FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void* w, const float* w_scale, int F, void* out, int out_type,
                             int weights_final, void* scratch, long long scratch_bytes, int* status, cudaStream_t stream) {
     if (T == 0) return 0;
     FRB_CHECK_ARG(K >= 1 && K <= FRB_8BIT_MOST_INNER, "linear in 8 bits: %d entries are outside 1..%d", K, FRB_8BIT_MOST_INNER);
     Scratch s(scratch);
-    int8_t* codes = s.take<int8_t>((long long)T * up_to(K, FRB_8BIT_KBLOCK));
-    float* scales = s.take<float>(T);
+    int8_t* codes = nullptr;
+    float* scales = nullptr;
+    if (!tokens_fit(T, K)) {
+        codes = s.take<int8_t>((long long)T * up_to(K, FRB_8BIT_KBLOCK));
+        scales = s.take<float>(T);
+    }
     FRB_CHECK_ARG(s.at <= scratch_bytes, "linear in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
     Product p = {};
     p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K; p.rows = T; p.out = out; p.out_type = out_type; p.status = status;

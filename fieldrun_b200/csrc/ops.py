@@ -1986,22 +1986,25 @@ def weight_8bit(*parts: torch.Tensor, codes: Optional[torch.Tensor] = None, scal
     return codes, scales
 
 
-def _weight_8bit_of(what: str, codes: torch.Tensor, scales: torch.Tensor, experts: Optional[int], parts: int, features: int, inner: int) -> None:
+def _weight_8bit_of(what: str, codes: torch.Tensor, scales: torch.Tensor, experts: Optional[int], parts: int, features: int, inner: int) -> int:
+    """How many experts' weights these are; raises unless they are what the call needs."""
     shape = codes.shape
+    if codes.dtype is torch.int8 and scales.dtype is torch.float32 and len(shape) == 4:
+        count = shape[0] if experts is None else experts
+        if count >= 1 and shape == (count, parts, (features + 15) // 16 * 16, (inner + 127) // 128 * 128) and scales.shape == shape[:3]:
+            return count
     if codes.dtype is not torch.int8 or scales.dtype is not torch.float32:
         raise KernelError(f"{what}: codes are int8 and scales float32, found {codes.dtype} and {scales.dtype}")
-    if len(shape) != 4 or shape[1] != parts or shape[2] != -(-features // 16) * 16 or shape[3] != -(-inner // 128) * 128 or shape[0] < 1 \
-            or (experts is not None and shape[0] != experts) or scales.shape != shape[:3]:
-        wanted = list(weight_8bit_shape(experts or 1, parts, features, inner))
-        raise KernelError(f"{what}: codes of shape {list(shape)} with scales of {list(scales.shape)}, not {wanted if experts else ['experts'] + wanted[1:]} "
-                          f"with scales of the first three sizes")
+    wanted = list(weight_8bit_shape(experts or 1, parts, features, inner))
+    raise KernelError(f"{what}: codes of shape {list(shape)} with scales of {list(scales.shape)}, not {wanted if experts else ['experts'] + wanted[1:]} "
+                      f"with scales of the first three sizes")
 
 
-def _rows_in_and_out(x: torch.Tensor, out: torch.Tensor, features: Optional[int]) -> tuple[int, int, int]:
-    if x.dim() != 2 or out.dim() != 2 or x.shape[0] != out.shape[0] or not 1 <= x.shape[1] <= EIGHT_BIT_MOST_INNER or out.shape[1] < 1 \
-            or (features is not None and out.shape[1] != features):
-        raise KernelError(f"rows of shape {list(x.shape)} with results of {list(out.shape)}")
-    return x.shape[0], x.shape[1], out.shape[1]
+def _rows_in_and_out(x: torch.Tensor, out: torch.Tensor, same_width: bool = False) -> tuple[int, int, int]:
+    xs, ys = x.shape, out.shape
+    if len(xs) != 2 or len(ys) != 2 or xs[0] != ys[0] or not 1 <= xs[1] <= EIGHT_BIT_MOST_INNER or ys[1] < 1 or (same_width and xs[1] != ys[1]):
+        raise KernelError(f"rows of shape {list(xs)} with results of {list(ys)}")
+    return xs[0], xs[1], ys[1]
 
 
 def _scratch_8bit(scratch: Optional[torch.Tensor], need: int, device) -> torch.Tensor:
@@ -2012,9 +2015,16 @@ def _scratch_8bit(scratch: Optional[torch.Tensor], need: int, device) -> torch.T
     return scratch
 
 
+def _status_at(device) -> int:
+    status = _TC_STATUS.get(str(device))
+    return (tc_status(device) if status is None else status).data_ptr()
+
+
 def linear_8bit_scratch(rows: int, inner: int) -> int:
-    """Bytes of scratch that :func:`linear_8bit` needs."""
-    return _up(rows * _up(inner, EIGHT_BIT_KBLOCK), 256) + _up(4 * rows, 256)
+    """Bytes of scratch that :func:`linear_8bit` needs (none for a few tokens, which the product rounds itself)."""
+    if rows <= 8 and inner <= 14336 and inner <= (16384, 16384, 8192, 4096, 4096, 2048)[min(rows, 5)]:
+        return 0
+    return _rows_scratch(rows, inner)
 
 
 def linear_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out: torch.Tensor, *, weights_final: bool = False,
@@ -2024,17 +2034,23 @@ def linear_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out:
     scale of the token * scale of the channel * sum.  A row's results depend on that row alone, to the last bit.  ``weights_final`` (a promise):
     codes and scales were complete before the kernel before this call in the stream began, so that they may be read while that one still
     runs.  ``scratch``: uint8 of :func:`linear_8bit_scratch` bytes, for the call's own use."""
-    rows, inner, features = _rows_in_and_out(x, out, None)
+    rows, inner, features = _rows_in_and_out(x, out)
     _weight_8bit_of("linear_8bit", codes, scales, 1, 1, features, inner)
-    scratch = _scratch_8bit(scratch, linear_8bit_scratch(rows, inner), x.device)
+    need = linear_8bit_scratch(rows, inner)
+    if need or scratch is not None:
+        scratch = _scratch_8bit(scratch, need, x.device)
     at = _addresses(x, codes, scales, out, scratch)
-    _call("frb_linear_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], features, at[3], _code(out.dtype), int(weights_final), at[4],
-          scratch.numel(), _ptr(tc_status(x.device)))
+    _call("frb_linear_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], features, at[3], _code(out.dtype), int(weights_final), at[4], need,
+          _status_at(x.device))
+
+
+def _rows_scratch(rows: int, inner: int) -> int:
+    return _up(rows * _up(inner, EIGHT_BIT_KBLOCK), 256) + _up(4 * rows, 256)
 
 
 def gated_8bit_scratch(rows: int, inner: int, width: int) -> int:
     """Bytes of scratch that :func:`gated_8bit` needs."""
-    return linear_8bit_scratch(rows, inner) + _up(4 * rows * width, 256) + linear_8bit_scratch(rows, width)
+    return _rows_scratch(rows, inner) + _up(4 * rows * width, 256) + _rows_scratch(rows, width)
 
 
 def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor, out: torch.Tensor, *,
@@ -2043,7 +2059,7 @@ def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor,
     """A gated feed-forward block in 8-bit integers: h = act(x W_gate^T) * (x W_up^T) with ``activation`` silu or gelu_tanh (``gate_limit`` > 0:
     the clamped gate, as in the expert products), out [T, d] = h W_down^T.  Both products are as in :func:`linear_8bit`; h is made in float32
     and rounded to codes row by row.  ``in_codes`` [1, 2, width up to 16, d up to 128] (gate, up), ``down_codes`` [1, 1, d up to 16, width up to 128]."""
-    rows, inner, _ = _rows_in_and_out(x, out, x.shape[-1])
+    rows, inner, _ = _rows_in_and_out(x, out, True)
     if not 1 <= width <= EIGHT_BIT_MOST_INNER or activation not in GATES_8BIT or gate_limit < 0.0 or (gate_limit > 0.0 and activation != "silu"):
         raise KernelError(f"gated_8bit: a width of {width}, activation {activation!r} and a gate limit of {gate_limit}")
     _weight_8bit_of("gated_8bit, gate and up", in_codes, in_scales, 1, 2, width, inner)
@@ -2051,7 +2067,7 @@ def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor,
     scratch = _scratch_8bit(scratch, gated_8bit_scratch(rows, inner, width), x.device)
     at = _addresses(x, in_codes, in_scales, down_codes, down_scales, out, scratch)
     _call("frb_gated_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], width, at[3], at[4], GATES_8BIT[activation], float(gate_limit), at[5],
-          _code(out.dtype), int(weights_final), at[6], scratch.numel(), _ptr(tc_status(x.device)))
+          _code(out.dtype), int(weights_final), at[6], scratch.numel(), _status_at(x.device))
 
 
 def expert_tile_rows_8bit(assignments: int, experts: int) -> int:
@@ -2093,7 +2109,7 @@ def expert_rows_8bit(x: torch.Tensor, row_of_assign: torch.Tensor, lists: tuple,
     scratch = _scratch_8bit(scratch, expert_rows_8bit_scratch(tokens, top_k, inner, width), x.device)
     at = _addresses(x, row_of_assign, *lists, in_codes, in_scales, down_codes, down_scales, y, scratch)
     _call("frb_expert_rows_8bit", at[0], _code(x.dtype), tokens, inner, top_k, *at[1:6], max_tiles, tile_rows, at[6], at[7], in_codes.shape[0], width,
-          at[8], at[9], float(gate_limit), at[10], at[11], scratch.numel(), _ptr(tc_status(x.device)))
+          at[8], at[9], float(gate_limit), at[10], at[11], scratch.numel(), _status_at(x.device))
 
 
 def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor,
@@ -2101,7 +2117,7 @@ def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_c
     """Routed experts in 8-bit integers: out[t] = sum over r of ``weights[t, r]`` * (gated block of expert ``ids[t, r]`` on x[t]), the
     blocks as :func:`expert_rows_8bit` computes them, their sum in float32 in the order of r, rounded once to out's type.  ``ids`` int32 and
     ``weights`` float32 [T, top_k]; an id that names no expert (-1) adds nothing."""
-    tokens, inner, _ = _rows_in_and_out(x, out, x.shape[-1])
+    tokens, inner, _ = _rows_in_and_out(x, out, True)
     if ids.dim() != 2 or ids.shape[0] != tokens or weights.shape != ids.shape or not 1 <= ids.shape[1] <= 128:
         raise KernelError(f"ids of shape {list(ids.shape)} and weights of {list(weights.shape)} for {tokens} tokens (1 to 128 experts each)")
     _want_ints("the experts' ids", ids)
@@ -2114,7 +2130,7 @@ def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_c
     scratch = _scratch_8bit(scratch, experts_8bit_scratch(tokens, top_k, experts, inner, width), x.device)
     at = _addresses(x, ids, weights, in_codes, in_scales, down_codes, down_scales, out, scratch)
     _call("frb_experts_8bit", at[0], _code(x.dtype), tokens, inner, top_k, at[1], at[2], at[3], at[4], experts, width, at[5], at[6], float(gate_limit),
-          expert_tile_rows_8bit(tokens * top_k, experts), at[7], _code(out.dtype), at[8], scratch.numel(), _ptr(tc_status(x.device)))
+          expert_tile_rows_8bit(tokens * top_k, experts), at[7], _code(out.dtype), at[8], scratch.numel(), _status_at(x.device))
 
 
 def wait_probe(device, limit_cycles: int = 100_000) -> int:

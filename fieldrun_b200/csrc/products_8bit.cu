@@ -16,6 +16,7 @@
 // rounded to codes by every block for itself, into shared memory, while its first weights are on their way: one launch instead of two.
 //
 // Every wait on an mbarrier gives up after about a second, records a code in `status` and lets the block leave through the common exit.
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -30,7 +31,8 @@ namespace frb_products8 {
 #define P8_EPILOGUE_WARPS 8
 #define P8_THREADS (64 + 32 * P8_EPILOGUE_WARPS)
 #define P8_MAX_STAGES 16
-#define P8_SMEM (220 * 1024)
+#define P8_SMEM (222 * 1024)
+#define P8_STAGED_BYTES (4096 * P8_EPILOGUE_WARPS)
 
 // The gates in one form, g' sigmoid(g' (a + b g'^2)) (u' + add): silu a = 1, b = 0; tanh-gelu, 0.5 g (1 + tanh(z)) = g sigmoid(2 z) with
 // z = sqrt(2 / pi) (g + 0.044715 g^3); the clamped gate a = 1.702, g' = min(g, L), u' = clamp(u, -L, L), add 1.  NaN stays NaN.  The hardware's
@@ -62,6 +64,7 @@ struct Params {
     const void* x;         // tokens as they are (kernels that round them themselves)
     int K, whole_rows;     // their entries; whether every row starts on 16 bytes
     int weights_final;
+    int staged;            // results go through shared memory
     int out_align;         // 2: rows of 32-byte multiples from a 32-byte boundary, 1: of 16, 0: neither
 };
 
@@ -156,13 +159,19 @@ __device__ __forceinline__ void everybody() {
 
 // ----------------------------------------------------------------------------- out of the kernel
 
+__device__ __forceinline__ void load_sums(uint32_t from, uint32_t (&sums)[16]) { tmem_ld16(from, sums); }
+__device__ __forceinline__ void load_sums(uint32_t from, uint32_t (&sums)[32]) {
+    tmem_ld16(from, reinterpret_cast<uint32_t (&)[16]>(sums[0]));
+    tmem_ld16(from + 16, reinterpret_cast<uint32_t (&)[16]>(sums[16]));
+}
+
 __device__ __forceinline__ void store_32_bytes(void* at, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
                  ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
 // 16 neighbouring channels of a token, `left` of them inside the row.
-__device__ __forceinline__ void store16(float* at, const float (&v)[16], int left, int align) {
+__device__ __forceinline__ void store16(float* at, const float* v, int left, int align) {
     if (left >= 16 && align == 2) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -179,7 +188,7 @@ __device__ __forceinline__ void store16(float* at, const float (&v)[16], int lef
         for (int i = 0; i < 16; ++i) if (i < left) at[i] = v[i];
     }
 }
-__device__ __forceinline__ void store16(bf16* at, const float (&v)[16], int left, int align) {
+__device__ __forceinline__ void store16(bf16* at, const float* v, int left, int align) {
     uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
@@ -201,6 +210,22 @@ __device__ __forceinline__ float gated(float g, float u, const Gate& gate) {
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * fmaf(gate.b * g, g, gate.a)));
     return __fdividef(g, 1.0f + e) * (u + gate.add);
+}
+
+// The same as chunk `chunk` of a 128-byte row whose 16-byte pieces are swizzled by `swizzle`.
+template <typename OutT>
+__device__ __forceinline__ void put16(uint8_t* row, int chunk, int swizzle, const float* v) {
+    if constexpr (sizeof(OutT) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<float4*>(row + (((4 * chunk + i) ^ swizzle) << 4)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint4*>(row + (((2 * chunk + i) ^ swizzle) << 4)) =
+                make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]), pack_bf16x2(v[8 * i + 2], v[8 * i + 3]), pack_bf16x2(v[8 * i + 4], v[8 * i + 5]),
+                           pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
+    }
 }
 
 // ----------------------------------------------------------------------------- the kernel
@@ -265,6 +290,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     __shared__ uint64_t tokens_bar;
     __shared__ uint32_t tmem_slot, token_tops[1][P8_EPILOGUE_WARPS];
     __shared__ float token_scales[8];
+    __shared__ __align__(16) float w_scales[2][256];
     __shared__ int failed_flag;
     constexpr bool ROUNDS = !std::is_same<InT, int8_t>::value;
     volatile int* failed = &failed_flag;
@@ -408,57 +434,104 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             if (lane == 0) bar_arrive(&tokens_bar);
             asm volatile("bar.sync 1, %0;" ::"n"(32 * P8_EPILOGUE_WARPS) : "memory");       // the scales are there
         }
+        // Staged results: a warp's 32 tokens by 128 bytes of channels go through a buffer of its own (16-byte pieces swizzled by the token) and from
+        // there in whole lines; otherwise every lane stores its token's channels.  (8,192 tokens, 1024 x 8192, float32: 109 us without.  Copies by TMA,
+        // with their fence, wait and map, took 92.)
+        // A step is 32 channels, or 16 of gate and up.
+        constexpr int STEP = PARTS == 1 ? 32 : 16, GROUP_STEPS = 128 / (int)sizeof(OutT) / STEP;        // steps in 128 bytes
+        const int shift = p.staged ? (GROUP_STEPS == 1 ? 0 : 1) : 0;
+        uint8_t* buffer = ring + (size_t)p.stages * stage_bytes + (warp - 2) * 4096;
+        const auto step_at = [&](int i) { return STEP * ((((i >> shift) * 2 + turn) << shift) + (i & ((1 << shift) - 1))); };
         int half = 0;
         uint32_t sums_parity = 0;                                 // one bit for each half
+        // A tile's scales are read while the one before it is computed.
+        float next_x = 0.f, next_w = 0.f;
+        const auto ask = [&](int item) {
+            if (item >= items) return;
+            int row0, expert, channel;
+            place(item, row0, expert, channel);
+            const int rows = listed ? min(p.lists.tile_rows, p.lists.offsets[expert + 1] - row0) : p.rows - row0;
+            const int within = side * 128 + quarter * 32 + lane, i = threadIdx.x - 64;
+            if (!ROUNDS && within < rows && quarter * 32 + lane < p.x_box) next_x = p.x_scale[row0 + within];
+            if (i < p.columns) {
+                const int part = PARTS == 2 && i >= p.n ? 1 : 0, c = i - part * p.n;
+                next_w = channel + c < p.F ? p.w_scale[((size_t)expert * PARTS + part) * p.FP + channel + c] : 0.f;
+            }
+        };
+        ask(first);
         for (int item = first; item < items; item += step) {
             int row0, expert, channel;
             place(item, row0, expert, channel);
             const int rows = listed ? min(p.lists.tile_rows, p.lists.offsets[expert + 1] - row0) : p.rows - row0;
-            const int within = side * 128 + quarter * 32 + lane;
+            const int warp_row = side * 128 + quarter * 32, within = warp_row + lane;
             const bool mine = within < rows && quarter * 32 + lane < p.x_box;
-            const bool any = side * 128 + quarter * 32 < rows && quarter * 32 < p.x_box;
+            const bool any = warp_row < rows && quarter * 32 < p.x_box;
             const int row = row0 + within;
-            const float x_scale = !mine ? 0.f : ROUNDS ? token_scales[within & 7] : p.x_scale[row];
-            const float* w_scale = p.w_scale + (size_t)expert * PARTS * p.FP + channel;
+            const float x_scale = !mine ? 0.f : ROUNDS ? token_scales[within & 7] : next_x;
             const int channels = min(p.n, p.F - channel);
-            if (!__all_sync(0xffffffffu, bar_wait(&sums_bar[half], (sums_parity >> half) & 1, failed))) { if (lane == 0) atomicExch(p.status, 125); break; }
+            float* scales = w_scales[half];
+            scales[threadIdx.x - 64] = next_w;                        // (there are as many threads as columns at most)
+            ask(item + step);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * P8_EPILOGUE_WARPS) : "memory");
+            // (a warp whose wait ran out goes through the other items without work: all warps meet at the barrier above)
+            const bool done = __all_sync(0xffffffffu, bar_wait(&sums_bar[half], (sums_parity >> half) & 1, failed));
+            if (!done && lane == 0) atomicExch(p.status, 125);
             sums_parity ^= 1u << half;
             fence_after_sync();
-            if (any) {
+            if (any && done) {
                 const uint32_t sums = lanes + half * p.columns;
                 OutT* dst = out + (size_t)row * p.F + channel;
-                uint32_t acc[2][PARTS][16];
-                int c = 16 * turn;
-                if (c < channels) {
+                uint32_t acc[2][PARTS][STEP];
+                if (step_at(0) < channels) {
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q) tmem_ld16(sums + q * p.n + c, acc[0][q]);
+                    for (int q = 0; q < PARTS; ++q) load_sums(sums + q * p.n + step_at(0), acc[0][q]);
                 }
 #pragma unroll 1
-                for (; c < channels; c += 64) {
+                for (int turns = 0; step_at(turns) < channels; turns += 2) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int c0 = c + 32 * h;
+                        const int c0 = step_at(turns + h), next = step_at(turns + h + 1);
                         if (c0 >= channels) break;
-                        float scale[PARTS][16];
-#pragma unroll
-                        for (int q = 0; q < PARTS; ++q)
-#pragma unroll
-                            for (int i = 0; i < 16; i += 4) {
-                                const float4 v = __ldg(reinterpret_cast<const float4*>(w_scale + (size_t)q * p.FP + c0 + i));
-                                scale[q][i] = v.x; scale[q][i + 1] = v.y; scale[q][i + 2] = v.z; scale[q][i + 3] = v.w;
-                            }
                         tmem_wait_ld();
-                        if (c0 + 32 < channels) {
+                        if (next < channels) {
 #pragma unroll
-                            for (int q = 0; q < PARTS; ++q) tmem_ld16(sums + q * p.n + c0 + 32, acc[h ^ 1][q]);
+                            for (int q = 0; q < PARTS; ++q) load_sums(sums + q * p.n + next, acc[h ^ 1][q]);
                         }
-                        float v[16];
+                        float v[STEP];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            v[i] = (float)(int)acc[h][0][i] * x_scale * scale[0][i];
-                            if (PARTS == 2) v[i] = gated(v[i], (float)(int)acc[h][PARTS - 1][i] * x_scale * scale[PARTS - 1][i], p.gate);
+                        for (int i = 0; i < STEP; i += 4) {
+                            const float4 s0 = *reinterpret_cast<const float4*>(scales + c0 + i), s1 = *reinterpret_cast<const float4*>(scales + (PARTS - 1) * p.n + c0 + i);
+                            const float first_scale[4] = {s0.x, s0.y, s0.z, s0.w}, second_scale[4] = {s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                v[i + j] = (float)(int)acc[h][0][i + j] * x_scale * first_scale[j];
+                                if (PARTS == 2) v[i + j] = gated(v[i + j], (float)(int)acc[h][PARTS - 1][i + j] * x_scale * second_scale[j], p.gate);
+                            }
                         }
-                        if (mine) store16(dst + c0, v, channels - c0, p.out_align);
+                        if (!p.staged) {
+#pragma unroll
+                            for (int i = 0; i < STEP; i += 16)
+                                if (mine && c0 + i < channels) store16(dst + c0 + i, v + i, channels - c0 - i, p.out_align);
+                            continue;
+                        }
+                        const int in_group = (turns + h) & (GROUP_STEPS - 1);
+#pragma unroll
+                        for (int i = 0; i < STEP; i += 16) put16<OutT>(buffer + lane * 128, in_group * (STEP / 16) + i / 16, lane & 7, v + i);
+                        if (in_group == GROUP_STEPS - 1 || next >= channels) {
+                            __syncwarp();
+                            const int piece = lane & 7, from = c0 - STEP * in_group + piece * (16 / (int)sizeof(OutT));
+                            uint4 w[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {             // four tokens at a time, 128 bytes of each
+                                const int r = 4 * i + (lane >> 3);
+                                w[i] = *reinterpret_cast<const uint4*>(buffer + r * 128 + ((piece ^ (r & 7)) << 4));
+                            }
+                            __syncwarp();
+                            OutT* to = out + (size_t)(row0 + warp_row + (lane >> 3)) * p.F + channel + from;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i, to += 4 * (size_t)p.F)
+                                if (warp_row + 4 * i + (lane >> 3) < rows && from < channels) *reinterpret_cast<uint4*>(to) = w[i];
+                        }
                     }
                 }
                 tmem_wait_ld();
@@ -531,7 +604,7 @@ static Shape choose(const Product& p, int sms) {
         if (listed ? (p.lists.tile_rows > 128) != (ctas == 2) : ctas == 2 && p.rows <= 128) continue;
         const long long row_tiles = listed ? p.lists.max_tiles : (p.rows + 128 * ctas - 1) / (128 * ctas);
         const int x_box = tokens_box(p, ctas), x_rows = rounds ? 0 : x_box;
-        const int ring = P8_SMEM - 1024 - (x_box < 128 ? 128 * 128 : 0) - (rounds ? k_blocks * 1024 : 0);
+        const int ring = P8_SMEM - 1024 - (x_box < 128 ? 128 * 128 : P8_STAGED_BYTES) - (rounds ? k_blocks * 1024 : 0);
         for (int n = 16 * ctas; n * p.parts <= 256; n += 16 * ctas) {
             const int columns = n * p.parts, block = (x_rows + columns / ctas) * 128;
             int per_stage = 1;
@@ -547,6 +620,17 @@ static Shape choose(const Product& p, int sms) {
         }
     }
     return best;
+}
+
+// Lets a kernel have a block's whole shared memory: asked for once a kernel and device.
+template <auto KERNEL>
+static void may_have_shared() {
+    static std::atomic<unsigned> asked{0};
+    int device = 0;
+    cudaGetDevice(&device);
+    const unsigned bit = 1u << (device & 31);
+    if (asked.load(std::memory_order_relaxed) & bit) return;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM) == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
 }
 
 int product(const Product& q, cudaStream_t stream) {
@@ -577,13 +661,14 @@ int product(const Product& q, cudaStream_t stream) {
     p.columns = p.n * q.parts;
     p.x_box = tokens_box(q, ctas);
     p.n_box = p.columns / ctas;
-    const int two = 2 * p.columns;
+    // (steps of 32 columns may read behind the second half's last)
+    const int two = p.columns + up_to(p.columns, 32);
     p.tmem_columns = two <= 32 ? 32 : two <= 64 ? 64 : two <= 128 ? 128 : two <= 256 ? 256 : 512;
     p.per_stage = shape.per_stage;
     p.stages = shape.stages;
     // the A operand of an MMA is 128 rows, whatever was copied: the last stage's has to end inside the block's shared memory
     const size_t smem = 1024 + (rounds ? p.k_blocks * 1024 : 0) + (size_t)p.stages * p.per_stage * ((rounds ? 0 : p.x_box) + p.n_box) * 128 +
-                        (p.x_box < 128 ? 128 * 128 : 0);
+                        (p.x_box < 128 ? 128 * 128 : P8_STAGED_BYTES);
     FRB_CHECK_ARG(p.stages >= 2 && p.stages <= P8_MAX_STAGES && smem <= P8_SMEM, "product in 8 bits: %d stages in %zu bytes", p.stages, smem);
     p.x = q.x; p.K = q.K; p.weights_final = q.weights_final;
     p.whole_rows = q.K % 8 == 0 && ((uintptr_t)q.x & 15) == 0;
@@ -593,6 +678,8 @@ int product(const Product& q, cudaStream_t stream) {
     FRB_CHECK_ARG(most < (1ll << 31) - 4096, "product in 8 bits: %d rows of %d channels exceed the count of tiles", q.rows, q.F);
     const int row_bytes = q.F * (q.out_type == FRB_F32 ? 4 : 2);
     p.out_align = row_bytes % 32 == 0 && ((uintptr_t)q.out & 31) == 0 ? 2 : row_bytes % 16 == 0 && ((uintptr_t)q.out & 15) == 0 ? 1 : 0;
+    // tiles of 128 tokens go out through shared memory where the results' rows are multiples of 16 bytes and tiles end with 128 bytes
+    p.staged = p.x_box == 128 && p.out_align >= 1 && p.n % (q.out_type == FRB_F32 ? 32 : 64) == 0;
     CUtensorMap map_x, map_w;
     const int box_parts = ctas == 2 ? 1 : q.parts;
     FRB_CHECK_ARG((rounds || map_tokens(&map_x, q.x, q.rows, KP, p.x_box, p.per_stage)) &&
@@ -611,10 +698,10 @@ int product(const Product& q, cudaStream_t stream) {
     attributes[1].val.clusterDim.x = (unsigned)ctas;
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
-    config.numAttrs = 2;
+    config.numAttrs = ctas == 2 ? 2 : 1;
 #define LAUNCH(CTAS, PARTS, OutT, InT)                                                                                                \
     do {                                                                                                                              \
-        cudaFuncSetAttribute(product_8bit_kernel<CTAS, PARTS, OutT, InT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P8_SMEM);       \
+        may_have_shared<product_8bit_kernel<CTAS, PARTS, OutT, InT>>();                                                               \
         cudaLaunchKernelEx(&config, product_8bit_kernel<CTAS, PARTS, OutT, InT>, map_x, map_w, p);                                    \
     } while (0)
     FRB_CHECK_ARG(q.parts == 1 || q.out_type == FRB_F32, "product in 8 bits: gated units come out in float32");

@@ -58,8 +58,10 @@ def test_what_a_linear_layer_refuses():
             (1, w.float(), "codes are int8"), (1, w[0, 0], "codes of shape"), (1, w[:, :, :33], "codes of shape"), (1, w[..., :100], "codes of shape"),
             (1, torch.zeros(2, 1, 48, 128, dtype=torch.int8), "codes of shape"), (2, s.double(), "scales float32"), (2, s[..., :33], "with scales of"),
             (3, torch.zeros(3, 60), "codes of shape"), (3, torch.zeros(4, 33), "with results of"), (3, torch.zeros(3, 0), "with results of"),
-            ("scratch", torch.zeros(64, dtype=torch.uint8), "are needed"), ("scratch", torch.zeros(4096), "as scratch")]:
+            ("scratch", torch.zeros(4096), "as scratch")]:
         refuses(ops.linear_8bit, args, {}, at, value, match)
+    refuses(ops.linear_8bit, (torch.zeros(9, 100), w, s, torch.zeros(9, 33)), {}, "scratch", torch.zeros(64, dtype=torch.uint8), "are needed")
+    assert ops.linear_8bit_scratch(3, 100) == 0 and ops.linear_8bit_scratch(9, 100) == 9 * 128 + 128 + 256      # runs of 256 bytes
 
 
 def test_what_a_gated_block_refuses():
@@ -104,7 +106,7 @@ def test_what_expert_rows_refuse():
 def test_entry_points_refuse_sizes_by_a_message():
     # the C entry points' own checks, which come before anything is launched
     lib = ops.library("products8")
-    assert lib.frb_linear_8bit(None, 0, 3, 100, None, None, 33, None, 0, 0, None, ops.linear_8bit_scratch(3, 100) - 1, None, None) == -1
+    assert lib.frb_linear_8bit(None, 0, 9, 100, None, None, 33, None, 0, 0, None, ops.linear_8bit_scratch(9, 100) - 1, None, None) == -1
     assert b"are needed" in lib.frb_last_error()
     assert lib.frb_linear_8bit(None, 0, 3, 131073, None, None, 33, None, 0, 0, None, 1 << 40, None, None) == -1
     assert b"131073 entries" in lib.frb_last_error()
