@@ -64,6 +64,7 @@ struct Params {
     const void* x;         // tokens as they are (kernels that round them themselves)
     int K, whole_rows;     // their entries; whether every row starts on 16 bytes
     int weights_final;
+    int m;                 // tokens of an MMA: 128 a block, or 64 where a tile has no more
     int staged;            // results go through shared memory
     int out_align;         // 2: rows of 32-byte multiples from a 32-byte boundary, 1: of 16, 0: neither
 };
@@ -124,27 +125,30 @@ __device__ __forceinline__ uint32_t first_blocks(uint64_t* bar) {
 
 // Boxes of the tokens' codes (coordinates: entry of a k-block, token, k-block) and of the weights' (entry, channel, part, k-block) into this
 // block's shared memory, k-block after k-block; the bytes count on the (first) block's barrier.
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 template <int CTAS>
-__device__ __forceinline__ void load_tokens_box(void* dst, const CUtensorMap* map, int row, int k_block, uint32_t bar) {
+__device__ __forceinline__ void load_tokens_box(uint32_t dst, const CUtensorMap* map, int row, int k_block, uint32_t bar) {
     if constexpr (CTAS == 2)
         asm volatile(
             "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(k_block) : "memory");
+            ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(k_block) : "memory");
     else
         asm volatile(
             "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(k_block) : "memory");
+            ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(k_block) : "memory");
 }
 template <int CTAS>
-__device__ __forceinline__ void load_weights_box(void* dst, const CUtensorMap* map, int channel, int part, int k_block, uint32_t bar) {
+__device__ __forceinline__ void load_weights_box(uint32_t dst, const CUtensorMap* map, int channel, int part, int k_block, uint32_t bar) {
     if constexpr (CTAS == 2)
         asm volatile(
             "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(channel), "r"(part), "r"(k_block) : "memory");
+            ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(channel), "r"(part), "r"(k_block) : "memory");
     else
         asm volatile(
             "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-            ::"r"(smem_addr(dst)), "l"(map), "r"(bar), "r"(0), "r"(channel), "r"(part), "r"(k_block) : "memory");
+            ::"r"(dst), "l"(map), "r"(bar), "r"(0), "r"(channel), "r"(part), "r"(k_block) : "memory");
 }
 
 template <int CTAS>
@@ -335,45 +339,52 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             expert = 0;
         }
     };
-    const int stages_per_item = (p.k_blocks + p.per_stage - 1) / p.per_stage;
 
+    // The whole warp goes through the loops that issue copies and MMAs, one of its lanes issues them (elect_one, tcgen05.cuh); addresses and
+    // descriptors go on by additions: a stage of 8 KB costs each of the two loops more than its copies and MMAs do otherwise.
     if (warp == 0) {
-        if (lane == 0) {
-            const auto barrier_at = [&](int s) { return CTAS == 2 ? first_blocks(&full_bar[s]) : smem_addr(&full_bar[s]); };
-            // (boxes that end behind the last k-block are filled with zeros there)
-            const auto load_weights = [&](int s, int st, int expert, int channel) {
-                if (side == 0) bar_expect(&full_bar[s], stage_bytes * CTAS);
-                const bool by_part = CTAS == 2 && PARTS == 2;  // of a pair, the first block brings the gate's rows and the second the up's
-                load_weights_box<CTAS>(ring + (size_t)s * stage_bytes + stage_x, &map_w, by_part ? channel : channel + side * p.n_box,
-                                       expert * PARTS + (by_part ? side : 0), st * p.per_stage, barrier_at(s));
-            };
-            const auto load_tokens = [&](int s, int st, int row0) {
-                if (!ROUNDS) load_tokens_box<CTAS>(ring + (size_t)s * stage_bytes, &map_x, row0 + side * 128, st * p.per_stage, barrier_at(s));
-            };
-            // The first stages' weights before the wait for the tokens' codes, then their tokens, then stage after stage.
-            int row0, expert, channel, ahead = 0;
-            if (!p.weights_final) wait_for_previous_kernel();
-            for (int item = first; item < items && ahead < p.stages; item += step) {
-                place(item, row0, expert, channel);
-                for (int st = 0; st < stages_per_item && ahead < p.stages; ++st) load_weights(ahead++, st, expert, channel);
-            }
-            wait_for_previous_kernel();
-            let_next_kernel_start();
-            int issued = 0, s = 0;
-            uint32_t parity = 1;                              // of the phase in which the stage's earlier use was given back
-            bool ok = true;
-            for (int item = first; item < items && ok; item += step) {
-                place(item, row0, expert, channel);
-                for (int st = 0; st < stages_per_item; ++st) {
-                    if (issued >= ahead) {
-                        if (!bar_wait(&empty_bar[s], parity, failed)) { atomicExch(p.status, 121); ok = false; break; }
-                        load_weights(s, st, expert, channel);
+        const uint32_t ring_at = smem_addr(ring), empty_at = smem_addr(empty_bar), own_full = smem_addr(full_bar);
+        const uint32_t full_at = CTAS == 2 ? first_blocks(full_bar) : own_full;
+        const bool by_part = CTAS == 2 && PARTS == 2;          // of a pair, the first block brings the gate's rows and the second the up's
+        const int side_channel = by_part ? 0 : side * p.n_box, side_part = by_part ? side : 0;
+        // (boxes that end behind the last k-block are filled with zeros there)
+        const auto load_weights = [&](int s, int k_block, int part, int channel) {
+            if (side == 0) expect_bytes(own_full + 8 * s, stage_bytes * CTAS);
+            load_weights_box<CTAS>(ring_at + s * stage_bytes + stage_x, &map_w, channel, part, k_block, full_at + 8 * s);
+        };
+        // The first stages' weights before the wait for the tokens' codes, then their tokens, then stage after stage.
+        int row0, expert, channel, ahead = 0;
+        if (!p.weights_final) wait_for_previous_kernel();
+        for (int item = first; item < items && ahead < p.stages; item += step) {
+            place(item, row0, expert, channel);
+            for (int k = 0; k < p.k_blocks && ahead < p.stages; k += p.per_stage, ++ahead)
+                if (elect_one()) load_weights(ahead, k, expert * PARTS + side_part, channel + side_channel);
+        }
+        __syncwarp();
+        wait_for_previous_kernel();
+        let_next_kernel_start();
+        int issued = 0, s = 0;
+        uint32_t parity = 1;                                   // of the phase in which the stage's earlier use was given back
+        bool ok = true;
+        for (int item = first; item < items && ok; item += step) {
+            place(item, row0, expert, channel);
+            const int part = expert * PARTS + side_part, from = channel + side_channel, token = row0 + side * 128;
+            for (int k = 0; k < p.k_blocks; k += p.per_stage) {
+                if (issued >= ahead) {
+                    if (!bar_try(empty_at + 8 * s, parity) && !warp_wait(&empty_bar[s], parity, failed)) {
+                        if (lane == 0) atomicExch(p.status, 121);
+                        ok = false;
+                        break;
                     }
-                    load_tokens(s, st, row0);
-                    ++issued;
-                    if (++s == p.stages) { s = 0; parity ^= 1; }
+                    if (elect_one()) load_weights(s, k, part, from);
                 }
+                if (!ROUNDS && elect_one()) load_tokens_box<CTAS>(ring_at + s * stage_bytes, &map_x, token, k, full_at + 8 * s);
+                ++issued;
+                if (++s == p.stages) { s = 0; parity ^= 1; }
             }
+        }
+        __syncwarp();
+        if (lane == 0) {
             // every stage has come back before the block may leave (a pair's first block signals this one's barriers)
             for (int back = 0; back < p.stages && back < issued; ++back) {
                 const int q = issued - 1 - back;
@@ -387,7 +398,9 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
     } else if (warp == 1) {
         if (side == 0) {
-            const uint32_t idesc = instr_desc_i8(128 * CTAS, p.columns), ring_at = smem_addr(ring);
+            const uint32_t idesc = instr_desc_i8(p.m * CTAS, p.columns);
+            const uint64_t first_x = tile_desc(smem_addr(ROUNDS ? tokens : ring)), first_w = tile_desc(smem_addr(ring) + stage_x);
+            const uint32_t stage_step = stage_bytes >> 4, x_step = ROUNDS ? 64 : x_bytes >> 4, w_step = w_bytes >> 4;      // in 16 bytes
             int s = 0, half = 0;
             uint32_t parity = 0, read_parity = 3;             // (one bit of the latter for each half)
             bool ok = true;
@@ -397,22 +410,22 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 read_parity ^= 1u << half;
                 fence_after_sync();
                 const uint32_t sums = tmem + half * p.columns;
-                for (int st = 0; st < stages_per_item; ++st) {
+                uint32_t add = 0;                             // 0: the item's first MMA sets the sums
+                for (int left = p.k_blocks, at = 0; left > 0; left -= p.per_stage, at += p.per_stage) {
                     if (!warp_wait(&full_bar[s], parity, failed)) { if (lane == 0) atomicExch(p.status, 124); ok = false; break; }
                     fence_after_sync();
-                    const int blocks = min(p.per_stage, p.k_blocks - st * p.per_stage);
                     if (elect_one()) {
-                        for (int b = 0; b < blocks; ++b) {
-                            const uint64_t desc_x = ROUNDS ? tile_desc(smem_addr(tokens) + (st * p.per_stage + b) * 1024)
-                                                           : tile_desc(ring_at + s * stage_bytes + b * x_bytes);
-                            const uint64_t desc_w = tile_desc(ring_at + s * stage_bytes + stage_x + b * w_bytes);
+                        uint64_t desc_x = first_x + (ROUNDS ? at * 64 : s * stage_step), desc_w = first_w + s * stage_step;
+                        const int blocks = min(p.per_stage, left);
+                        for (int b = 0; b < blocks; ++b, desc_x += x_step, desc_w += w_step) {
 #pragma unroll
-                            for (int k = 0; k < FRB_8BIT_KBLOCK / 32; ++k)           // 32 k per MMA: 32 bytes along the swizzled row
-                                i8_mma<CTAS>(sums, desc_x + 2 * k, desc_w + 2 * k, idesc, (st | b | k) != 0);
+                            for (int k = 0; k < FRB_8BIT_KBLOCK / 32; ++k, add = 1)           // 32 k per MMA: 32 bytes along the swizzled row
+                                i8_mma<CTAS>(sums, desc_x + 2 * k, desc_w + 2 * k, idesc, add);
                         }
                         commit<CTAS>(&empty_bar[s]);
-                        if (st == stages_per_item - 1) commit<CTAS>(&sums_bar[half]);
+                        if (left <= p.per_stage) commit<CTAS>(&sums_bar[half]);
                     }
+                    add = 1;
                     __syncwarp();
                     if (++s == p.stages) { s = 0; parity ^= 1; }
                 }
@@ -422,7 +435,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     } else {
         // Warp w may read the 32 lanes of tensor memory that are numbered by w & 3; the two warps of a quarter take the groups of 16
         // channels in turn.
-        const int quarter = warp & 3, turn = (warp - 2) >> 2;
+        const int quarter = warp & 3, turn = (warp - 2) >> 2, span = p.m >> 2;               // (64 tokens lie in the first 16 lanes of each quarter)
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         OutT* out = (OutT*)p.out;
         wait_for_previous_kernel();
@@ -451,8 +464,8 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             int row0, expert, channel;
             place(item, row0, expert, channel);
             const int rows = listed ? min(p.lists.tile_rows, p.lists.offsets[expert + 1] - row0) : p.rows - row0;
-            const int within = side * 128 + quarter * 32 + lane, i = threadIdx.x - 64;
-            if (!ROUNDS && within < rows && quarter * 32 + lane < p.x_box) next_x = p.x_scale[row0 + within];
+            const int within = side * 128 + quarter * span + lane, i = threadIdx.x - 64;
+            if (!ROUNDS && within < rows && lane < span && quarter * span + lane < p.x_box) next_x = p.x_scale[row0 + within];
             if (i < p.columns) {
                 const int part = PARTS == 2 && i >= p.n ? 1 : 0, c = i - part * p.n;
                 next_w = channel + c < p.F ? p.w_scale[((size_t)expert * PARTS + part) * p.FP + channel + c] : 0.f;
@@ -463,9 +476,9 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             int row0, expert, channel;
             place(item, row0, expert, channel);
             const int rows = listed ? min(p.lists.tile_rows, p.lists.offsets[expert + 1] - row0) : p.rows - row0;
-            const int warp_row = side * 128 + quarter * 32, within = warp_row + lane;
-            const bool mine = within < rows && quarter * 32 + lane < p.x_box;
-            const bool any = warp_row < rows && quarter * 32 < p.x_box;
+            const int warp_row = side * 128 + quarter * span, within = warp_row + lane;
+            const bool mine = within < rows && lane < span && quarter * span + lane < p.x_box;
+            const bool any = warp_row < rows && quarter * span < p.x_box;
             const int row = row0 + within;
             const float x_scale = !mine ? 0.f : ROUNDS ? token_scales[within & 7] : next_x;
             const int channels = min(p.n, p.F - channel);
@@ -604,7 +617,7 @@ static Shape choose(const Product& p, int sms) {
         if (listed ? (p.lists.tile_rows > 128) != (ctas == 2) : ctas == 2 && p.rows <= 128) continue;
         const long long row_tiles = listed ? p.lists.max_tiles : (p.rows + 128 * ctas - 1) / (128 * ctas);
         const int x_box = tokens_box(p, ctas), x_rows = rounds ? 0 : x_box;
-        const int ring = P8_SMEM - 1024 - (x_box < 128 ? 128 * 128 : P8_STAGED_BYTES) - (rounds ? k_blocks * 1024 : 0);
+        const int ring = P8_SMEM - 1024 - (x_box < 128 ? (x_box <= 64 ? 64 : 128) * 128 : P8_STAGED_BYTES) - (rounds ? k_blocks * 1024 : 0);
         for (int n = 16 * ctas; n * p.parts <= 256; n += 16 * ctas) {
             const int columns = n * p.parts, block = (x_rows + columns / ctas) * 128;
             int per_stage = 1;
@@ -661,14 +674,15 @@ int product(const Product& q, cudaStream_t stream) {
     p.columns = p.n * q.parts;
     p.x_box = tokens_box(q, ctas);
     p.n_box = p.columns / ctas;
+    p.m = p.x_box <= 64 ? 64 : 128;
     // (steps of 32 columns may read behind the second half's last)
     const int two = p.columns + up_to(p.columns, 32);
     p.tmem_columns = two <= 32 ? 32 : two <= 64 ? 64 : two <= 128 ? 128 : two <= 256 ? 256 : 512;
     p.per_stage = shape.per_stage;
     p.stages = shape.stages;
-    // the A operand of an MMA is 128 rows, whatever was copied: the last stage's has to end inside the block's shared memory
+    // the A operand of an MMA is 64 or 128 rows, whatever was copied: the last stage's has to end inside the block's shared memory
     const size_t smem = 1024 + (rounds ? p.k_blocks * 1024 : 0) + (size_t)p.stages * p.per_stage * ((rounds ? 0 : p.x_box) + p.n_box) * 128 +
-                        (p.x_box < 128 ? 128 * 128 : P8_STAGED_BYTES);
+                        (p.x_box < 128 ? p.m * 128 : P8_STAGED_BYTES);
     FRB_CHECK_ARG(p.stages >= 2 && p.stages <= P8_MAX_STAGES && smem <= P8_SMEM, "product in 8 bits: %d stages in %zu bytes", p.stages, smem);
     p.x = q.x; p.K = q.K; p.weights_final = q.weights_final;
     p.whole_rows = q.K % 8 == 0 && ((uintptr_t)q.x & 15) == 0;
