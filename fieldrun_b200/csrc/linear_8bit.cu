@@ -17,6 +17,9 @@ struct Scratch {
     }
 };
 
+// From one row of a unit's middle to the next: whole lines, whatever the width.
+static int hidden_stride(int I) { return up_to(I, 32); }
+
 #define FRB_TRY(call)                         \
     do {                                      \
         const int status_ = (call);           \
@@ -25,12 +28,12 @@ struct Scratch {
 
 // Rows and the product that reads them: one launch where the product rounds them itself, else rows as codes in the scratch first.  The kernel
 // that makes those lets the product start only after its own wait, so that the weights, whoever wrote them, are complete by then.
-static int rows_and_product(Product& p, const void* x, int x_type, int8_t* codes, float* scales, bool weights_final, cudaStream_t stream) {
+static int rows_and_product(Product& p, const void* x, int x_type, int x_stride, int8_t* codes, float* scales, bool weights_final, cudaStream_t stream) {
     if (!p.lists.tile_expert && tokens_fit(p.rows, p.K)) {
-        p.x = x; p.x_type = x_type; p.x_scale = nullptr; p.weights_final = weights_final;
+        p.x = x; p.x_type = x_type; p.x_stride = x_stride; p.x_scale = nullptr; p.weights_final = weights_final;
         return product(p, stream);
     }
-    FRB_TRY(rows_codes(x, x_type, p.rows, p.K, nullptr, 1, codes, scales, stream));
+    FRB_TRY(rows_codes(x, x_type, x_stride, p.rows, p.K, nullptr, 1, codes, scales, stream));
     p.x = codes; p.x_scale = scales; p.weights_final = true;
     return product(p, stream);
 }
@@ -50,8 +53,9 @@ FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void*
     }
     FRB_CHECK_ARG(s.at <= scratch_bytes, "linear in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
     Product p = {};
-    p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K; p.rows = T; p.out = out; p.out_type = out_type; p.status = status;
-    return rows_and_product(p, x, x_type, codes, scales, weights_final != 0, stream);
+    p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K; p.rows = T; p.out = out; p.out_stride = F; p.out_type = out_type;
+    p.status = status;
+    return rows_and_product(p, x, x_type, K, codes, scales, weights_final != 0, stream);
 }
 
 // h = act(x Wg^T) * (x Wu^T) in float32, rounded to codes row by row, out [T, d] = h Wd^T.  w_in: codes [2][I up to 16][d up to 128] (gate, up),
@@ -66,16 +70,17 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     Scratch s(scratch);
     int8_t* codes = s.take<int8_t>((long long)T * up_to(d, FRB_8BIT_KBLOCK));
     float* scales = s.take<float>(T);
-    float* hidden = s.take<float>((long long)T * I);
+    const int IP = hidden_stride(I);
+    float* hidden = s.take<float>((long long)T * IP);
     int8_t* hidden_codes = s.take<int8_t>((long long)T * up_to(I, FRB_8BIT_KBLOCK));
     float* hidden_scales = s.take<float>(T);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "gated block in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
     Product p = {};
-    p.w = w_in; p.w_scale = in_scale; p.experts = 1; p.parts = 2; p.F = I; p.K = d; p.rows = T; p.out = hidden; p.out_type = FRB_F32; p.gate = gate;
-    p.limit = limit; p.status = status;
-    FRB_TRY(rows_and_product(p, x, x_type, codes, scales, weights_final != 0, stream));
-    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.out = out; p.out_type = out_type;
-    return rows_and_product(p, hidden, FRB_F32, hidden_codes, hidden_scales, true, stream);     // (the first product waited before it let this one start)
+    p.w = w_in; p.w_scale = in_scale; p.experts = 1; p.parts = 2; p.F = I; p.K = d; p.rows = T; p.out = hidden; p.out_stride = IP;
+    p.out_type = FRB_F32; p.gate = gate; p.limit = limit; p.status = status;
+    FRB_TRY(rows_and_product(p, x, x_type, d, codes, scales, weights_final != 0, stream));
+    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.out = out; p.out_stride = d; p.out_type = out_type;
+    return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, stream);     // (the first product waited before it let this one start)
 }
 
 // The experts' outputs y [N, d] (float32, in the order of the lists) for T tokens that were given their rows already: row_of_assign [T, top_k].
@@ -90,18 +95,19 @@ FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int to
     Scratch s(scratch);
     int8_t* codes = s.take<int8_t>((long long)N * up_to(d, FRB_8BIT_KBLOCK));
     float* scales = s.take<float>(N);
-    float* hidden = s.take<float>((long long)N * I);
+    const int IP = hidden_stride(I);
+    float* hidden = s.take<float>((long long)N * IP);
     int8_t* hidden_codes = s.take<int8_t>((long long)N * up_to(I, FRB_8BIT_KBLOCK));
     float* hidden_scales = s.take<float>(N);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
-    FRB_TRY(rows_codes(x, x_type, T, d, row_of_assign, top_k, codes, scales, stream));
+    FRB_TRY(rows_codes(x, x_type, d, T, d, row_of_assign, top_k, codes, scales, stream));
     Product p = {};
     p.w = w_in; p.w_scale = in_scale; p.experts = experts; p.parts = 2; p.F = I; p.K = d; p.rows = N; p.x = codes; p.x_scale = scales;
     p.lists = {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows};
-    p.out = hidden; p.out_type = FRB_F32; p.gate = FRB_GATE_SILU; p.limit = limit; p.status = status; p.weights_final = true;
+    p.out = hidden; p.out_stride = IP; p.out_type = FRB_F32; p.gate = FRB_GATE_SILU; p.limit = limit; p.status = status; p.weights_final = true;
     FRB_TRY(product(p, stream));
-    FRB_TRY(rows_codes(hidden, FRB_F32, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
-    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y;
+    FRB_TRY(rows_codes(hidden, FRB_F32, IP, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
+    p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y; p.out_stride = d;
     return product(p, stream);
 }
 

@@ -2050,7 +2050,7 @@ def _rows_scratch(rows: int, inner: int) -> int:
 
 def gated_8bit_scratch(rows: int, inner: int, width: int) -> int:
     """Bytes of scratch that :func:`gated_8bit` needs."""
-    return _rows_scratch(rows, inner) + _up(4 * rows * width, 256) + _rows_scratch(rows, width)
+    return _rows_scratch(rows, inner) + _up(4 * rows * _up(width, 32), 256) + _rows_scratch(rows, width)
 
 
 def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor, out: torch.Tensor, *,

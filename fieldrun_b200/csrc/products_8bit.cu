@@ -50,6 +50,7 @@ struct Params {
     void* out;
     int* status;
     int rows, F, FP;
+    int out_stride;
     int k_blocks;
     int n;                 // channels of a tile
     int columns;           // of one tile in tensor memory: n, or 2 n with gate and up
@@ -62,7 +63,7 @@ struct Params {
     int channel_tiles;
     Gate gate;
     const void* x;         // tokens as they are (kernels that round them themselves)
-    int K, whole_rows;     // their entries; whether every row starts on 16 bytes
+    int K, x_stride, whole_rows;      // their entries; from one to the next; whether every row starts on 16 bytes
     int weights_final;
     int m;                 // tokens of an MMA: 128 a block, or 64 where a tile has no more
     int staged;            // results go through shared memory
@@ -244,7 +245,7 @@ template <typename InT>
 __device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, uint8_t* codes, float* scales, uint32_t (*tops)[P8_EPILOGUE_WARPS]) {
     const int per_row = warps_a_token(p.rows), row = ew / per_row, sub = ew % per_row;
     const bool mine = row < p.rows;
-    const InT* src = (const InT*)p.x + (size_t)(mine ? row : 0) * p.K;
+    const InT* src = (const InT*)p.x + (size_t)(mine ? row : 0) * p.x_stride;
     const int KP = p.k_blocks * FRB_8BIT_KBLOCK, step = per_row * 256;
     const int first = (sub * 32 + lane) * 8;
     Eight<InT> kept[P8_KEPT];
@@ -493,7 +494,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             fence_after_sync();
             if (any && done) {
                 const uint32_t sums = lanes + half * p.columns;
-                OutT* dst = out + (size_t)row * p.F + channel;
+                OutT* dst = out + (size_t)row * p.out_stride + channel;
                 uint32_t acc[2][PARTS][STEP];
                 if (step_at(0) < channels) {
 #pragma unroll
@@ -540,9 +541,9 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                                 w[i] = *reinterpret_cast<const uint4*>(buffer + r * 128 + ((piece ^ (r & 7)) << 4));
                             }
                             __syncwarp();
-                            OutT* to = out + (size_t)(row0 + warp_row + (lane >> 3)) * p.F + channel + from;
+                            OutT* to = out + (size_t)(row0 + warp_row + (lane >> 3)) * p.out_stride + channel + from;
 #pragma unroll
-                            for (int i = 0; i < 8; ++i, to += 4 * (size_t)p.F)
+                            for (int i = 0; i < 8; ++i, to += 4 * (size_t)p.out_stride)
                                 if (warp_row + 4 * i + (lane >> 3) < rows && from < channels) *reinterpret_cast<uint4*>(to) = w[i];
                         }
                     }
@@ -604,7 +605,7 @@ static int tokens_box(const Product& p, int ctas) {
 struct Shape { int ctas, n, per_stage, stages; };
 
 // The form of a tile and of a stage: the one whose last block is done first.  Clocks of a k-block: the tensor core's 2 a column, but at
-// least 128 (it reads 128 tokens' codes from shared memory, however many there are), or those of the copies at 45 bytes a clock and SM;
+// least one a row of its M (it reads 64 or 128 tokens' codes from shared memory, however many there are), or those of the copies at 45 bytes a clock and SM;
 // of a stage at least 350 (the round from one copy to the next through both barriers); of a tile some 500 besides.  A stage is 52 KB at most
 // and holds several k-blocks where tiles are narrow: a box of them reads runs of several hundred bytes of a row at once.  Measured with a
 // 4096 x 24576 weight and one token, us: 32 channels and 1 k-block 56, 2 41, 8 30; 48 and 8 23; 64 and 4 23; 96 and 1 27, 4 22; 128 and 2 25.
@@ -616,15 +617,15 @@ static Shape choose(const Product& p, int sms) {
     for (int ctas = 1; ctas <= 2; ++ctas) {
         if (listed ? (p.lists.tile_rows > 128) != (ctas == 2) : ctas == 2 && p.rows <= 128) continue;
         const long long row_tiles = listed ? p.lists.max_tiles : (p.rows + 128 * ctas - 1) / (128 * ctas);
-        const int x_box = tokens_box(p, ctas), x_rows = rounds ? 0 : x_box;
-        const int ring = P8_SMEM - 1024 - (x_box < 128 ? (x_box <= 64 ? 64 : 128) * 128 : P8_STAGED_BYTES) - (rounds ? k_blocks * 1024 : 0);
+        const int x_box = tokens_box(p, ctas), x_rows = rounds ? 0 : x_box, m = x_box <= 64 ? 64 : 128;
+        const int ring = P8_SMEM - 1024 - (x_box < 128 ? m * 128 : P8_STAGED_BYTES) - (rounds ? k_blocks * 1024 : 0);
         for (int n = 16 * ctas; n * p.parts <= 256; n += 16 * ctas) {
             const int columns = n * p.parts, block = (x_rows + columns / ctas) * 128;
             int per_stage = 1;
             while (per_stage < 16 && per_stage < k_blocks && 2 * per_stage * block <= 52 * 1024 && 3 * 2 * per_stage * block <= ring) per_stage *= 2;
             const int fit = ring / (block * per_stage), stages = fit < P8_MAX_STAGES ? fit : P8_MAX_STAGES;
             if (stages < 2) continue;
-            const double math = 2.0 * columns > 128.0 ? 2.0 * columns : 128.0, feed = block / 45.0, both = per_stage * (math > feed ? math : feed);
+            const double math = 2.0 * columns > m ? 2.0 * columns : m, feed = block / 45.0, both = per_stage * (math > feed ? math : feed);
             const long long items = row_tiles * ((p.F + n - 1) / n), workers = sms / ctas;
             const double cost = (double)((items + workers - 1) / workers) * ((k_blocks + per_stage - 1) / per_stage * (both > 350.0 ? both : 350.0) + 500.0) +
                                 8.0 * columns;
@@ -684,13 +685,14 @@ int product(const Product& q, cudaStream_t stream) {
     const size_t smem = 1024 + (rounds ? p.k_blocks * 1024 : 0) + (size_t)p.stages * p.per_stage * ((rounds ? 0 : p.x_box) + p.n_box) * 128 +
                         (p.x_box < 128 ? p.m * 128 : P8_STAGED_BYTES);
     FRB_CHECK_ARG(p.stages >= 2 && p.stages <= P8_MAX_STAGES && smem <= P8_SMEM, "product in 8 bits: %d stages in %zu bytes", p.stages, smem);
-    p.x = q.x; p.K = q.K; p.weights_final = q.weights_final;
-    p.whole_rows = q.K % 8 == 0 && ((uintptr_t)q.x & 15) == 0;
+    p.x = q.x; p.K = q.K; p.x_stride = q.x_stride; p.weights_final = q.weights_final;
+    p.whole_rows = q.x_stride % 8 == 0 && ((uintptr_t)q.x & 15) == 0;
     p.row_tiles = (q.rows + 128 * ctas - 1) / (128 * ctas);
     p.channel_tiles = (q.F + p.n - 1) / p.n;
     const long long most = (long long)(q.lists.tile_expert ? q.lists.max_tiles : p.row_tiles) * p.channel_tiles;
     FRB_CHECK_ARG(most < (1ll << 31) - 4096, "product in 8 bits: %d rows of %d channels exceed the count of tiles", q.rows, q.F);
-    const int row_bytes = q.F * (q.out_type == FRB_F32 ? 4 : 2);
+    const int row_bytes = q.out_stride * (q.out_type == FRB_F32 ? 4 : 2);
+    p.out_stride = q.out_stride;
     p.out_align = row_bytes % 32 == 0 && ((uintptr_t)q.out & 31) == 0 ? 2 : row_bytes % 16 == 0 && ((uintptr_t)q.out & 15) == 0 ? 1 : 0;
     // tiles of 128 tokens go out through shared memory where the results' rows are multiples of 16 bytes and tiles end with 128 bytes
     p.staged = p.x_box == 128 && p.out_align >= 1 && p.n % (q.out_type == FRB_F32 ? 32 : 64) == 0;

@@ -39,21 +39,21 @@ struct Product {
     const float* w_scale;      // [experts][parts][F up to 16]
     int experts, parts;        // parts 2: gate and up
     int F, K;
-    const void* x;             // codes [rows][K up to 128], or (x_scale null) rows as they are, which the kernel rounds itself: tokens_fit()
+    const void* x;             // codes [rows][K up to 128], or (x_scale null) rows as they are, x_stride entries apart, which the kernel rounds itself
     const float* x_scale;      // [rows]
-    int x_type;                // without x_scale
+    int x_stride, x_type;      // without x_scale
     int rows;
     bool weights_final;        // the weights were complete before the kernel before this one began
     Lists lists;
-    void* out;                 // [rows][F]
-    int out_type;
+    void* out;                 // [rows], out_stride entries from one to the next
+    int out_stride, out_type;
     int gate;                  // parts 2: Frb8BitGate
     float limit;               // parts 2: > 0 the clamped gate
     int* status;               // 0, or the code of the wait that gave up
 };
 
 // rows_8bit.cu
-int rows_codes(const void* x, int x_type, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream);
+int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream);
 int plan(const int* ids, int tokens, int top_k, int experts, int tile_rows, int* offsets, int* row_of_assign, int* tile_expert, int* tile_row0,
          int* num_tiles, cudaStream_t stream);
 int combine(const float* y, const float* weights, const int* row_of_assign, int tokens, int top_k, int width, void* out, int out_type,
@@ -69,12 +69,12 @@ int product(const Product& p, cudaStream_t stream);
 #ifdef __CUDACC__
 namespace frb_products8 {
 
-// Eight neighbouring entries as they are stored.
+// Eight neighbouring entries as they are stored; those behind the row's end (`left`) are zeros.
 template <typename T> struct Eight;
 template <> struct Eight<float> {
     float v[8];
     __device__ __forceinline__ void read(const float* p, int left, bool whole) {
-        if (whole) {
+        if (whole && left >= 8) {
             const float4 a = load4(p), b = load4(p + 4);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
             return;
@@ -91,7 +91,7 @@ template <> struct Eight<float> {
 template <> struct Eight<bf16> {
     uint32_t w[4];
     __device__ __forceinline__ void read(const bf16* p, int left, bool whole) {
-        if (whole) {
+        if (whole && left >= 8) {
             const uint4 raw = *reinterpret_cast<const uint4*>(p);
             w[0] = raw.x; w[1] = raw.y; w[2] = raw.z; w[3] = raw.w;
             return;

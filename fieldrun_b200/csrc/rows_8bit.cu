@@ -13,7 +13,7 @@ namespace frb_products8 {
 // else to row t.
 template <typename T, int PER_ROW>
 __global__ void __launch_bounds__(PER_ROW < 128 ? 128 : PER_ROW, PER_ROW == 512 ? 2 : sizeof(T) == 4 ? 6 : 8)
-rows_8bit_kernel(const T* __restrict__ x, int rows, int K, int KP, const int* __restrict__ places, int copies, int8_t* __restrict__ codes,
+rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP, const int* __restrict__ places, int copies, int8_t* __restrict__ codes,
                  float* __restrict__ scales, int whole_rows) {
     constexpr int BLOCK = PER_ROW < 128 ? 128 : PER_ROW, AT_ONCE = BLOCK / PER_ROW;
     __shared__ uint32_t warp_top[2][BLOCK / 32];
@@ -22,7 +22,7 @@ rows_8bit_kernel(const T* __restrict__ x, int rows, int K, int KP, const int* __
     let_next_kernel_start();           // after the wait: the kernel after this one may read ahead what kernels before this one wrote
     int turn = 0;
     for (int row = blockIdx.x * AT_ONCE + threadIdx.x / PER_ROW; row < rows; row += gridDim.x * AT_ONCE, turn ^= 1) {
-        const T* src = x + (size_t)row * K;
+        const T* src = x + (size_t)row * x_stride;
         Eight<T> kept[RC_KEPT];
         uint32_t top = 0;
 #pragma unroll
@@ -93,19 +93,19 @@ rows_8bit_kernel(const T* __restrict__ x, int rows, int K, int KP, const int* __
     }
 }
 
-int rows_codes(const void* x, int x_type, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream) {
+int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream) {
     if (rows == 0) return 0;
     FRB_CHECK_ARG(K >= 1 && K <= FRB_8BIT_MOST_INNER, "rows in 8 bits: %d entries are outside 1..%d", K, FRB_8BIT_MOST_INNER);
     FRB_CHECK_ARG(copies >= 1, "rows in 8 bits: %d places a row", copies);
     FRB_CHECK_ARG(((uintptr_t)codes & 15) == 0, "rows in 8 bits: codes start on 16 bytes");
     const int KP = up_to(K, FRB_8BIT_KBLOCK);
-    // 16-byte loads where every row starts on 16 bytes and is a whole number of runs of 8 entries
-    const int whole = K % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    // 16-byte loads where every row starts on 16 bytes and its last run of 8 entries ends before the next
+    const int whole = x_stride % 8 == 0 && ((uintptr_t)x & 15) == 0;
 #define LAUNCH(PER_ROW)                                                                                                          \
     do {                                                                                                                         \
         const int at_once = PER_ROW < 128 ? 128 / PER_ROW : 1, blocks = (rows + at_once - 1) / at_once;                          \
         launch_dependent(rows_8bit_kernel<T, PER_ROW>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),                  \
-                         dim3(PER_ROW < 128 ? 128 : PER_ROW), 0, stream, (const T*)x, rows, K, KP, places, copies, (int8_t*)codes, scales, whole); \
+                         dim3(PER_ROW < 128 ? 128 : PER_ROW), 0, stream, (const T*)x, x_stride, rows, K, KP, places, copies, (int8_t*)codes, scales, whole); \
     } while (0)
     // as few threads a row as hold it in registers, where there are rows for every SM; else as many as there may be
     FRB_DISPATCH_DTYPE(x_type, T, {
@@ -223,5 +223,5 @@ int combine(const float* y, const float* weights, const int* row_of_assign, int 
 
 // Rows of x [rows, K] (float32 or bfloat16) as codes [.., K up to 128] and scales; row t goes to places[t * copies + c], or to row t.
 FRB_API int frb_rows_8bit(const void* x, int x_type, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream) {
-    return frb_products8::rows_codes(x, x_type, rows, K, places, copies, codes, scales, stream);
+    return frb_products8::rows_codes(x, x_type, K, rows, K, places, copies, codes, scales, stream);
 }
