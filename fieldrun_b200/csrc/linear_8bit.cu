@@ -83,7 +83,8 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, stream);     // (the first product waited before it let this one start)
 }
 
-// The experts' outputs y [N, d] (float32, in the order of the lists) for T tokens that were given their rows already: row_of_assign [T, top_k].
+// The experts' outputs y [N, d] (float32, in the order of the lists) for T tokens that were given their rows already: row_of_assign [T, top_k], or
+// null where x holds the rows in that order (top_k 1).
 // scratch as for frb_experts_8bit without lists and y.
 FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int top_k, const int* row_of_assign, const int* tile_expert, const int* tile_row0,
                                  const int* num_tiles, const int* offsets, int max_tiles, int tile_rows, const void* w_in, const float* in_scale, int experts,
@@ -91,6 +92,7 @@ FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int to
                                  cudaStream_t stream) {
     if (T == 0) return 0;
     FRB_CHECK_ARG((long long)T * top_k < (1ll << 31), "experts in 8 bits: %d tokens of %d experts", T, top_k);
+    FRB_CHECK_ARG(row_of_assign != nullptr || top_k == 1, "experts in 8 bits: rows in order go to one expert each, not %d", top_k);
     const int N = T * top_k;
     Scratch s(scratch);
     int8_t* codes = s.take<int8_t>((long long)N * up_to(d, FRB_8BIT_KBLOCK));

@@ -2088,20 +2088,22 @@ def experts_8bit_scratch(tokens: int, top_k: int, experts: int, inner: int, widt
             + expert_rows_8bit_scratch(tokens, top_k, inner, width))
 
 
-def expert_rows_8bit(x: torch.Tensor, row_of_assign: torch.Tensor, lists: tuple, max_tiles: int, tile_rows: int, in_codes: torch.Tensor,
+def expert_rows_8bit(x: torch.Tensor, row_of_assign: Optional[torch.Tensor], lists: tuple, max_tiles: int, tile_rows: int, in_codes: torch.Tensor,
                      in_scales: torch.Tensor, down_codes: torch.Tensor, down_scales: torch.Tensor, y: torch.Tensor, *, width: int,
                      gate_limit: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
     """The gated blocks (:func:`gated_8bit`) of a step's experts: ``y[row_of_assign[t * top_k + r]]`` (float32 [T * top_k, d]) becomes the block
     of token t's expert of rank r on x[t].  ``lists`` = (tile_expert, tile_row0, num_tiles, offsets) as :func:`expert_plan` makes them with tiles of
-    ``tile_rows`` (a value of ``EXPERT_TILES_8BIT``); ``in_codes`` [E, 2, width up to 16, d up to 128], ``down_codes`` [E, 1, d up to 16, width up to 128]."""
-    if x.dim() != 2 or x.shape[0] < 1 or row_of_assign.numel() % x.shape[0] or y.shape != (row_of_assign.numel(), x.shape[1]):
-        raise KernelError(f"rows of shape {list(x.shape)} with {row_of_assign.numel()} rows of experts and results of {list(y.shape)}")
+    ``tile_rows`` (a value of ``EXPERT_TILES_8BIT``); ``in_codes`` [E, 2, width up to 16, d up to 128], ``down_codes`` [E, 1, d up to 16, width up to 128].
+    ``row_of_assign`` None: x holds the experts' rows already in the order of the lists."""
+    given = x.shape[0] if row_of_assign is None else row_of_assign.numel()
+    if x.dim() != 2 or x.shape[0] < 1 or given % x.shape[0] or y.shape != (given, x.shape[1]):
+        raise KernelError(f"rows of shape {list(x.shape)} with {given} rows of experts and results of {list(y.shape)}")
     tokens, inner = x.shape
-    top_k = row_of_assign.numel() // tokens
+    top_k = given // tokens
     if tile_rows not in EXPERT_TILES_8BIT or max_tiles < 1 or not 1 <= width <= EIGHT_BIT_MOST_INNER or gate_limit < 0.0 or not 1 <= top_k <= 128:
         raise KernelError(f"expert_rows_8bit: {max_tiles} tiles of {tile_rows} rows, a width of {width}, {top_k} experts a token, a gate limit of {gate_limit}")
     _want(y, torch.float32, "expert outputs")
-    _want_ints("lists of the experts' rows", row_of_assign, *lists)
+    _want_ints("lists of the experts' rows", *lists, *(() if row_of_assign is None else (row_of_assign,)))
     _weight_8bit_of("expert_rows_8bit, gate and up", in_codes, in_scales, None, 2, width, inner)
     _weight_8bit_of("expert_rows_8bit, down", down_codes, down_scales, in_codes.shape[0], 1, inner, width)
     if lists[0].numel() < max_tiles or lists[1].numel() < max_tiles or lists[2].numel() != 1 or lists[3].numel() != in_codes.shape[0] + 1:

@@ -15,7 +15,8 @@ import torch
 from ..cache import CODE_DTYPES, CacheNeed, SequenceCache
 from ..config.plan import ModelPlan
 from ..parts import build_block, build_part
-from ..parts.linear import full_sums, require_true_float32, split_products_reach
+from ..parts.base import WEIGHT_DTYPES
+from ..parts.linear import Weight8, full_sums, require_true_float32, split_products_reach
 from ..weights.loader import TensorNeed, TensorSource
 from .context import StepContext
 
@@ -44,9 +45,20 @@ def parse_cache_dtype(name) -> str:
     raise ValueError(f"a cache of type {name!r}: known are {sorted(CODE_DTYPES)}, or None for the model's dtype")
 
 
+def parse_weight_dtype(name) -> str:
+    """What the matrices of the model's products are held in: "" (the model's dtype; also None) or a key of ``WEIGHT_DTYPES``."""
+    if name is None or name == "":
+        return ""
+    for codes, dtype in WEIGHT_DTYPES.items():
+        if name == dtype or (isinstance(name, str) and name.lower() == codes):
+            return codes
+    raise ValueError(f"weights of type {name!r}: known are {sorted(WEIGHT_DTYPES)}, or None for the model's dtype")
+
+
 class DecoderModel:
-    def __init__(self, plan: ModelPlan, dtype, cache_dtype=None):
-        """``cache_dtype``: "float8_e4m3fn" or "int8" holds the keys and values of every attention layer in 8 bits."""
+    def __init__(self, plan: ModelPlan, dtype, cache_dtype=None, weight_dtype=None):
+        """``cache_dtype``: "float8_e4m3fn" or "int8" holds the keys and values of every attention layer in 8 bits; ``weight_dtype``: "int8"
+        the matrices of attention's projections, feed-forwards and experts."""
         plan.check()
         self.plan = plan
         self.dtype = parse_dtype(dtype)
@@ -82,6 +94,9 @@ class DecoderModel:
         self.final_norm = build_part("norm", plan.final_norm, self.dtype)
         self.head = build_part("head", plan.head, self.dtype)
         self.head_is_tied = plan.head.tensors.get("weight") == plan.embedding.tensors.get("weight")
+        self.weight_codes = parse_weight_dtype(weight_dtype)
+        if self.weight_codes and not any([part.store_weights_as(self.weight_codes) for part in self.all_parts()]):
+            raise ValueError(f"weights in {self.weight_codes} were asked for, but no part's products have kernels for them")
         self.loaded = False
 
     # -- tensors -------------------------------------------------------------------------------------
@@ -145,9 +160,10 @@ class DecoderModel:
         seen, total = set(), 0
         for part in self.all_parts():
             for value in vars(part).values():
-                if isinstance(value, torch.Tensor) and value.data_ptr() not in seen:
-                    seen.add(value.data_ptr())
-                    total += value.numel() * value.element_size()
+                for tensor in value.pair if isinstance(value, Weight8) else (value,):
+                    if isinstance(tensor, torch.Tensor) and tensor.data_ptr() not in seen:
+                        seen.add(tensor.data_ptr())
+                        total += tensor.numel() * tensor.element_size()
         return total
 
     # -- cache ---------------------------------------------------------------------------------------

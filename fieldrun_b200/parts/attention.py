@@ -38,7 +38,8 @@ runs both maps of a prompt's head, of float32 outputs otherwise.
 
 The keys and values may be held in 8 bits (``store_cache_as``): they are written as codes with a scale per token and head, single
 tokens attend over the codes, and for a prompt the pages in sight are read back into bfloat16 pages first, which the same
-kernels then take as those of a bfloat16 cache.  Every query, a prompt's as well, sees what the cache holds.
+kernels then take as those of a bfloat16 cache.  Every query, a prompt's as well, sees what the cache holds.  So may the projections'
+weights (``store_weights_as``), apart from the head gates'.
 """
 from __future__ import annotations
 
@@ -50,7 +51,7 @@ from ..cache import CODE_DTYPES, PAGE_TOKENS, CacheNeed, LineView
 from ..csrc import ops
 from ..weights.loader import MATRIX, VECTOR, TensorNeed, TensorSource
 from .base import BiasedRows, Mixer, build_position, register_part
-from .linear import part_linear
+from .linear import Weight8, part_linear
 
 
 TC_ATTENTION_MIN_QUERIES = 64       # a step whose longest run of new tokens is shorter uses tiles of 16 queries
@@ -214,6 +215,12 @@ class GQAAttention(Mixer):
             self.q_norm = source.fetch(needs["q_norm"])
             self.k_norm = source.fetch(needs["k_norm"]) if "k_norm" in needs else None
 
+        if self.weight_codes:
+            self.w_qkv, self.w_o = Weight8.of(self.w_qkv), Weight8.of(self.w_o)
+
+    def store_weights_as(self, codes: str) -> bool:
+        return self._take_weights_as(codes)
+
     def _map_order(self, name: str, rows: torch.Tensor) -> torch.Tensor:
         """The query projection's rows (or bias) in the kernels' order of heads: [key head, map, query head of the group]
         instead of [key head, query head of the group, map].  Keys and values are in order as they are."""
@@ -237,7 +244,7 @@ class GQAAttention(Mixer):
             raise ValueError(f"keys and values in 8 bits are for bfloat16 models and the (key, value) head sizes {sorted(ops.MMA_HEAD_SIZES)}: "
                              f"this layer has {(self.head_dim, self.value_dim)} in {str(self.dtype).replace('torch.', '')}")
         self.codes = codes
-        self.kernel_groups = ("common", "streams", "attention", "cache8")
+        self.kernel_groups = tuple(dict.fromkeys((*self.kernel_groups, "cache8")))
 
     def prepare(self, num_positions: int, device) -> None:
         if self.position is not None and self.position.rotary_dim > 0:

@@ -16,6 +16,8 @@ Interfaces
 ``Mixer.cache_need()`` -> :class:`~fieldrun_b200.cache.CacheNeed`
 ``Mixer.store_cache_as(codes)``
     keys and values in 8 bits from now on (a key of ``CODE_DTYPES``), or a ValueError from a mixer that has no kernels for it.
+``Part.store_weights_as(codes)`` -> bool
+    the matrices of the part's products in 8 bits from the next ``load`` on (a key of ``WEIGHT_DTYPES``); whether it has any.
 ``FeedForward.forward(ctx, act, act32)`` -> float32 update [T, width]
 ``Position.tables(num_positions, device)`` -> (cos, sin) float32 [positions, dim/2]
 ``Block.forward(ctx, x, pending, line, writes_cache)`` -> (x, pending)
@@ -47,6 +49,9 @@ from ..config.plan import PartSpec
 from ..weights.loader import TensorNeed, TensorSource
 
 
+WEIGHT_DTYPES = {"int8": torch.int8}      # what the matrices of a bfloat16 model's products may be held in
+
+
 class Part:
     """Base of all parts: constants in, tensors by name, rows through.
 
@@ -59,6 +64,7 @@ class Part:
     # the libraries of kernels (groups of ``csrc/build.py``) that the part launches from; a model compiles and loads
     # the groups of its parts, and no others, before its first step
     kernel_groups: tuple[str, ...] = ("common", "streams")
+    weight_codes: str = ""            # what the part's matrices are held in, "" for the model's dtype
 
     def __init__(self, spec: PartSpec, dtype: torch.dtype):
         self.spec = spec
@@ -70,6 +76,20 @@ class Part:
     def dense_needs(self) -> list[TensorNeed]:
         """The tensors whose matrices are multiplied with a step's rows as dense products."""
         return self.tensor_needs()
+
+    def store_weights_as(self, codes: str) -> bool:
+        """Hold the matrices of the part's products in 8 bits (a part that has kernels for it; others stay as they are)."""
+        return False
+
+    def _take_weights_as(self, codes: str) -> bool:
+        """What a part with such kernels does."""
+        if codes not in WEIGHT_DTYPES:
+            raise ValueError(f"weights in {codes!r}: known are {sorted(WEIGHT_DTYPES)}")
+        if self.dtype != torch.bfloat16:
+            raise ValueError("weights in 8 bits are for bfloat16 models")
+        self.weight_codes = codes
+        self.kernel_groups = tuple(dict.fromkeys((*self.kernel_groups, "products8")))
+        return True
 
     def load(self, source: TensorSource) -> None:
         """Fetch the part's tensors.  A step's kernels read them ahead of their wait for the kernel before, so the last kernel that

@@ -19,6 +19,9 @@ scaled and sorted by a kernel of their own (product in float32, rounded once) an
 choice value, and only experts of the ``keep`` groups with the largest values can be picked.  ``shared_expert``
 ``{"width", "gate"}``: one more expert of the same form that every token uses; its output is added to the routed
 experts' sum, with ``gate`` multiplied by sigmoid(w_sg . x), one number per token.
+
+Every part's matrices may be held in 8 bits (``store_weights_as``): an expert's hidden row is then rounded to 8 bits between its two
+products.  Routers, and a shared expert with a gate per token, stay as they are.
 """
 from __future__ import annotations
 
@@ -29,7 +32,7 @@ import torch
 from ..csrc import ops
 from ..weights.loader import MATRIX, VECTOR, TensorNeed, TensorSource
 from .base import FeedForward, UpdateSum, WeightedRows, register_part
-from .linear import STREAM_ROWS, one_tile, part_linear
+from .linear import STREAM_ROWS, Weight8, one_tile, part_linear
 
 TILE_ROWS = 32        # rows of one expert that a block of the expert kernels takes
 # Above this many rows per expert (on average) a step's expert products run on tcgen05: tiles of 32 rows and more
@@ -176,17 +179,26 @@ class RoutedExperts(FeedForward):
             self.bias = source.fetch(TensorNeed(self.name_of("choice_bias"), (n,), VECTOR, "bias"))
         for e in range(n):
             gate, up, down = (source.fetch(need) for need in self._expert_needs(e))
+            if self.weight_codes:
+                if e == 0:
+                    self.w13, self.w2 = Weight8(i, d, gate.device, parts=2, experts=n), Weight8(d, i, gate.device, experts=n)
+                self.w13.put(e, gate, up)
+                self.w2.put(e, down)
+                continue
             if self.w13 is None:
                 self.w13 = torch.empty((n, 2 * i, d), dtype=gate.dtype, device=gate.device)
                 self.w2 = torch.empty((n, d, i), dtype=gate.dtype, device=gate.device)
             self.w13[e, :i].copy_(gate)
             self.w13[e, i:].copy_(up)
             self.w2[e].copy_(down)
-        if self.may_split and self.w13.is_cuda:
+        if self.may_split and not self.weight_codes and self.w13.is_cuda:
             self.split_scales = (ops.weight_scales(self.w13), ops.weight_scales(self.w2))
         if self.shared_width:
             fetched = [source.fetch(need) for need in self._shared_needs()]
             width = self.shared_width
+            if self.weight_codes and not self.shared_gate:
+                self.w_shared_in, self.w_shared_down = Weight8.of(*fetched[:2]), Weight8.of(fetched[2])
+                return
             rows = -(-(2 * width + 1) // 16) * 16           # a product's features in steps of 16 (the streaming kernels' rule)
             self.w_shared_in = torch.zeros((rows, d), dtype=fetched[0].dtype, device=fetched[0].device)
             self.w_shared_in[:width].copy_(fetched[0])
@@ -195,11 +207,19 @@ class RoutedExperts(FeedForward):
                 self.w_shared_in[2 * width].copy_(fetched[3].reshape(-1))
             self.w_shared_down = fetched[2]
 
+    def store_weights_as(self, codes: str) -> bool:
+        return self._take_weights_as(codes)
+
     def shared(self, ctx, act: torch.Tensor) -> torch.Tensor:
         """The shared expert's output [T, d] float32: silu(gate) * up, times the token's sigmoid gate where the part has one
         (put on the hidden rows: the product behind it is linear), then the product out.  Without that gate a few rows' and a
         prompt's first product carry the activation."""
         rows = act.shape[0]
+        if isinstance(self.w_shared_in, Weight8):
+            out = torch.empty((rows, self.hidden_size), dtype=torch.float32, device=act.device)
+            ops.gated_8bit(act, *self.w_shared_in.pair, *self.w_shared_down.pair, out, width=self.shared_width, weights_final=True,
+                           scratch=ctx.buffer("experts.shared_scratch", (ops.gated_8bit_scratch(rows, self.hidden_size, self.shared_width),), torch.uint8))
+            return out
         hidden = ctx.buffer("experts.shared_hidden", (rows, self.shared_width), self.dtype)
         if self.shared_fused:
             pair = self.w_shared_in[:2 * self.shared_width].view(1, 2 * self.shared_width, self.hidden_size)
@@ -263,6 +283,8 @@ class RoutedExperts(FeedForward):
         """Rows of one expert that one block takes: few when experts get few rows each, so that no block
         carries accumulators it does not need; enough that most experts fit one tile when they get many."""
         per_expert = assignments / self.num_experts
+        if self.weight_codes:
+            return ops.expert_tile_rows_8bit(assignments, self.num_experts)
         if self.on_tensor_cores(assignments, decode):
             return next((t for t in (32, 64, 128, 256) if t >= 1.3 * per_expert), 256)
         if self.on_split_products(assignments):
@@ -301,6 +323,14 @@ class RoutedExperts(FeedForward):
         y = ctx.buffer("experts.y", (p["rows"], self.hidden_size), torch.float32)
         limit = self.gate_limit
         sorted_token = p["sorted_token"]
+        if self.weight_codes:
+            tokens, top_k = act.shape[0] if scaled is None else p["rows"], self.top_k if scaled is None else 1
+            ops.expert_rows_8bit(act if scaled is None else scaled, p["row_of_assign"] if scaled is None else None,
+                                 (p["tile_expert"], p["tile_row0"], p["num_tiles"], p["offsets"]), p["max_tiles"], p["tile_rows"], *self.w13.pair,
+                                 *self.w2.pair, y, width=self.expert_width, gate_limit=limit,
+                                 scratch=ctx.buffer("experts.scratch", (ops.expert_rows_8bit_scratch(tokens, top_k, self.hidden_size, self.expert_width),),
+                                                    torch.uint8))
+            return y
         if scaled is not None:
             act, sorted_token = scaled, None
         if act.data_ptr() % 16 and (self.on_split_products(p["rows"]) or self.streams_float32(p["rows"])):
@@ -440,10 +470,21 @@ class DenseGatedUnit(FeedForward):
 
     def load(self, source: TensorSource) -> None:
         gate, up, down = (source.fetch(n) for n in self._needs())
+        if self.weight_codes:
+            self.w_gate_up, self.w_down = Weight8.of(gate, up), Weight8.of(down)
+            return
         self.w_gate_up = torch.cat([gate, up], dim=0).contiguous()
         self.w_down = down
 
+    def store_weights_as(self, codes: str) -> bool:
+        return self._take_weights_as(codes)
+
     def forward(self, ctx, act, act32):
+        if self.weight_codes:
+            out = torch.empty((act.shape[0], self.hidden_size), dtype=torch.float32, device=act.device)
+            ops.gated_8bit(act, *self.w_gate_up.pair, *self.w_down.pair, out, width=self.width, activation=self.activation, weights_final=True,
+                           scratch=ctx.buffer("dense.scratch", (ops.gated_8bit_scratch(act.shape[0], self.hidden_size, self.width),), torch.uint8))
+            return out
         both = part_linear(act, self.w_gate_up)                    # float32 [T, 2I]
         hidden = ctx.buffer("dense.hidden", (act.shape[0], self.width), self.dtype)
         ops.gated_unit(both, hidden, self.activation)
@@ -493,13 +534,18 @@ class DenseUnit(FeedForward):
     def load(self, source: TensorSource) -> None:
         self.w_up, self.w_down, *rest = (source.fetch(n) for n in self._needs())
         self.coefficients = rest[0] if rest else None
+        if self.weight_codes:
+            self.w_up, self.w_down = Weight8.of(self.w_up), Weight8.of(self.w_down)
+
+    def store_weights_as(self, codes: str) -> bool:
+        return self._take_weights_as(codes)
 
     def forward(self, ctx, act, act32):
         rows = act.shape[0]
         hidden = ctx.buffer("dense.hidden", (rows, self.width), self.dtype)
         if self.normed_powers:
             ops.poly_norm(part_linear(act, self.w_up), self.coefficients, self.norm_eps, hidden)
-        elif (self.dtype == torch.bfloat16 and rows >= FUSED_ACTIVATION_ROWS and not ctx.is_decode and self.width % 128 == 0
+        elif (self.dtype == torch.bfloat16 and not self.weight_codes and rows >= FUSED_ACTIVATION_ROWS and not ctx.is_decode and self.width % 128 == 0
                 and self.hidden_size % 64 == 0):
             # a prompt's rows: product and activation in one kernel on tcgen05, the result rounded once to bfloat16
             tile_expert, tile_row0, num_tiles, offsets, count, tile_rows = self.tiles.of(ctx, rows)

@@ -1,5 +1,6 @@
 """Plain dense matrix products: few rows as a stream over the weight, large float32 products on the tensor cores with their
-operands in parts, the others through the library (cuBLAS via torch.mm).
+operands in parts, products with a weight in 8 bits (:class:`Weight8`) in whole numbers, the others through the library (cuBLAS via
+torch.mm).
 
 The reference's dense products (``Bundle::mm``, src/bundle.rs:644-683) are a
 library call as well: ndarray's ``dot`` over matrixmultiply or cblas.  Weights
@@ -42,6 +43,30 @@ SPLIT_ROWS = 48
 SPLIT_TILES = 32
 SPLIT_PRODUCTS = 1 << 31
 LONG_STEP = 16384         # tokens of the longest step that the generation loop runs
+
+
+class Weight8:
+    """A weight in 8 bits: int8 codes with a float32 scale per output channel (``ops.weight_8bit``), for one matrix [features, inner], for gate
+    and up of that shape (``parts`` 2), or for as many of either as there are ``experts``."""
+
+    def __init__(self, features: int, inner: int, device, parts: int = 1, experts: int = 1):
+        self.features, self.inner = features, inner
+        shape = ops.weight_8bit_shape(experts, parts, features, inner)
+        self.codes = torch.zeros(shape, dtype=torch.int8, device=device)
+        self.scales = torch.zeros(shape[:3], dtype=torch.float32, device=device)
+
+    @classmethod
+    def of(cls, *matrices: torch.Tensor) -> "Weight8":
+        weight = cls(*matrices[0].shape, matrices[0].device, parts=len(matrices))
+        weight.put(0, *matrices)
+        return weight
+
+    def put(self, expert: int, *matrices: torch.Tensor) -> None:
+        ops.weight_8bit(*(m.contiguous() for m in matrices), codes=self.codes[expert:expert + 1], scales=self.scales[expert:expert + 1])
+
+    @property
+    def pair(self) -> tuple[torch.Tensor, torch.Tensor]:
+        return self.codes, self.scales
 
 
 def split_products_reach(needs) -> bool:
@@ -91,12 +116,18 @@ def float32_kernels_read(rows: torch.Tensor, weight: torch.Tensor, out: Optional
             and rows.is_contiguous() and weight.is_contiguous() and rows.data_ptr() % 16 == 0 and weight.data_ptr() % 16 == 0)
 
 
-def linear(rows: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tensor] = None, rounded: bool = False,
+def linear(rows: torch.Tensor, weight, out: Optional[torch.Tensor] = None, rounded: bool = False,
            split: bool = True, weight_final: bool = False) -> torch.Tensor:
     """rows [T, in] @ weight[out, in]^T -> float32 [T, out]; ``split``: whether a large float32 product may run as split products
     on the tensor cores; with ``rounded`` (bfloat16 rows only) the float32 sums rounded once
     to bfloat16, for a reader that takes its operands in that type anyway.  ``weight_final``: the weight was complete before the
-    kernel before this product in the stream began, so that a product of few rows may read it while that one still runs."""
+    kernel before this product in the stream began, so that a product of few rows may read it while that one still runs.  ``weight`` may be
+    a :class:`Weight8` (of one matrix); the rows are then rounded to 8 bits, too."""
+    if isinstance(weight, Weight8):
+        if out is None:
+            out = torch.empty((rows.shape[0], weight.features), dtype=torch.bfloat16 if rounded else torch.float32, device=rows.device)
+        ops.linear_8bit(rows, weight.codes, weight.scales, out, weights_final=weight_final)
+        return out
     if rounded:
         if rows.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16 or not rows.is_cuda or out is not None:
             raise RuntimeError(f"a rounded matrix product of {rows.dtype} rows with a {weight.dtype} weight on {rows.device}")
