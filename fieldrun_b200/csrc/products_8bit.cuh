@@ -10,6 +10,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "pairs.cuh"
 
 #define FRB_8BIT_KBLOCK 128            // entries of a k-block; rows of codes are multiples of it
 #define FRB_8BIT_ROWS 16               // a weight's rows are filled up to multiples of it
@@ -138,21 +139,25 @@ __device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool 
     near = false;
     if (factor == 0.f) return make_uint2(0u, 0u);
     float t[8];
+    const uint64_t factors = pair_of(factor, factor), whole = pair_of(FRB_8BIT_WHOLE, FRB_8BIT_WHOLE), less = pair_of(-1.f, -1.f);
+    float middle = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = fmaf(v.entry(i), factor, FRB_8BIT_WHOLE);
-    if (sizeof(T) == 2) {
-        if (check) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float r = t[i] - FRB_8BIT_WHOLE;
-                if (fmaf(fabsf(r), 1e-6f, fabsf(fmaf(v.entry(i), factor, -r))) >= 0.5f && (__float_as_uint(t[i]) & 1u)) t[i] -= copysignf(1.f, r);
-            }
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t x = pair_of(v.entry(i), v.entry(i + 1)), sums = fma_pairs(x, factors, whole);
+        halves_of(sums, t[i], t[i + 1]);
+        if (sizeof(T) == 4) {
+            float r0, r1;
+            halves_of(fma_pairs(x, factors, fma_pairs(sums, less, whole)), r0, r1);
+            middle = fmaxf(middle, fmaxf(fabsf(r0), fabsf(r1)));
         }
-    } else {
-        float middle = 0.f;
+    }
+    if (sizeof(T) == 4) near = middle > FRB_8BIT_BORDER;
+    if (sizeof(T) == 2 && check) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) middle = fmaxf(middle, fabsf(fmaf(v.entry(i), factor, FRB_8BIT_WHOLE - t[i])));
-        near = middle > FRB_8BIT_BORDER;
+        for (int i = 0; i < 8; ++i) {
+            const float r = t[i] - FRB_8BIT_WHOLE;
+            if (fmaf(fabsf(r), 1e-6f, fabsf(fmaf(v.entry(i), factor, -r))) >= 0.5f && (__float_as_uint(t[i]) & 1u)) t[i] -= copysignf(1.f, r);
+        }
     }
     uint32_t w[8];
 #pragma unroll

@@ -8,11 +8,12 @@ namespace frb_products8 {
 
 #define RC_KEPT 4                      // runs of 8 entries that a thread keeps in registers; what is beyond is read a second time (from L1)
 
-// A row is taken by PER_ROW threads, a block of 128 or 512 holds one or several.  Bound by memory where there are many rows, by two trips to it
-// and the row's maximum where there are few.  `places`: row t goes to the rows places[t * copies + c] of the result (negative: nowhere),
+// A row is taken by PER_ROW threads, a block of 128 or more holds one or several.  Bound by memory where there are many rows (2,048 of 8192
+// float32 by 512 threads each 24 us, by 256 with all of their entries in registers 16), by two trips to it and the row's maximum where there
+// are few.  `places`: row t goes to the rows places[t * copies + c] of the result (negative: nowhere),
 // else to row t.
 template <typename T, int PER_ROW>
-__global__ void __launch_bounds__(PER_ROW < 128 ? 128 : PER_ROW, PER_ROW == 512 ? 2 : sizeof(T) == 4 ? 6 : 8)
+__global__ void __launch_bounds__(PER_ROW < 128 ? 128 : PER_ROW, PER_ROW == 512 ? 2 : (sizeof(T) == 4 ? 6 : 8) / (PER_ROW == 256 ? 2 : 1))
 rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP, const int* __restrict__ places, int copies, int8_t* __restrict__ codes,
                  float* __restrict__ scales, int whole_rows) {
     constexpr int BLOCK = PER_ROW < 128 ? 128 : PER_ROW, AT_ONCE = BLOCK / PER_ROW;
@@ -21,8 +22,10 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
     wait_for_previous_kernel();
     let_next_kernel_start();           // after the wait: the kernel after this one may read ahead what kernels before this one wrote
     int turn = 0;
-    for (int row = blockIdx.x * AT_ONCE + threadIdx.x / PER_ROW; row < rows; row += gridDim.x * AT_ONCE, turn ^= 1) {
-        const T* src = x + (size_t)row * x_stride;
+    for (int base = blockIdx.x * AT_ONCE; base < rows; base += gridDim.x * AT_ONCE, turn ^= 1) {
+        const int row = base + threadIdx.x / PER_ROW;
+        const bool there = AT_ONCE == 1 || row < rows;          // (a block's last rows may be none; its barrier is for all)
+        const T* src = x + (size_t)(there ? row : 0) * x_stride;
         Eight<T> kept[RC_KEPT];
         uint32_t top = 0;
 #pragma unroll
@@ -42,8 +45,10 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
         if (PER_ROW > 32) {
             if (lane == 0) warp_top[turn][warp] = top;
             __syncthreads();           // (two sets of maxima in turn: a warp that is ahead writes the other)
-            top = __reduce_max_sync(0xffffffffu, lane < BLOCK / 32 ? warp_top[turn][lane] : 0u);
+            constexpr int WARPS = PER_ROW / 32;                   // of a row
+            top = __reduce_max_sync(0xffffffffu, lane < WARPS ? warp_top[turn][warp / WARPS * WARPS + lane] : 0u);
         }
+        if (!there) continue;
         const float a = __uint_as_float(top);
         float factor, scale;
         bool check;
@@ -109,8 +114,10 @@ int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const i
     } while (0)
     // as few threads a row as hold it in registers, where there are rows for every SM; else as many as there may be
     FRB_DISPATCH_DTYPE(x_type, T, {
-        if (rows <= 2 * frb_sm_count() || K > 128 * 8 * RC_KEPT) LAUNCH(512);
-        else if (K > 32 * 8 * RC_KEPT) LAUNCH(128);
+        if (rows <= 2 * frb_sm_count() || K > 256 * 8 * RC_KEPT) LAUNCH(512);
+        else if (K > 128 * 8 * RC_KEPT) LAUNCH(256);
+        else if (K > 64 * 8 * RC_KEPT) LAUNCH(128);
+        else if (K > 32 * 8 * RC_KEPT) LAUNCH(64);
         else LAUNCH(32);
     });
 #undef LAUNCH
