@@ -83,10 +83,10 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, stream);     // (the first product waited before it let this one start)
 }
 
-// The experts' outputs y [N, d] (rows y_stride apart, in the order of the lists) for T tokens that were given their rows already: row_of_assign
+// The experts' outputs y [N, d] (float32, rows y_stride apart, in the order of the lists) for T tokens that were given their rows already: row_of_assign
 // [T, top_k], or null where x holds the rows in that order (top_k 1).
 static int expert_rows(const void* x, int x_type, int T, int d, int top_k, const int* row_of_assign, const Lists& lists, const void* w_in,
-                       const float* in_scale, int experts, int I, const void* w_down, const float* down_scale, float limit, void* y, int y_type, int y_stride,
+                       const float* in_scale, int experts, int I, const void* w_down, const float* down_scale, float limit, float* y, int y_stride,
                        Scratch& s, long long scratch_bytes, int* status, cudaStream_t stream) {
     FRB_CHECK_ARG(row_of_assign != nullptr || top_k == 1, "experts in 8 bits: rows in order go to one expert each, not %d", top_k);
     const int N = T * top_k;
@@ -105,11 +105,10 @@ static int expert_rows(const void* x, int x_type, int T, int d, int top_k, const
     FRB_TRY(product(p, stream));
     FRB_TRY(rows_codes(hidden, FRB_F32, IP, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
     p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y; p.out_stride = y_stride;
-    p.out_type = y_type;
     return product(p, stream);
 }
 
-// The same with float32 outputs, one row behind another.
+// The same with one row behind another.
 FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int top_k, const int* row_of_assign, const int* tile_expert, const int* tile_row0,
                                  const int* num_tiles, const int* offsets, int max_tiles, int tile_rows, const void* w_in, const float* in_scale, int experts,
                                  int I, const void* w_down, const float* down_scale, float limit, float* y, void* scratch, long long scratch_bytes, int* status,
@@ -118,7 +117,7 @@ FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int to
     FRB_CHECK_ARG((long long)T * top_k < (1ll << 31), "experts in 8 bits: %d tokens of %d experts", T, top_k);
     Scratch s(scratch);
     return expert_rows(x, x_type, T, d, top_k, row_of_assign, {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows}, w_in, in_scale, experts, I,
-                       w_down, down_scale, limit, y, FRB_F32, d, s, scratch_bytes, status, stream);
+                       w_down, down_scale, limit, y, d, s, scratch_bytes, status, stream);
 }
 
 // out [T, d] = sum over r of weights[t, r] * unit of expert ids[t, r] on x[t].  w_in: codes [experts][2][I up to 16][d up to 128], w_down:
@@ -138,11 +137,11 @@ FRB_API int frb_experts_8bit(const void* x, int x_type, int T, int d, int top_k,
     int* tile_row0 = s.take<int>(max_tiles);
     int* num_tiles = s.take<int>(1);
     const int y_stride = hidden_stride(d);
-    char* y = s.take<char>((long long)N * y_stride * (out_type == FRB_F32 ? 4 : 2));
+    float* y = s.take<float>((long long)N * y_stride);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, more are needed", scratch_bytes);
     FRB_TRY(plan(ids, T, top_k, experts, tile_rows, offsets, row_of_assign, tile_expert, tile_row0, num_tiles, stream));
     FRB_TRY(expert_rows(x, x_type, T, d, top_k, row_of_assign, {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows}, w_in, in_scale, experts, I,
-                        w_down, down_scale, limit, y, out_type, y_stride, s, scratch_bytes, status, stream));
+                        w_down, down_scale, limit, y, y_stride, s, scratch_bytes, status, stream));
     return combine(y, y_stride, weights, row_of_assign, T, top_k, d, out, out_type, stream);
 }
 

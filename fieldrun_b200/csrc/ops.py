@@ -2121,7 +2121,7 @@ def expert_rows_8bit(x: torch.Tensor, row_of_assign: Optional[torch.Tensor], lis
 def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor, down_codes: torch.Tensor,
                  down_scales: torch.Tensor, out: torch.Tensor, *, width: int, gate_limit: float = 0.0, scratch: Optional[torch.Tensor] = None) -> None:
     """Routed experts in 8-bit integers: out[t] = sum over r of ``weights[t, r]`` * (gated block of expert ``ids[t, r]`` on x[t]), the
-    blocks as :func:`expert_rows_8bit` computes them, their outputs rounded to out's type, the sum in float32 in the order of r, rounded once.  ``ids`` int32 and
+    blocks as :func:`expert_rows_8bit` computes them, their sum in float32 in the order of r, rounded once to out's type.  ``ids`` int32 and
     ``weights`` float32 [T, top_k]; an id that names no expert (-1) adds nothing."""
     tokens, inner, _ = _rows_in_and_out(x, out, True)
     if ids.dim() != 2 or ids.shape[0] != tokens or weights.shape != ids.shape or not 1 <= ids.shape[1] <= 128:

@@ -57,7 +57,7 @@ struct Product {
 int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const int* places, int copies, void* codes, float* scales, cudaStream_t stream);
 int plan(const int* ids, int tokens, int top_k, int experts, int tile_rows, int* offsets, int* row_of_assign, int* tile_expert, int* tile_row0,
          int* num_tiles, cudaStream_t stream);
-int combine(const void* y, int y_stride, const float* weights, const int* row_of_assign, int tokens, int top_k, int width, void* out, int type,
+int combine(const float* y, int y_stride, const float* weights, const int* row_of_assign, int tokens, int top_k, int width, void* out, int out_type,
             cudaStream_t stream);
 // products_8bit.cu
 bool tokens_fit(int rows, int K);

@@ -264,8 +264,7 @@ def check_experts(x, ids, weights, parts, limit=0.0, dtype=F32):
             exact.index_add_(0, token, y * weight)
             bound.index_add_(0, token, off * weight.abs())
             size.index_add_(0, token, y.abs() * weight.abs())
-    # a product and a sum a rank, and an expert's output travels in the result's type
-    plain.agree(out, exact, bound + ((ids.shape[1] + 1) * plain.U + plain.HALF_STEP[dtype]) * size)
+    plain.agree(out, exact, bound + (ids.shape[1] + 1) * plain.U * size)            # a product and a sum a rank
     return out
 
 
