@@ -15,6 +15,7 @@ struct Scratch {
         at += (count * (long long)sizeof(T) + 255) / 256 * 256;
         return here;
     }
+    bool starts_well() const { return ((uintptr_t)base & 15) == 0; }
 };
 
 // From one row of a unit's middle to the next: whole lines, whatever the width.
@@ -52,6 +53,10 @@ FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void*
         scales = s.take<float>(T);
     }
     FRB_CHECK_ARG(s.at <= scratch_bytes, "linear in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
+    FRB_CHECK_ARG(s.starts_well(), "linear in 8 bits: the scratch starts on 16 bytes");
+    const size_t x_bytes = (size_t)T * K * (x_type == FRB_F32 ? 4 : 2), out_bytes = (size_t)T * F * (out_type == FRB_F32 ? 4 : 2);
+    FRB_CHECK_ARG((uintptr_t)x + x_bytes <= (uintptr_t)out || (uintptr_t)out + out_bytes <= (uintptr_t)x,
+                  "linear in 8 bits: the results lie on the rows that they are made of");
     Product p = {};
     p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K; p.rows = T; p.out = out; p.out_stride = F; p.out_type = out_type;
     p.status = status;
@@ -75,6 +80,7 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     int8_t* hidden_codes = s.take<int8_t>((long long)T * up_to(I, FRB_8BIT_KBLOCK));
     float* hidden_scales = s.take<float>(T);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "gated block in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
+    FRB_CHECK_ARG(s.starts_well(), "gated block in 8 bits: the scratch starts on 16 bytes");
     Product p = {};
     p.w = w_in; p.w_scale = in_scale; p.experts = 1; p.parts = 2; p.F = I; p.K = d; p.rows = T; p.out = hidden; p.out_stride = IP;
     p.out_type = FRB_F32; p.gate = gate; p.limit = limit; p.status = status;
@@ -97,6 +103,7 @@ static int expert_rows(const void* x, int x_type, int T, int d, int top_k, const
     int8_t* hidden_codes = s.take<int8_t>((long long)N * up_to(I, FRB_8BIT_KBLOCK));
     float* hidden_scales = s.take<float>(N);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
+    FRB_CHECK_ARG(s.starts_well(), "experts in 8 bits: the scratch starts on 16 bytes");
     FRB_TRY(rows_codes(x, x_type, d, T, d, row_of_assign, top_k, codes, scales, stream));
     Product p = {};
     p.w = w_in; p.w_scale = in_scale; p.experts = experts; p.parts = 2; p.F = I; p.K = d; p.rows = N; p.x = codes; p.x_scale = scales;
@@ -114,7 +121,7 @@ FRB_API int frb_expert_rows_8bit(const void* x, int x_type, int T, int d, int to
                                  int I, const void* w_down, const float* down_scale, float limit, float* y, void* scratch, long long scratch_bytes, int* status,
                                  cudaStream_t stream) {
     if (T == 0) return 0;
-    FRB_CHECK_ARG((long long)T * top_k < (1ll << 31), "experts in 8 bits: %d tokens of %d experts", T, top_k);
+    FRB_CHECK_ARG((long long)T * top_k < (1ll << 30), "experts in 8 bits: %d tokens of %d experts", T, top_k);
     Scratch s(scratch);
     return expert_rows(x, x_type, T, d, top_k, row_of_assign, {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows}, w_in, in_scale, experts, I,
                        w_down, down_scale, limit, y, d, s, scratch_bytes, status, stream);
@@ -126,7 +133,7 @@ FRB_API int frb_experts_8bit(const void* x, int x_type, int T, int d, int top_k,
                              const float* in_scale, int experts, int I, const void* w_down, const float* down_scale, float limit, int tile_rows, void* out,
                              int out_type, void* scratch, long long scratch_bytes, int* status, cudaStream_t stream) {
     if (T == 0) return 0;
-    FRB_CHECK_ARG((long long)T * top_k < (1ll << 31), "experts in 8 bits: %d tokens of %d experts", T, top_k);
+    FRB_CHECK_ARG((long long)T * top_k < (1ll << 30), "experts in 8 bits: %d tokens of %d experts", T, top_k);
     FRB_CHECK_ARG(experts >= 1 && experts <= 8192, "experts in 8 bits: %d experts are outside 1..8192", experts);
     FRB_CHECK_ARG(tile_rows >= 1, "experts in 8 bits: tiles of %d rows", tile_rows);
     const int N = T * top_k, max_tiles = N / tile_rows + (experts < N ? experts : N);

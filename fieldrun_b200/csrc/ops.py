@@ -2015,6 +2015,11 @@ def _scratch_8bit(scratch: Optional[torch.Tensor], need: int, device) -> torch.T
     return scratch
 
 
+def _rounded_by_the_product(rows: int, inner: int) -> bool:
+    """Whether a product rounds its few rows itself (tokens_fit in products_8bit.cu): one kernel instead of two."""
+    return rows <= 8 and inner <= (14336, 14336, 8192, 4096, 4096, 2048)[min(rows, 5)]
+
+
 def _status_at(device) -> int:
     status = _TC_STATUS.get(str(device))
     return (tc_status(device) if status is None else status).data_ptr()
@@ -2022,7 +2027,7 @@ def _status_at(device) -> int:
 
 def linear_8bit_scratch(rows: int, inner: int) -> int:
     """Bytes of scratch that :func:`linear_8bit` needs (none for a few tokens, which the product rounds itself)."""
-    if rows <= 8 and inner <= 14336 and inner <= (16384, 16384, 8192, 4096, 4096, 2048)[min(rows, 5)]:
+    if _rounded_by_the_product(rows, inner):
         return 0
     return _rows_scratch(rows, inner)
 
@@ -2042,6 +2047,8 @@ def linear_8bit(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, out:
     at = _addresses(x, codes, scales, out, scratch)
     _call("frb_linear_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], features, at[3], _code(out.dtype), int(weights_final), at[4], need,
           _status_at(x.device))
+    if need == 0:
+        count_launches(-1 if rows else -2)
 
 
 def _rows_scratch(rows: int, inner: int) -> int:
@@ -2068,6 +2075,7 @@ def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor,
     at = _addresses(x, in_codes, in_scales, down_codes, down_scales, out, scratch)
     _call("frb_gated_8bit", at[0], _code(x.dtype), rows, inner, at[1], at[2], width, at[3], at[4], GATES_8BIT[activation], float(gate_limit), at[5],
           _code(out.dtype), int(weights_final), at[6], scratch.numel(), _status_at(x.device))
+    count_launches(-(int(_rounded_by_the_product(rows, inner)) + int(_rounded_by_the_product(rows, width)) if rows else 4))
 
 
 def expert_tile_rows_8bit(assignments: int, experts: int) -> int:

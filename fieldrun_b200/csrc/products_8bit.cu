@@ -49,7 +49,7 @@ struct Params {
     const float* x_scale;
     void* out;
     int* status;
-    int rows, F, FP;
+    int rows, experts, F, FP;
     int out_stride;
     int k_blocks;
     int n;                 // channels of a tile
@@ -323,7 +323,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
     const bool listed = p.lists.tile_expert != nullptr;
-    const int items = __shfl_sync(0xffffffffu, (listed ? p.lists.num_tiles[0] : p.row_tiles) * p.channel_tiles, 0);
+    const int items = __shfl_sync(0xffffffffu, (listed ? min(p.lists.num_tiles[0], p.lists.max_tiles) : p.row_tiles) * p.channel_tiles, 0);
     const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
     // Neighbouring items: with lists the channel tiles of one expert's rows (its weights are read once), without the tiles of tokens
     // over the same weights.
@@ -331,8 +331,8 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         if (listed) {
             const int tile = item / p.channel_tiles;
             channel = (item - tile * p.channel_tiles) * p.n;
-            expert = p.lists.tile_expert[tile];
-            row0 = p.lists.tile_row0[tile];
+            expert = min(max(p.lists.tile_expert[tile], 0), p.experts - 1);       // (nothing is read out of place, whatever a list says)
+            row0 = min(max(p.lists.tile_row0[tile], 0), p.rows);
         } else {
             const int t = item / p.row_tiles;
             channel = t * p.n;
@@ -464,7 +464,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             if (item >= items) return;
             int row0, expert, channel;
             place(item, row0, expert, channel);
-            const int rows = listed ? min(p.lists.tile_rows, p.lists.offsets[expert + 1] - row0) : p.rows - row0;
+            const int rows = listed ? min(p.lists.tile_rows, min(p.lists.offsets[expert + 1], p.rows) - row0) : p.rows - row0;
             const int within = side * 128 + quarter * span + lane, i = threadIdx.x - 64;
             if (!ROUNDS && within < rows && lane < span && quarter * span + lane < p.x_box) next_x = p.x_scale[row0 + within];
             if (i < p.columns) {
@@ -476,12 +476,18 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         for (int item = first; item < items; item += step) {
             int row0, expert, channel;
             place(item, row0, expert, channel);
-            const int rows = listed ? min(p.lists.tile_rows, p.lists.offsets[expert + 1] - row0) : p.rows - row0;
+            const int rows = listed ? min(p.lists.tile_rows, min(p.lists.offsets[expert + 1], p.rows) - row0) : p.rows - row0;
             const int warp_row = side * 128 + quarter * span, within = warp_row + lane;
             const bool mine = within < rows && lane < span && quarter * span + lane < p.x_box;
             const bool any = warp_row < rows && quarter * span < p.x_box;
             const int row = row0 + within;
+            // A sum times the token's scale times the channel's; a token's scale of one and more (or NaN) comes last, in a branch that hardly ever is
+            // taken, so that no product on the way leaves float32's range where the result does not (scales are 2^-103 and more, sums below 2^31).
+            // With gate and up the channel's scale always comes first (the branch's instructions cost one token's block 1.4 us of 34): the
+            // same for channels' scales below 2^96.
             const float x_scale = !mine ? 0.f : ROUNDS ? token_scales[within & 7] : next_x;
+            const float x_first = x_scale < 1.f ? x_scale : 1.f, x_last = x_scale < 1.f ? 1.f : x_scale;
+            const bool large = __any_sync(0xffffffffu, !(x_scale < 1.f));
             const int channels = min(p.n, p.F - channel);
             float* scales = w_scales[half];
             scales[threadIdx.x - 64] = next_w;                        // (there are as many threads as columns at most)
@@ -518,8 +524,13 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                             const float first_scale[4] = {s0.x, s0.y, s0.z, s0.w}, second_scale[4] = {s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                v[i + j] = (float)(int)acc[h][0][i + j] * x_scale * first_scale[j];
-                                if (PARTS == 2) v[i + j] = gated(v[i + j], (float)(int)acc[h][PARTS - 1][i + j] * x_scale * second_scale[j], p.gate);
+                                if (PARTS == 1) {
+                                    v[i + j] = (float)(int)acc[h][0][i + j] * x_first * first_scale[j];
+                                    if (large) v[i + j] *= x_last;
+                                } else {
+                                    v[i + j] = gated((float)(int)acc[h][0][i + j] * first_scale[j] * x_scale,
+                                                     (float)(int)acc[h][PARTS - 1][i + j] * second_scale[j] * x_scale, p.gate);
+                                }
                             }
                         }
                         if (!p.staged) {
@@ -665,7 +676,7 @@ int product(const Product& q, cudaStream_t stream) {
     FRB_CHECK_ARG(ctas != 0, "product in 8 bits: no form for %d rows of %d entries", q.rows, q.K);
     Params p;
     p.lists = q.lists; p.w_scale = q.w_scale; p.x_scale = q.x_scale; p.out = q.out; p.status = q.status;
-    p.rows = q.rows; p.F = q.F; p.FP = FP; p.k_blocks = KP / FRB_8BIT_KBLOCK; 
+    p.rows = q.rows; p.experts = q.experts; p.F = q.F; p.FP = FP; p.k_blocks = KP / FRB_8BIT_KBLOCK; 
     const float log2e = 1.4426950408889634f, slope = q.limit > 0.f ? FRB_CLAMPED_GATE_SLOPE : q.gate == FRB_GATE_GELU_TANH ? 1.5957691216057308f : 1.0f;
     p.gate.a = -log2e * slope;
     p.gate.b = q.limit <= 0.f && q.gate == FRB_GATE_GELU_TANH ? -log2e * slope * 0.044715f : 0.f;

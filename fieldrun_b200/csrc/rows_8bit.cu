@@ -10,11 +10,11 @@ namespace frb_products8 {
 
 // A row is taken by PER_ROW threads, a block of 128 or more holds one or several.  Bound by memory where there are many rows (2,048 of 8192
 // float32 by 512 threads each 24 us, by 256 with all of their entries in registers 16), by two trips to it and the row's maximum where there
-// are few.  `places`: row t goes to the rows places[t * copies + c] of the result (negative: nowhere),
+// are few.  `places`: row t goes to the rows places[t * copies + c] of the result (nowhere where that is none of them),
 // else to row t.
 template <typename T, int PER_ROW>
 __global__ void __launch_bounds__(PER_ROW < 128 ? 128 : PER_ROW, PER_ROW == 512 ? 2 : (sizeof(T) == 4 ? 6 : 8) / (PER_ROW == 256 ? 2 : 1))
-rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP, const int* __restrict__ places, int copies, int8_t* __restrict__ codes,
+rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP, const int* __restrict__ places, int copies, int places_end, int8_t* __restrict__ codes,
                  float* __restrict__ scales, int whole_rows) {
     constexpr int BLOCK = PER_ROW < 128 ? 128 : PER_ROW, AT_ONCE = BLOCK / PER_ROW;
     __shared__ uint32_t warp_top[2][BLOCK / 32];
@@ -65,7 +65,7 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
 #pragma unroll 1
         for (int i = 0; i < count; ++i) {
             const int to = places ? places[(size_t)row * copies + i] : row;
-            if (to < 0) continue;
+            if ((unsigned)to >= (unsigned)places_end) continue;
             int8_t* dst = codes + (size_t)to * KP;
 #pragma unroll
             for (int j = 0; j < RC_KEPT; ++j) {
@@ -78,7 +78,7 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
 #pragma unroll 1
             for (int i = 0; i < count; ++i) {
                 const int to = places ? places[(size_t)row * copies + i] : row;
-                if (to >= 0) *reinterpret_cast<uint2*>(codes + (size_t)to * KP + k) = c;
+                if ((unsigned)to < (unsigned)places_end) *reinterpret_cast<uint2*>(codes + (size_t)to * KP + k) = c;
             }
         };
 #pragma unroll 1
@@ -110,7 +110,7 @@ int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const i
     do {                                                                                                                         \
         const int at_once = PER_ROW < 128 ? 128 / PER_ROW : 1, blocks = (rows + at_once - 1) / at_once;                          \
         launch_dependent(rows_8bit_kernel<T, PER_ROW>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),                  \
-                         dim3(PER_ROW < 128 ? 128 : PER_ROW), 0, stream, (const T*)x, x_stride, rows, K, KP, places, copies, (int8_t*)codes, scales, whole); \
+                         dim3(PER_ROW < 128 ? 128 : PER_ROW), 0, stream, (const T*)x, x_stride, rows, K, KP, places, copies, places ? rows * copies : rows, (int8_t*)codes, scales, whole); \
     } while (0)
     // as few threads a row as hold it in registers, where there are rows for every SM; else as many as there may be
     FRB_DISPATCH_DTYPE(x_type, T, {

@@ -184,6 +184,48 @@ def test_results_beyond_32_bits_of_places():
         plain.agree(out[some], exact, bound)
 
 
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_scales_at_the_ends_of_the_range(rows):
+    # a token's scale of 2^96 and more, a channel's of 2^-100: no product on the way is infinite or loses places
+    gen = generator(rows)
+    codes, _, w, s = plain.random_weight(gen, 1, 1, 64, 512, DEV)
+    x = torch.randn((rows, 512), generator=gen, device=DEV)
+    for of_x, of_w in ((2.0 ** 120, 2.0 ** -100), (2.0 ** -90, 2.0 ** 110), (2.0 ** -60, 2.0 ** -50), (2.0 ** 30, 2.0 ** 60), (2.0 ** -80, 2.0 ** 80)):
+        scales = torch.full((64,), of_w, device=DEV)
+        s[0, 0, :64] = scales
+        exact, bound = plain.product(x * of_x, codes[0, 0], scales)
+        assert 2.0 ** -125 < exact.abs().min() and exact.abs().max() < 2.0 ** 127
+        plain.agree(linear(x * of_x, w, s, 64), exact, bound, (of_x, of_w))
+
+
+def test_places_that_are_refused():
+    gen = generator(7)
+    x = rows_of(gen, 20, 128)
+    _, _, w, s = plain.random_weight(gen, 1, 1, 128, 128, DEV)
+    with pytest.raises(ops.KernelError, match="lie on the rows"):
+        ops.linear_8bit(x, w, s, x)
+    flat = rows_of(gen, 64, 128, F32).reshape(-1)
+    with pytest.raises(ops.KernelError, match="lie on the rows"):
+        ops.linear_8bit(flat[:2560].view(20, 128), w, s, flat[2000:4560].view(20, 128))
+    odd = torch.zeros(1 << 16, dtype=torch.uint8, device=DEV)[1:]
+    with pytest.raises(ops.KernelError, match="scratch starts on 16 bytes"):
+        linear(x, w, s, 128, scratch=odd)
+    _, _, w_in, s_in = plain.random_weight(gen, 1, 2, 64, 128, DEV)
+    _, _, w_down, s_down = plain.random_weight(gen, 1, 1, 128, 64, DEV)
+    for rows in (1, 20):
+        with pytest.raises(ops.KernelError, match="scratch starts on 16 bytes"):
+            ops.gated_8bit(x[:rows], w_in, s_in, w_down, s_down, torch.empty((rows, 128), device=DEV), width=64, scratch=odd)
+    room = torch.zeros(w.numel() + 64, dtype=torch.int8, device=DEV)
+    with pytest.raises(ops.KernelError, match="start on 16 bytes"):
+        linear(x, room[1:1 + w.numel()].view(w.shape), s, 128)
+    for wrong in (x.to(torch.float16), x.to(torch.float64)):
+        with pytest.raises(ops.KernelError, match="float32 and bfloat16"):
+            linear(wrong, w, s, 128)
+    with pytest.raises(ops.KernelError, match="not contiguous"):
+        linear(rows_of(gen, 128, 20).t(), *plain.random_weight(gen, 1, 1, 128, 128, DEV)[2:], 128)
+    torch.cuda.synchronize()
+
+
 def test_no_rows():
     _, _, w, s = plain.random_weight(generator(), 1, 1, 40, 100, DEV)
     ops.linear_8bit(torch.zeros((0, 100), device=DEV), w, s, torch.zeros((0, 40), device=DEV))
@@ -314,6 +356,24 @@ def test_experts_with_lists_of_the_frameworks_own():
         out = torch.empty((300, 256), device=DEV)
         ops.expert_combine(y, weights, row_of_assign, out)
         assert torch.equal(out, want), tile_rows
+
+
+def test_lists_that_point_out_of_place_reach_nothing_outside():
+    gen = generator(13)
+    x, _, _, parts = experts_case(gen, 24, 256, 128, 3, 1)
+    (ic, iscale, w_in, s_in), (dc, dscale, w_down, s_down) = parts
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    room = torch.full((24 * 256 + 512,), 5.0, device=DEV)
+    y = room[256:256 + 24 * 256].view(24, 256)
+    order = torch.arange(24, dtype=torch.int32, device=DEV)
+    order[5], order[6] = -1, 1 << 20
+    # tiles of experts 0 .. 2 in their places, then ones of no expert and of no rows; more of them than the lists hold
+    lists = (ints(0, 1, 2, 99, -7, 1), ints(0, 8, 16, 1 << 20, -100, 1 << 28), ints(1 << 20), ints(0, 8, 16, 24))
+    ops.expert_rows_8bit(x, order, lists, 6, 8, w_in, s_in, w_down, s_down, y, width=128)
+    torch.cuda.synchronize()
+    exact, bound = plain.block(x[8:16], ic[1], iscale[1], dc[1, 0], dscale[1, 0])
+    plain.agree(y[8:16], exact, bound)
+    assert (room[:256] == 5).all() and (room[256 + 24 * 256:] == 5).all()
 
 
 # ------------------------------------------------------------------------------------------------ streams and graphs
