@@ -10,7 +10,9 @@ per expert, as in a step of 16k prompt tokens),
 ``experts_stream`` (decode-sized expert products: the persistent TMA-fed stream; ``experts_stream_mma``: the kernel that
 loads weights into registers, kept for inner sizes that are no multiple of 64), ``attention_decode`` (pages by TMA),
 ``attention_decode_mma`` (pages loaded into registers), ``attention_decode_8bit`` (pages of e4m3 codes; ``..._int8``: int8; ``..._long``: one sequence
-of 131,072 keys), ``cache_8bit_write`` (rows of a prompt of 2,048 tokens into 8-bit pages) and ``cache_8bit_read`` (512 pages read back), ``attention_prefill``
+of 131,072 keys), ``cache_8bit_write`` (rows of a prompt of 2,048 tokens into 8-bit pages) and ``cache_8bit_read`` (512 pages read back), ``linear_8bit`` (8,192 tokens
+through a weight of 8-bit codes; ``..._token``: one), ``gated_8bit`` (2,048 tokens through a gated block; ``..._token``: one) and ``experts_8bit`` (8 tokens through
+MiniMax-M2's experts), ``attention_prefill``
 (mma.sync tiles of 16 queries), ``attention_prefill_tc`` (tcgen05 tiles of 128 queries; ``attention_prefill_tc_long``: one prompt of 16,384 tokens),
 ``latent_attention_prefill`` (attention over shared key rows of 512 + 64 entries, tcgen05; ``latent_attention_prefill_mma``: the
 mma.sync kernel), ``latent_attention_decode`` and ``latent_attention_decode_small`` (single tokens in chunks of keys, with the join; ``..._mma``: the mma.sync kernel),
@@ -206,6 +208,39 @@ def cache_8bit(kind: str, launches: int) -> dict:
     ops.tc_status_check(torch.device(DEV))
     return {"case": ("cache_8bit_" if kind in ("write", "read") else "") + kind, "ms": round(ms, 4), "batch": batch, "context": context,
             "gb_per_s": round(moved / ms / 1e6, 1)}
+
+
+def products_8bit(kind: str, launches: int) -> dict:
+    def weight(experts, parts, features, inner):
+        shape = ops.weight_8bit_shape(experts, parts, features, inner)
+        return torch.randint(-127, 128, shape, dtype=torch.int8, device=DEV), torch.rand(shape[:3], device=DEV) * 1e-4
+    tokens = 1 if kind.endswith("token") else {"linear": 8192, "gated": 2048, "experts": 8}[kind]
+    inner, width, turn = (HIDDEN, WIDTH, iter(range(1 << 30))) if kind == "experts" else (4096, 12288, iter(range(1 << 30)))
+    x = torch.randn(tokens, inner, device=DEV).to(torch.bfloat16)
+    if kind.startswith("linear"):
+        weights, out = [weight(1, 1, width, inner) for _ in range(6)], torch.empty(tokens, width, dtype=torch.bfloat16, device=DEV)
+        launch = lambda: ops.linear_8bit(x, *weights[next(turn) % 6], out)
+        products, codes = tokens * inner * width, inner * width
+    else:
+        experts = 256 if kind == "experts" else 1
+        weights = [(weight(experts, 2, width, inner), weight(experts, 1, inner, width)) for _ in range(1 if experts > 1 else 4)]
+        out = torch.empty(tokens, inner, dtype=torch.bfloat16, device=DEV)
+        picks = [torch.randn(tokens, experts, device=DEV).topk(8)[1].to(torch.int32) for _ in range(4)] if experts > 1 else []
+        scores = torch.full((tokens, 8), 0.125, device=DEV)
+
+        def launch():
+            n = next(turn)
+            gate_up, down = weights[n % len(weights)]
+            if experts > 1:
+                ops.experts_8bit(x, picks[n % 4], scores, *gate_up, *down, out, width=width)
+            else:
+                ops.gated_8bit(x, *gate_up, *down, out, width=width)
+        products = tokens * 3 * inner * width * (8 if experts > 1 else 1)
+        codes = 3 * inner * width * (len(torch.unique(picks[0])) if experts > 1 else 1)
+    ms = _time_recorded(launch, launches)
+    ops.tc_status_check(torch.device(DEV))
+    return {"case": kind.replace("linear", "linear_8bit").replace("gated", "gated_8bit").replace("experts", "experts_8bit"), "ms": round(ms, 4),
+            "tokens": tokens, "weights_gb_per_s": round(codes / ms / 1e6, 1), "tera_operations": round(2 * products / ms / 1e9, 1)}
 
 
 LATENT_HEADS, LATENT_RANK, LATENT_ROT = 16, 512, 64
@@ -821,6 +856,11 @@ CASES = {
     "attention_decode_8bit_long": lambda n: cache_8bit("attention_decode_8bit_long", n),
     "cache_8bit_write": lambda n: cache_8bit("write", n),
     "cache_8bit_read": lambda n: cache_8bit("read", n),
+    "linear_8bit": lambda n: products_8bit("linear", n),
+    "linear_8bit_token": lambda n: products_8bit("linear_token", n),
+    "gated_8bit": lambda n: products_8bit("gated", n),
+    "gated_8bit_token": lambda n: products_8bit("gated_token", n),
+    "experts_8bit": lambda n: products_8bit("experts", n),
     "attention_prefill": lambda n: attention("prefill", n),
     "attention_prefill_tc": lambda n: attention("prefill_tc", n),
     "attention_prefill_tc_long": lambda n: attention("prefill_tc_long", n),
