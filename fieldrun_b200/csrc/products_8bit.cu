@@ -286,7 +286,9 @@ __device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, 
 }
 
 // InT int8_t: the tokens' codes come with the weights, stage by stage; otherwise they are rounded here (at most eight, CTAS 1, no lists).
-template <int CTAS, int PARTS, typename OutT, typename InT>
+// WHOLE: tiles of 128 tokens a block, whose results are many; without, the way out is short code in place of a fast one (one token's gated block
+// of 4096 and 12288: 34.8 us with the code of whole tiles, most of it waiting for instructions, 31.9 without).
+template <int CTAS, int PARTS, typename OutT, typename InT, bool WHOLE>
 __global__ void __launch_bounds__(P8_THREADS, 1)
 product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Params p) {
     extern __shared__ uint8_t smem_raw[];
@@ -452,8 +454,9 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         // there in whole lines; otherwise every lane stores its token's channels.  (8,192 tokens, 1024 x 8192, float32: 109 us without.  Copies by TMA,
         // with their fence, wait and map, took 92.)
         // A step is 32 channels, or 16 of gate and up.
-        constexpr int STEP = PARTS == 1 ? 32 : 16, GROUP_STEPS = 128 / (int)sizeof(OutT) / STEP;        // steps in 128 bytes
-        const int shift = p.staged ? (GROUP_STEPS == 1 ? 0 : 1) : 0;
+        constexpr int STEP = PARTS == 1 && WHOLE ? 32 : 16, HALVES = WHOLE ? 2 : 1, GROUP_STEPS = 128 / (int)sizeof(OutT) / STEP;        // steps in 128 bytes
+        const bool staged = WHOLE && p.staged;
+        const int shift = staged ? (GROUP_STEPS == 1 ? 0 : 1) : 0;
         uint8_t* buffer = ring + (size_t)p.stages * stage_bytes + (warp - 2) * 4096;
         const auto step_at = [&](int i) { return STEP * ((((i >> shift) * 2 + turn) << shift) + (i & ((1 << shift) - 1))); };
         int half = 0;
@@ -501,21 +504,25 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             if (any && done) {
                 const uint32_t sums = lanes + half * p.columns;
                 OutT* dst = out + (size_t)row * p.out_stride + channel;
-                uint32_t acc[2][PARTS][STEP];
-                if (step_at(0) < channels) {
+                uint32_t acc[HALVES][PARTS][STEP];                 // (two: the next step's sums come while this one's are scaled)
+                if (HALVES == 2 && step_at(0) < channels) {
 #pragma unroll
                     for (int q = 0; q < PARTS; ++q) load_sums(sums + q * p.n + step_at(0), acc[0][q]);
                 }
 #pragma unroll 1
-                for (int turns = 0; step_at(turns) < channels; turns += 2) {
+                for (int turns = 0; step_at(turns) < channels; turns += HALVES) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
+                    for (int h = 0; h < HALVES; ++h) {
                         const int c0 = step_at(turns + h), next = step_at(turns + h + 1);
                         if (c0 >= channels) break;
-                        tmem_wait_ld();
-                        if (next < channels) {
+                        if (HALVES == 1) {
 #pragma unroll
-                            for (int q = 0; q < PARTS; ++q) load_sums(sums + q * p.n + next, acc[h ^ 1][q]);
+                            for (int q = 0; q < PARTS; ++q) load_sums(sums + q * p.n + c0, acc[0][q]);
+                        }
+                        tmem_wait_ld();
+                        if (HALVES == 2 && next < channels) {
+#pragma unroll
+                            for (int q = 0; q < PARTS; ++q) load_sums(sums + q * p.n + next, acc[HALVES - 1 - h][q]);
                         }
                         float v[STEP];
 #pragma unroll
@@ -533,7 +540,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                                 }
                             }
                         }
-                        if (!p.staged) {
+                        if (!staged) {
 #pragma unroll
                             for (int i = 0; i < STEP; i += 16)
                                 if (mine && c0 + i < channels) store16(dst + c0 + i, v + i, channels - c0 - i, p.out_align);
@@ -726,21 +733,23 @@ int product(const Product& q, cudaStream_t stream) {
     attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = ctas == 2 ? 2 : 1;
-#define LAUNCH(CTAS, PARTS, OutT, InT)                                                                                                \
+#define LAUNCH(CTAS, PARTS, OutT, InT, WHOLE)                                                                                         \
     do {                                                                                                                              \
-        may_have_shared<product_8bit_kernel<CTAS, PARTS, OutT, InT>>();                                                               \
-        cudaLaunchKernelEx(&config, product_8bit_kernel<CTAS, PARTS, OutT, InT>, map_x, map_w, p);                                    \
+        may_have_shared<product_8bit_kernel<CTAS, PARTS, OutT, InT, WHOLE>>();                                                         \
+        cudaLaunchKernelEx(&config, product_8bit_kernel<CTAS, PARTS, OutT, InT, WHOLE>, map_x, map_w, p);                             \
     } while (0)
     FRB_CHECK_ARG(q.parts == 1 || q.out_type == FRB_F32, "product in 8 bits: gated units come out in float32");
     if (q.parts == 2) {
-        if (rounds) { FRB_DISPATCH_DTYPE(q.x_type, InT, LAUNCH(1, 2, float, InT)); }
-        else if (ctas == 2) LAUNCH(2, 2, float, int8_t);
-        else LAUNCH(1, 2, float, int8_t);
+        if (rounds) { FRB_DISPATCH_DTYPE(q.x_type, InT, LAUNCH(1, 2, float, InT, false)); }
+        else if (ctas == 2) LAUNCH(2, 2, float, int8_t, true);
+        else if (p.x_box == 128) LAUNCH(1, 2, float, int8_t, true);
+        else LAUNCH(1, 2, float, int8_t, false);
     } else {
         FRB_DISPATCH_DTYPE(q.out_type, OutT, {
-            if (rounds) { FRB_DISPATCH_DTYPE(q.x_type, InT, LAUNCH(1, 1, OutT, InT)); }
-            else if (ctas == 2) LAUNCH(2, 1, OutT, int8_t);
-            else LAUNCH(1, 1, OutT, int8_t);
+            if (rounds) { FRB_DISPATCH_DTYPE(q.x_type, InT, LAUNCH(1, 1, OutT, InT, false)); }
+            else if (ctas == 2) LAUNCH(2, 1, OutT, int8_t, true);
+            else if (p.x_box == 128) LAUNCH(1, 1, OutT, int8_t, true);
+            else LAUNCH(1, 1, OutT, int8_t, false);
         });
     }
 #undef LAUNCH
