@@ -253,8 +253,8 @@ __device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, 
 #pragma unroll
     for (int j = 0; j < P8_KEPT; ++j) {
         const int k = first + j * step;
+        kept[j].clear();
         if (mine && k < p.K) kept[j].read(src + k, p.K - k, p.whole_rows);
-        else kept[j].clear();
     }
 #pragma unroll
     for (int j = 0; j < P8_KEPT; ++j) top = top_of(kept[j], top);
@@ -272,15 +272,15 @@ __device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, 
 #pragma unroll
     for (int j = 0; j < P8_KEPT; ++j) {
         const int k = first + j * step;
-        if (k >= KP) continue;
+        if (k >= KP) break;
         bool near;
-        *place(k) = codes_of(kept[j], factor, check, near);
+        *place(k) = codes_of<InT, false>(kept[j], factor, check, near);
         again |= (uint32_t)near << j;
     }
 #pragma unroll 1
     for (int j = 0; again >> j; ++j) {
         const int k = first + j * step;
-        if (again >> j & 1) *place(k) = slow_codes(src + k, p.K - k, factor, __uint_as_float(top));
+        if ((again >> j & 1) && k < p.K) *place(k) = slow_codes(src + k, p.K - k, factor, __uint_as_float(top));
     }
     if (sub == 0 && lane == 0) scales[row] = scale;
 }

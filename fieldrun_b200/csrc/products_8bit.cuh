@@ -134,7 +134,8 @@ __device__ __forceinline__ void row_factor(uint32_t top, float& factor, float& s
 
 // 127 x / a rounded half to even, for eight entries; `near`: one of them is so near to the middle of two codes that slow_codes() has to decide.  In a
 // row of bfloat16 that is to be checked an entry nearer than 1e-6 of itself to a middle is one, and was rounded up: an odd code goes back by one.
-template <typename T>
+// MENDS: that is done here; without, slow_codes() does it (for one in 128 tokens, in code that comes cold and is to be short).
+template <typename T, bool MENDS = true>
 __device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool check, bool& near) {
     near = false;
     if (factor == 0.f) return make_uint2(0u, 0u);
@@ -152,7 +153,8 @@ __device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool 
         }
     }
     if (sizeof(T) == 4) near = middle > FRB_8BIT_BORDER;
-    if (sizeof(T) == 2 && check) {
+    if (sizeof(T) == 2 && !MENDS) near = check;
+    if (sizeof(T) == 2 && MENDS && check) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float r = t[i] - FRB_8BIT_WHOLE;

@@ -6,7 +6,9 @@ namespace frb_products8 {
 
 // ----------------------------------------------------------------------------- rows as codes
 
-#define RC_KEPT 4                      // runs of 8 entries that a thread keeps in registers; what is beyond is read a second time (from L1)
+// Runs of 8 entries that a thread keeps in registers; what is beyond is read a second time (from L1).  512 threads a row are for few rows: one run
+// each, and code that is short, since it comes cold.
+constexpr int kept_runs(int per_row) { return per_row == 512 ? 1 : 4; }
 
 // A row is taken by PER_ROW threads, a block of 128 or more holds one or several.  Bound by memory where there are many rows (2,048 of 8192
 // float32 by 512 threads each 24 us, by 256 with all of their entries in registers 16), by two trips to it and the row's maximum where there
@@ -16,7 +18,7 @@ template <typename T, int PER_ROW>
 __global__ void __launch_bounds__(PER_ROW < 128 ? 128 : PER_ROW, PER_ROW == 512 ? 2 : (sizeof(T) == 4 ? 6 : 8) / (PER_ROW == 256 ? 2 : 1))
 rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP, const int* __restrict__ places, int copies, int places_end, int8_t* __restrict__ codes,
                  float* __restrict__ scales, int whole_rows) {
-    constexpr int BLOCK = PER_ROW < 128 ? 128 : PER_ROW, AT_ONCE = BLOCK / PER_ROW;
+    constexpr int BLOCK = PER_ROW < 128 ? 128 : PER_ROW, AT_ONCE = BLOCK / PER_ROW, KEPT = kept_runs(PER_ROW);
     __shared__ uint32_t warp_top[2][BLOCK / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = threadIdx.x % PER_ROW;
     wait_for_previous_kernel();
@@ -26,17 +28,17 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
         const int row = base + threadIdx.x / PER_ROW;
         const bool there = AT_ONCE == 1 || row < rows;          // (a block's last rows may be none; its barrier is for all)
         const T* src = x + (size_t)(there ? row : 0) * x_stride;
-        Eight<T> kept[RC_KEPT];
+        Eight<T> kept[KEPT];
         uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < RC_KEPT; ++j) {
+        for (int j = 0; j < KEPT; ++j) {
             const int k = (j * PER_ROW + me) * 8;
             if (k < K) kept[j].read(src + k, K - k, whole_rows);
             else kept[j].clear();
         }
 #pragma unroll
-        for (int j = 0; j < RC_KEPT; ++j) top = top_of(kept[j], top);
-        for (int k = (RC_KEPT * PER_ROW + me) * 8; k < K; k += PER_ROW * 8) {
+        for (int j = 0; j < KEPT; ++j) top = top_of(kept[j], top);
+        for (int k = (KEPT * PER_ROW + me) * 8; k < K; k += PER_ROW * 8) {
             Eight<T> v;
             v.read(src + k, K - k, whole_rows);
             top = top_of(v, top);
@@ -53,10 +55,10 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
         float factor, scale;
         bool check;
         row_factor<T>(top, factor, scale, check);
-        uint2 made[RC_KEPT];
+        uint2 made[KEPT];
         uint32_t again = 0;            // one bit for each run of eight entries that slow_codes() decides
 #pragma unroll
-        for (int j = 0; j < RC_KEPT; ++j) {
+        for (int j = 0; j < KEPT; ++j) {
             bool near;
             made[j] = codes_of(kept[j], factor, check, near);
             again |= (uint32_t)near << j;
@@ -68,7 +70,7 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
             if ((unsigned)to >= (unsigned)places_end) continue;
             int8_t* dst = codes + (size_t)to * KP;
 #pragma unroll
-            for (int j = 0; j < RC_KEPT; ++j) {
+            for (int j = 0; j < KEPT; ++j) {
                 const int k = (j * PER_ROW + me) * 8;
                 if (k < KP) *reinterpret_cast<uint2*>(dst + k) = made[j];
             }
@@ -84,10 +86,10 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
 #pragma unroll 1
         for (int j = 0; again >> j; ++j) {
             const int k = (j * PER_ROW + me) * 8;
-            if (again >> j & 1) put(k, slow_codes(src + k, K - k, factor, a));
+            if ((again >> j & 1) && k < K) put(k, slow_codes(src + k, K - k, factor, a));
         }
 #pragma unroll 1
-        for (int k = (RC_KEPT * PER_ROW + me) * 8; k < KP; k += PER_ROW * 8) {
+        for (int k = (KEPT * PER_ROW + me) * 8; k < KP; k += PER_ROW * 8) {
             Eight<T> v;
             if (k < K) v.read(src + k, K - k, whole_rows);
             else v.clear();
@@ -114,10 +116,10 @@ int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const i
     } while (0)
     // as few threads a row as hold it in registers, where there are rows for every SM; else as many as there may be
     FRB_DISPATCH_DTYPE(x_type, T, {
-        if (rows <= 2 * frb_sm_count() || K > 256 * 8 * RC_KEPT) LAUNCH(512);
-        else if (K > 128 * 8 * RC_KEPT) LAUNCH(256);
-        else if (K > 64 * 8 * RC_KEPT) LAUNCH(128);
-        else if (K > 32 * 8 * RC_KEPT) LAUNCH(64);
+        if (rows <= 2 * frb_sm_count() || K > 256 * 8 * kept_runs(256)) LAUNCH(512);
+        else if (K > 128 * 8 * kept_runs(128)) LAUNCH(256);
+        else if (K > 64 * 8 * kept_runs(64)) LAUNCH(128);
+        else if (K > 32 * 8 * kept_runs(32)) LAUNCH(64);
         else LAUNCH(32);
     });
 #undef LAUNCH
