@@ -28,13 +28,15 @@ static int hidden_stride(int I) { return up_to(I, 32); }
     } while (0)
 
 // Rows and the product that reads them: one launch where the product rounds them itself, else rows as codes in the scratch first.  The kernel
-// that makes those lets the product start only after its own wait, so that the weights, whoever wrote them, are complete by then.
-static int rows_and_product(Product& p, const void* x, int x_type, int x_stride, int8_t* codes, float* scales, bool weights_final, cudaStream_t stream) {
+// that makes those lets the product start only after its own wait, so that the weights, whoever wrote them, are complete by then; behind another
+// product (in_chain), which has waited so itself, before it.
+static int rows_and_product(Product& p, const void* x, int x_type, int x_stride, int8_t* codes, float* scales, bool weights_final, bool in_chain,
+                            cudaStream_t stream) {
     if (!p.lists.tile_expert && tokens_fit(p.rows, p.K)) {
         p.x = x; p.x_type = x_type; p.x_stride = x_stride; p.x_scale = nullptr; p.weights_final = weights_final;
         return product(p, stream);
     }
-    FRB_TRY(rows_codes(x, x_type, x_stride, p.rows, p.K, nullptr, 1, codes, scales, stream));
+    FRB_TRY(rows_codes(x, x_type, x_stride, p.rows, p.K, nullptr, 1, codes, scales, in_chain, stream));
     p.x = codes; p.x_scale = scales; p.weights_final = true;
     return product(p, stream);
 }
@@ -60,7 +62,7 @@ FRB_API int frb_linear_8bit(const void* x, int x_type, int T, int K, const void*
     Product p = {};
     p.w = w; p.w_scale = w_scale; p.experts = 1; p.parts = 1; p.F = F; p.K = K; p.rows = T; p.out = out; p.out_stride = F; p.out_type = out_type;
     p.status = status;
-    return rows_and_product(p, x, x_type, K, codes, scales, weights_final != 0, stream);
+    return rows_and_product(p, x, x_type, K, codes, scales, weights_final != 0, false, stream);
 }
 
 // h = act(x Wg^T) * (x Wu^T) in float32, rounded to codes row by row, out [T, d] = h Wd^T.  w_in: codes [2][I up to 16][d up to 128] (gate, up),
@@ -84,9 +86,9 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     Product p = {};
     p.w = w_in; p.w_scale = in_scale; p.experts = 1; p.parts = 2; p.F = I; p.K = d; p.rows = T; p.out = hidden; p.out_stride = IP;
     p.out_type = FRB_F32; p.gate = gate; p.limit = limit; p.status = status;
-    FRB_TRY(rows_and_product(p, x, x_type, d, codes, scales, weights_final != 0, stream));
+    FRB_TRY(rows_and_product(p, x, x_type, d, codes, scales, weights_final != 0, false, stream));
     p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.out = out; p.out_stride = d; p.out_type = out_type;
-    return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, stream);     // (the first product waited before it let this one start)
+    return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, true, stream);     // (the first product waited before it let this one start)
 }
 
 // The experts' outputs y [N, d] (float32, rows y_stride apart, in the order of the lists) for T tokens that were given their rows already: row_of_assign
@@ -104,13 +106,13 @@ static int expert_rows(const void* x, int x_type, int T, int d, int top_k, const
     float* hidden_scales = s.take<float>(N);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, %lld are needed", scratch_bytes, s.at);
     FRB_CHECK_ARG(s.starts_well(), "experts in 8 bits: the scratch starts on 16 bytes");
-    FRB_TRY(rows_codes(x, x_type, d, T, d, row_of_assign, top_k, codes, scales, stream));
+    FRB_TRY(rows_codes(x, x_type, d, T, d, row_of_assign, top_k, codes, scales, false, stream));
     Product p = {};
     p.w = w_in; p.w_scale = in_scale; p.experts = experts; p.parts = 2; p.F = I; p.K = d; p.rows = N; p.x = codes; p.x_scale = scales;
     p.lists = lists;
     p.out = hidden; p.out_stride = IP; p.out_type = FRB_F32; p.gate = FRB_GATE_SILU; p.limit = limit; p.status = status; p.weights_final = true;
     FRB_TRY(product(p, stream));
-    FRB_TRY(rows_codes(hidden, FRB_F32, IP, N, I, nullptr, 1, hidden_codes, hidden_scales, stream));
+    FRB_TRY(rows_codes(hidden, FRB_F32, IP, N, I, nullptr, 1, hidden_codes, hidden_scales, true, stream));
     p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.x = hidden_codes; p.x_scale = hidden_scales; p.out = y; p.out_stride = y_stride;
     return product(p, stream);
 }
