@@ -461,25 +461,24 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         const auto step_at = [&](int i) { return STEP * ((((i >> shift) * 2 + turn) << shift) + (i & ((1 << shift) - 1))); };
         int half = 0;
         uint32_t sums_parity = 0;                                 // one bit for each half
-        // A tile's scales are read while the one before it is computed.
+        // A tile's place and scales are read while the one before it is computed.
         float next_x = 0.f, next_w = 0.f;
+        int next_row0 = 0, next_channel = 0, next_rows = 0;
         const auto ask = [&](int item) {
             if (item >= items) return;
-            int row0, expert, channel;
-            place(item, row0, expert, channel);
-            const int rows = listed ? min(p.lists.tile_rows, min(p.lists.offsets[expert + 1], p.rows) - row0) : p.rows - row0;
+            int expert;
+            place(item, next_row0, expert, next_channel);
+            next_rows = listed ? min(p.lists.tile_rows, min(p.lists.offsets[expert + 1], p.rows) - next_row0) : p.rows - next_row0;
             const int within = side * 128 + quarter * span + lane, i = threadIdx.x - 64;
-            if (!ROUNDS && within < rows && lane < span && quarter * span + lane < p.x_box) next_x = p.x_scale[row0 + within];
+            if (!ROUNDS && within < next_rows && lane < span && quarter * span + lane < p.x_box) next_x = p.x_scale[next_row0 + within];
             if (i < p.columns) {
                 const int part = PARTS == 2 && i >= p.n ? 1 : 0, c = i - part * p.n;
-                next_w = channel + c < p.F ? p.w_scale[((size_t)expert * PARTS + part) * p.FP + channel + c] : 0.f;
+                next_w = next_channel + c < p.F ? p.w_scale[((size_t)expert * PARTS + part) * p.FP + next_channel + c] : 0.f;
             }
         };
         ask(first);
         for (int item = first; item < items; item += step) {
-            int row0, expert, channel;
-            place(item, row0, expert, channel);
-            const int rows = listed ? min(p.lists.tile_rows, min(p.lists.offsets[expert + 1], p.rows) - row0) : p.rows - row0;
+            const int row0 = next_row0, channel = next_channel, rows = next_rows;
             const int warp_row = side * 128 + quarter * span, within = warp_row + lane;
             const bool mine = within < rows && lane < span && quarter * span + lane < p.x_box;
             const bool any = warp_row < rows && quarter * span < p.x_box;
