@@ -28,15 +28,15 @@ static int hidden_stride(int I) { return up_to(I, 32); }
     } while (0)
 
 // Rows and the product that reads them: one launch where the product rounds them itself, else rows as codes in the scratch first.  The kernel
-// that makes those lets the product start only after its own wait, so that the weights, whoever wrote them, are complete by then; behind another
-// product (in_chain), which has waited so itself, before it.
+// that makes those lets the product start only after its own wait, so that the weights, whoever wrote them, are complete by then; before it where
+// they are so anyway: behind another product (in_chain), which has waited so itself, and by the caller's word.
 static int rows_and_product(Product& p, const void* x, int x_type, int x_stride, int8_t* codes, float* scales, bool weights_final, bool in_chain,
                             cudaStream_t stream) {
     if (!p.lists.tile_expert && tokens_fit(p.rows, p.K)) {
         p.x = x; p.x_type = x_type; p.x_stride = x_stride; p.x_scale = nullptr; p.weights_final = weights_final;
         return product(p, stream);
     }
-    FRB_TRY(rows_codes(x, x_type, x_stride, p.rows, p.K, nullptr, 1, codes, scales, in_chain, stream));
+    FRB_TRY(rows_codes(x, x_type, x_stride, p.rows, p.K, nullptr, 1, codes, scales, in_chain || weights_final, stream));
     p.x = codes; p.x_scale = scales; p.weights_final = true;
     return product(p, stream);
 }
@@ -88,7 +88,7 @@ FRB_API int frb_gated_8bit(const void* x, int x_type, int T, int d, const void* 
     p.out_type = FRB_F32; p.gate = gate; p.limit = limit; p.status = status;
     FRB_TRY(rows_and_product(p, x, x_type, d, codes, scales, weights_final != 0, false, stream));
     p.w = w_down; p.w_scale = down_scale; p.parts = 1; p.F = d; p.K = I; p.out = out; p.out_stride = d; p.out_type = out_type;
-    return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, true, stream);     // (the first product waited before it let this one start)
+    return rows_and_product(p, hidden, FRB_F32, IP, hidden_codes, hidden_scales, true, true, stream);
 }
 
 // The experts' outputs y [N, d] (float32, rows y_stride apart, in the order of the lists) for T tokens that were given their rows already: row_of_assign

@@ -53,8 +53,8 @@ struct Product {
     int* status;               // 0, or the code of the wait that gave up
 };
 
-// rows_8bit.cu; in_chain: the kernel before this one is a product of the same call, which lets this one start only after its own wait
-int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const int* places, int copies, void* codes, float* scales, bool in_chain, cudaStream_t stream);
+// rows_8bit.cu; early: the kernel after this one may start before this one's wait is over (what it reads ahead is complete)
+int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const int* places, int copies, void* codes, float* scales, bool early, cudaStream_t stream);
 int plan(const int* ids, int tokens, int top_k, int experts, int tile_rows, int* offsets, int* row_of_assign, int* tile_expert, int* tile_row0,
          int* num_tiles, cudaStream_t stream);
 int combine(const float* y, int y_stride, const float* weights, const int* row_of_assign, int tokens, int top_k, int width, void* out, int out_type,
