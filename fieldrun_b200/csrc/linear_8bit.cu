@@ -148,6 +148,7 @@ FRB_API int frb_experts_8bit(const void* x, int x_type, int T, int d, int top_k,
     const int y_stride = hidden_stride(d);
     float* y = s.take<float>((long long)N * y_stride);
     FRB_CHECK_ARG(s.at <= scratch_bytes, "experts in 8 bits: %lld bytes of scratch, more are needed", scratch_bytes);
+    FRB_CHECK_ARG(s.starts_well(), "experts in 8 bits: the scratch starts on 16 bytes");       // (the lists, too, are written into it)
     FRB_TRY(plan(ids, T, top_k, experts, tile_rows, offsets, row_of_assign, tile_expert, tile_row0, num_tiles, stream));
     FRB_TRY(expert_rows(x, x_type, T, d, top_k, row_of_assign, {tile_expert, tile_row0, num_tiles, offsets, max_tiles, tile_rows}, w_in, in_scale, experts, I,
                         w_down, down_scale, limit, y, y_stride, s, scratch_bytes, status, stream));
