@@ -62,7 +62,6 @@ attention_pair_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     constexpr uint32_t STAGE_BYTES = 2 * K_STEP + AP_STEP_PAGES * V_BYTES;
     constexpr uint32_t SP_COL0 = 0, O_COL0 = 2 * AP_STEP_KEYS, TMEM_COLS = 512;
 
-    let_next_kernel_start();
     const int tile = gridDim.x - 1 - blockIdx.x, head = blockIdx.y;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int group = p.heads / p.v_heads, vh = head / group;
@@ -94,7 +93,7 @@ attention_pair_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-    wait_for_previous_kernel();
+    after_previous_kernel();                                   // (the next one starts not before this block has its columns: tmem_alloc())
 
     if (warp == 0) {
         if (lane == 0) {

@@ -80,7 +80,6 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
 
     // The step's tables are not the work of the kernel before this one (it writes queries, keys and values): they
     // are read, and barriers and tensor memory set up, while that kernel still runs.
-    let_next_kernel_start();
     const int tile = gridDim.x - 1 - blockIdx.x, head = blockIdx.y;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int group = p.num_heads / p.num_kv_heads, kvh = head / group;
@@ -116,7 +115,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-    wait_for_previous_kernel();
+    after_previous_kernel();                                   // (the next one starts not before this block has its columns: tmem_alloc())
 
     if (warp == 0) {
         if (lane == 0) {

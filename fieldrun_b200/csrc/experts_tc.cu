@@ -63,7 +63,6 @@ expert_gemm_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     // run side by side read the same rows (which stay in L2) and, where an expert has several tiles, the same
     // weights soon after.  The ring of stages runs on from item to item, so the next item's first tiles arrive
     // while the epilogue still reads this item's accumulators.
-    let_next_kernel_start();
     const int feature_blocks = p.F / BLOCK_FEATS;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int f_total = PAIRED ? 2 * p.F : p.F;
@@ -86,7 +85,7 @@ expert_gemm_tc_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem_base_slot, 0);
-    wait_for_previous_kernel();                                  // barriers and tensor memory were set up while it still ran
+    after_previous_kernel();                                     // barriers and tensor memory were set up while it still ran
     const int num_items = p.num_tiles[0] * feature_blocks;
 
     if (warp == 0) {

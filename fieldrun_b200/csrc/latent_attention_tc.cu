@@ -111,7 +111,6 @@ latent_attention_tc_kernel(const __grid_constant__ CUtensorMap map_ql, const __g
     __shared__ int failed_flag;
     volatile int* failed = &failed_flag;
 
-    let_next_kernel_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int TQ = p.tokens_per_block, HB = p.heads_per_block, T = p.num_tokens, H = p.num_heads;
     const int chunk = p.chunk_pages > 0 ? (int)blockIdx.x % p.num_chunks : 0;
@@ -143,7 +142,7 @@ latent_attention_tc_kernel(const __grid_constant__ CUtensorMap map_ql, const __g
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    wait_for_previous_kernel();
+    after_previous_kernel();                                   // (the next one starts not before this block has its columns: tmem_alloc())
 
     if (warp == 0) {
         if (lane == 0) {

@@ -97,7 +97,9 @@ __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fenc
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // One warp of the block allocates `columns` (a power of two, at least 32) of tensor memory and leaves their
-// address in *slot (shared memory); the same warp frees them before the block ends.
+// address in *slot (shared memory); the same warp frees them before the block ends.  The allocation waits, without a limit, for columns
+// that other blocks of the SM hold.  So a kernel that takes columns lets the next one start only once it has them: the next
+// one may take its own ahead of its wait for this kernel, and must not get in before.
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(slot)), "r"(columns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");

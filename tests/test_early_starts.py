@@ -1,0 +1,62 @@
+"""How kernels that start before the one before them has ended are written, read from their sources on the host.
+
+A kernel that was written the other way round may wait for ever, so what these rules forbid is not run."""
+import glob
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "fieldrun_b200", "csrc")
+LETS_NEXT = re.compile(r"\b(let_next_kernel_start|after_previous_kernel)\(\)")
+WAITS = re.compile(r"\b(wait_for_previous_kernel|after_previous_kernel)\(\)")
+TAKES_COLUMNS = re.compile(r"\b(tmem_alloc|alloc_columns<\w+>)\(&")
+
+
+def without_comments(text):
+    return re.sub(r"//[^\n]*", "", re.sub(r"/\*.*?\*/", "", text, flags=re.S))
+
+
+def body_at(text, at):
+    """The braces' contents from the first brace at or behind `at`."""
+    start = text.index("{", at)
+    depth = 0
+    for i in range(start, len(text)):
+        depth += {"{": 1, "}": -1}.get(text[i], 0)
+        if depth == 0:
+            return text[start + 1:i]
+    raise AssertionError("braces do not match")
+
+
+def kernels():
+    """(file and name, body) of every kernel."""
+    found = []
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu"))):
+        with open(path) as handle:
+            text = without_comments(handle.read())
+        for m in re.finditer(r"__global__\s+void\s+(?:__launch_bounds__\((?:[^()]|\([^()]*\))*\)\s*)?(\w+)\s*\(", text):
+            depth, i = 1, m.end()
+            while depth:
+                depth += {"(": 1, ")": -1}.get(text[i], 0)
+                i += 1
+            if text[i:].lstrip().startswith("{"):
+                found.append((f"{os.path.basename(path)}:{m.group(1)}", body_at(text, i)))
+    return found
+
+
+KERNELS = dict(kernels())
+WITH_COLUMNS = [name for name, body in KERNELS.items() if TAKES_COLUMNS.search(body)]
+
+
+def test_the_kernels_are_found():
+    assert len(KERNELS) > 100 and {name.split(":")[0] for name in WITH_COLUMNS} == {
+        "attention_f32_tc.cu", "attention_pair_tc.cu", "attention_tc.cu", "delta_chunks.cu", "experts_tc.cu", "latent_attention_tc.cu", "products_8bit.cu",
+        "products_f32.cu", "state_space_chunks.cu"}
+
+
+@pytest.mark.parametrize("name", WITH_COLUMNS)
+def test_a_kernel_with_tensor_memory_lets_the_next_one_start_only_once_it_has_its_columns(name):
+    """Else the next kernel's block could take them first and wait for this kernel, whose block waits for the columns."""
+    body = KERNELS[name]
+    lets = LETS_NEXT.search(body)
+    assert lets is None or lets.start() > TAKES_COLUMNS.search(body).end()
