@@ -401,6 +401,7 @@ product_8bit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
     } else if (warp == 1) {
         if (side == 0) {
+            wait_for_previous_kernel();                       // no tokens before that; the limits of the waits below are for this kernel's own work
             const uint32_t idesc = instr_desc_i8(p.m * CTAS, p.columns);
             const uint64_t first_x = tile_desc(smem_addr(ROUNDS ? tokens : ring)), first_w = tile_desc(smem_addr(ring) + stage_x);
             const uint32_t stage_step = stage_bytes >> 4, x_step = ROUNDS ? 64 : x_bytes >> 4, w_step = w_bytes >> 4;      // in 16 bytes

@@ -60,3 +60,30 @@ def test_a_kernel_with_tensor_memory_lets_the_next_one_start_only_once_it_has_it
     body = KERNELS[name]
     lets = LETS_NEXT.search(body)
     assert lets is None or lets.start() > TAKES_COLUMNS.search(body).end()
+
+
+BOUNDED_WAIT = re.compile(r"\b(warp_wait|bar_wait|warp_wait_both)\(")
+
+
+def roles(body):
+    """The contents of a kernel's branches `if (warp == 0) {..} else if (warp == 1) {..} else {..}`."""
+    at = re.search(r"\bif \(warp == 0\) \{", body).start()
+    found = []
+    while True:
+        found.append(body_at(body, at))
+        end = body.index(found[-1], at) + len(found[-1]) + 1
+        follows = re.match(r"\s*else\b", body[end:])
+        if not follows:
+            return found
+        at = end + follows.end()
+
+
+def test_the_products_roles_wait_for_the_kernel_before_ahead_of_any_wait_with_a_limit():
+    """A wait's limit of about a second is for the kernel's own copies and products: what the kernel before still does, beside which this one has
+    started, must not be charged to it."""
+    body = KERNELS["products_8bit.cu:product_8bit_kernel"]
+    assert not BOUNDED_WAIT.search(body[:re.search(r"\bif \(warp == 0\) \{", body).start()])
+    branches = roles(body)
+    assert len(branches) == 3
+    for branch in branches:
+        assert WAITS.search(branch).start() < BOUNDED_WAIT.search(branch).start()
