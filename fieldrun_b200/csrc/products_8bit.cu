@@ -726,13 +726,18 @@ int product(const Product& q, cudaStream_t stream) {
     config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attributes[2];
-    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attributes[0].val.programmaticStreamSerializationAllowed = 1;
-    attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = (unsigned)ctas;
-    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
-    config.numAttrs = ctas == 2 ? 2 : 1;
+    if (ctas == 2) {
+        cudaLaunchAttribute& pairs = attributes[config.numAttrs++];
+        pairs.id = cudaLaunchAttributeClusterDimension;
+        pairs.val.clusterDim.x = 2;
+        pairs.val.clusterDim.y = pairs.val.clusterDim.z = 1;
+    }
+    if ((long)config.gridDim.x <= frb_dependent_launch_blocks()) {
+        cudaLaunchAttribute& early = attributes[config.numAttrs++];
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+    }
 #define LAUNCH(CTAS, PARTS, OutT, InT, WHOLE)                                                                                         \
     do {                                                                                                                              \
         may_have_shared<product_8bit_kernel<CTAS, PARTS, OutT, InT, WHOLE>>();                                                         \

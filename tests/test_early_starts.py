@@ -87,3 +87,11 @@ def test_the_products_roles_wait_for_the_kernel_before_ahead_of_any_wait_with_a_
     assert len(branches) == 3
     for branch in branches:
         assert WAITS.search(branch).start() < BOUNDED_WAIT.search(branch).start()
+
+
+def test_every_early_start_asks_the_switch():
+    """FIELDRUN_B200_PDL sets the largest grid that starts early, 0 none."""
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))):
+        with open(path) as handle:
+            text = without_comments(handle.read())
+        assert text.count("cudaLaunchAttributeProgrammaticStreamSerialization") <= len(re.findall(r"<= (?:per_sm \* )?frb_dependent_launch_blocks\(\)", text)), path
