@@ -172,9 +172,10 @@ __device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool 
 // p + e and c a = q + f, both sums of two float32, the remainder against half of a is (p - q -+ a/2) + (e - f), where both differences in the
 // first bracket are of numbers within a factor of two of one another and so without rounding, and so is e - f: every term is a
 // whole multiple of x's last place, e below 2^7 and f below 2^15 of them (a is less than 2^8 times x, or its code were 0).
+// (p, q and their difference by name: a compiler may join a product and a subtraction into one rounding, and e and f would then count twice.)
 __device__ __forceinline__ float decided_code(float x, float c, float a) {
     if (a > 1.2676506e30f) { x *= 9.5367432e-7f; a *= 9.5367432e-7f; }               // above 2^100: times 2^-20, or 127 x would be infinite
-    const float p = 127.f * x, e = fmaf(127.f, x, -p), q = c * a, f = fmaf(c, a, -q), d = p - q;
+    const float p = __fmul_rn(127.f, x), e = fmaf(127.f, x, -p), q = __fmul_rn(c, a), f = fmaf(c, a, -q), d = __fsub_rn(p, q);
     const float toward = copysignf(1.f, d), over = toward * ((d - toward * (0.5f * a)) + (e - f));
     return over > 0.f || (over == 0.f && ((int)c & 1)) ? c + toward : c;
 }
