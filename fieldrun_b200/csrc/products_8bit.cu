@@ -264,8 +264,7 @@ __device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, 
     top = 0;
     for (int i = 0; i < per_row; ++i) top = max(top, tops[0][ew - sub + i]);
     float factor, scale;
-    bool check;
-    row_factor<InT>(top, factor, scale, check);
+    row_factor<InT>(top, factor, scale);
     if (!mine) return;
     const auto place = [&](int k) { return reinterpret_cast<uint2*>(codes + (k >> 7) * 1024 + row * 128 + ((((k >> 4) & 7) ^ row) << 4) + (k & 8)); };
     uint32_t again = 0;                                       // one bit for each run of eight entries that slow_codes() decides
@@ -274,7 +273,7 @@ __device__ __forceinline__ void round_tokens(const Params& p, int ew, int lane, 
         const int k = first + j * step;
         if (k >= KP) break;
         bool near;
-        *place(k) = codes_of<InT, false>(kept[j], factor, check, near);
+        *place(k) = codes_of(kept[j], factor, near);
         again |= (uint32_t)near << j;
     }
 #pragma unroll 1

@@ -114,17 +114,16 @@ __device__ __forceinline__ uint32_t top_of(const Eight<T>& v, uint32_t top) {
     return top;
 }
 
-// What a row's largest magnitude a (its bits) gives: the factor of its entries before they are rounded, the scale that is stored, and whether
-// a bfloat16 row's products with the factor have to be looked at for values in the middle of two codes.
+// What a row's largest magnitude a (its bits) gives: the factor of its entries before they are rounded, and the scale that is stored.
 //
-// bfloat16: with the factor rounded up they need not, but for one row in 128.  Let x and a be integers of 8 bits, 127 x / (a 2^s) their quotient.  If
-// it is not a middle n + 1/2, it is at least 1 / (254 x) > 1.5e-5 of itself from one, and the factor's error (2^-23 of itself) takes it past none.
-// If it is one, (2 n + 1) a 2^s = 254 x; unless 127 divides a (a = 254), 127 divides 2 n + 1, so n = 63, and rounding up gives the even code, 64.
+// bfloat16: with the factor rounded up every product is rounded as the quotient is.  Let x and a be integers of 8 bits, 127 x / (a 2^s) their quotient.
+// If it is not a middle n + 1/2, it is at least 1 / (254 x) > 1.5e-5 of itself from one, and the factor's error (2^-23 of itself) takes it past none.
+// If it is one, (2 n + 1) a 2^s = 254 x.  Either 127 divides a, so a = 254: the factor is a power of two and the product exact.  Or 127 divides
+// 2 n + 1, so n = 63, and rounding up gives the even code, 64.
 template <typename T>
-__device__ __forceinline__ void row_factor(uint32_t top, float& factor, float& scale, bool& check) {
+__device__ __forceinline__ void row_factor(uint32_t top, float& factor, float& scale) {
     const float a = __uint_as_float(top);
     factor = scale = 0.f;
-    check = sizeof(T) == 2 && (top >> 16 & 0x7f) == 126;
     if (top >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);
     else if (a >= FRB_8BIT_SMALLEST_ROW) { factor = sizeof(T) == 4 ? __fdiv_rn(127.f, a) : __fdiv_ru(127.f, a); scale = __fdiv_rn(a, 127.f); }
 }
@@ -132,11 +131,10 @@ __device__ __forceinline__ void row_factor(uint32_t top, float& factor, float& s
 #define FRB_8BIT_WHOLE 12582912.f      // 1.5 * 2^23: a number added to it is rounded to a whole one, whose lowest byte is the sum's
 #define FRB_8BIT_BORDER 0.49998f       // the factor is off by 2^-23 of itself at most, a product by 127 * 2^-23 < 1.6e-5
 
-// 127 x / a rounded half to even, for eight entries; `near`: one of them is so near to the middle of two codes that slow_codes() has to decide.  In a
-// row of bfloat16 that is to be checked an entry nearer than 1e-6 of itself to a middle is one, and was rounded up: an odd code goes back by one.
-// MENDS: that is done here; without, slow_codes() does it (for one in 128 tokens, in code that comes cold and is to be short).
-template <typename T, bool MENDS = true>
-__device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool check, bool& near) {
+// 127 x / a rounded half to even, for eight entries; `near`: one of them (of float32) is so near to the middle of two codes that slow_codes() has to
+// decide.
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool& near) {
     near = false;
     if (factor == 0.f) return make_uint2(0u, 0u);
     float t[8];
@@ -152,15 +150,7 @@ __device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float factor, bool 
             middle = fmaxf(middle, fmaxf(fabsf(r0), fabsf(r1)));
         }
     }
-    if (sizeof(T) == 4) near = middle > FRB_8BIT_BORDER;
-    if (sizeof(T) == 2 && !MENDS) near = check;
-    if (sizeof(T) == 2 && MENDS && check) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float r = t[i] - FRB_8BIT_WHOLE;
-            if (fmaf(fabsf(r), 1e-6f, fabsf(fmaf(v.entry(i), factor, -r))) >= 0.5f && (__float_as_uint(t[i]) & 1u)) t[i] -= copysignf(1.f, r);
-        }
-    }
+    near = sizeof(T) == 4 && middle > FRB_8BIT_BORDER;
     uint32_t w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(t[i]);
@@ -180,7 +170,7 @@ __device__ __forceinline__ float decided_code(float x, float c, float a) {
     return over > 0.f || (over == 0.f && ((int)c & 1)) ? c + toward : c;
 }
 
-// The codes of eight entries that stand at p, decided one after another.  (Few runs come here; the code is short, and the registers of those
+// The codes of eight float32 entries that stand at p, decided one after another.  (Few runs come here; the code is short, and the registers of those
 // that do not come are left alone.)
 template <typename T>
 __device__ __forceinline__ uint2 slow_codes(const T* p, int left, float factor, float top) {

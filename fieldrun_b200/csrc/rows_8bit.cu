@@ -56,14 +56,13 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
         if (!there) continue;
         const float a = __uint_as_float(top);
         float factor, scale;
-        bool check;
-        row_factor<T>(top, factor, scale, check);
+        row_factor<T>(top, factor, scale);
         uint2 made[KEPT];
         uint32_t again = 0;            // one bit for each run of eight entries that slow_codes() decides
 #pragma unroll
         for (int j = 0; j < KEPT; ++j) {
             bool near;
-            made[j] = codes_of(kept[j], factor, check, near);
+            made[j] = codes_of(kept[j], factor, near);
             again |= (uint32_t)near << j;
         }
         const int count = places ? copies : 1;
@@ -97,7 +96,7 @@ rows_8bit_kernel(const T* __restrict__ x, int x_stride, int rows, int K, int KP,
             if (k < K) v.read(src + k, K - k, whole_rows);
             else v.clear();
             bool near;
-            const uint2 c = codes_of(v, factor, check, near);
+            const uint2 c = codes_of(v, factor, near);
             put(k, near ? slow_codes(src + k, K - k, factor, a) : c);
         }
     }

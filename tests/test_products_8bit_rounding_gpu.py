@@ -69,3 +69,44 @@ def test_a_rows_results_are_its_own_however_it_was_rounded(dtype):
         out = torch.empty((count, 700), device=DEV)
         ops.linear_8bit(x[first:first + count], w, s, out)
         assert torch.equal(out, whole[first:first + count]), (first, count)
+
+
+def test_every_pair_of_bfloat16_significands():
+    """Row a has the largest entry a = 128 .. 255 and every entry of eight bits, halved up to eight times, that is at most a."""
+    x = torch.arange(128, 256, device=DEV)[None, :] * torch.exp2(-torch.arange(9.0, device=DEV))[:, None]
+    x = torch.cat([x.reshape(-1), torch.zeros(2048 - x.numel(), device=DEV)]).expand(128, -1)
+    a = torch.arange(128.0, 256.0, device=DEV)[:, None]
+    x = torch.where(x <= a, x, a)
+    x[:, 1::2] *= -1
+    for power in (-90, 0, 100):
+        rows = (x * 2.0 ** power).to(BF16)
+        want, _ = plain.codes_of(rows)
+        assert torch.equal(codes_by_rows(rows), want)
+        for first in range(0, 128, 8):
+            assert torch.equal(codes_by_product(rows[first:first + 8]), want[first:first + 8])
+
+
+def test_tokens_take_the_same_time_whatever_their_largest_entry():
+    """No largest entry sends a bfloat16 token to a slower code: 254 and 255, 8 tokens, the least of several recorded runs, with half as much to spare."""
+    gen = generator(3)
+    x = torch.randint(-250, 250, (8, 2048), generator=gen, device=DEV).float().to(BF16)
+    weights = [plain.random_weight(gen, 1, 1, 6144, 2048, DEV)[2:] for _ in range(4)]
+    out, took = torch.empty((8, 6144), device=DEV), {}
+    for top in (255, 254):
+        x[:, 5] = top
+        ops.linear_8bit(x, *weights[0], out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for n in range(40):
+                ops.linear_8bit(x, *weights[n % 4], out)
+        times = []
+        for _ in range(8):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            graph.replay()
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end))
+        took[top] = min(times)
+    assert took[254] < 1.5 * took[255], took
