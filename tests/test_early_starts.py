@@ -95,3 +95,22 @@ def test_every_early_start_asks_the_switch():
         with open(path) as handle:
             text = without_comments(handle.read())
         assert text.count("cudaLaunchAttributeProgrammaticStreamSerialization") <= len(re.findall(r"<= (?:per_sm \* )?frb_dependent_launch_blocks\(\)", text)), path
+
+
+@pytest.mark.parametrize("name", [name for name in KERNELS if name.split(":")[0] in ("rows_8bit.cu", "products_8bit.cu")])
+def test_kernels_of_products_in_8_bits_let_the_next_one_start_behind_their_own_wait(name):
+    """A product asks for weights and reads lists ahead of its wait: what wrote them, two kernels before, has ended by then only if the kernel between
+    has waited for it first.  `early` is the callers' word that there is nothing to wait for."""
+    body = KERNELS[name]
+    waits = WAITS.search(body).start()
+    for m in LETS_NEXT.finditer(body):
+        assert m.start() > waits or body[:m.start()].rstrip().endswith("if (early)")
+
+
+def test_rows_as_codes_let_the_product_start_early_only_where_its_weights_are_final():
+    with open(os.path.join(CSRC, "linear_8bit.cu")) as handle:
+        text = without_comments(handle.read())
+    early = [re.sub(r"\s+", " ", call).split(", ")[-2] for call in re.findall(r"rows_codes\(([^;]*)\)\)", text)]
+    assert early == ["in_chain || weights_final", "false", "true"]
+    # behind the experts' first product, which has waited for the rows before it
+    assert re.search(r"FRB_TRY\(product\(p, stream\)\);\s*FRB_TRY\(rows_codes\(hidden,[^;]*, true, stream\)\)", text)
