@@ -2067,7 +2067,7 @@ def gated_8bit(x: torch.Tensor, in_codes: torch.Tensor, in_scales: torch.Tensor,
     the clamped gate, as in the expert products), out [T, d] = h W_down^T.  Both products are as in :func:`linear_8bit`; h is made in float32
     and rounded to codes row by row.  ``in_codes`` [1, 2, width up to 16, d up to 128] (gate, up), ``down_codes`` [1, 1, d up to 16, width up to 128]."""
     rows, inner, _ = _rows_in_and_out(x, out, True)
-    if not 1 <= width <= EIGHT_BIT_MOST_INNER or activation not in GATES_8BIT or gate_limit < 0.0 or (gate_limit > 0.0 and activation != "silu"):
+    if not 1 <= width <= EIGHT_BIT_MOST_INNER or activation not in GATES_8BIT or not gate_limit >= 0.0 or (gate_limit > 0.0 and activation != "silu"):
         raise KernelError(f"gated_8bit: a width of {width}, activation {activation!r} and a gate limit of {gate_limit}")
     _weight_8bit_of("gated_8bit, gate and up", in_codes, in_scales, 1, 2, width, inner)
     _weight_8bit_of("gated_8bit, down", down_codes, down_scales, 1, 1, inner, width)
@@ -2112,7 +2112,7 @@ def expert_rows_8bit(x: torch.Tensor, row_of_assign: Optional[torch.Tensor], lis
         raise KernelError(f"rows of shape {list(x.shape)} with {given} rows of experts and results of {list(y.shape)}")
     tokens, inner = x.shape
     top_k = given // tokens
-    if tile_rows not in EXPERT_TILES_8BIT or max_tiles < 1 or not 1 <= width <= EIGHT_BIT_MOST_INNER or gate_limit < 0.0 or not 1 <= top_k <= 128:
+    if tile_rows not in EXPERT_TILES_8BIT or max_tiles < 1 or not 1 <= width <= EIGHT_BIT_MOST_INNER or not gate_limit >= 0.0 or not 1 <= top_k <= 128:
         raise KernelError(f"expert_rows_8bit: {max_tiles} tiles of {tile_rows} rows, a width of {width}, {top_k} experts a token, a gate limit of {gate_limit}")
     _want(y, torch.float32, "expert outputs")
     _want_ints("lists of the experts' rows", *lists, *(() if row_of_assign is None else (row_of_assign,)))
@@ -2136,7 +2136,7 @@ def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_c
         raise KernelError(f"ids of shape {list(ids.shape)} and weights of {list(weights.shape)} for {tokens} tokens (1 to 128 experts each)")
     _want_ints("the experts' ids", ids)
     _want(weights, torch.float32, "the experts' weights")
-    if not 1 <= width <= EIGHT_BIT_MOST_INNER or gate_limit < 0.0:
+    if not 1 <= width <= EIGHT_BIT_MOST_INNER or not gate_limit >= 0.0:
         raise KernelError(f"experts_8bit: a width of {width} and a gate limit of {gate_limit}")
     _weight_8bit_of("experts_8bit, gate and up", in_codes, in_scales, None, 2, width, inner)
     experts, top_k = in_codes.shape[0], ids.shape[1]

@@ -1,5 +1,6 @@
 """Products in 8-bit integers on the host: what the entry points refuse before anything is launched."""
 import pytest
+import torch
 
 from fieldrun_b200.csrc import ops
 
@@ -17,3 +18,29 @@ def test_scratch_off_16_bytes_is_refused_before_any_kernel_writes_to_it(place):
     for what, call in calls.items():
         assert call() == -1, what
         assert lib.frb_last_error().decode() == f"{what.strip()} in 8 bits: the scratch starts on 16 bytes"
+
+
+def weight(experts, parts, features, inner):
+    shape = ops.weight_8bit_shape(experts, parts, features, inner)
+    return torch.zeros(shape, dtype=torch.int8), torch.zeros(shape[:3])
+
+
+def ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def blocks(tokens):
+    """Calls of the gated operators for so many tokens, each with options of its own."""
+    x, w_in, w_down = torch.zeros(tokens, 100), weight(5, 2, 40, 100), weight(5, 1, 100, 40)
+    lists = (ints(6), ints(6), ints(1), ints(6))
+    return {
+        "gated_8bit": lambda **more: ops.gated_8bit(x, *weight(1, 2, 40, 100), *weight(1, 1, 100, 40), x.clone(), width=40, **more),
+        "expert_rows_8bit": lambda **more: ops.expert_rows_8bit(x, None, lists, 6, 8, *w_in, *w_down, x.clone(), width=40, **more),
+        "experts_8bit": lambda **more: ops.experts_8bit(x, ints(tokens, 2), torch.zeros(tokens, 2), *w_in, *w_down, x.clone(), width=40, **more)}
+
+
+@pytest.mark.parametrize("limit", [float("nan"), -1.0, -float("inf")])
+def test_a_gate_limit_that_is_none_is_refused(limit):
+    for name, call in blocks(3).items():
+        with pytest.raises(ops.KernelError, match=f"{name}: .*a gate limit of {limit}"):
+            call(gate_limit=limit)
