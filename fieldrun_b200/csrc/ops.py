@@ -2145,6 +2145,8 @@ def experts_8bit(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, in_c
     at = _addresses(x, ids, weights, in_codes, in_scales, down_codes, down_scales, out, scratch)
     _call("frb_experts_8bit", at[0], _code(x.dtype), tokens, inner, top_k, at[1], at[2], at[3], at[4], experts, width, at[5], at[6], float(gate_limit),
           expert_tile_rows_8bit(tokens * top_k, experts), at[7], _code(out.dtype), at[8], scratch.numel(), _status_at(x.device))
+    if tokens == 0:
+        count_launches(-_KERNELS_PER_CALL["frb_experts_8bit"])
 
 
 def wait_probe(device, limit_cycles: int = 100_000) -> int:

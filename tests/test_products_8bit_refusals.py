@@ -44,3 +44,17 @@ def test_a_gate_limit_that_is_none_is_refused(limit):
     for name, call in blocks(3).items():
         with pytest.raises(ops.KernelError, match=f"{name}: .*a gate limit of {limit}"):
             call(gate_limit=limit)
+
+
+@pytest.mark.parametrize("tokens", [0, 3])
+def test_kernels_counted(tokens, monkeypatch):
+    """What a call of no tokens launches is nothing; three tokens' linear layer is one kernel, their gated block two, their experts six."""
+    monkeypatch.setattr(ops, "_addresses", lambda *tensors: [0] * len(tensors))
+    monkeypatch.setattr(ops, "_status_at", lambda device: 0)
+    monkeypatch.setattr(ops, "_call", lambda name, *args: ops.count_launches(ops._KERNELS_PER_CALL[name]))
+    calls = blocks(tokens)
+    calls["linear_8bit"] = lambda: ops.linear_8bit(torch.zeros(tokens, 100), *weight(1, 1, 40, 100), torch.zeros(tokens, 40))
+    for name, kernels in {"linear_8bit": 1, "gated_8bit": 2, "experts_8bit": 6}.items():
+        before = ops.launches()
+        calls[name]()
+        assert ops.launches() - before == (kernels if tokens else 0), name
