@@ -1972,14 +1972,16 @@ def weight_8bit(*parts: torch.Tensor, codes: Optional[torch.Tensor] = None, scal
     """A weight's rows (one or two matrices [features, inner], gate and up; float32 or bfloat16) as codes [1, parts, features up to 16,
     inner up to 128] with scales [1, parts, features up to 16], as the products take them: every row as :func:`rows_8bit` stores it.  ``codes``
     and ``scales``: one expert's places in larger tensors (filled with zeros where no weights go)."""
-    features, inner = parts[0].shape if parts[0].dim() == 2 else (0, 0)
+    features, inner = parts[0].shape if parts and parts[0].dim() == 2 else (0, 0)
     if not 1 <= len(parts) <= 2 or features < 1 or any(part.shape != (features, inner) for part in parts):
         raise KernelError(f"weights of shapes {[list(part.shape) for part in parts]}: one matrix, or gate and up of one shape")
     shape = weight_8bit_shape(1, len(parts), features, inner)
+    if (codes is None) != (scales is None):
+        raise KernelError("a weight's codes and scales come together or not at all")
     if codes is None:
         codes = torch.zeros(shape, dtype=torch.int8, device=parts[0].device)
         scales = torch.zeros(shape[:3], dtype=torch.float32, device=parts[0].device)
-    if codes.shape != shape or scales is None or scales.shape != shape[:3]:
+    if codes.shape != shape or scales.shape != shape[:3]:
         raise KernelError(f"codes of shape {list(codes.shape)}, not {list(shape)}, for {len(parts)} matrices of {features} x {inner}")
     for part, part_codes, part_scales in zip(parts, codes[0], scales[0]):
         rows_8bit(part, part_codes[:features], part_scales[:features])

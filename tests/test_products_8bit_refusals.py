@@ -58,3 +58,15 @@ def test_kernels_counted(tokens, monkeypatch):
         before = ops.launches()
         calls[name]()
         assert ops.launches() - before == (kernels if tokens else 0), name
+
+
+def test_a_weights_places_come_together():
+    codes, scales = weight(1, 1, 40, 100)
+    matrix = torch.zeros(40, 100)
+    for more in (dict(codes=codes), dict(scales=scales)):
+        with pytest.raises(ops.KernelError, match="codes and scales come together"):
+            ops.weight_8bit(matrix, **more)
+    with pytest.raises(ops.KernelError, match="weights of shapes \\[\\]: one matrix"):
+        ops.weight_8bit()
+    with pytest.raises(ops.KernelError, match="a CPU tensor was given"):
+        ops.weight_8bit(matrix, codes=codes, scales=scales)
