@@ -7,7 +7,8 @@ namespace frb_products8 {
 // ----------------------------------------------------------------------------- rows as codes
 
 // Runs of 8 entries that a thread keeps in registers; what is beyond is read a second time (from L1).  512 threads a row are for few rows: one run
-// each, and code that is short, since it comes cold (200 rows of 4,096 bfloat16: 3.4 us with four, 2.2 with one).
+// each, and code that is short, since it comes cold (200 rows of 4,096 bfloat16: 3.4 us with four, 2.2 with one).  They also take the rows that are too
+// long for 256 threads' registers, however many there are; of these all entries behind the first 4,096 are read twice.
 constexpr int kept_runs(int per_row) { return per_row == 512 ? 1 : 4; }
 
 // A row is taken by PER_ROW threads, a block of 128 or more holds one or several.  Bound by memory where there are many rows (2,048 of 8192
@@ -116,7 +117,7 @@ int rows_codes(const void* x, int x_type, int x_stride, int rows, int K, const i
         launch_dependent(rows_8bit_kernel<T, PER_ROW>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),                  \
                          dim3(PER_ROW < 128 ? 128 : PER_ROW), 0, stream, (const T*)x, x_stride, rows, K, KP, places, copies, places ? rows * copies : rows, (int8_t*)codes, scales, whole, (int)early); \
     } while (0)
-    // as few threads a row as hold it in registers, where there are rows for every SM; else as many as there may be
+    // as few threads a row as hold it in registers, where there are rows for every SM and it is no longer than 8,192 entries; else as many as there may be
     FRB_DISPATCH_DTYPE(x_type, T, {
         if (rows <= 2 * frb_sm_count() || K > 256 * 8 * kept_runs(256)) LAUNCH(512);
         else if (K > 128 * 8 * kept_runs(128)) LAUNCH(256);
